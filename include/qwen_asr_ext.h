@@ -219,6 +219,76 @@ int32_t qwen_asr_pool_stream_push_many(QwenAsrPool* pool, QwenAsrStreamState* co
  * `workers` workers, longest first to the least-loaded worker. Returns 0 or -1. */
 int32_t qwen_asr_debug_assign_longest_first(const int64_t* lengths, int32_t n, int32_t workers, int32_t* worker_of);
 
+/* ---- 8-bit operators on device memory -------------------------------------------------
+ * The operators of the engine's int8 prefill and int8 KV cache, for callers who keep their
+ * own tensors. All pointers are device pointers of one GPU; `device` is its ordinal (-1: the
+ * caller's current device), `stream` a cudaStream_t of it (NULL: the default stream). A call
+ * enqueues its kernels and returns: no allocation, no workspace, no synchronisation, so it can
+ * be captured into a CUDA graph and calls on different streams share nothing. Returns 0, or -1
+ * with the reason in qwen_asr_last_error() and nothing enqueued. Row strides are in elements. */
+enum { QWEN_ASR_F32 = 0, QWEN_ASR_BF16 = 1 };
+
+/* h = x + residual (h = x without one), rounded to dtype; u = h * weight; int8 row
+ * q = rint(127 u / max|u|) and scale = max|u| / sqrt(mean(h^2) + eps) / 127 (1 for a row of
+ * zeros), so that q * scale is the normalised row. A row with a NaN or an infinity gets scale
+ * NaN and q = 0. h may be x or residual (in place), and NULL without a residual. rows x d,
+ * d <= 32768; bytes [d, ldq) of a q row are left as they were. */
+int32_t qwen_asr_rms_norm_int8(const void* x, int64_t ldx, const void* residual, int64_t ldr, const float* weight,
+                               float eps, int32_t dtype, int64_t rows, int32_t d, int8_t* q, int64_t ldq, float* scale,
+                               void* h, int64_t ldh, int32_t device, void* stream);
+
+/* y[m][n] = (sum_k xq[m][k] * wq[n][k]) * xs[m] * ws[n] with exact int32 sums, then
+ * STORE: out = y; RESID: out = y + residual (out may be residual); SWIGLU: rows of wq are
+ * interleaved gate0, up0, gate1, ... and out[m][j] = silu(y[m][2j]) * y[m][2j + 1], n / 2 wide.
+ * xq and wq start on 16-byte boundaries with row strides that are multiples of 16;
+ * k <= 131071. A row's result does not depend on the rows it shares the call with. */
+enum { QWEN_ASR_LINEAR_STORE = 0, QWEN_ASR_LINEAR_RESID = 1, QWEN_ASR_LINEAR_SWIGLU = 2 };
+int32_t qwen_asr_linear_int8(const int8_t* xq, int64_t ldx, const float* xs, const int8_t* wq, int64_t ldw,
+                             const float* ws, int64_t m, int32_t n, int32_t k, int32_t epilogue, const void* residual,
+                             int64_t ldr, void* out, int64_t ldo, int32_t dtype, int32_t device, void* stream);
+
+/* An int8 KV cache of n_seq sequences: k and v [n_seq][n_kv][capacity][head_dim], and an f32
+ * scale for each block of 16 tokens of a head, [n_seq][n_kv][capacity / 16]. capacity is a
+ * multiple of 16, head_dim 64 or 128; seq_stride / scale_stride are the elements from one
+ * sequence to the next (a layer of a larger cache is a pointer into it and its strides). */
+typedef struct QwenAsrKv8 {
+  int8_t *k, *v;
+  float *k_scale, *v_scale;
+  int64_t seq_stride, scale_stride;
+  int32_t n_seq, n_kv, capacity, head_dim;
+} QwenAsrKv8;
+/* Rows [n_seq][rows] of heads x head_dim contiguous elements. */
+typedef struct QwenAsrRows {
+  void* data;
+  int64_t seq_stride, row_stride;
+} QwenAsrRows;
+/* In the three calls below sequence b's rows are at positions starts[b * index_stride] on, and
+ * counts[b * index_stride] of the `rows` rows are in use (counts NULL: all). Both are read on
+ * the device when the call runs. A sequence with a negative start has no rows in use. */
+
+/* Writes k and v behind `starts`. A block's scale becomes max(scale, max|new value| / 127) and
+ * the rows it holds before `start` are re-coded when it grew; a block written from its first
+ * token on starts anew. Values are q = rint(x / scale). A NaN or an infinity makes the block's
+ * scale NaN. Rows past the capacity are dropped. */
+int32_t qwen_asr_kv8_append(const QwenAsrKv8* cache, const QwenAsrRows* k, const QwenAsrRows* v, int32_t dtype,
+                            int32_t rows, const int32_t* starts, const int32_t* counts, int32_t index_stride,
+                            int32_t device, void* stream);
+/* Reads values back: q * scale, zeros in rows that are not in use or past the capacity. k_out
+ * or v_out may be NULL. */
+int32_t qwen_asr_kv8_read(const QwenAsrKv8* cache, const QwenAsrRows* k_out, const QwenAsrRows* v_out, int32_t dtype,
+                          int32_t rows, const int32_t* starts, const int32_t* counts, int32_t index_stride,
+                          int32_t device, void* stream);
+/* Causal attention: query row r of sequence b attends positions 0 .. starts[b] + r of its
+ * cache, head h to KV head h / (heads / n_kv): softmax(scale * q k^T) v. Rows not in use get
+ * zeros. max_len bounds the positions any row sees (0: the capacity); it only shapes the launch,
+ * a row that sees more is still right. */
+int32_t qwen_asr_kv8_attention(const QwenAsrKv8* cache, const QwenAsrRows* q, const QwenAsrRows* out, int32_t dtype,
+                               int32_t rows, int32_t heads, const int32_t* starts, const int32_t* counts,
+                               int32_t index_stride, float scale, int32_t max_len, int32_t device, void* stream);
+/* Nonzero (and cleared) when a bounded wait inside qwen_asr_linear_int8 gave up on `device`: its
+ * output is not to be used. Waits for the device. */
+int32_t qwen_asr_ops_error(int32_t device);
+
 #ifdef __cplusplus
 }
 #endif

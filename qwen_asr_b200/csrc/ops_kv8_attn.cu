@@ -1,0 +1,548 @@
+// Attention over the int8 KV cache (ops_kv8.cu): o = softmax(scale q K^T) V per head, causal over
+// positions 0 .. start + row, grouped query heads.
+//
+// Tensor-core tiles of 16 tokens, the cache's scale block, so a tile has one K and one V scale.
+// int8 values are exact in f16 (the byte x + 128 under the exponent of 1024 is 1152 + x), so K
+// and V enter as they are, and the scales stay in f32: the K scale multiplies the scores, the V
+// scale the tile's product. A query row is first scaled by a power of two that puts its largest
+// value into [1/2, 1).
+//   f32 rows: q and the probabilities enter as two f16 planes, v = hi + lo, which holds them to
+//     2^-25 of the row's largest (below f32's own rounding of it). The two planes are rows r and
+//     r + 8 of the same 16-row operand: a tile holds 8 query rows and both planes cost one product.
+//   bf16 rows: one plane (a bf16 value is exact in f16 down to 2^-14 of the row's largest, and
+//     the probabilities' 2^-11 is an eighth of the output's own 2^-8), 16 rows a tile.
+// Scores, the running maximum and sum and the output stay in f32 registers.
+//
+// Fragments straight from the cache's layout: the order of the head's dimensions within the score
+// product, and that of the output columns, are free as long as both operands agree. A thread takes
+// 16 contiguous bytes of a token for both products; V's token pairs are interleaved in registers.
+//
+// Step kernel (few query rows): one cluster per (KV head, row tile, sequence); its CTAs split the
+// sequence's actual length, their warps take tiles in turn, each with its own ring of asynchronous
+// copies and its own softmax state. States are merged in warp order, then in rank order over
+// distributed shared memory: no workspace, no atomics, the same bits every time.
+// Prompt kernel (many query rows): warps split the rows and share the CTA's ring of K/V tiles.
+//
+// Bound: step - DRAM (the cache is read once per KV head); prompt - the tensor pipe (mma.sync).
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "bulk.cuh"
+#include "dev_util.cuh"
+#include "ops.h"
+
+namespace qasr {
+namespace {
+
+constexpr int kTok = kKv8Block;  // tokens of a tile
+constexpr float kNone = -1.0e30f;  // running maximum before any key (finite: differences stay defined)
+
+struct AttnArgs {
+  Kv8 c;
+  const void* q;
+  void* out;
+  long long q_seq, q_row, o_seq, o_row;
+  const int *starts, *counts;
+  int idx_stride, rows, heads, group, row_tiles;
+  float scale;
+};
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Two bytes of w (already x + 128) as f16 values x.
+template <uint32_t SEL>
+__device__ __forceinline__ uint32_t bytes_f16(uint32_t w) {
+  const uint32_t p = __byte_perm(w, 0x64646464u, SEL);  // 1024 + byte
+  const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&p), __half2half2(__ushort_as_half(0x6480)));
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack_rest(float a, float b, uint32_t hi) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+  return pack_f16(a - f.x, b - f.y);
+}
+
+// Shared-memory tile: 16 tokens of HD bytes, K then V then the two scales. 16-byte chunks are
+// permuted within a row so that the fragment loads hit distinct banks.
+template <int HD>
+struct Tile {
+  static constexpr int kChunks = HD / 16;
+  static constexpr int kBytes = 2 * kTok * HD + 16;
+  __device__ static uint32_t k_at(int row, int chunk) {
+    return row * HD + (HD == 128 ? (chunk ^ ((row & 1) << 2)) : chunk) * 16;
+  }
+  __device__ static uint32_t v_at(int row, int chunk) {
+    return kTok * HD + row * HD + (HD == 128 ? chunk ^ (((row >> 1) & 3) << 1) : chunk ^ ((row >> 1) & 3)) * 16;
+  }
+  // One tile's copies by `n` threads (n a multiple of 32, i the thread's index among them).
+  __device__ static void fetch(uint32_t st, const int8_t* k, const int8_t* v, const float* ks, const float* vs,
+                               int tile, int i, int n) {
+    const long long off = (long long)tile * kTok * HD;
+    for (int c = i; c < kTok * kChunks; c += n) {
+      const int row = c / kChunks, ch = c % kChunks;
+      cp16(st + k_at(row, ch), k + off + row * HD + ch * 16);
+      cp16(st + v_at(row, ch), v + off + row * HD + ch * 16);
+    }
+    if (i == 0) cp4(st + 2 * kTok * HD, ks + tile);
+    if (i == 1) cp4(st + 2 * kTok * HD + 4, vs + tile);
+  }
+};
+
+// One warp's query rows and softmax state. PL planes (2: f32 accuracy, 8 rows; 1: 16 rows).
+template <int HD, int PL>
+struct WarpState {
+  static constexpr int kRows = PL == 2 ? 8 : 16;
+  static constexpr int kR = PL == 2 ? 1 : 2;    // rows a thread holds: g (and g + 8)
+  static constexpr int kSteps = HD / 16;        // k steps of the score product
+  static constexpr int kNt = HD / 8;            // column tiles of the output
+  uint32_t q[kSteps][4];
+  float fac[kR];   // scale * log2(e) * the row's power of two
+  int last[kR];    // last position the row sees (-1: none)
+  float m[kR], l[kR];
+  float acc[kNt][2 * kR];
+
+  // dims of k step j that thread t of a quad holds: 4 from here
+  __device__ static int dim0(int t, int j) { return (j & 3) * 4 + t * 16 + (j >> 2) * 64; }
+  // output dims of column tile j: column n is dim n * kNt + j
+  __device__ static int out_dim(int n, int j) { return n * kNt + j; }
+
+  __device__ void init(const AttnArgs& a, int seq, int kvh, int row0, int start, int count, bool bf16) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int j = 0; j < kNt; ++j)
+#pragma unroll
+      for (int i = 0; i < 2 * kR; ++i) acc[j][i] = 0.f;
+#pragma unroll
+    for (int h = 0; h < kR; ++h) {
+      const int rr = row0 + g + h * 8, s = rr / a.group;
+      const bool live = s < count;  // rows past the operand too: count <= rows
+      last[h] = live ? min(start + s, a.c.capacity - 1) : -1;
+      m[h] = kNone;
+      l[h] = 0.f;
+      float f[kSteps][4];
+      float mx = 0.f;
+      const long long off =
+          seq * a.q_seq + (long long)s * a.q_row + (long long)(kvh * a.group + rr % a.group) * HD;
+#pragma unroll
+      for (int j = 0; j < kSteps; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          f[j][i] = 0.f;
+          if (live) {
+            const long long at = off + dim0(t, j) + i;
+            f[j][i] = bf16 ? __bfloat162float(((const __nv_bfloat16*)a.q)[at]) : ((const float*)a.q)[at];
+          }
+          mx = fmaxf(mx, fabsf(f[j][i]));
+        }
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      int e = 0;
+      if (mx > 0.f && mx < __int_as_float(0x7F800000)) frexpf(mx, &e);
+      fac[h] = scalbnf(a.scale * 1.4426950408889634f, e);
+#pragma unroll
+      for (int j = 0; j < kSteps; ++j) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[j][i] = scalbnf(f[j][i], -e);
+        const uint32_t h0 = pack_f16(f[j][0], f[j][1]), h1 = pack_f16(f[j][2], f[j][3]);
+        q[j][h] = h0;
+        q[j][2 + h] = h1;
+        if (PL == 2) {
+          q[j][1] = pack_rest(f[j][0], f[j][1], h0);
+          q[j][3] = pack_rest(f[j][2], f[j][3], h1);
+        }
+      }
+    }
+  }
+
+  // One tile of 16 tokens from position pos0, staged at st.
+  __device__ void tile(const unsigned char* st, int pos0) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const float ks = *reinterpret_cast<const float*>(st + 2 * kTok * HD);
+    const float vs = *reinterpret_cast<const float*>(st + 2 * kTok * HD + 4);
+    float vr[kR];  // a row that sees nothing of the tile takes nothing of its scale either (it may be NaN)
+#pragma unroll
+    for (int h = 0; h < kR; ++h) vr[h] = pos0 <= last[h] ? vs : 0.f;
+    float s[2][4];
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[nt][i] = 0.f;
+#pragma unroll
+      for (int c = 0; c < HD / 64; ++c) {
+        const uint4 w4 = *reinterpret_cast<const uint4*>(st + Tile<HD>::k_at(nt * 8 + g, t + 4 * c));
+        const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t u = w[i] ^ 0x80808080u;
+          mma16816(s[nt], q[c * 4 + i], bytes_f16<0x4140>(u), bytes_f16<0x4342>(u));
+        }
+      }
+    }
+    // scores of row g (+ 8h) at tokens nt * 8 + 2t + {0, 1}, in units of log2
+    uint32_t p[4];
+    bool grew = false;
+    float corr[kR];
+#pragma unroll
+    for (int h = 0; h < kR; ++h) {
+      float x[4];
+      const float f = fac[h] * ks;
+      float mx = kNone;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int nt = i >> 1, o = i & 1;
+        const float sum = PL == 2 ? s[nt][o] + s[nt][2 + o] : s[nt][2 * h + o];
+        x[i] = pos0 + nt * 8 + 2 * t + o <= last[h] ? sum * f : -__int_as_float(0x7F800000);
+        mx = fmaxf(mx, x[i]);
+      }
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      const float mn = fmaxf(m[h], mx);
+      corr[h] = ex2(m[h] - mn);
+      grew |= mn > m[h];
+      m[h] = mn;
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[i] = ex2(x[i] - mn);
+        sum += x[i];
+      }
+      l[h] = l[h] * corr[h] + sum;
+      p[h] = pack_f16(x[0], x[1]);
+      p[2 + h] = pack_f16(x[2], x[3]);
+      if (PL == 2) {
+        p[1] = pack_rest(x[0], x[1], p[0]);
+        p[3] = pack_rest(x[2], x[3], p[2]);
+      }
+    }
+    if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+      for (int j = 0; j < kNt; ++j)
+#pragma unroll
+        for (int i = 0; i < 2 * kR; ++i) acc[j][i] *= corr[i >> 1];
+    }
+    // V: tokens 2t, 2t + 1 and 2t + 8, 2t + 9, kNt dims from g * kNt
+    constexpr int W = kNt / 4;  // words a thread takes of a token
+    uint32_t v[4][W];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int row = 2 * t + (r & 1) + (r >> 1) * 8;
+      if constexpr (HD == 128) {
+        const uint4 w = *reinterpret_cast<const uint4*>(st + Tile<HD>::v_at(row, g));
+        v[r][0] = w.x; v[r][1] = w.y; v[r][2] = w.z; v[r][3] = w.w;
+      } else {
+        const uint2 w = *reinterpret_cast<const uint2*>(st + Tile<HD>::v_at(row, g >> 1) + (g & 1) * 8);
+        v[r][0] = w.x; v[r][1] = w.y;
+      }
+#pragma unroll
+      for (int i = 0; i < W; ++i) v[r][i] ^= 0x80808080u;
+    }
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      const uint32_t a0 = __byte_perm(v[0][i], v[1][i], 0x5140), a1 = __byte_perm(v[0][i], v[1][i], 0x7362);
+      const uint32_t b0 = __byte_perm(v[2][i], v[3][i], 0x5140), b1 = __byte_perm(v[2][i], v[3][i], 0x7362);
+      const uint32_t lo[4] = {bytes_f16<0x4140>(a0), bytes_f16<0x4342>(a0), bytes_f16<0x4140>(a1),
+                              bytes_f16<0x4342>(a1)};
+      const uint32_t hi[4] = {bytes_f16<0x4140>(b0), bytes_f16<0x4342>(b0), bytes_f16<0x4140>(b1),
+                              bytes_f16<0x4342>(b1)};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float o[4] = {0.f, 0.f, 0.f, 0.f};
+        mma16816(o, p, lo[k], hi[k]);
+        float* d = acc[i * 4 + k];
+        if (PL == 2) {
+          d[0] = fmaf(o[0] + o[2], vr[0], d[0]);
+          d[1] = fmaf(o[1] + o[3], vr[0], d[1]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) d[e % (2 * kR)] = fmaf(o[e], vr[(e >> 1) % kR], d[e % (2 * kR)]);
+        }
+      }
+    }
+  }
+
+  __device__ void finish_sum() {
+#pragma unroll
+    for (int h = 0; h < kR; ++h) {
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+    }
+  }
+};
+
+__device__ __forceinline__ void put(void* out, long long i, float v, bool bf16) {
+  if (bf16)
+    ((__nv_bfloat16*)out)[i] = __float2bfloat16_rn(v);
+  else
+    ((float*)out)[i] = v;
+}
+
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float ld_peer(uint32_t addr, int rank) {
+  uint32_t r;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(r) : "memory");
+  return v;
+}
+
+// A sequence's first position (at most the capacity) and live rows.
+__device__ __forceinline__ void live_rows(const AttnArgs& a, int seq, int& start, int& count) {
+  start = a.starts[(long long)seq * a.idx_stride];
+  count = a.rows;
+  if (a.counts) count = min(max(a.counts[(long long)seq * a.idx_stride], 0), a.rows);
+  if (start < 0) count = 0;
+  start = min(start, a.c.capacity);
+}
+
+// ------------------------------------------------------------------ step kernel
+constexpr int kStepWarps = 4, kStepStages = 4;
+template <int HD>
+constexpr int step_smem() {
+  return kStepWarps * kStepStages * Tile<HD>::kBytes;
+}
+
+// grid (splits, n_kv * row_tiles, n_seq), cluster (splits, 1, 1)
+template <int HD, int PL>
+__global__ void __launch_bounds__(kStepWarps * 32) step_kernel(const AttnArgs a) {
+  using S = WarpState<HD, PL>;
+  constexpr int R = S::kRows;
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ float wm[kStepWarps][R], wl[kStepWarps][R], cm[R], cl[R];
+  __shared__ float part[R][HD];  // the CTA's merged output
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int splits = gridDim.x, rank = blockIdx.x;
+  const int kvh = blockIdx.y / a.row_tiles, row0 = (blockIdx.y % a.row_tiles) * R, seq = blockIdx.z;
+  int start, count;
+  live_rows(a, seq, start, count);
+  // tokens any row of the tile sees
+  const int s_last = min(count - 1, (row0 + R - 1) / a.group);
+  const int len = s_last >= row0 / a.group ? (int)min((long long)start + s_last + 1, (long long)a.c.capacity) : 0;
+  const int tiles = (len + kTok - 1) / kTok;
+  const int t0 = (int)((long long)tiles * rank / splits), t1 = (int)((long long)tiles * (rank + 1) / splits);
+
+  const long long blocks = a.c.capacity / kTok;
+  const int8_t* k = a.c.k + seq * a.c.seq_stride + (long long)kvh * a.c.capacity * HD;
+  const int8_t* v = a.c.v + seq * a.c.seq_stride + (long long)kvh * a.c.capacity * HD;
+  const float* ks = a.c.ks + seq * a.c.scale_stride + kvh * blocks;
+  const float* vs = a.c.vs + seq * a.c.scale_stride + kvh * blocks;
+  unsigned char* ring = smem + warp * kStepStages * Tile<HD>::kBytes;
+  const uint32_t ring_a = smem_u32(ring);
+  const int mine = t1 - t0 > warp ? (t1 - t0 - warp + kStepWarps - 1) / kStepWarps : 0;
+#pragma unroll
+  for (int i = 0; i < kStepStages - 1; ++i) {
+    if (i < mine) Tile<HD>::fetch(ring_a + i * Tile<HD>::kBytes, k, v, ks, vs, t0 + warp + i * kStepWarps, lane, 32);
+    cp_commit();
+  }
+  S st;
+  st.init(a, seq, kvh, row0, start, count, PL == 1);
+  for (int i = 0; i < mine; ++i) {
+    const int nx = i + kStepStages - 1;
+    if (nx < mine)
+      Tile<HD>::fetch(ring_a + nx % kStepStages * Tile<HD>::kBytes, k, v, ks, vs, t0 + warp + nx * kStepWarps, lane, 32);
+    cp_commit();
+    cp_wait<kStepStages - 1>();
+    __syncwarp();
+    st.tile(ring + i % kStepStages * Tile<HD>::kBytes, (t0 + warp + i * kStepWarps) * kTok);
+    __syncwarp();
+  }
+  cp_wait<0>();
+  st.finish_sum();
+  __syncthreads();  // every ring is idle: it holds the warps' outputs now
+  float* wo = reinterpret_cast<float*>(smem);  // [warp][R][HD]
+  static_assert(kStepWarps * R * HD * 4 <= step_smem<HD>(), "the warps' outputs reuse the rings");
+#pragma unroll
+  for (int h = 0; h < S::kR; ++h) {
+    const int r = g + h * 8;
+    if (t == 0) {
+      wm[warp][r] = st.m[h];
+      wl[warp][r] = st.l[h];
+    }
+#pragma unroll
+    for (int j = 0; j < S::kNt; ++j) {
+      wo[(warp * R + r) * HD + S::out_dim(2 * t, j)] = st.acc[j][2 * h];
+      wo[(warp * R + r) * HD + S::out_dim(2 * t + 1, j)] = st.acc[j][2 * h + 1];
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < R * HD; i += kStepWarps * 32) {
+    const int r = i / HD, d = i % HD;
+    float mm = wm[0][r], ll = 0.f, o = 0.f;
+#pragma unroll
+    for (int w = 1; w < kStepWarps; ++w) mm = fmaxf(mm, wm[w][r]);
+#pragma unroll
+    for (int w = 0; w < kStepWarps; ++w) {
+      const float f = ex2(wm[w][r] - mm);
+      ll = fmaf(wl[w][r], f, ll);
+      o = fmaf(wo[(w * R + r) * HD + d], f, o);
+    }
+    part[r][d] = o;
+    if (d == 0) {
+      cm[r] = mm;
+      cl[r] = ll;
+    }
+  }
+  if (splits > 1)
+    cluster_barrier();
+  else
+    __syncthreads();
+  const int n_rows = a.rows * a.group;
+  for (int i = rank * kStepWarps * 32 + threadIdx.x; i < R * HD; i += splits * kStepWarps * 32) {
+    const int r = i / HD, d = i % HD, rr = row0 + r;
+    if (rr >= n_rows) continue;
+    float ll, o;
+    if (splits > 1) {
+      float mm = kNone;
+      for (int p = 0; p < splits; ++p) mm = fmaxf(mm, ld_peer(smem_u32(&cm[r]), p));
+      ll = 0.f;
+      o = 0.f;
+      for (int p = 0; p < splits; ++p) {
+        const float f = ex2(ld_peer(smem_u32(&cm[r]), p) - mm);
+        ll = fmaf(ld_peer(smem_u32(&cl[r]), p), f, ll);
+        o = fmaf(ld_peer(smem_u32(&part[r][d]), p), f, o);
+      }
+    } else {
+      ll = cl[r];
+      o = part[r][d];
+    }
+    const float inv = ll == 0.f ? 0.f : __fdiv_rn(1.0f, ll);
+    put(a.out, seq * a.o_seq + (long long)(rr / a.group) * a.o_row + (long long)(kvh * a.group + rr % a.group) * HD + d,
+        __fmul_rn(o, inv), PL == 1);
+  }
+  __syncwarp();
+  if (splits > 1) cluster_barrier();  // no CTA leaves while a peer reads its part
+}
+
+// ------------------------------------------------------------------ prompt kernel
+constexpr int kPromptWarps = 8, kPromptTiles = 4, kPromptStages = 2;  // 64 tokens a stage
+template <int HD>
+constexpr int prompt_smem() {
+  return kPromptStages * kPromptTiles * Tile<HD>::kBytes;
+}
+
+// grid (row tiles of kPromptWarps * kRows, n_kv, n_seq)
+template <int HD, int PL>
+__global__ void __launch_bounds__(kPromptWarps * 32) prompt_kernel(const AttnArgs a) {
+  using S = WarpState<HD, PL>;
+  constexpr int R = S::kRows, CR = R * kPromptWarps, N = kPromptWarps * 32;
+  extern __shared__ __align__(128) unsigned char smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int kvh = blockIdx.y, seq = blockIdx.z;
+  // the last rows see the most keys: they start first
+  const int base = (gridDim.x - 1 - blockIdx.x) * CR, row0 = base + warp * R;
+  int start, count;
+  live_rows(a, seq, start, count);
+  auto tokens = [&](int r_first, int r_last) {  // tokens that query rows r_first .. r_last see
+    const int s_last = min(count - 1, r_last / a.group);
+    return s_last >= r_first / a.group ? (int)min((long long)start + s_last + 1, (long long)a.c.capacity) : 0;
+  };
+  const int tiles = (tokens(base, base + CR - 1) + kTok - 1) / kTok;
+  const int own_tiles = (tokens(row0, row0 + R - 1) + kTok - 1) / kTok;
+  const long long blocks = a.c.capacity / kTok;
+  const int8_t* k = a.c.k + seq * a.c.seq_stride + (long long)kvh * a.c.capacity * HD;
+  const int8_t* v = a.c.v + seq * a.c.seq_stride + (long long)kvh * a.c.capacity * HD;
+  const float* ks = a.c.ks + seq * a.c.scale_stride + kvh * blocks;
+  const float* vs = a.c.vs + seq * a.c.scale_stride + kvh * blocks;
+  const uint32_t ring_a = smem_u32(smem);
+  constexpr int kStage = kPromptTiles * Tile<HD>::kBytes;
+  const int stages = (tiles + kPromptTiles - 1) / kPromptTiles;
+  auto fetch = [&](int i) {
+    for (int b = 0; b < kPromptTiles; ++b) {
+      const int tl = i * kPromptTiles + b;
+      if (tl < tiles)
+        Tile<HD>::fetch(ring_a + (i % kPromptStages) * kStage + b * Tile<HD>::kBytes, k, v, ks, vs, tl, threadIdx.x, N);
+    }
+  };
+  if (stages > 0) fetch(0);
+  cp_commit();
+  S st;
+  st.init(a, seq, kvh, row0, start, count, PL == 1);
+  for (int i = 0; i < stages; ++i) {
+    if (i + 1 < stages) fetch(i + 1);
+    cp_commit();
+    cp_wait<1>();
+    __syncthreads();
+    for (int b = 0; b < kPromptTiles; ++b) {
+      const int tl = i * kPromptTiles + b;
+      if (tl < own_tiles) st.tile(smem + (i % kPromptStages) * kStage + b * Tile<HD>::kBytes, tl * kTok);
+    }
+    __syncthreads();
+  }
+  st.finish_sum();
+  const int n_rows = a.rows * a.group;
+#pragma unroll
+  for (int h = 0; h < S::kR; ++h) {
+    const int rr = row0 + g + h * 8;
+    if (rr >= n_rows) continue;
+    const float inv = st.l[h] == 0.f ? 0.f : __fdiv_rn(1.0f, st.l[h]);
+    const long long o = seq * a.o_seq + (long long)(rr / a.group) * a.o_row +
+                        (long long)(kvh * a.group + rr % a.group) * HD;
+#pragma unroll
+    for (int j = 0; j < S::kNt; ++j)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        put(a.out, o + S::out_dim(2 * t + e, j), __fmul_rn(st.acc[j][2 * h + e], inv), PL == 1);
+  }
+}
+
+template <int HD, int PL>
+cudaError_t launch(AttnArgs a, int max_len, cudaStream_t s) {
+  constexpr int R = WarpState<HD, PL>::kRows;
+  const int n_rows = a.rows * a.group;
+  if (n_rows > 8 * R) {
+    const dim3 g((n_rows + R * kPromptWarps - 1) / (R * kPromptWarps), a.c.n_kv, a.c.n_seq);
+    static OncePerDevice once;
+    const cudaError_t e = once.smem(prompt_kernel<HD, PL>, prompt_smem<HD>());
+    if (e != cudaSuccess) return e;
+    return ops_launch(prompt_kernel<HD, PL>, g, dim3(kPromptWarps * 32), prompt_smem<HD>(), s, 1, a);
+  }
+  a.row_tiles = (n_rows + R - 1) / R;
+  const long long ctas = (long long)a.c.n_kv * a.row_tiles * a.c.n_seq;
+  const int tiles = (max_len + kTok - 1) / kTok;
+  int splits = 1;
+  while (splits < 8 && splits * 2 * kStepWarps <= tiles && ctas * splits < 6LL * ops_sm_count()) splits *= 2;
+  static OncePerDevice once;
+  const cudaError_t e = once.smem(step_kernel<HD, PL>, step_smem<HD>());
+  if (e != cudaSuccess) return e;
+  return ops_launch(step_kernel<HD, PL>, dim3(splits, a.c.n_kv * a.row_tiles, a.c.n_seq), dim3(kStepWarps * 32),
+                    step_smem<HD>(), s, splits, a);
+}
+
+}  // namespace
+
+cudaError_t kv8_attention(const Kv8& c, const void* q, long long q_seq, long long q_row, void* out, long long o_seq,
+                          long long o_row, OpsDtype dt, int rows, int heads, const int* starts, const int* counts,
+                          int idx_stride, float scale, int max_len, cudaStream_t s) {
+  if (rows <= 0 || c.n_seq <= 0) return cudaSuccess;
+  AttnArgs a{c, q, out, q_seq, q_row, o_seq, o_row, starts, counts, idx_stride, rows, heads, heads / c.n_kv, 1, scale};
+  if (max_len <= 0 || max_len > c.capacity) max_len = c.capacity;
+  if (c.head_dim == 128)
+    return dt == OPS_BF16 ? launch<128, 1>(a, max_len, s) : launch<128, 2>(a, max_len, s);
+  return dt == OPS_BF16 ? launch<64, 1>(a, max_len, s) : launch<64, 2>(a, max_len, s);
+}
+
+}  // namespace qasr
