@@ -22,21 +22,7 @@ _I32P = C.POINTER(C.c_int32)
 _I64P = C.POINTER(C.c_int64)
 _U8P = C.POINTER(C.c_uint8)
 _VP = C.c_void_p
-
-
-class Kv8Desc(C.Structure):
-    """QwenAsrKv8: an int8 KV cache (include/qwen_asr_ext.h)."""
-    _fields_ = [("k", _VP), ("v", _VP), ("k_scale", _VP), ("v_scale", _VP), ("seq_stride", C.c_int64),
-                ("scale_stride", C.c_int64), ("n_seq", C.c_int32), ("n_kv", C.c_int32), ("capacity", C.c_int32),
-                ("head_dim", C.c_int32)]
-
-
-class RowsDesc(C.Structure):
-    """QwenAsrRows: rows of contiguous heads."""
-    _fields_ = [("data", _VP), ("seq_stride", C.c_int64), ("row_stride", C.c_int64)]
-
-
-_I32, _I64, _KV8P, _ROWSP = C.c_int32, C.c_int64, C.POINTER(Kv8Desc), C.POINTER(RowsDesc)
+_I32, _I64 = C.c_int32, C.c_int64
 
 # name: (restype, argtypes)
 SIGNATURES = {
@@ -128,9 +114,9 @@ SIGNATURES = {
                                       _I64, _I32, _VP]),
     "qwen_asr_linear_int8": (_I32, [_VP, _I64, _VP, _VP, _I64, _VP, _I64, _I32, _I32, _I32, _VP, _I64, _VP, _I64,
                                     _I32, _I32, _VP]),
-    "qwen_asr_kv8_append": (_I32, [_KV8P, _ROWSP, _ROWSP, _I32, _I32, _VP, _VP, _I32, _I32, _VP]),
-    "qwen_asr_kv8_read": (_I32, [_KV8P, _ROWSP, _ROWSP, _I32, _I32, _VP, _VP, _I32, _I32, _VP]),
-    "qwen_asr_kv8_attention": (_I32, [_KV8P, _ROWSP, _ROWSP, _I32, _I32, _I32, _VP, _VP, _I32, C.c_float, _I32, _I32,
+    "qwen_asr_kv8_append": (_I32, [_VP, _VP, _VP, _I32, _I32, _VP, _VP, _I32, _I32, _VP]),
+    "qwen_asr_kv8_read": (_I32, [_VP, _VP, _VP, _I32, _I32, _VP, _VP, _I32, _I32, _VP]),
+    "qwen_asr_kv8_attention": (_I32, [_VP, _VP, _VP, _I32, _I32, _I32, _VP, _VP, _I32, C.c_float, _I32, _I32,
                                       _VP]),
     "qwen_asr_ops_error": (_I32, [_I32]),
     "qwen_asr_debug_fix_timestamps": (None, [C.POINTER(C.c_float), C.c_int32]),

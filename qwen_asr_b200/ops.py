@@ -15,18 +15,23 @@ raises RuntimeError. There is no CPU form.
 """
 from __future__ import annotations
 
-import ctypes as C
 import math
+import struct
 from typing import NamedTuple
 
 import torch
 
-from . import Kv8Desc, RowsDesc, last_error, lib
+from . import last_error, lib
 
 BLOCK = 16  # cache tokens that share a scale
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
 _FLOATS = (torch.float32, torch.bfloat16)
+_F32, _INT8, _INT32 = torch.float32, torch.int8, torch.int32
+_KV8 = struct.Struct("@PPPPqqiiii")  # QwenAsrKv8
+_ROWS = struct.Struct("@Pqq")        # QwenAsrRows
+_grad = torch.is_grad_enabled
+_raw_stream = torch._C._cuda_getCurrentRawStream  # the current stream's handle, without a Stream object
 
 
 class Kv8Cache(NamedTuple):
@@ -46,6 +51,9 @@ def kv8_cache(n_seq: int, n_kv: int, capacity: int, head_dim: int = 128, device=
     return Kv8Cache(*q, *s)
 
 
+# A call of a few microseconds has no time for a check of its arguments one by one: each operator asks
+# whether everything is as it should be in one expression, and only where it is not does the slow
+# form below look for the argument to name.
 def _tensor(t, name, dims, dtypes, device=None, shape=None):
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor, not {type(t).__name__}")
@@ -53,56 +61,66 @@ def _tensor(t, name, dims, dtypes, device=None, shape=None):
         raise TypeError(f"{name} must be {' or '.join(str(d) for d in dtypes)}, not {t.dtype}")
     if not t.is_cuda:
         raise ValueError(f"{name} must be on a CUDA device")
-    if device is not None and t.device != device:
-        raise ValueError(f"{name} is on {t.device}, not on {device}")
+    if device is not None and t.get_device() != device:
+        raise ValueError(f"{name} is on {t.device}, not on cuda:{device}")
     if t.dim() != dims:
         raise ValueError(f"{name} must have {dims} dimensions, not {t.dim()}")
     if shape is not None and tuple(t.shape) != tuple(shape):
         raise ValueError(f"{name} must have shape {tuple(shape)}, not {tuple(t.shape)}")
-    if t.requires_grad and torch.is_grad_enabled():
+    if t.requires_grad and _grad():
         raise ValueError(f"{name} requires a gradient, which the 8-bit operators do not have")
     return t
 
 
-def _rows2d(t, name):
+def _is(t, dtype, device, shape):
+    return (isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == device and t.shape == shape
+            and not (t.requires_grad and _grad()))
+
+
+def _pitch(t, name):
     """Row stride of a matrix whose rows are contiguous."""
-    if t.shape[1] > 1 and t.stride(1) != 1:
+    ld, one = t.stride()
+    rows, width = t.shape
+    if one != 1 and width > 1:
         raise ValueError(f"{name}: rows must be contiguous")
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+    return ld if rows > 1 else max(ld, width)
 
 
-def _call(fn, *args):
-    if fn(*args) != 0:
-        raise RuntimeError(last_error())
-
-
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+def _failed():
+    raise RuntimeError(last_error())
 
 
 def rms_norm_int8(x, weight, eps: float = 1e-6, residual=None):
     """(q, scale, h) of x [rows, d] (f32 or bf16): h = x + residual in x's type (x itself without a
     residual), q int8 [rows, d] and scale f32 [rows] with q * scale[:, None] the RMS-normalised
     rows times weight (f32 [d]). q's row stride is d rounded up to 16, as linear_int8 wants it."""
-    _tensor(x, "x", 2, _FLOATS)
-    rows, d = x.shape
-    _tensor(weight, "weight", 1, (torch.float32,), x.device, (d,))
-    if residual is not None:
-        _tensor(residual, "residual", 2, (x.dtype,), x.device, (rows, d))
+    _x = isinstance(x, torch.Tensor)
+    code = _DTYPES.get(x.dtype) if _x else None
+    if code is None or x.dim() != 2 or not x.is_cuda or (x.requires_grad and _grad()):
+        _tensor(x, "x", 2, _FLOATS)
+    dev, shape, dtype = x.get_device(), x.shape, x.dtype
+    rows, d = shape
+    if not _is(weight, _F32, dev, (d,)):
+        _tensor(weight, "weight", 1, (_F32,), dev, (d,))
     if not 1 <= d <= 32768:
         raise ValueError("d must be 1 .. 32768")
     if not eps >= 0:
         raise ValueError("eps must not be negative")
-    w = weight if d == 1 or weight.stride(0) == 1 else weight.contiguous()
+    if d > 1 and weight.stride(0) != 1:
+        weight = weight.contiguous()
     ld = -(-d // 16) * 16
-    q = torch.empty(rows, ld, dtype=torch.int8, device=x.device)
-    scale = torch.empty(rows, dtype=torch.float32, device=x.device)
-    h = x if residual is None else torch.empty(rows, d, dtype=x.dtype, device=x.device)
-    ldx = _rows2d(x, "x")
-    ldr = 0 if residual is None else _rows2d(residual, "residual")
-    _call(lib().qwen_asr_rms_norm_int8, x.data_ptr(), ldx, None if residual is None else residual.data_ptr(), ldr,
-          w.data_ptr(), eps, _DTYPES[x.dtype], rows, d, q.data_ptr(), ld, scale.data_ptr(),
-          None if residual is None else h.data_ptr(), d, x.device.index, _stream(x.device))
+    q = torch.empty((rows, ld), dtype=_INT8, device=x.device)
+    scale = torch.empty(rows, dtype=_F32, device=x.device)
+    if residual is None:
+        h, hp, rp, ldr = x, None, None, 0
+    else:
+        if not _is(residual, dtype, dev, shape):
+            _tensor(residual, "residual", 2, (dtype,), dev, shape)
+        h = torch.empty(shape, dtype=dtype, device=x.device)
+        hp, rp, ldr = h.data_ptr(), residual.data_ptr(), _pitch(residual, "residual")
+    if lib().qwen_asr_rms_norm_int8(x.data_ptr(), _pitch(x, "x"), rp, ldr, weight.data_ptr(), eps, code, rows, d,
+                                    q.data_ptr(), ld, scale.data_ptr(), hp, d, dev, _raw_stream(dev)):
+        _failed()
     return (q if ld == d else q[:, :d]), scale, h
 
 
@@ -111,85 +129,105 @@ def linear_int8(xq, xs, wq, ws, residual=None, swiglu: bool = False, dtype=torch
     (f32 or bf16), with exact integer sums. residual [m, n] (in dtype) is added; swiglu takes the
     rows of wq as gate0, up0, gate1, ... and returns silu(gate) * up, [m, n / 2]. Rows of xq and wq
     start on 16-byte boundaries (row strides that are multiples of 16)."""
-    _tensor(xq, "xq", 2, (torch.int8,))
-    m, k = xq.shape
-    dev = xq.device
-    _tensor(wq, "wq", 2, (torch.int8,), dev)
+    if not (isinstance(xq, torch.Tensor) and xq.dtype is _INT8 and xq.is_cuda and xq.dim() == 2):
+        _tensor(xq, "xq", 2, (_INT8,))
+    dev, (m, k) = xq.get_device(), xq.shape
+    if not (isinstance(wq, torch.Tensor) and wq.dtype is _INT8 and wq.get_device() == dev and wq.dim() == 2):
+        _tensor(wq, "wq", 2, (_INT8,), dev)
     n = wq.shape[0]
     if wq.shape[1] != k:
         raise ValueError(f"xq has rows of {k} values, wq of {wq.shape[1]}")
-    if dtype not in _DTYPES:
+    code = _DTYPES.get(dtype)
+    if code is None:
         raise TypeError(f"dtype must be torch.float32 or torch.bfloat16, not {dtype}")
-    _tensor(xs, "xs", 1, (torch.float32,), dev, (m,))
-    _tensor(ws, "ws", 1, (torch.float32,), dev, (n,))
+    if not (_is(xs, _F32, dev, (m,)) and _is(ws, _F32, dev, (n,))):
+        _tensor(xs, "xs", 1, (_F32,), dev, (m,))
+        _tensor(ws, "ws", 1, (_F32,), dev, (n,))
     if not (xs.is_contiguous() and ws.is_contiguous()):
         raise ValueError("xs and ws must be contiguous")
-    if residual is not None:
-        _tensor(residual, "residual", 2, (dtype,), dev, (m, n))
-        if swiglu:
-            raise ValueError("swiglu and residual exclude each other")
     if not 1 <= k <= 131071:
         raise ValueError("k must be 1 .. 131071")
     if n < 1 or (swiglu and n % 2):
         raise ValueError("n must be positive, and even for swiglu")
-    ldx, ldw = _rows2d(xq, "xq"), _rows2d(wq, "wq")
-    if m == 1:
-        ldx = -(-k // 16) * 16
-    if n == 1:
-        ldw = -(-k // 16) * 16
-    if ldx % 16 or ldw % 16 or xq.data_ptr() % 16 or wq.data_ptr() % 16:
+    epi, rp, ldr, width = 0, None, 0, n
+    if swiglu:
+        epi, width = 2, n // 2
+    if residual is not None:
+        if not _is(residual, dtype, dev, (m, n)):
+            _tensor(residual, "residual", 2, (dtype,), dev, (m, n))
+        if swiglu:
+            raise ValueError("swiglu and residual exclude each other")
+        epi, rp, ldr = 1, residual.data_ptr(), _pitch(residual, "residual")
+    k16 = -(-k // 16) * 16
+    ldx = _pitch(xq, "xq") if m > 1 else k16 if k == 1 or xq.stride(1) == 1 else _pitch(xq, "xq")
+    ldw = _pitch(wq, "wq") if n > 1 else k16 if k == 1 or wq.stride(1) == 1 else _pitch(wq, "wq")
+    xp, wp = xq.data_ptr(), wq.data_ptr()
+    if (ldx | ldw | xp | wp) & 15:
         raise ValueError("rows of xq and wq must start on 16-byte boundaries")
-    width = n // 2 if swiglu else n
-    out = torch.empty(m, width, dtype=dtype, device=dev)
-    if m == 0:
-        return out
-    _call(lib().qwen_asr_linear_int8, xq.data_ptr(), ldx, xs.data_ptr(), wq.data_ptr(), ldw, ws.data_ptr(), m, n, k,
-          2 if swiglu else 0 if residual is None else 1, None if residual is None else residual.data_ptr(),
-          0 if residual is None else _rows2d(residual, "residual"), out.data_ptr(), width, _DTYPES[dtype], dev.index,
-          _stream(dev))
+    out = torch.empty((m, width), dtype=dtype, device=xq.device)
+    if m and lib().qwen_asr_linear_int8(xp, ldx, xs.data_ptr(), wp, ldw, ws.data_ptr(), m, n, k, epi, rp, ldr,
+                                        out.data_ptr(), width, code, dev, _raw_stream(dev)):
+        _failed()
     return out
 
 
 def _cache(cache):
+    """(descriptor, device, n_seq, n_kv, head_dim) of a cache."""
     k, v, ks, vs = cache
-    _tensor(k, "cache.k", 4, (torch.int8,))
-    n_seq, n_kv, cap, hd = k.shape
-    dev = k.device
-    _tensor(v, "cache.v", 4, (torch.int8,), dev, k.shape)
-    _tensor(ks, "cache.k_scale", 3, (torch.float32,), dev, (n_seq, n_kv, cap // BLOCK))
-    _tensor(vs, "cache.v_scale", 3, (torch.float32,), dev, (n_seq, n_kv, cap // BLOCK))
+    try:
+        shape, st, ss = k.shape, k.stride(), ks.stride()
+        n, h, cap, hd = shape
+        dev, blocks = k.get_device(), cap // BLOCK
+        if (k.dtype is _INT8 and v.dtype is _INT8 and ks.dtype is _F32 and vs.dtype is _F32 and v.shape == shape
+                and v.stride() == st and st[1:] == (cap * hd, hd, 1) and ks.shape == (n, h, blocks)
+                and vs.shape == ks.shape and vs.stride() == ss and ss[1:] == (blocks, 1) and (hd == 128 or hd == 64)
+                and blocks > 0 and cap == blocks * BLOCK and dev >= 0 and v.get_device() == dev
+                and ks.get_device() == dev and vs.get_device() == dev
+                and not ((ks.requires_grad or vs.requires_grad) and _grad())):
+            return (_KV8.pack(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), st[0], ss[0], n, h, cap, hd),
+                    dev, n, h, hd)
+    except (AttributeError, ValueError):
+        pass
+    _tensor(k, "cache.k", 4, (_INT8,))
+    n, h, cap, hd = k.shape
+    dev = k.get_device()
+    _tensor(v, "cache.v", 4, (_INT8,), dev, k.shape)
+    _tensor(ks, "cache.k_scale", 3, (_F32,), dev, (n, h, cap // BLOCK))
+    _tensor(vs, "cache.v_scale", 3, (_F32,), dev, (n, h, cap // BLOCK))
     if hd not in (64, 128):
         raise ValueError("head_dim must be 64 or 128")
     if cap < BLOCK or cap % BLOCK:
         raise ValueError("the capacity must be a positive multiple of 16")
-    if k[0].is_contiguous() and v[0].is_contiguous() and ks[0].is_contiguous() and vs[0].is_contiguous():
-        if n_seq == 1 or (k.stride(0) == v.stride(0) and ks.stride(0) == vs.stride(0)):
-            return Kv8Desc(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), k.stride(0), ks.stride(0), n_seq,
-                           n_kv, cap, hd), dev
+    if n < 1 or h < 1:
+        raise ValueError("a cache needs a sequence and a head")
+    if all(t[0].is_contiguous() for t in (k, v, ks, vs)) and (
+            n == 1 or (k.stride(0) == v.stride(0) and ks.stride(0) == vs.stride(0))):
+        return (_KV8.pack(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), k.stride(0), ks.stride(0), n, h,
+                          cap, hd), dev, n, h, hd)
     raise ValueError("each sequence of the cache must be contiguous, with the same strides for k and v")
 
 
-def _index(t, name, dev, n_seq):
-    _tensor(t, name, 1, (torch.int32,), dev, (n_seq,))
-    if n_seq > 1 and t.stride(0) < 1:
-        raise ValueError(f"{name} must not be an expanded tensor")
-    return t
-
-
-def _indices(starts, counts, dev, n_seq):
-    """(starts, counts) with one stride for both."""
-    _index(starts, "starts", dev, n_seq)
+def _indices(starts, counts, dev, n):
+    """(starts, counts, address of starts, of counts or None, their stride)."""
+    if not _is(starts, _INT32, dev, (n,)):
+        _tensor(starts, "starts", 1, (_INT32,), dev, (n,))
+    stride = starts.stride(0) if n > 1 else 1
     if counts is not None:
-        _index(counts, "counts", dev, n_seq)
-        if n_seq > 1 and counts.stride(0) != starts.stride(0):
-            starts, counts = starts.contiguous(), counts.contiguous()
-    return starts, counts, (starts.stride(0) if n_seq > 1 else 1)
+        if not _is(counts, _INT32, dev, (n,)):
+            _tensor(counts, "counts", 1, (_INT32,), dev, (n,))
+        if n > 1 and counts.stride(0) != stride:
+            starts, counts, stride = starts.contiguous(), counts.contiguous(), 1
+    if stride < 1:
+        raise ValueError("starts and counts must not be expanded tensors")
+    return starts, counts, starts.data_ptr(), None if counts is None else counts.data_ptr(), stride
 
 
-def _rows4d(t, name):
-    if (t.shape[3] > 1 and t.stride(3) != 1) or (t.shape[2] > 1 and t.stride(2) != t.shape[3]):
+def _rows(t, name):
+    """Descriptor of rows [n_seq, rows, heads, head_dim] whose heads are contiguous."""
+    seq, row, head, one = t.stride()
+    if (one != 1 and t.shape[3] > 1) or (head != t.shape[3] and t.shape[2] > 1):
         raise ValueError(f"{name}: the heads of a row must be contiguous")
-    return RowsDesc(t.data_ptr(), t.stride(0), t.stride(1))
+    return _ROWS.pack(t.data_ptr(), seq, row)
 
 
 def kv8_append(cache: Kv8Cache, k, v, starts, counts=None) -> None:
@@ -197,35 +235,38 @@ def kv8_append(cache: Kv8Cache, k, v, starts, counts=None) -> None:
     (int32, on the device) of each sequence; counts[b] says how many of the rows it has (default
     all). The scale of a block of 16 tokens only grows while it fills, and what it holds is
     re-coded; rows past the capacity are dropped, and a negative start skips the sequence."""
-    desc, dev = _cache(cache)
-    _tensor(k, "k", 4, _FLOATS, dev)
+    desc, dev, n, h, hd = _cache(cache)
+    code = _DTYPES.get(k.dtype) if isinstance(k, torch.Tensor) else None
+    if code is None or k.dim() != 4:
+        _tensor(k, "k", 4, _FLOATS, dev)
     rows = k.shape[1]
-    shape = (desc.n_seq, rows, desc.n_kv, desc.head_dim)
-    _tensor(k, "k", 4, _FLOATS, dev, shape)
-    _tensor(v, "v", 4, (k.dtype,), dev, shape)
-    starts, counts, stride = _indices(starts, counts, dev, desc.n_seq)
-    if rows == 0:
-        return
-    _call(lib().qwen_asr_kv8_append, C.byref(desc), C.byref(_rows4d(k, "k")), C.byref(_rows4d(v, "v")),
-          _DTYPES[k.dtype], rows, starts.data_ptr(), None if counts is None else counts.data_ptr(), stride, dev.index,
-          _stream(dev))
+    shape = (n, rows, h, hd)
+    if not (_is(k, k.dtype, dev, shape) and _is(v, k.dtype, dev, shape)):
+        _tensor(k, "k", 4, _FLOATS, dev, shape)
+        _tensor(v, "v", 4, (k.dtype,), dev, shape)
+    starts, counts, sp, cp, stride = _indices(starts, counts, dev, n)
+    if rows and lib().qwen_asr_kv8_append(desc, _rows(k, "k"), _rows(v, "v"), code, rows, sp, cp, stride, dev,
+                                          _raw_stream(dev)):
+        _failed()
 
 
 def kv8_read(cache: Kv8Cache, starts, rows: int, counts=None, dtype=torch.float32):
     """(k, v) [n_seq, rows, n_kv, head_dim]: the values of positions starts[b] + r, zeros from row
     counts[b] and from the capacity on."""
-    desc, dev = _cache(cache)
-    if dtype not in _DTYPES:
+    desc, dev, n, h, hd = _cache(cache)
+    code = _DTYPES.get(dtype)
+    if code is None:
         raise TypeError(f"dtype must be torch.float32 or torch.bfloat16, not {dtype}")
     if rows < 0:
         raise ValueError("rows must not be negative")
-    starts, counts, stride = _indices(starts, counts, dev, desc.n_seq)
-    k = torch.empty(desc.n_seq, rows, desc.n_kv, desc.head_dim, dtype=dtype, device=dev)
+    starts, counts, sp, cp, stride = _indices(starts, counts, dev, n)
+    k = torch.empty((n, rows, h, hd), dtype=dtype, device=starts.device)
     v = torch.empty_like(k)
-    if rows:
-        _call(lib().qwen_asr_kv8_read, C.byref(desc), C.byref(_rows4d(k, "k")), C.byref(_rows4d(v, "v")),
-              _DTYPES[dtype], rows, starts.data_ptr(), None if counts is None else counts.data_ptr(), stride,
-              dev.index, _stream(dev))
+    width = h * hd
+    if rows and lib().qwen_asr_kv8_read(desc, _ROWS.pack(k.data_ptr(), rows * width, width),
+                                        _ROWS.pack(v.data_ptr(), rows * width, width), code, rows, sp, cp, stride,
+                                        dev, _raw_stream(dev)):
+        _failed()
     return k, v
 
 
@@ -234,20 +275,25 @@ def kv8_attention(q, cache: Kv8Cache, starts, counts=None, scale: float | None =
     the cache: row r of sequence b attends positions 0 .. starts[b] + r; rows from counts[b] on get
     zeros. scale defaults to 1 / sqrt(head_dim). max_len, an upper bound of starts + rows when the
     caller knows one, only shapes the launch."""
-    desc, dev = _cache(cache)
-    _tensor(q, "q", 4, _FLOATS, dev)
-    rows, heads = q.shape[1], q.shape[2]
-    _tensor(q, "q", 4, _FLOATS, dev, (desc.n_seq, rows, heads, desc.head_dim))
-    if heads < 1 or heads % desc.n_kv or heads > 256 * desc.n_kv:
-        raise ValueError(f"{heads} query heads do not fit {desc.n_kv} cached ones")
-    starts, counts, stride = _indices(starts, counts, dev, desc.n_seq)
+    desc, dev, n, h, hd = _cache(cache)
+    code = _DTYPES.get(q.dtype) if isinstance(q, torch.Tensor) else None
+    if code is None or q.dim() != 4:
+        _tensor(q, "q", 4, _FLOATS, dev)
+    shape = q.shape
+    rows, heads = shape[1], shape[2]
+    if shape != (n, rows, heads, hd) or q.get_device() != dev or (q.requires_grad and _grad()):
+        _tensor(q, "q", 4, _FLOATS, dev, (n, rows, heads, hd))
+    if heads < 1 or heads % h or heads > 256 * h:
+        raise ValueError(f"{heads} query heads do not fit {h} cached ones")
+    starts, counts, sp, cp, stride = _indices(starts, counts, dev, n)
     if scale is None:
-        scale = 1.0 / math.sqrt(desc.head_dim)
-    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    if rows:
-        _call(lib().qwen_asr_kv8_attention, C.byref(desc), C.byref(_rows4d(q, "q")), C.byref(_rows4d(out, "out")),
-              _DTYPES[q.dtype], rows, heads, starts.data_ptr(), None if counts is None else counts.data_ptr(), stride,
-              scale, max_len, dev.index, _stream(dev))
+        scale = 1.0 / math.sqrt(hd)
+    out = torch.empty(shape, dtype=q.dtype, device=q.device)
+    width = heads * hd
+    if rows and lib().qwen_asr_kv8_attention(desc, _rows(q, "q"), _ROWS.pack(out.data_ptr(), rows * width, width),
+                                             code, rows, heads, sp, cp, stride, scale, max_len, dev,
+                                             _raw_stream(dev)):
+        _failed()
     return out
 
 

@@ -1,6 +1,6 @@
 """The 8-bit operators' C entry points refuse what they cannot run, before anything is enqueued: every
 call here has one argument wrong and must return -1 with the reason (no GPU is needed for that)."""
-import ctypes as C
+import struct
 
 import pytest
 
@@ -27,11 +27,11 @@ def cache(**kw):
     a = dict(k=P, v=P, k_scale=P, v_scale=P, seq_stride=2 * 32 * 128, scale_stride=4, n_seq=2, n_kv=2, capacity=32,
              head_dim=128)
     a.update(kw)
-    return C.byref(Q.Kv8Desc(*a.values()))
+    return struct.pack("@PPPPqqiiii", *(x or 0 for x in a.values()))
 
 
 def rows(data=P, seq=256, row=256):
-    return C.byref(Q.RowsDesc(data, seq, row))
+    return struct.pack("@Pqq", data or 0, seq, row)
 
 
 def append(c=None, k=None, v=None, dtype=0, n=1, starts=P, counts=None, stride=1):
