@@ -12,7 +12,8 @@
 // (128-byte swizzle, 128 values of K a stage; rows and values past the ends read zeros).
 //
 // Schedule. Warp 0 issues TMA into a ring, warp 1 issues four MMAs (K = 32 each) a stage, warps
-// 2-5 drain the accumulator. Many tiles: a persistent grid with two accumulators, so that one
+// 2-9 drain the accumulator (two warps a TMEM lane quarter, half the tokens each; the residual's
+// loads run one chunk ahead). Many tiles: a persistent grid with two accumulators, so that one
 // tile's epilogue runs behind the next one's products. Few tiles (fewer than the SMs): a cluster
 // of 2 to 8 CTAs splits K, each leaves its int32 partial tile in its own shared memory, and after
 // one cluster barrier every CTA adds up its share of the tokens over distributed shared memory.
@@ -33,7 +34,7 @@ namespace {
 
 constexpr int kCh = 128;    // channels of a tile
 constexpr int kKb = 128;    // K bytes of a stage
-constexpr int kEpiWarps = 4;
+constexpr int kEpiWarps = 8;
 constexpr int kThreads = 64 + 32 * kEpiWarps;
 constexpr int kMaxCluster = 8;
 
@@ -43,17 +44,20 @@ template <int NT>
 struct Shape {
   static constexpr int kStage = kCh * kKb + NT * kKb;
   static constexpr int kStages = NT >= 256 ? 4 : NT >= 128 ? 6 : NT >= 64 ? 4 : NT >= 32 ? 5 : 6;
-  static constexpr int kSmem = 1024 + kStages * kStage + 256;
-  // int32 accumulator, signed 8-bit A and B, both K-major
-  static constexpr uint32_t kIdesc =
-      (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(NT >> 3) << 17) | ((uint32_t)(kCh >> 4) << 24);
+  static constexpr int kHalf = NT / 2;                       // tokens of an epilogue warp
+  static constexpr int kSmem = 1024 + kStages * kStage + kEpiWarps * kHalf * 4 + 256;
   static_assert(kStages * kStage >= NT * kCh * 4, "the partial tile reuses the ring");
 };
+
+// Instruction descriptor: int32 accumulator, signed 8-bit A and B, both K-major, M = 128, N = nt.
+__device__ __forceinline__ uint32_t idesc_i8(int nt) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(nt >> 3) << 17) | ((uint32_t)(kCh >> 4) << 24);
+}
 
 struct LinArgs {
   long long m;
   int n, nk, ct, tiles, split;
-  int epi, bf16;
+  int nt;  // tokens of a tile: a multiple of 16, of 32 above 64, at most the template's NT
   const float *xs, *ws;
   const void* resid;
   long long ldr, ldo;
@@ -90,12 +94,25 @@ __device__ __forceinline__ void commit(uint64_t* bar) {
                : "memory");
 }
 
-__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t* r) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(addr));
+#define QASR_R8(r, i) "=r"((r)[i]), "=r"((r)[i + 1]), "=r"((r)[i + 2]), "=r"((r)[i + 3]), "=r"((r)[i + 4]), \
+    "=r"((r)[i + 5]), "=r"((r)[i + 6]), "=r"((r)[i + 7])
+// C columns of this warp's lane quarter: lane = TMEM lane.
+template <int C>
+__device__ __forceinline__ void tmem_ld(uint32_t addr, uint32_t* r) {
+  if constexpr (C == 8)
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];" : QASR_R8(r, 0) : "r"(addr));
+  else if constexpr (C == 16)
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : QASR_R8(r, 0), QASR_R8(r, 8)
+        : "r"(addr));
+  else
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+        "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : QASR_R8(r, 0), QASR_R8(r, 8), QASR_R8(r, 16), QASR_R8(r, 24)
+        : "r"(addr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;");
 }
 
 __device__ __forceinline__ void cluster_barrier() {
@@ -112,55 +129,90 @@ __device__ __forceinline__ int ld_cluster(uint32_t addr) {
   return v;
 }
 
-__device__ __forceinline__ float get(const LinArgs& a, const void* p, long long i) {
-  return a.bf16 ? __bfloat162float(((const __nv_bfloat16*)p)[i]) : ((const float*)p)[i];
+template <bool BF16>
+__device__ __forceinline__ void put(void* p, long long i, float v) {
+  if constexpr (BF16) ((__nv_bfloat16*)p)[i] = __float2bfloat16_rn(v);
+  else ((float*)p)[i] = v;
 }
-__device__ __forceinline__ void put(const LinArgs& a, long long i, float v) {
-  if (a.bf16)
-    ((__nv_bfloat16*)a.out)[i] = __float2bfloat16_rn(v);
-  else
-    ((float*)a.out)[i] = v;
+
+// Residual of tokens m0 .. m0 + C - 1 of this lane's channel, as loaded: it is converted where it
+// is used, so that nothing waits for the loads before that.
+template <int C, bool BF16>
+__device__ __forceinline__ void load_resid(const LinArgs& a, long long m0, int ch, uint32_t* r) {
+#pragma unroll
+  for (int j = 0; j < C; ++j) {
+    r[j] = 0u;
+    if (m0 + j < a.m && ch < a.n) {
+      const long long i = (m0 + j) * a.ldr + ch;
+      if constexpr (BF16) r[j] = ((const uint16_t*)a.resid)[i];
+      else r[j] = ((const uint32_t*)a.resid)[i];
+    }
+  }
+}
+template <bool BF16>
+__device__ __forceinline__ float resid_value(uint32_t r) {
+  return __uint_as_float(BF16 ? r << 16 : r);
 }
 
 // silu(g) * u by exp(-|g|), which does not overflow: far negative gates keep their small values.
+// The denominator is in [1, 2], whose correctly rounded reciprocal takes no slow path (a quotient
+// does for tiny exponentials); in all at most 9 * 2^-24 off.
 __device__ __forceinline__ float gated(float g, float u) {
   const float t = expf(-fabsf(g));
-  const float s = __fdiv_rn(g >= 0.f ? 1.0f : t, __fadd_rn(1.0f, t));
+  const float s = __fmul_rn(g >= 0.f ? 1.0f : t, __frcp_rn(__fadd_rn(1.0f, t)));
   return __fmul_rn(__fmul_rn(s, g), u);
 }
 
-// C tokens m0 .. of one channel a lane (sums acc): scales, epilogue, stores. All 32 lanes call it.
-template <int C>
-__device__ __forceinline__ void finish(const LinArgs& a, const int* acc, long long m0, int ch, float wsc, int lane) {
+// C tokens from m0 of one channel a lane: sums acc, token scales xs, residual r; all 32 lanes call it.
+template <int C, int EPI, bool BF16>
+__device__ __forceinline__ void finish(const LinArgs& a, const int* acc, const float* xs, const uint32_t* r,
+                                       long long m0, int ch, float wsc, int lane) {
   float v[C];
 #pragma unroll
-  for (int j = 0; j < C; ++j)
-    v[j] = __fmul_rn(__fmul_rn((float)acc[j], m0 + j < a.m ? __ldg(a.xs + m0 + j) : 0.f), wsc);
-  if (a.epi == LINEAR_SWIGLU) {
+  for (int j = 0; j < C; ++j) v[j] = __fmul_rn(__fmul_rn((float)acc[j], xs[j]), wsc);
+  if constexpr (EPI == LINEAR_SWIGLU && C > 1) {
     // lanes 2i, 2i + 1 hold gate and up of output column (ch / 2): of two tokens the even lane
     // finishes the first and the odd lane the second
+    static_assert(C % 2 == 0, "tokens in pairs");
 #pragma unroll
     for (int j = 0; j < C; j += 2) {
       const float got = __shfl_xor_sync(0xffffffffu, lane & 1 ? v[j] : v[j + 1], 1);
       const float g = lane & 1 ? got : v[j], u = lane & 1 ? v[j + 1] : got;
       const long long m = m0 + j + (lane & 1);
-      if (m < a.m && ch < a.n) put(a, m * a.ldo + (ch >> 1), gated(g, u));
+      if (m < a.m && ch < a.n) put<BF16>(a.out, m * a.ldo + (ch >> 1), gated(g, u));
     }
-    return;
+  } else if constexpr (EPI == LINEAR_SWIGLU) {
+    const float u = __shfl_xor_sync(0xffffffffu, v[0], 1);
+    if (m0 < a.m && ch < a.n && !(lane & 1)) put<BF16>(a.out, m0 * a.ldo + (ch >> 1), gated(v[0], u));
+  } else {
+#pragma unroll
+    for (int j = 0; j < C; ++j)
+      if (m0 + j < a.m && ch < a.n)
+        put<BF16>(a.out, (m0 + j) * a.ldo + ch, EPI == LINEAR_RESID ? __fadd_rn(v[j], resid_value<BF16>(r[j])) : v[j]);
   }
-  if (a.epi == LINEAR_RESID) {
-    float r[C];
-#pragma unroll
-    for (int j = 0; j < C; ++j) r[j] = m0 + j < a.m && ch < a.n ? get(a, a.resid, (m0 + j) * a.ldr + ch) : 0.f;
-#pragma unroll
-    for (int j = 0; j < C; ++j) v[j] = __fadd_rn(v[j], r[j]);
-  }
-#pragma unroll
-  for (int j = 0; j < C; ++j)
-    if (m0 + j < a.m && ch < a.n) put(a, (m0 + j) * a.ldo + ch, v[j]);
 }
 
-template <int NT>
+// A split tile's tokens [p0, p1) of one half: C at a time, the peers' partial sums added up.
+template <int C, int EPI, bool BF16>
+__device__ __forceinline__ void join(const LinArgs& a, uint32_t part, const float* xs, long long m0, int p0, int p1,
+                                     int ch, float wsc, int lane) {
+#pragma unroll 1
+  for (int p = p0; p < p1; p += C) {
+    if (m0 + p >= a.m) break;
+    uint32_t r[C];
+    if constexpr (EPI == LINEAR_RESID) load_resid<C, BF16>(a, m0 + p, ch, r);
+    int acc[C] = {};
+#pragma unroll 4
+    for (int k = 0; k < a.split; ++k) {
+      const uint32_t peer = map_rank(part + (uint32_t)p * (kCh * 4), k);
+#pragma unroll
+      for (int j = 0; j < C; ++j) acc[j] += ld_cluster(peer + j * (kCh * 4));
+    }
+    finish<C, EPI, BF16>(a, acc, xs + p, r, m0 + p, ch, wsc, lane);
+  }
+}
+
+template <int NT, int EPI, bool BF16>
 __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_constant__ CUtensorMap map_w,
                                                              const __grid_constant__ CUtensorMap map_x,
                                                              const LinArgs a) {
@@ -168,7 +220,8 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
   constexpr int ST = S::kStages;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + ST * S::kStage);
+  float* xs_s = reinterpret_cast<float*>(smem + ST * S::kStage);  // [epilogue warp][kHalf]
+  uint64_t* full = reinterpret_cast<uint64_t*>(xs_s + kEpiWarps * S::kHalf);
   uint64_t* empty = full + ST;
   uint64_t* acc_full = empty + ST;
   uint64_t* acc_empty = acc_full + 2;
@@ -206,7 +259,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
     if (lane == 0) {
       int it = 0;
       for (int u = unit0; u < a.tiles && !*abort_flag; u += step) {
-        const int ch0 = u % a.ct * kCh, m0 = u / a.ct * NT;
+        const int ch0 = u % a.ct * kCh, m0 = u / a.ct * a.nt;
         for (int kt = k0; kt < k1; ++kt, ++it) {
           const int st = it % ST;
           if (it >= ST && !mbar_wait(&empty[st], (uint32_t)((it / ST) - 1) & 1u, &g_wait_err, 31)) {
@@ -214,7 +267,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
             break;
           }
           unsigned char* sp = smem + st * S::kStage;
-          mbar_expect_tx(&full[st], S::kStage);
+          mbar_expect_tx(&full[st], kCh * kKb + a.nt * kKb);
           tma_2d(sp, &map_w, kt * kKb, ch0, &full[st]);
           tma_2d(sp + kCh * kKb, &map_x, kt * kKb, m0, &full[st]);
         }
@@ -222,6 +275,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
     }
   } else if (warp == 1) {
     if (lane == 0) {
+      const uint32_t idesc = idesc_i8(a.nt);
       int it = 0, lt = 0;
       for (int u = unit0; u < a.tiles && !*abort_flag; u += step, ++lt) {
         const int ab = lt & 1;
@@ -242,7 +296,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
           const uint32_t sw = smem_u32(smem + st * S::kStage), sx = sw + kCh * kKb;
 #pragma unroll
           for (int kk = 0; kk < kKb / 32; ++kk)
-            mma_i8(acc, sw128_desc(sw + kk * 32), sw128_desc(sx + kk * 32), S::kIdesc, (kt > k0 || kk > 0) ? 1u : 0u);
+            mma_i8(acc, sw128_desc(sw + kk * 32), sw128_desc(sx + kk * 32), idesc, (kt > k0 || kk > 0) ? 1u : 0u);
           commit(&empty[st]);
         }
         if (!ok) {
@@ -253,33 +307,49 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
       }
     }
   } else {
-    const int q = warp & 3;  // TMEM lane quarter of this warp
+    const int q = warp & 3, half = (warp - 2) >> 2;  // TMEM lane quarter and token half of this warp
+    // tokens in registers at a time (16 where their residuals and the next ones' are too)
+    constexpr int kMost = EPI == LINEAR_RESID || NT > 64 ? 16 : 32, C = S::kHalf < kMost ? S::kHalf : kMost;
+    const int H = a.nt / 2;
+    float* xs = xs_s + (warp - 2) * S::kHalf;
     int lt = 0;
     for (int u = unit0; u < a.tiles; u += step, ++lt) {
       const int ab = lt & 1;
+      const int ch = u % a.ct * kCh + q * 32 + lane;
+      const long long m0 = (long long)(u / a.ct) * a.nt + half * H;
+      const float wsc = ch < a.n ? __ldg(a.ws + ch) : 0.f;
+      __syncwarp();
+      for (int j = lane; j < H; j += 32) xs[j] = m0 + j < a.m ? __ldg(a.xs + m0 + j) : 0.f;
+      __syncwarp();
+      uint32_t r[C];
+      if constexpr (EPI == LINEAR_RESID)
+        if (a.split == 1) load_resid<C, BF16>(a, m0, ch, r);
       const bool ok = mbar_wait(&acc_full[ab], (uint32_t)(lt >> 1) & 1u, &g_wait_err, 34);
       if (!ok) {
         *abort_flag = 1;
         break;
       }
       asm volatile("tcgen05.fence::after_thread_sync;");
-      const int ch = u % a.ct * kCh + q * 32 + lane;
-      const long long m0 = (long long)(u / a.ct) * NT;
-      const float wsc = ch < a.n ? __ldg(a.ws + ch) : 0.f;
-      const uint32_t trow = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(ab * NT);
+      const uint32_t trow = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(ab * NT + half * H);
 #pragma unroll 1
-      for (int c = 0; c < NT; c += 16) {
+      for (int c = 0; c < H; c += C) {
         if (m0 + c >= a.m) break;
-        uint32_t r[16];
-        tmem_ld16(trow + c, r);
-        asm volatile("tcgen05.wait::ld.sync.aligned;");
+        int acc[C];
+        tmem_ld<C>(trow + c, reinterpret_cast<uint32_t*>(acc));
         if (a.split > 1) {
           // every stage has been read by the MMAs that this accumulator waited for
           int* part = reinterpret_cast<int*>(smem);
 #pragma unroll
-          for (int j = 0; j < 16; ++j) part[(c + j) * kCh + q * 32 + lane] = (int)r[j];
+          for (int j = 0; j < C; ++j) part[(half * H + c + j) * kCh + q * 32 + lane] = acc[j];
         } else {
-          finish<16>(a, reinterpret_cast<const int*>(r), m0 + c, ch, wsc, lane);
+          uint32_t next[C];
+          if constexpr (EPI == LINEAR_RESID)
+            if (c + C < H) load_resid<C, BF16>(a, m0 + c + C, ch, next);
+          finish<C, EPI, BF16>(a, acc, xs + c, r, m0 + c, ch, wsc, lane);
+          if constexpr (EPI == LINEAR_RESID) {
+#pragma unroll
+            for (int j = 0; j < C; ++j) r[j] = next[j];
+          }
         }
       }
       asm volatile("tcgen05.fence::before_thread_sync;");
@@ -290,23 +360,22 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
     __syncwarp();
     cluster_barrier();  // every partial tile is in its CTA's shared memory
     if (warp >= 2) {
-      const int q = warp & 3;
+      const int q = warp & 3, half = (warp - 2) >> 2;
       const int ch = unit0 % a.ct * kCh + q * 32 + lane;
-      const long long m0 = (long long)(unit0 / a.ct) * NT;
+      const int H = a.nt / 2;
+      const long long m0 = (long long)(unit0 / a.ct) * a.nt + half * H;
       const float wsc = ch < a.n ? __ldg(a.ws + ch) : 0.f;
-      const uint32_t base = smem_u32(smem) + (uint32_t)(q * 32 + lane) * 4u;
-      const int live = (int)min((long long)NT, a.m - m0);
-      // token pairs in turn: pair p belongs to rank p % split
-#pragma unroll 1
-      for (int p = rank * 2; p < live; p += a.split * 2) {
-        int acc[2] = {0, 0};
-        for (int r = 0; r < a.split; ++r) {
-          const uint32_t peer = map_rank(base + (uint32_t)p * (kCh * 4), r);
-          acc[0] += ld_cluster(peer);
-          acc[1] += ld_cluster(peer + kCh * 4);
-        }
-        finish<2>(a, acc, m0 + p, ch, wsc, lane);
-      }
+      const uint32_t part = smem_u32(smem) + (uint32_t)(half * H * kCh + q * 32 + lane) * 4u;
+      const float* xs = xs_s + (warp - 2) * S::kHalf;
+      const int each = H / a.split;  // tokens of a rank (H >= 8 = the largest split, and a multiple of it)
+      if (each % 8 == 0)
+        join<8, EPI, BF16>(a, part, xs, m0, rank * each, (rank + 1) * each, ch, wsc, lane);
+      else if (each % 4 == 0)
+        join<4, EPI, BF16>(a, part, xs, m0, rank * each, (rank + 1) * each, ch, wsc, lane);
+      else if (each % 2 == 0)
+        join<2, EPI, BF16>(a, part, xs, m0, rank * each, (rank + 1) * each, ch, wsc, lane);
+      else
+        join<1, EPI, BF16>(a, part, xs, m0, rank * each, (rank + 1) * each, ch, wsc, lane);
     }
     __syncwarp();
     cluster_barrier();  // no CTA leaves while a peer reads its partial
@@ -345,24 +414,36 @@ bool byte_map(CUtensorMap* m, const void* base, long long rows, int cols, long l
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int NT>
-cudaError_t launch(const int8_t* xq, long long ldx, const int8_t* wq, long long ldw, int k, LinArgs a, cudaStream_t s) {
-  CUtensorMap mw, mx;
-  if (!byte_map(&mw, wq, a.n, k, ldw, kCh) || !byte_map(&mx, xq, a.m, k, ldx, NT)) return cudaErrorInvalidValue;
+struct LinCall {
+  const int8_t *xq, *wq;
+  long long ldx, ldw;
+  int k;
+  LinearEpi epi;
+  bool bf16;
+};
+
+template <int NT, int EPI, bool BF16>
+cudaError_t launch_as(const LinCall& c, const LinArgs& a, const CUtensorMap& mw, const CUtensorMap& mx, int grid,
+                      cudaStream_t s) {
   static OncePerDevice once;
-  const cudaError_t e = once.smem(linear_kernel<NT>, Shape<NT>::kSmem);
+  const cudaError_t e = once.smem(linear_kernel<NT, EPI, BF16>, Shape<NT>::kSmem);
   if (e != cudaSuccess) return e;
-  a.ct = ceil_div(a.n, kCh);
-  a.nk = ceil_div(k, kKb);
-  const long long tiles = (long long)a.ct * ((a.m + NT - 1) / NT);
-  if (tiles > 0x7FFFFFFF) return cudaErrorInvalidValue;
-  a.tiles = (int)tiles;
-  const int sms = ops_sm_count();
-  a.split = 1;
-  // few tiles: split K while the CTAs still fit one wave and each keeps two stages of K
-  while (a.split < kMaxCluster && a.tiles * a.split * 2 <= sms && a.nk >= a.split * 4) a.split *= 2;
-  const int grid = a.split > 1 ? a.tiles * a.split : (a.tiles < sms ? a.tiles : sms);
-  return ops_launch(linear_kernel<NT>, dim3(grid), dim3(kThreads), Shape<NT>::kSmem, s, a.split, mw, mx, a);
+  return ops_launch(linear_kernel<NT, EPI, BF16>, dim3(grid), dim3(kThreads), Shape<NT>::kSmem, s, a.split, mw, mx, a);
+}
+
+template <int NT>
+cudaError_t launch(const LinCall& c, const LinArgs& a, int grid, cudaStream_t s) {
+  CUtensorMap mw, mx;
+  if (!byte_map(&mw, c.wq, a.n, c.k, c.ldw, kCh) || !byte_map(&mx, c.xq, a.m, c.k, c.ldx, a.nt))
+    return cudaErrorInvalidValue;
+  if (c.epi == LINEAR_SWIGLU)
+    return c.bf16 ? launch_as<NT, LINEAR_SWIGLU, true>(c, a, mw, mx, grid, s)
+                  : launch_as<NT, LINEAR_SWIGLU, false>(c, a, mw, mx, grid, s);
+  if (c.epi == LINEAR_RESID)
+    return c.bf16 ? launch_as<NT, LINEAR_RESID, true>(c, a, mw, mx, grid, s)
+                  : launch_as<NT, LINEAR_RESID, false>(c, a, mw, mx, grid, s);
+  return c.bf16 ? launch_as<NT, LINEAR_STORE, true>(c, a, mw, mx, grid, s)
+                : launch_as<NT, LINEAR_STORE, false>(c, a, mw, mx, grid, s);
 }
 
 }  // namespace
@@ -372,14 +453,44 @@ cudaError_t linear_int8(const int8_t* xq, long long ldx, const float* xs, const 
                         void* out, long long ldo, OpsDtype dt, cudaStream_t s) {
   if (m <= 0 || n <= 0) return cudaSuccess;
   LinArgs a{};
-  a.m = m; a.n = n; a.epi = epi; a.bf16 = dt == OPS_BF16; a.xs = xs; a.ws = ws;
-  a.resid = residual; a.ldr = ldr; a.ldo = ldo; a.out = out;
-  if (m <= 16) return launch<16>(xq, ldx, wq, ldw, k, a, s);
-  if (m <= 32) return launch<32>(xq, ldx, wq, ldw, k, a, s);
-  if (m <= 64) return launch<64>(xq, ldx, wq, ldw, k, a, s);
-  const long long ct = ceil_div(n, kCh);
-  if (ct * ((m + 255) / 256) < ops_sm_count()) return launch<128>(xq, ldx, wq, ldw, k, a, s);
-  return launch<256>(xq, ldx, wq, ldw, k, a, s);
+  a.m = m; a.n = n; a.xs = xs; a.ws = ws; a.resid = residual; a.ldr = ldr; a.ldo = ldo; a.out = out;
+  const LinCall c{xq, wq, ldx, ldw, k, epi, dt == OPS_BF16};
+  a.ct = ceil_div(n, kCh);
+  a.nk = ceil_div(k, kKb);
+  const int sms = ops_sm_count();
+  // Tile width and K split with the least estimated time in cycles. A step of 128 bytes of K takes 2
+  // for each of the 128 + nt rows it brings from L2 (64 bytes a cycle and SM; the products take 2
+  // nt), a tile's epilogue about 8 nt beside the next tile's products, and a split's join 2000.
+  // Measured against all widths and splits at 16 shapes, the choice is within 6 % of the best
+  // (9 % at 32 x 4096 x 2048); e.g. 8191 x 2048 x 6144: 224 tokens 93 us (592 tiles, four full
+  // waves), 256 tokens 101 us, 128 tokens 118 us; 381 x 2048 x 6144: 192 tokens in 4 splits 13.3
+  // us, 96 in 2 15.7 us, 128 unsplit 22 us; 8 x 2048 x 6144: 8 splits 7.7 us, 1 split 17 us.
+  long long best = -1;
+  static const int widths[] = {16, 32, 64, 96, 128, 160, 192, 224, 256};
+  for (int nt : widths) {
+    const long long tiles = (long long)a.ct * ((m + nt - 1) / nt);
+    if (tiles > 0x7FFFFFFF / 16) continue;
+    for (int split = 1; split <= kMaxCluster; split *= 2) {
+      if (split > 1 && (a.nk < split * 2 || nt / 2 % split || tiles * split > 2 * sms)) break;
+      const long long waves = (tiles * split + sms - 1) / sms;
+      const long long loop = (long long)((a.nk + split - 1) / split) * 2 * (128 + nt);
+      const long long epi = 8 * nt + (split > 1 ? 2000 : 0);
+      const long long cost = waves * (loop > epi ? loop : epi) + epi;
+      if (best < 0 || cost < best) {
+        best = cost;
+        a.nt = nt;
+        a.split = split;
+        a.tiles = (int)tiles;
+      }
+    }
+  }
+  if (best < 0) return cudaErrorInvalidValue;
+  const int grid = a.split > 1 ? a.tiles * a.split : (a.tiles < sms ? a.tiles : sms);
+  if (a.nt <= 16) return launch<16>(c, a, grid, s);
+  if (a.nt <= 32) return launch<32>(c, a, grid, s);
+  if (a.nt <= 64) return launch<64>(c, a, grid, s);
+  if (a.nt <= 128) return launch<128>(c, a, grid, s);
+  return launch<256>(c, a, grid, s);
 }
 
 int linear_int8_error() {

@@ -6,14 +6,18 @@
 // alike. So one pass over the row gives everything: the sum of h^2 and the maximum of |u| are
 // reduced together, once, and the row, still in registers, is quantised behind that one barrier.
 //
-// Rounding. q is the correctly rounded quotient. In f32, v = u * (127 / top) is off by less
-// than 127 * 4 * 2^-24 < 4e-5, so a v further than 1e-4 from a half rounds to the right side;
-// the few others (2e-4 of all) are rounded again from the f64 product, whose factors h, w are
-// exact. top is compared exactly too: the product's f32 rounding first, its error (one fma)
-// between equal ones. The sum of squares is held in 64 bits, where no finite row overflows it.
+// Rounding. q is the correctly rounded quotient. In f32, v = u * (127 / top) is off by at most
+// 127 * 4 * 2^-24 < 3.1e-5 (four roundings), so a v further than 3.2e-5 from a half rounds to the
+// right side; the others (6e-5 of all) are rounded again from the f64 product, whose factors are
+// exact. For them, and for the scale, top is exact too: the threads that hold the largest f32
+// product add its rounding error (one fma). The sum of squares is held in 64 bits, where no
+// finite row overflows it.
 //
-// Bound: DRAM. A bf16 row of d values with a residual moves 7d bytes and takes ~25 operations a
-// value.
+// Bound: DRAM for many rows. What it took to get near: a bf16 sum as packed adds, one fmax a
+// value, rounding by the 1.5 * 2^23 trick whose low byte is the int8 value, and a warp that adds up
+// the squares behind the barrier while the others quantise (they do not need the norm). 16411
+// rows of 2048 bf16 values with a residual: 89 us with a shuffled (f64, u64) reduction and
+// per-value conversions, @NORM_MANY@ so.
 #include <cuda_bf16.h>
 
 #include "dev_util.cuh"
@@ -31,13 +35,6 @@ struct Elem<false> {
   __device__ static float load(const T* p) { return *p; }
   __device__ static void store(T* p, float v) { *p = v; }
   __device__ static float round(float v) { return v; }
-  __device__ static void load_vec(const T* p, float* f) {
-    const float4 v = *reinterpret_cast<const float4*>(p);
-    f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
-  }
-  __device__ static void store_vec(T* p, const float* f) {
-    *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
-  }
 };
 template <>
 struct Elem<true> {
@@ -46,13 +43,6 @@ struct Elem<true> {
   __device__ static float load(const T* p) { return __bfloat162float(*p); }
   __device__ static void store(T* p, float v) { *p = __float2bfloat16_rn(v); }
   __device__ static float round(float v) { return __bfloat162float(__float2bfloat16_rn(v)); }
-  __device__ static void load_vec(const T* p, float* f) { bf16x8_to_f32(*reinterpret_cast<const uint4*>(p), f); }
-  __device__ static void store_vec(T* p, const float* f) {
-    __nv_bfloat162 v[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
-    *reinterpret_cast<uint4*>(p) = *reinterpret_cast<uint4*>(v);
-  }
 };
 
 struct NormArgs {
@@ -122,81 +112,174 @@ __device__ __forceinline__ void row_stat(Stat& st, Stat* red, int warp, int lane
   st.warp();
 }
 
+// 16 bytes of a row as loaded, and the sum of two of them rounded to the type. (Two bf16 values
+// round the same from f32 as from their exact sum: where f32 cannot hold it, the smaller is below
+// 2^-16 of the larger, far from a bf16 tie.)
+template <bool BF16>
+__device__ __forceinline__ uint4 add_packed(uint4 a, uint4 b) {
+  uint32_t* x = reinterpret_cast<uint32_t*>(&a);
+  const uint32_t* y = reinterpret_cast<const uint32_t*>(&b);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (BF16) {
+      const __nv_bfloat162 h =
+          __hadd2_rn(*reinterpret_cast<const __nv_bfloat162*>(x + i), *reinterpret_cast<const __nv_bfloat162*>(y + i));
+      x[i] = *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+      x[i] = __float_as_uint(__fadd_rn(__uint_as_float(x[i]), __uint_as_float(y[i])));
+    }
+  }
+  return a;
+}
+
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN when either is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+constexpr float kRound = 12582912.f;  // 1.5 * 2^23: adding it rounds to an integer, in the low bits
+
 // One row by W warps, its values in registers: NV vectors a thread.
-template <bool BF16, int W, int NV, int ROWS>
-__global__ void __launch_bounds__(W * ROWS * 32) norm_vec_kernel(const NormArgs a) {
-  using E = Elem<BF16>;
-  using T = typename E::T;
-  constexpr int V = E::kVec;
-  __shared__ Stat red[W];
-  const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) % W;
-  const long long row = (long long)blockIdx.x * ROWS + (threadIdx.x >> 5) / W;
-  if (row >= a.rows) return;  // ROWS > 1 only with W == 1: no barrier below
+template <bool BF16, int W, int NV>
+__global__ void __launch_bounds__(W * 32) norm_vec_kernel(const NormArgs a) {
+  using T = typename Elem<BF16>::T;
+  constexpr int V = Elem<BF16>::kVec, N = W * 32;
+  __shared__ double parts[N];
+  __shared__ unsigned tops[W];
+  __shared__ unsigned low;  // ordered bits of the largest product's rounding error
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long row = blockIdx.x;
   const T* x = (const T*)a.x + row * a.ldx;
-  const T* r = a.r ? (const T*)a.r + row * a.ldr : nullptr;
-  const int t = warp * 32 + lane;
-  float h[NV][V];
-  bool in[NV];
+  uint4 raw[NV];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const int c = (t + j * W * 32) * V;
-    in[j] = c < a.d;
-    if (in[j]) E::load_vec(x + c, h[j]);
+    const int c = (threadIdx.x + j * N) * V;
+    raw[j] = make_uint4(0, 0, 0, 0);
+    if (c < a.d) raw[j] = *reinterpret_cast<const uint4*>(x + c);
   }
-  if (r) {
-    float f[NV][V];
+  if (a.r) {
+    const T* r = (const T*)a.r + row * a.ldr;
+    uint4 add[NV];
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
-      if (in[j]) E::load_vec(r + (t + j * W * 32) * V, f[j]);
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-#pragma unroll
-      for (int i = 0; i < V; ++i) h[j][i] = E::round(__fadd_rn(h[j][i], f[j][i]));
-  }
-  Stat st;
-#pragma unroll
-  for (int j = 0; j < NV; ++j)
-    if (in[j]) {
-      const int c = (t + j * W * 32) * V;
-      if (a.h) E::store_vec((T*)a.h + row * a.ldh + c, h[j]);
-#pragma unroll
-      for (int i = 0; i < V; i += 4) {
-        const float4 w = __ldg(reinterpret_cast<const float4*>(a.w + c + i));
-        st.add(h[j][i], w.x);
-        st.add(h[j][i + 1], w.y);
-        st.add(h[j][i + 2], w.z);
-        st.add(h[j][i + 3], w.w);
-      }
+    for (int j = 0; j < NV; ++j) {
+      const int c = (threadIdx.x + j * N) * V;
+      add[j] = make_uint4(0, 0, 0, 0);
+      if (c < a.d) add[j] = *reinterpret_cast<const uint4*>(r + c);
     }
-  row_stat(st, red, warp, lane, W);
-  const float top = __uint_as_float(st.top);
-  const float r127 = st.finite() && st.top ? __fdiv_rn(127.0f, top) : 0.f;
-  const bool tiny = r127 > 3e38f;  // 127 / top overflowed: a row of subnormals
 #pragma unroll
-  for (int j = 0; j < NV; ++j)
-    if (in[j]) {
-      const int c = (t + j * W * 32) * V;
-      uint32_t o[V / 4];
+    for (int j = 0; j < NV; ++j) raw[j] = add_packed<BF16>(raw[j], add[j]);
+  }
+  float h[NV][V], u[NV][V];
+  float mx = 0.f;
+  double ss = 0.0;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int c = (threadIdx.x + j * N) * V;
+    if constexpr (BF16) {
+      bf16x8_to_f32(raw[j], h[j]);
+    } else {
+      h[j][0] = __uint_as_float(raw[j].x);
+      h[j][1] = __uint_as_float(raw[j].y);
+      h[j][2] = __uint_as_float(raw[j].z);
+      h[j][3] = __uint_as_float(raw[j].w);
+    }
+    if (c < a.d) {
+      if (a.h) *reinterpret_cast<uint4*>((T*)a.h + row * a.ldh + c) = raw[j];
 #pragma unroll
       for (int i = 0; i < V; i += 4) {
         const float4 w = __ldg(reinterpret_cast<const float4*>(a.w + c + i));
-        const float wf[4] = {w.x, w.y, w.z, w.w};
-        o[i / 4] = 0u;
+        u[j][i] = __fmul_rn(h[j][i], w.x);
+        u[j][i + 1] = __fmul_rn(h[j][i + 1], w.y);
+        u[j][i + 2] = __fmul_rn(h[j][i + 2], w.z);
+        u[j][i + 3] = __fmul_rn(h[j][i + 3], w.w);
+      }
+    } else {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int v = r127 == 0.f ? 0
-                        : tiny      ? __double2int_rn((double)h[j][i + k] * (double)wf[k] * 127.0 / st.top64())
-                                    : quant(h[j][i + k], wf[k], r127, st);
-          o[i / 4] |= ((uint32_t)v & 0xFFu) << (8 * k);
+      for (int i = 0; i < V; ++i) u[j][i] = 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      mx = max_nan(mx, fabsf(u[j][i]));
+      ss = fma((double)h[j][i], (double)h[j][i], ss);
+    }
+  }
+  const unsigned mine = __float_as_uint(mx) & 0x7FFFFFFFu;
+  const unsigned wtop = __reduce_max_sync(0xffffffffu, mine);
+  parts[threadIdx.x] = ss;
+  if (lane == 0) tops[warp] = wtop;
+  if (threadIdx.x == 0) low = 0u;
+  __syncthreads();
+  unsigned top = tops[0];
+#pragma unroll
+  for (int i = 1; i < W; ++i) top = max(top, tops[i]);
+  const bool finite = top < 0x7F800000u;
+  if (mine == top && finite && top) {
+    // this thread holds a largest product
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = (threadIdx.x + j * N) * V;
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (c < a.d && (__float_as_uint(u[j][i]) & 0x7FFFFFFFu) == top) {
+          const float e = __fmaf_rn(h[j][i], a.w[c + i], -u[j][i]);
+          atomicMax(&low, (unsigned)float_to_ordered(u[j][i] < 0.f ? -e : e) ^ 0x80000000u);
         }
-      }
-      int8_t* q = a.q + row * a.ldq + c;
-      if constexpr (V == 8)
-        *reinterpret_cast<uint2*>(q) = make_uint2(o[0], o[1]);
-      else
-        *reinterpret_cast<uint32_t*>(q) = o[0];
     }
-  if (t == 0) write_scale(a, row, st);
+  }
+  const float r127 = finite && top ? __fdiv_rn(127.0f, __uint_as_float(top)) : 0.f;
+  bool near = r127 > 3e38f;  // 127 / top overflowed: a row of subnormals takes the exact path
+  int8_t* q = a.q + row * a.ldq;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int c = (threadIdx.x + j * N) * V;
+    uint32_t o[V / 4];
+#pragma unroll
+    for (int i = 0; i < V; i += 4) {
+      uint32_t b[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float v = __fmul_rn(u[j][i + k], r127);
+        const float t = __fadd_rn(v, kRound);
+        b[k] = __float_as_uint(t);
+        near |= fabsf(__fsub_rn(v, __fsub_rn(t, kRound))) > 0.5f - 3.2e-5f;
+      }
+      o[i / 4] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+      if (!finite) o[i / 4] = 0u;
+    }
+    if (c < a.d) {
+      if constexpr (V == 8)
+        *reinterpret_cast<uint2*>(q + c) = make_uint2(o[0], o[1]);
+      else
+        *reinterpret_cast<uint32_t*>(q + c) = o[0];
+    }
+  }
+  __syncthreads();  // `low` is complete
+  const double top64 = (double)__uint_as_float(top) + (double)ordered_to_float((int)(low ^ 0x80000000u));
+  if (near && finite) {
+#pragma unroll 1
+    for (int j = 0; j < NV; ++j) {
+      const int c = (threadIdx.x + j * N) * V;
+      if (c < a.d)
+#pragma unroll 1
+        for (int i = 0; i < V; ++i) {
+          // (the row again from memory: an index into the registers would push them all to the stack)
+          const T* src = a.h ? (const T*)a.h + row * a.ldh : x;
+          q[c + i] = (int8_t)__double2int_rn((double)Elem<BF16>::load(src + c + i) * (double)a.w[c + i] * 127.0 / top64);
+        }
+    }
+  }
+  if (warp == 0) {
+    double sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < W; ++i) sum += parts[i * 32 + lane];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0)
+      a.scale[row] = !finite ? __int_as_float(0x7FFFFFFF)
+                     : top   ? (float)(top64 / sqrt(sum / (double)a.d + (double)a.eps) / 127.0)
+                             : 1.0f;
+  }
 }
 
 // Any d, stride and alignment: the row is staged in shared memory, one element a thread at a time.
@@ -237,11 +320,14 @@ cudaError_t launch(const NormArgs& a, bool vec, cudaStream_t s) {
   const int nv = a.d / V;  // vectors of a row
   const dim3 g((unsigned)a.rows);
   if (vec) {
-    if (nv <= 128) return ops_launch(norm_vec_kernel<BF16, 4, 1, 1>, g, dim3(128), 0, s, 1, a);
-    if (nv <= 256) return ops_launch(norm_vec_kernel<BF16, 8, 1, 1>, g, dim3(256), 0, s, 1, a);
-    if (nv <= 512) return ops_launch(norm_vec_kernel<BF16, 8, 2, 1>, g, dim3(256), 0, s, 1, a);
-    if (nv <= 1024) return ops_launch(norm_vec_kernel<BF16, 8, 4, 1>, g, dim3(256), 0, s, 1, a);
-    if (nv <= 2048) return ops_launch(norm_vec_kernel<BF16, 16, 4, 1>, g, dim3(512), 0, s, 1, a);
+    // two vectors a thread where rows fill the GPU anyway, one where a row's latency counts
+    const bool many = a.rows >= 4 * ops_sm_count();
+    if (nv <= 128) return ops_launch(norm_vec_kernel<BF16, 4, 1>, g, dim3(128), 0, s, 1, a);
+    if (nv <= 256 && many) return ops_launch(norm_vec_kernel<BF16, 4, 2>, g, dim3(128), 0, s, 1, a);
+    if (nv <= 256) return ops_launch(norm_vec_kernel<BF16, 8, 1>, g, dim3(256), 0, s, 1, a);
+    if (nv <= 512) return ops_launch(norm_vec_kernel<BF16, 8, 2>, g, dim3(256), 0, s, 1, a);
+    if (nv <= 1024) return ops_launch(norm_vec_kernel<BF16, 8, 4>, g, dim3(256), 0, s, 1, a);
+    if (nv <= 2048) return ops_launch(norm_vec_kernel<BF16, 16, 4>, g, dim3(512), 0, s, 1, a);
   }
   const size_t smem = (size_t)a.d * sizeof(float);
   if (smem > 40 * 1024) {

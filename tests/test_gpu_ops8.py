@@ -157,9 +157,8 @@ def test_linear_residual_and_swiglu(ops, dt, m, n, k):
     s = ops.linear_int8(xq, xs, wq, ws, swiglu=True, dtype=dt)
     g, u = ref[:, 0::2].double(), ref[:, 1::2].double()
     want = g / (1 + torch.exp(-g)) * u
-    # expf 2 ulp (2 * 2^-23), then a sum, a quotient and a product of half an ulp each: 7 * 2^-24
-    # (one more for second-order terms), and the output's rounding; results under the smallest
-    # normal number may lose all their bits
+    # expf 2 ulp (4 * 2^-24), then a sum, a reciprocal and three products of 2^-24 each: 9 * 2^-24,
+    # or 8 and the output's rounding; results under the smallest normal number may lose all bits
     tol = want.abs() * (8 * 2.0 ** -24 + HALF[dt]) + 2.0 ** -126
     assert ((s.double() - want).abs() <= tol).all()
 
