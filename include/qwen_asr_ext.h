@@ -26,6 +26,15 @@ void qwen_asr_set_skip_silence(QwenAsrEngine* engine, int32_t on);
 /* Decode weights: 0 = int8 per-row (the reference's decode, decoder.rs:106-118, default),
  * 1 = bf16 (the reference's bf16 matvec family, kernels/mod.rs:630-835). */
 int32_t qwen_asr_set_decode_mode(QwenAsrEngine* engine, int32_t mode);
+/* Prefill products: 0 = bf16 weights with f32-accurate activations (the reference's f32 sgemm,
+ * default), 1 = the int8 decode weights times int8 rows with a scale each (the operators at the
+ * end of this header): several times faster, with int8 decode's accuracy. 0 ok, -1 bad mode. */
+int32_t qwen_asr_set_prefill_mode(QwenAsrEngine* engine, int32_t mode);
+/* KV cache: 0 = f32 (the reference's, default), 1 = int8 with a scale for each 16 tokens of a
+ * head, about a quarter of the memory a position. A change empties the cache: streams prefill
+ * their prompt from scratch on the next chunk. 0 ok, -1 bad mode or out of memory (then nothing
+ * changed). */
+int32_t qwen_asr_set_kv_mode(QwenAsrEngine* engine, int32_t mode);
 /* Benchmark mode: run exactly n decode steps per segment, ignoring EOS (0 = off). */
 void qwen_asr_set_force_n_tokens(QwenAsrEngine* engine, int32_t n);
 /* Pushes audio to `count` distinct streams at once: each stream runs exactly the chunks
@@ -206,6 +215,8 @@ QwenAsrEngine* qwen_asr_pool_engine(QwenAsrPool* pool, int32_t i);
 void qwen_asr_pool_set_segment_sec(QwenAsrPool* pool, float sec);
 int32_t qwen_asr_pool_set_language(QwenAsrPool* pool, const char* language);
 void qwen_asr_pool_set_decode_mode(QwenAsrPool* pool, int32_t mode); /* 0 int8, 1 bf16 */
+int32_t qwen_asr_pool_set_prefill_mode(QwenAsrPool* pool, int32_t mode); /* 0 bf16, 1 int8 */
+int32_t qwen_asr_pool_set_kv_mode(QwenAsrPool* pool, int32_t mode);      /* 0 f32, 1 int8 */
 void qwen_asr_pool_set_force_n_tokens(QwenAsrPool* pool, int32_t n);
 void qwen_asr_pool_stream_set_max_new_tokens(QwenAsrPool* pool, int32_t n);
 /* Like qwen_asr_transcribe_pcm, the segments spread over the pool's GPUs. */

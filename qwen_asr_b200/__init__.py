@@ -50,6 +50,8 @@ SIGNATURES = {
     "qwen_asr_set_past_text": (None, [_VP, C.c_int32]),
     "qwen_asr_set_skip_silence": (None, [_VP, C.c_int32]),
     "qwen_asr_set_decode_mode": (C.c_int32, [_VP, C.c_int32]),
+    "qwen_asr_set_prefill_mode": (C.c_int32, [_VP, C.c_int32]),
+    "qwen_asr_set_kv_mode": (C.c_int32, [_VP, C.c_int32]),
     "qwen_asr_set_force_n_tokens": (None, [_VP, C.c_int32]),
     "qwen_asr_set_use_graph": (None, [_VP, C.c_int32]),
     "qwen_asr_set_decode_batch": (C.c_int32, [_VP, C.c_int32]),
@@ -76,6 +78,8 @@ SIGNATURES = {
     "qwen_asr_pool_set_segment_sec": (None, [_VP, C.c_float]),
     "qwen_asr_pool_set_language": (C.c_int32, [_VP, C.c_char_p]),
     "qwen_asr_pool_set_decode_mode": (None, [_VP, C.c_int32]),
+    "qwen_asr_pool_set_prefill_mode": (C.c_int32, [_VP, C.c_int32]),
+    "qwen_asr_pool_set_kv_mode": (C.c_int32, [_VP, C.c_int32]),
     "qwen_asr_pool_set_force_n_tokens": (None, [_VP, C.c_int32]),
     "qwen_asr_pool_stream_set_max_new_tokens": (None, [_VP, C.c_int32]),
     "qwen_asr_pool_transcribe_pcm": (_VP, [_VP, _F32P, C.c_int32]),
@@ -222,6 +226,16 @@ class Engine:
     def set_decode_mode(self, mode: str):
         if lib().qwen_asr_set_decode_mode(self._h, {"int8": 0, "bf16": 1}[mode]) != 0:
             raise ValueError(mode)
+
+    def set_prefill_mode(self, mode: str):
+        """"bf16" (f32-accurate prefill products, default) or "int8" (int8 weights and rows)."""
+        if lib().qwen_asr_set_prefill_mode(self._h, {"bf16": 0, "int8": 1}[mode]) != 0:
+            raise ValueError(mode)
+
+    def set_kv_mode(self, mode: str):
+        """"f32" (default) or "int8" (a quarter of the memory a position); a change empties the cache."""
+        if lib().qwen_asr_set_kv_mode(self._h, {"f32": 0, "int8": 1}[mode]) != 0:
+            raise RuntimeError(last_error())
 
     def set_force_n_tokens(self, n: int):
         lib().qwen_asr_set_force_n_tokens(self._h, n)
@@ -435,6 +449,14 @@ class Pool:
 
     def set_decode_mode(self, mode: str):
         lib().qwen_asr_pool_set_decode_mode(self._h, 1 if mode == "bf16" else 0)
+
+    def set_prefill_mode(self, mode: str):
+        if lib().qwen_asr_pool_set_prefill_mode(self._h, {"bf16": 0, "int8": 1}[mode]) != 0:
+            raise ValueError(mode)
+
+    def set_kv_mode(self, mode: str):
+        if lib().qwen_asr_pool_set_kv_mode(self._h, {"f32": 0, "int8": 1}[mode]) != 0:
+            raise RuntimeError(last_error())
 
     def set_force_n_tokens(self, n: int):
         lib().qwen_asr_pool_set_force_n_tokens(self._h, n)

@@ -283,6 +283,15 @@ int32_t qwen_asr_set_decode_mode(QwenAsrEngine* e, int32_t mode) {
   e->ctx.eng.set_decode_mode(mode == 0 ? qasr::DECODE_INT8 : qasr::DECODE_BF16);
   return 0;
 }
+int32_t qwen_asr_set_prefill_mode(QwenAsrEngine* e, int32_t mode) {
+  if (!e || (mode != 0 && mode != 1)) return -1;
+  e->ctx.eng.set_prefill_mode(mode == 1 ? qasr::PREFILL_INT8 : qasr::PREFILL_BF16);
+  return 0;
+}
+int32_t qwen_asr_set_kv_mode(QwenAsrEngine* e, int32_t mode) {
+  if (!e || (mode != 0 && mode != 1)) return -1;
+  return e->ctx.set_kv_mode(mode == 1 ? qasr::KV_INT8 : qasr::KV_F32) ? 0 : -1;
+}
 void qwen_asr_set_force_n_tokens(QwenAsrEngine* e, int32_t n) {
   if (e) e->ctx.force_n_tokens = n > 0 ? n : 0;
 }

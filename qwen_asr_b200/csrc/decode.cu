@@ -1684,8 +1684,9 @@ bool decode_stage_once() {
   return on;
 }
 
-int decode_batched_step_launches(int layers, bool int8) {
-  return int8 && decode_stage_once() ? 9 * layers + 2 : 5 * layers + 1;
+int decode_batched_step_launches(int layers, bool int8, bool kv8) {
+  const int more = kv8 ? 2 * layers : 0;  // norm + RoPE, append, attention instead of one kernel
+  return more + (int8 && decode_stage_once() ? 9 * layers + 2 : 5 * layers + 1);
 }
 
 void decode_kernels_init() {
@@ -1809,7 +1810,7 @@ bool decode_step(const DecodeArgs& a, cudaStream_t s) {
     m.B = B;
     return m;
   };
-  const bool split = B > 1 || decode_split_qkv(a.hidden, a.q_heads, a.kv_heads, a.int8);
+  const bool split = B > 1 || a.kv8.k || decode_split_qkv(a.hidden, a.q_heads, a.kv_heads, a.int8);
   for (int l = 0; l < a.layers; ++l) {
     // QKV projection + attention, one cluster per (kv head, sequence). The first kernel of a
     // step is a plain launch: it starts only after the previous step (which advanced
@@ -1832,7 +1833,28 @@ bool decode_step(const DecodeArgs& a, cudaStream_t s) {
       if (a.on_launch) a.on_launch(a.hook_ctx, 0);
       check("qkv_proj", l);
     }
-    {
+    if (a.kv8.k) {
+      // int8 cache: norm and RoPE of the projected rows in place, then the cache's own operators
+      const int* pos = &a.st->pos;
+      constexpr int kStride = sizeof(StepState) / sizeof(int);
+      if (!qk_norm_rope_rows(a.qkv, B, pos, kStride, a.q_heads, a.kv_heads, a.qn[l], a.kn[l], a.eps, a.rope_cos,
+                             a.rope_sin, s)) {
+        set_error("decode: norm and RoPE launch failed");
+        ok = false;
+      }
+      Kv8 c = a.kv8;
+      c.n_seq = B;
+      c.k += (size_t)l * a.kv8_layer_stride;
+      c.v += (size_t)l * a.kv8_layer_stride;
+      c.ks += (size_t)l * (a.kv8_layer_stride / kHd / kKv8Block);
+      c.vs += (size_t)l * (a.kv8_layer_stride / kHd / kKv8Block);
+      const float* k = a.qkv + (size_t)a.q_heads * kHd;
+      launched(kv8_append(c, k, nqkv, nqkv, k + (size_t)a.kv_heads * kHd, nqkv, nqkv, OPS_F32, 1, pos, nullptr, kStride, s));
+      launched(kv8_attention(c, a.qkv, nqkv, nqkv, a.attn, qd, qd, OPS_F32, 1, a.q_heads, pos, nullptr, kStride,
+                             1.0f / sqrtf((float)kHd), 0, s, kKv8Splits));
+      if (a.on_launch) a.on_launch(a.hook_ctx, 1);
+      check("kv8_attention", l);
+    } else {
       QkvAttnArgs q{};
       q.x = a.x;
       if (l == 0) {

@@ -310,6 +310,9 @@ bool Engine::ensure_kv(int needed) {
   if (needed <= max_seq_ && rope_cap_ >= max_seq_) return true;
   int nm = max_seq_ > 0 ? max_seq_ : 2048;
   while (nm < needed) nm *= 2;
+  if (kv_mode_ == KV_INT8) {
+    if (!resize_kv8(slots_, nm, (size_t)(slots_ > 1 ? max_seq_ : kv_len_))) return false;
+  } else {
   size_t per = (size_t)slots_ * c.dec_layers * c.dec_kv_heads * nm * 128;
   float *nk = nullptr, *nv = nullptr;
   CUDA_OK(cudaMalloc(&nk, per * 4), false);
@@ -334,6 +337,7 @@ bool Engine::ensure_kv(int needed) {
   kc_.n = per;
   vc_.p = nv;
   vc_.n = per;
+  }
   max_seq_ = nm;
   std::vector<float> rc, rs;
   build_rope_tables(nm, 128, c.dec_rope_theta, rc, rs);
@@ -353,8 +357,86 @@ bool Engine::ensure_kv(int needed) {
   return true;
 }
 
+// The int8 cache for `slots` slots of `seq` positions, with the first `used` positions of every
+// (slot, layer, head) of the present one.
+bool Engine::resize_kv8(int slots, int seq, size_t used) {
+  const size_t lh = (size_t)cfg_.dec_layers * cfg_.dec_kv_heads, runs = (size_t)slots * lh, old_runs = (size_t)slots_ * lh;
+  const size_t blocks = (size_t)seq / kKv8Block;
+  DevBuf<int8_t> nk, nv;
+  DevBuf<float> nks, nvs;
+  if (!nk.alloc(runs * seq * 128) || !nv.alloc(runs * seq * 128) || !nks.alloc(runs * blocks) || !nvs.alloc(runs * blocks))
+    return false;
+  if (k8_.p && max_seq_ > 0 && used > 0) {
+    const size_t used_blocks = (used + kKv8Block - 1) / kKv8Block, old_blocks = (size_t)max_seq_ / kKv8Block;
+    struct Move {
+      void* to;
+      const void* from;
+      size_t pitch, old_pitch, bytes;
+    } moves[] = {{nk.p, k8_.p, (size_t)seq * 128, (size_t)max_seq_ * 128, used * 128},
+                 {nv.p, v8_.p, (size_t)seq * 128, (size_t)max_seq_ * 128, used * 128},
+                 {nks.p, k8s_.p, blocks * 4, old_blocks * 4, used_blocks * 4},
+                 {nvs.p, v8s_.p, blocks * 4, old_blocks * 4, used_blocks * 4}};
+    for (const Move& m : moves)
+      CUDA_OK(cudaMemcpy2DAsync(m.to, m.pitch, m.from, m.old_pitch, m.bytes, old_runs, cudaMemcpyDeviceToDevice, stream_),
+              false);
+  }
+  CUDA_OK(cudaStreamSynchronize(stream_), false);
+  std::swap(k8_.p, nk.p);
+  std::swap(k8_.n, nk.n);
+  std::swap(v8_.p, nv.p);
+  std::swap(v8_.n, nv.n);
+  std::swap(k8s_.p, nks.p);
+  std::swap(k8s_.n, nks.n);
+  std::swap(v8s_.p, nvs.p);
+  std::swap(v8s_.n, nvs.n);
+  return true;
+}
+
+Kv8 Engine::kv8_at(int slot, int layer, int n_seq) const {
+  const size_t run = ((size_t)slot * cfg_.dec_layers + layer) * cfg_.dec_kv_heads;
+  const size_t blocks = (size_t)max_seq_ / kKv8Block;
+  return Kv8{k8_.p + run * max_seq_ * 128, v8_.p + run * max_seq_ * 128, k8s_.p + run * blocks, v8s_.p + run * blocks,
+             (long long)kv_slot_stride(), (long long)(kv_slot_stride() / 128 / kKv8Block), n_seq, cfg_.dec_kv_heads,
+             max_seq_, 128};
+}
+
+bool Engine::set_kv_mode(KvMode m) {
+  if (m == kv_mode_) return true;
+  cudaSetDevice(device_);
+  CUDA_OK(cudaStreamSynchronize(stream_), false);
+  if (max_seq_ > 0) {
+    const size_t per = (size_t)slots_ * kv_slot_stride();
+    if (m == KV_INT8) {
+      if (!resize_kv8(slots_, max_seq_, 0)) return false;
+    } else if (!kc_.alloc(per) || !vc_.alloc(per)) {
+      kc_.release();
+      vc_.release();
+      return false;
+    }
+  }
+  if (m == KV_INT8) {
+    kc_.release();
+    vc_.release();
+  } else {
+    k8_.release();
+    v8_.release();
+    k8s_.release();
+    v8s_.release();
+  }
+  kv_mode_ = m;
+  kv_len_ = 0;
+  ++graph_gen_;
+  return true;
+}
+
 bool Engine::ensure_slots(int n) {
   if (n <= slots_) return true;
+  if (kv_mode_ == KV_INT8) {
+    if (!resize_kv8(n, max_seq_, (size_t)max_seq_)) return false;
+    slots_ = n;
+    ++graph_gen_;
+    return true;
+  }
   const size_t old = (size_t)slots_ * kv_slot_stride(), per = (size_t)n * kv_slot_stride();
   float *nk = nullptr, *nv = nullptr;
   CUDA_OK(cudaMalloc(&nk, per * 4), false);
@@ -589,6 +671,10 @@ bool Engine::gemm_stage_ok(long fallbacks_before) {
     set_error("tensor-core attention: a device-side wait timed out (code " + std::to_string(e) + ")");
     return false;
   }
+  if (int e = prefill_mode_ == PREFILL_INT8 ? linear_int8_error() : 0) {
+    set_error("int8 product: a device-side wait timed out (code " + std::to_string(e) + ")");
+    return false;
+  }
   if (int e = gemm_tc_error()) {
     set_error("tensor-core GEMM: a device-side wait timed out (code " + std::to_string(e) + ")");
     return false;
@@ -609,17 +695,18 @@ bool Engine::prefill_layers(float* x, int R, const std::vector<RowBlock>& blocks
   const int ldq = qd + 2 * kvd;
   const float scale = 1.0f / sqrtf(128.f);
   if (R <= 0) return true;
-  if (!pl_a_.alloc(split_planes_elems(R, h)) || !pl_b_.alloc(split_planes_elems(R, inter)) ||
-      !pl_c_.alloc(split_planes_elems(R, qd)))
-    return false;
+  const bool i8 = prefill_mode_ == PREFILL_INT8, kv8 = kv_mode_ == KV_INT8;
+  if (!i8 && (!pl_a_.alloc(split_planes_elems(R, h)) || !pl_b_.alloc(split_planes_elems(R, inter)))) return false;
+  if (!pl_c_.alloc(split_planes_elems(R, qd))) return false;
+  if (i8 && (!q8_.alloc((size_t)R * std::max(h, std::max(qd, inter))) || !q8s_.alloc(R))) return false;
   const long long plH = (long long)R * h, plI = (long long)R * inter, plQ = (long long)R * qd;
   const bool simt_att = simt_attention();
   AttnPlan plan;
-  if (!simt_att) {
+  if (!simt_att || kv8) {
     std::vector<AttnBlock> ab;
     for (const RowBlock& bk : blocks)
       if (bk.S > 0) ab.push_back({bk.off, bk.S, bk.start, bk.slot});
-    if (!prefill_attention_plan(ab, c.dec_heads, kv_slot_stride(), stream_, plan)) {
+    if (!kv8 && !prefill_attention_plan(ab, c.dec_heads, kv_slot_stride(), stream_, plan)) {
       set_error("prefill: could not set up the attention work items");
       return false;
     }
@@ -637,13 +724,42 @@ bool Engine::prefill_layers(float* x, int R, const std::vector<RowBlock>& blocks
   }
   for (int l = 0; l < c.dec_layers; ++l) {
     const DecLayerW& L = dec_layers_[l];
+    if (i8) {
+      CUDA_OK(rms_norm_int8(x, h, nullptr, 0, L.n1, c.dec_rms_norm_eps, OPS_F32, R, h, q8_.p, h, q8s_.p, nullptr, 0,
+                            stream_),
+              false);
+      CUDA_OK(linear_int8(q8_.p, h, q8s_.p, L.qqkv, h, L.sqkv, R, ldq, h, LINEAR_STORE, nullptr, 0, pqkv_.p, ldq,
+                          OPS_F32, stream_),
+              false);
+    } else {
     rms_norm_rows(x, pxn_.p, R, h, L.n1, c.dec_rms_norm_eps, stream_, pl_a_.p, plH);
     GemmArgs a;
     a.M = R; a.N = ldq; a.K = h; a.A = pxn_.p; a.lda = h; a.B = L.wqkv; a.ldb = h;
     a.C = pqkv_.p; a.ldc = ldq;
     a.a_split = pl_a_.p; a.a_split_ld = h; a.a_split_plane = plH;
     gemm(a, stream_);
-    if (simt_att) {
+    }
+    if (kv8) {
+      // norm and RoPE of all rows in place, then each sequence's rows into its slot and over it
+      if (!qk_norm_rope_rows(pqkv_.p, R, prow_pos_.p, 1, c.dec_heads, c.dec_kv_heads, L.qn, L.kn, c.dec_rms_norm_eps,
+                             rope_cos_, rope_sin_, stream_)) {
+        set_error("prefill: norm and RoPE launch failed");
+        return false;
+      }
+      launches += 1;
+      for (const RowBlock& bk : blocks) {
+        if (bk.S == 0) continue;
+        const Kv8 cache = kv8_at(bk.slot, l, 1);
+        const int* start = prow_pos_.p + bk.off;
+        const float* q = pqkv_.p + (size_t)bk.off * ldq;
+        CUDA_OK(kv8_append(cache, q + qd, 0, ldq, q + qd + kvd, 0, ldq, OPS_F32, bk.S, start, nullptr, 1, stream_),
+                false);
+        CUDA_OK(kv8_attention(cache, q, 0, ldq, patt_.p + (size_t)bk.off * qd, 0, qd, OPS_F32, bk.S, c.dec_heads,
+                              start, nullptr, 1, scale, 0, stream_, kKv8Splits),
+                false);
+        launches += 2;
+      }
+    } else if (simt_att) {
       for (const RowBlock& bk : blocks) {
         if (bk.S == 0) continue;
         const size_t so = (size_t)bk.slot * kv_slot_stride() + (size_t)l * c.dec_kv_heads * max_seq_ * 128;
@@ -662,7 +778,7 @@ bool Engine::prefill_layers(float* x, int R, const std::vector<RowBlock>& blocks
       launches += 1;
     }
     // every sequence's attention of this layer in one tensor-core launch
-    if (!simt_att) {
+    if (!simt_att && !kv8) {
       if (!prefill_attention_tc(plan, pqkv_.p, c.dec_heads, c.dec_kv_heads, kc_.p, vc_.p,
                                 (long long)l * c.dec_kv_heads * max_seq_ * 128, max_seq_, scale, patt_.p, pl_c_.p,
                                 plQ, stream_)) {
@@ -671,10 +787,28 @@ bool Engine::prefill_layers(float* x, int R, const std::vector<RowBlock>& blocks
       }
       launches += 1;
     }
+    if (i8) {
+      // attention rows -> int8 -> o projection; its sum with x is the next norm's; gate/up; down
+      CUDA_OK(quant_rows_int8(patt_.p, qd, R, qd, q8_.p, qd, q8s_.p, stream_), false);
+      CUDA_OK(linear_int8(q8_.p, qd, q8s_.p, L.qo, qd, L.so, R, h, qd, LINEAR_STORE, nullptr, 0, pxn_.p, h, OPS_F32,
+                          stream_),
+              false);
+      CUDA_OK(rms_norm_int8(x, h, pxn_.p, h, L.n2, c.dec_rms_norm_eps, OPS_F32, R, h, q8_.p, h, q8s_.p, x, h, stream_),
+              false);
+      CUDA_OK(linear_int8(q8_.p, h, q8s_.p, L.qgu, h, L.sgu, R, 2 * inter, h, LINEAR_SWIGLU, nullptr, 0, pmid_.p,
+                          inter, OPS_F32, stream_),
+              false);
+      CUDA_OK(quant_rows_int8(pmid_.p, inter, R, inter, q8_.p, inter, q8s_.p, stream_), false);
+      CUDA_OK(linear_int8(q8_.p, inter, q8s_.p, L.qdown, inter, L.sdown, R, h, inter, LINEAR_RESID, x, h, x, h,
+                          OPS_F32, stream_),
+              false);
+      launches += 8;
+      continue;
+    }
     GemmArgs o;
     o.M = R; o.N = h; o.K = qd; o.A = patt_.p; o.lda = qd; o.B = L.wo; o.ldb = qd;
     o.C = x; o.ldc = h; o.epi = EPI_RESID; o.resid = x; o.ldr = h;
-    if (!simt_att) {
+    if (!simt_att && !kv8) {
       o.a_split = pl_c_.p; o.a_split_ld = qd; o.a_split_plane = plQ;
     }
     gemm(o, stream_);
@@ -903,6 +1037,26 @@ bool Engine::copy_kv(int slot, int layer, int n_pos, float* k, float* v) {
     return false;
   }
   CUDA_OK(cudaStreamSynchronize(stream_), false);
+  if (kv_mode_ == KV_INT8) {
+    const Kv8 cache = kv8_at(slot, layer, 1);
+    const size_t n = (size_t)n_pos * c.dec_kv_heads * 128;
+    DevBuf<float> rows[2];
+    DevBuf<int> zero;
+    const int z = 0;
+    std::vector<float> host(n);
+    if (!rows[0].alloc(n) || !rows[1].alloc(n) || !zero.upload(&z, 1, stream_)) return false;
+    const long long ld = (long long)c.dec_kv_heads * 128;
+    CUDA_OK(kv8_read(cache, rows[0].p, 0, ld, rows[1].p, 0, ld, OPS_F32, n_pos, zero.p, nullptr, 1, stream_), false);
+    CUDA_OK(cudaStreamSynchronize(stream_), false);
+    for (int i = 0; i < 2 && n; ++i) {
+      CUDA_OK(cudaMemcpy(host.data(), rows[i].p, n * 4, cudaMemcpyDeviceToHost), false);
+      for (int p = 0; p < n_pos; ++p)
+        for (int hh = 0; hh < c.dec_kv_heads; ++hh)
+          memcpy((i ? v : k) + ((size_t)hh * n_pos + p) * 128, host.data() + ((size_t)p * c.dec_kv_heads + hh) * 128,
+                 128 * 4);
+    }
+    return true;
+  }
   for (int hh = 0; hh < c.dec_kv_heads; ++hh) {
     const size_t off = (size_t)slot * kv_slot_stride() + ((size_t)layer * c.dec_kv_heads + hh) * max_seq_ * 128;
     CUDA_OK(cudaMemcpy(k + (size_t)hh * n_pos * 128, kc_.p + off, (size_t)n_pos * 128 * 4, cudaMemcpyDeviceToHost),
@@ -973,13 +1127,19 @@ DecodeArgs Engine::dargs(const int* forced, float* logits, int slot) {
   a.lm_w = i8 ? (const void*)lm_q_ : (const void*)lm_bf16_; a.lm_s = lm_s_; a.final_norm = final_norm_;
   a.embed = embed_; a.rope_cos = rope_cos_; a.rope_sin = rope_sin_;
   a.k_cache = kc_.p; a.v_cache = vc_.p; a.layers = c.dec_layers;
+  if (kv_mode_ == KV_INT8) {
+    a.kv8 = kv8_at(slot, 0, 1);
+    a.kv8_layer_stride = (size_t)c.dec_kv_heads * max_seq_ * 128;
+  }
   a.x = dx_.p; a.qkv = dqkv_.p; a.attn = dattn_.p; a.ffn = dffn_.p; a.part = dpart_.p; a.ticket = dticket_.p;
   a.am_ticket = dam_ticket_.p; a.am_part = dam_part_.p; a.st = dstate_.p; a.tokens = dtokens_.p;
   a.staged = dstaged_.p;
   a.kv_slot_stride = kv_slot_stride(); a.tokens_ld = tokens_ld_; a.batch = 1;
   if (slot > 0) {  // one sequence in its own slot: offset the per-sequence buffers
-    a.k_cache += (size_t)slot * kv_slot_stride();
-    a.v_cache += (size_t)slot * kv_slot_stride();
+    if (kv_mode_ == KV_F32) {
+      a.k_cache += (size_t)slot * kv_slot_stride();
+      a.v_cache += (size_t)slot * kv_slot_stride();
+    }
     a.x += (size_t)slot * c.dec_hidden;
     a.st += slot;
     a.tokens += (size_t)slot * tokens_ld_;
@@ -997,7 +1157,8 @@ bool Engine::enqueue_step(const DecodeArgs& a) { return decode_step(a, stream_);
 // qkv+attention, o, gate/up, down per layer, then lm_head (batched steps add a q/k/v matvec)
 int Engine::decode_step_launches_1() const {
   const bool split = decode_split_qkv(cfg_.dec_hidden, cfg_.dec_heads, cfg_.dec_kv_heads, mode_ == DECODE_INT8);
-  return (split ? 5 : 4) * cfg_.dec_layers + 1;
+  const int per_layer = kv_mode_ == KV_INT8 ? 7 : split ? 5 : 4;
+  return per_layer * cfg_.dec_layers + 1;
 }
 
 bool Engine::decode(int max_steps, bool stop_on_eos, std::vector<int>& out, const std::vector<int>* forced,
@@ -1334,7 +1495,7 @@ bool Engine::decode_batch(int B, int max_steps, bool stop_on_eos, std::vector<st
     return false;
   }
   CUDA_OK(cudaGetLastError(), false);
-  launches += (long)launched * (B > 1 ? decode_batched_step_launches(cfg_.dec_layers, mode_ == DECODE_INT8) : decode_step_launches_1());
+  launches += (long)launched * (B > 1 ? decode_batched_step_launches(cfg_.dec_layers, mode_ == DECODE_INT8, kv_mode_ == KV_INT8) : decode_step_launches_1());
   int herr = 0;
   CUDA_OK(cudaMemcpy(&herr, derr_.p, sizeof(int), cudaMemcpyDeviceToHost), false);
   if (herr) {

@@ -32,6 +32,8 @@ struct DecLayerW {
 };
 
 enum DecodeMode { DECODE_INT8 = 0, DECODE_BF16 = 1 };
+enum PrefillMode { PREFILL_BF16 = 0, PREFILL_INT8 = 1 };
+enum KvMode { KV_F32 = 0, KV_INT8 = 1 };
 
 // Per-stage timings of the last call, in milliseconds (CUDA events).
 struct StagePerf {
@@ -113,6 +115,14 @@ class Engine {
     ++graph_gen_;
   }
   DecodeMode decode_mode() const { return mode_; }
+  // Prefill products: bf16 weights times three-plane f32 activations (the reference's f32 sgemm
+  // accuracy), or the decode's int8 weights times int8 rows (ops.h).
+  void set_prefill_mode(PrefillMode m) { prefill_mode_ = m; }
+  PrefillMode prefill_mode() const { return prefill_mode_; }
+  // KV cache in f32 (the reference's), or in int8 with a scale for 16 tokens of a head. A change
+  // empties every slot. false: out of memory, nothing changed.
+  bool set_kv_mode(KvMode m);
+  KvMode kv_mode() const { return kv_mode_; }
   StagePerf perf;
   bool use_graph = true;
   long launches = 0;  // kernels enqueued by this engine (graph replays count their nodes)
@@ -154,6 +164,8 @@ class Engine {
   int device_ = 0;
   cudaStream_t stream_ = nullptr;
   DecodeMode mode_ = DECODE_INT8;
+  PrefillMode prefill_mode_ = PREFILL_BF16;
+  KvMode kv_mode_ = KV_F32;
   std::vector<void*> allocs_;
   void* dalloc(size_t bytes);
   template <typename T>
@@ -185,10 +197,17 @@ class Engine {
   DevBuf<int> win_starts_;
   DevBuf<float> px_, pxn_, pqkv_, patt_, pmid_;
   DevBuf<int> ids_;
+  DevBuf<int8_t> q8_;           // int8 prefill: rows of the next product, and their scales
+  DevBuf<float> q8s_;
   DevBuf<float> mel_keep_, cls_x_, cls_xn_, cls_logits_;
   DevBuf<int> cls_ids_, cls_out_;
   // KV cache [slot][layers][kv][max_seq][128] f32
   DevBuf<float> kc_, vc_;
+  // in KV_INT8 mode instead: the same layout in int8, and scales [slot][layers][kv][max_seq / 16]
+  DevBuf<int8_t> k8_, v8_;
+  DevBuf<float> k8s_, v8s_;
+  bool resize_kv8(int slots, int seq, size_t used);  // moves `used` positions of every row run
+  Kv8 kv8_at(int slot, int layer, int n_seq) const;
   int max_seq_ = 0;
   int kv_len_ = 0;
   int slots_ = 1;

@@ -6,6 +6,8 @@
 #include <cstdint>
 #include <vector>
 
+#include "ops.h"
+
 namespace qasr {
 
 // ---------------------------------------------------------------- GEMM
@@ -165,6 +167,10 @@ void prefill_qk_rope_kv(float* qkv, int S, int start, int n_heads, int n_kv, con
 void prefill_qk_rope_kv_packed(float* qkv, int R, const int* row_pos, const long long* row_kv, int n_heads, int n_kv,
                                const float* qn, const float* kn, float eps, const float* rope_cos,
                                const float* rope_sin, float* kc, float* vc, int max_seq, cudaStream_t s);
+// Per-head RMSNorm + NeoX RoPE of q and k in place, R rows at positions row_pos[r * pos_stride]
+// (the int8 KV cache is written from these rows by kv8_append). false: the launch was refused.
+bool qk_norm_rope_rows(float* qkv, int R, const int* row_pos, int pos_stride, int n_heads, int n_kv, const float* qn,
+                       const float* kn, float eps, const float* rope_cos, const float* rope_sin, cudaStream_t s);
 // Causal GQA attention of S queries at positions start.. over the cache; out [S][n_heads*128].
 void prefill_attention(const float* qkv, int S, int start, int n_heads, int n_kv, const float* kc,
                        const float* vc, int max_seq, float scale, float* out, cudaStream_t s);
@@ -242,6 +248,10 @@ struct DecodeArgs {
   int batch = 1;
   size_t kv_slot_stride = 0;
   int tokens_ld = 0;
+  // Int8 KV cache instead of k_cache / v_cache (null k: the f32 cache): this batch's first slot,
+  // layer 0; a layer is layer_stride further, its scales layer_stride / (16 * 128).
+  Kv8 kv8{};
+  size_t kv8_layer_stride = 0;
   // Batched steps: device buffer of decode_staged_bytes() where each matvec's inputs are
   // staged once (stage_kernel) instead of by every CTA; null stages in every CTA.
   void* staged = nullptr;
@@ -254,7 +264,7 @@ int decode_max_batch(int hidden, int inter, int q_heads, int kv_heads, bool int8
 // (QASR_STAGE_ONCE=0 turns it off); kernels a batched step launches.
 size_t decode_staged_bytes(int hidden, int q_dim, int inter);
 bool decode_stage_once();
-int decode_batched_step_launches(int layers, bool int8);
+int decode_batched_step_launches(int layers, bool int8, bool kv8);
 // Whether a single-sequence step projects q/k/v with a separate matvec (5 kernels per layer).
 bool decode_split_qkv(int hidden, int q_heads, int kv_heads, bool int8);
 // Per-device kernel attributes (dynamic shared memory limits); call once per device.

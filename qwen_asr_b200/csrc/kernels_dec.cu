@@ -68,13 +68,14 @@ __global__ void __launch_bounds__(128) prefill_qk_rope_kv_kernel(float* __restri
                                                                  const float* __restrict__ rs, float* __restrict__ kc,
                                                                  float* __restrict__ vc, int max_seq,
                                                                  const int* __restrict__ row_pos,
-                                                                 const long long* __restrict__ row_kv) {
+                                                                 const long long* __restrict__ row_kv,
+                                                                 int pos_stride = 1) {
   __shared__ float sh[kHd];
   __shared__ float red[4];
   const int row = blockIdx.x, hh = blockIdx.y, d = threadIdx.x;
   const int ld = (n_heads + 2 * n_kv) * kHd;
   // packed rows of several sequences: each row's own position and KV slot offset
-  const int pos = row_pos ? row_pos[row] : start + row;
+  const int pos = row_pos ? row_pos[(size_t)row * pos_stride] : start + row;
   if (row_kv) {
     kc += row_kv[row];
     vc += row_kv[row];
@@ -88,6 +89,10 @@ __global__ void __launch_bounds__(128) prefill_qk_rope_kv_kernel(float* __restri
     int kh = hh - n_heads;
     float v = base[(n_heads + kh) * kHd + d];
     float r = head_norm_rope(v, kn, eps, c, sn, sh, red);
+    if (!kc) {  // no f32 cache: k stays in its row
+      base[(n_heads + kh) * kHd + d] = r;
+      return;
+    }
     size_t off = ((size_t)kh * max_seq + pos) * kHd + d;
     kc[off] = r;
     vc[off] = base[(n_heads + n_kv + kh) * kHd + d];
@@ -110,6 +115,15 @@ void prefill_qk_rope_kv_packed(float* qkv, int R, const int* row_pos, const long
   dim3 grid(R, n_heads + n_kv);
   prefill_qk_rope_kv_kernel<<<grid, 128, 0, s>>>(qkv, 0, n_heads, n_kv, qn, kn, eps, rope_cos, rope_sin, kc, vc,
                                                  max_seq, row_pos, row_kv);
+}
+
+bool qk_norm_rope_rows(float* qkv, int R, const int* row_pos, int pos_stride, int n_heads, int n_kv, const float* qn,
+                       const float* kn, float eps, const float* rope_cos, const float* rope_sin, cudaStream_t s) {
+  if (R <= 0) return true;
+  dim3 grid(R, n_heads + n_kv);
+  prefill_qk_rope_kv_kernel<<<grid, 128, 0, s>>>(qkv, 0, n_heads, n_kv, qn, kn, eps, rope_cos, rope_sin, nullptr,
+                                                 nullptr, 0, row_pos, nullptr, pos_stride);
+  return cudaPeekAtLastError() == cudaSuccess;
 }
 
 // ------------------------------------------------------------------ prefill attention

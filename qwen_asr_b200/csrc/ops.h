@@ -22,6 +22,10 @@ cudaError_t rms_norm_int8(const void* x, long long ldx, const void* residual, lo
                           OpsDtype dt, long long rows, int d, int8_t* q, long long ldq, float* scale, void* h,
                           long long ldh, cudaStream_t s);
 
+// int8 rows of x without a norm: q as above for u = x, scale = top / 127.
+cudaError_t quant_rows_int8(const float* x, long long ldx, long long rows, int d, int8_t* q, long long ldq,
+                            float* scale, cudaStream_t s);
+
 enum LinearEpi { LINEAR_STORE = 0, LINEAR_RESID = 1, LINEAR_SWIGLU = 2 };
 
 // out[m][n] = (sum_k xq[m][k] * wq[n][k]) * xs[m] * ws[n], exact int32 sums; LINEAR_RESID adds
@@ -34,6 +38,7 @@ cudaError_t linear_int8(const int8_t* xq, long long ldx, const float* xs, const 
 // int8 K/V of n_seq sequences: [n_seq][n_kv][capacity][head_dim] with an f32 scale for each
 // block of kKv8Block tokens of a head, [n_seq][n_kv][capacity / kKv8Block].
 constexpr int kKv8Block = 16;
+constexpr int kKv8Splits = 8;  // the engine's decode steps: a sequence's bits do not depend on the batch
 struct Kv8 {
   int8_t *k, *v;
   float *ks, *vs;
@@ -59,10 +64,12 @@ cudaError_t kv8_read(const Kv8& c, void* k_out, long long k_seq, long long k_row
 // out[b][r] = softmax(scale * q[b][r] K^T) V per head over positions 0 .. starts[b] + r;
 // q / out [n_seq][rows][heads * head_dim] (element strides). Rows from counts[b] on, and
 // sequences with a negative start, get zeros. max_len: an upper bound of the positions any row
-// sees (only the launch shape depends on it; <= 0: the capacity).
+// sees (only the launch shape depends on it; <= 0: the capacity). splits: CTAs that share a
+// sequence's length when there are few query rows, 1, 2, 4 or 8 (0: by max_len and the sequences
+// at hand; a fixed number makes a sequence's result independent of the others).
 cudaError_t kv8_attention(const Kv8& c, const void* q, long long q_seq, long long q_row, void* out, long long o_seq,
                           long long o_row, OpsDtype dt, int rows, int heads, const int* starts, const int* counts,
-                          int idx_stride, float scale, int max_len, cudaStream_t s);
+                          int idx_stride, float scale, int max_len, cudaStream_t s, int splits = 0);
 
 // Nonzero once a bounded wait inside linear_int8 gave up on the current device (clears it).
 int linear_int8_error();

@@ -510,7 +510,7 @@ __global__ void __launch_bounds__(kPromptWarps * 32) prompt_kernel(const AttnArg
 }
 
 template <int HD, int PL>
-cudaError_t launch(AttnArgs a, int max_len, cudaStream_t s) {
+cudaError_t launch(AttnArgs a, int max_len, int splits, cudaStream_t s) {
   constexpr int R = WarpState<HD, PL>::kRows;
   const int n_rows = a.rows * a.group;
   if (n_rows > 8 * R) {
@@ -523,8 +523,10 @@ cudaError_t launch(AttnArgs a, int max_len, cudaStream_t s) {
   a.row_tiles = (n_rows + R - 1) / R;
   const long long ctas = (long long)a.c.n_kv * a.row_tiles * a.c.n_seq;
   const int tiles = (max_len + kTok - 1) / kTok;
-  int splits = 1;
-  while (splits < 8 && splits * 2 * kStepWarps <= tiles && ctas * splits < 6LL * ops_sm_count()) splits *= 2;
+  if (splits < 1) {
+    splits = 1;
+    while (splits < 8 && splits * 2 * kStepWarps <= tiles && ctas * splits < 6LL * ops_sm_count()) splits *= 2;
+  }
   static OncePerDevice once;
   const cudaError_t e = once.smem(step_kernel<HD, PL>, step_smem<HD>());
   if (e != cudaSuccess) return e;
@@ -536,13 +538,13 @@ cudaError_t launch(AttnArgs a, int max_len, cudaStream_t s) {
 
 cudaError_t kv8_attention(const Kv8& c, const void* q, long long q_seq, long long q_row, void* out, long long o_seq,
                           long long o_row, OpsDtype dt, int rows, int heads, const int* starts, const int* counts,
-                          int idx_stride, float scale, int max_len, cudaStream_t s) {
+                          int idx_stride, float scale, int max_len, cudaStream_t s, int splits) {
   if (rows <= 0 || c.n_seq <= 0) return cudaSuccess;
   AttnArgs a{c, q, out, q_seq, q_row, o_seq, o_row, starts, counts, idx_stride, rows, heads, heads / c.n_kv, 1, scale};
   if (max_len <= 0 || max_len > c.capacity) max_len = c.capacity;
   if (c.head_dim == 128)
-    return dt == OPS_BF16 ? launch<128, 1>(a, max_len, s) : launch<128, 2>(a, max_len, s);
-  return dt == OPS_BF16 ? launch<64, 1>(a, max_len, s) : launch<64, 2>(a, max_len, s);
+    return dt == OPS_BF16 ? launch<128, 1>(a, max_len, splits, s) : launch<128, 2>(a, max_len, splits, s);
+  return dt == OPS_BF16 ? launch<64, 1>(a, max_len, splits, s) : launch<64, 2>(a, max_len, splits, s);
 }
 
 }  // namespace qasr

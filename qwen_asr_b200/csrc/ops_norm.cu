@@ -53,7 +53,7 @@ struct NormArgs {
   float* scale;
   long long ldx, ldr, ldh, ldq, rows;
   int d;
-  float eps;
+  float eps;  // negative: int8 rows without a norm (w null, scale = top / 127)
 };
 
 // Running row statistics: the sum of squares, and the largest |u| as (f32 rounding, error).
@@ -92,12 +92,17 @@ __device__ __forceinline__ int quant(float h, float w, float r127, const Stat& s
   return (int)t;
 }
 
+__device__ __forceinline__ float scale_of(const NormArgs& a, double top, double ss) {
+  const double rms = a.eps < 0.f ? 1.0 : sqrt(ss / (double)a.d + (double)a.eps);
+  return (float)(top / rms / 127.0);
+}
+
 __device__ __forceinline__ void write_scale(const NormArgs& a, long long row, const Stat& st) {
   float sc = 1.0f;
   if (!st.finite())
     sc = __int_as_float(0x7FFFFFFF);
   else if (st.top)
-    sc = (float)(st.top64() / sqrt(st.ss / (double)a.d + (double)a.eps) / 127.0);
+    sc = scale_of(a, st.top64(), st.ss);
   a.scale[row] = sc;
 }
 
@@ -188,7 +193,7 @@ __global__ void __launch_bounds__(W * 32) norm_vec_kernel(const NormArgs a) {
       if (a.h) *reinterpret_cast<uint4*>((T*)a.h + row * a.ldh + c) = raw[j];
 #pragma unroll
       for (int i = 0; i < V; i += 4) {
-        const float4 w = __ldg(reinterpret_cast<const float4*>(a.w + c + i));
+        const float4 w = a.w ? __ldg(reinterpret_cast<const float4*>(a.w + c + i)) : make_float4(1.f, 1.f, 1.f, 1.f);
         u[j][i] = __fmul_rn(h[j][i], w.x);
         u[j][i + 1] = __fmul_rn(h[j][i + 1], w.y);
         u[j][i + 2] = __fmul_rn(h[j][i + 2], w.z);
@@ -222,7 +227,7 @@ __global__ void __launch_bounds__(W * 32) norm_vec_kernel(const NormArgs a) {
 #pragma unroll
       for (int i = 0; i < V; ++i)
         if (c < a.d && (__float_as_uint(u[j][i]) & 0x7FFFFFFFu) == top) {
-          const float e = __fmaf_rn(h[j][i], a.w[c + i], -u[j][i]);
+          const float e = a.w ? __fmaf_rn(h[j][i], a.w[c + i], -u[j][i]) : 0.f;
           atomicMax(&low, (unsigned)float_to_ordered(u[j][i] < 0.f ? -e : e) ^ 0x80000000u);
         }
     }
@@ -265,7 +270,8 @@ __global__ void __launch_bounds__(W * 32) norm_vec_kernel(const NormArgs a) {
         for (int i = 0; i < V; ++i) {
           // (the row again from memory: an index into the registers would push them all to the stack)
           const T* src = a.h ? (const T*)a.h + row * a.ldh : x;
-          q[c + i] = (int8_t)__double2int_rn((double)Elem<BF16>::load(src + c + i) * (double)a.w[c + i] * 127.0 / top64);
+          const double w = a.w ? (double)a.w[c + i] : 1.0;
+          q[c + i] = (int8_t)__double2int_rn((double)Elem<BF16>::load(src + c + i) * w * 127.0 / top64);
         }
     }
   }
@@ -277,7 +283,7 @@ __global__ void __launch_bounds__(W * 32) norm_vec_kernel(const NormArgs a) {
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0)
       a.scale[row] = !finite ? __int_as_float(0x7FFFFFFF)
-                     : top   ? (float)(top64 / sqrt(sum / (double)a.d + (double)a.eps) / 127.0)
+                     : top   ? scale_of(a, top64, sum)
                              : 1.0f;
   }
 }
@@ -299,13 +305,13 @@ __global__ void __launch_bounds__(512) norm_any_kernel(const NormArgs a) {
     if (r) h = E::round(__fadd_rn(h, E::load(r + c)));
     hrow[c] = h;
     if (a.h) E::store((T*)a.h + row * a.ldh + c, h);
-    st.add(h, a.w[c]);
+    st.add(h, a.w ? a.w[c] : 1.0f);
   }
   row_stat(st, red, warp, lane, 16);
   const float r127 = st.finite() && st.top ? __fdiv_rn(127.0f, __uint_as_float(st.top)) : 0.f;
   const bool tiny = r127 > 3e38f;
   for (int c = threadIdx.x; c < a.d; c += 512) {
-    const float h = hrow[c], w = a.w[c];
+    const float h = hrow[c], w = a.w ? a.w[c] : 1.0f;
     const int v = r127 == 0.f ? 0
                   : tiny      ? __double2int_rn((double)h * (double)w * 127.0 / st.top64())
                               : quant(h, w, r127, st);
@@ -340,16 +346,24 @@ cudaError_t launch(const NormArgs& a, bool vec, cudaStream_t s) {
 
 }  // namespace
 
+static cudaError_t run_rows(const NormArgs& a, OpsDtype dt, cudaStream_t s) {
+  if (a.rows == 0) return cudaSuccess;
+  const int V = dt == OPS_BF16 ? 8 : 4;
+  auto ok = [&](const void* p, long long ld) { return !p || ((uintptr_t)p % 16 == 0 && ld % V == 0); };
+  const bool vec = a.d % V == 0 && ok(a.x, a.ldx) && ok(a.r, a.ldr) && ok(a.h, a.ldh) && (uintptr_t)a.w % 16 == 0 &&
+                   (uintptr_t)a.q % V == 0 && a.ldq % V == 0;
+  return dt == OPS_BF16 ? launch<true>(a, vec, s) : launch<false>(a, vec, s);
+}
+
 cudaError_t rms_norm_int8(const void* x, long long ldx, const void* residual, long long ldr, const float* w, float eps,
                           OpsDtype dt, long long rows, int d, int8_t* q, long long ldq, float* scale, void* h,
                           long long ldh, cudaStream_t s) {
-  if (rows == 0) return cudaSuccess;
-  NormArgs a{x, residual, h, w, q, scale, ldx, ldr, ldh, ldq, rows, d, eps};
-  const int V = dt == OPS_BF16 ? 8 : 4;
-  auto ok = [&](const void* p, long long ld) { return !p || ((uintptr_t)p % 16 == 0 && ld % V == 0); };
-  const bool vec = d % V == 0 && ok(x, ldx) && ok(residual, ldr) && ok(h, ldh) && (uintptr_t)w % 16 == 0 &&
-                   (uintptr_t)q % V == 0 && ldq % V == 0;
-  return dt == OPS_BF16 ? launch<true>(a, vec, s) : launch<false>(a, vec, s);
+  return run_rows(NormArgs{x, residual, h, w, q, scale, ldx, ldr, ldh, ldq, rows, d, eps}, dt, s);
+}
+
+cudaError_t quant_rows_int8(const float* x, long long ldx, long long rows, int d, int8_t* q, long long ldq,
+                            float* scale, cudaStream_t s) {
+  return run_rows(NormArgs{x, nullptr, nullptr, nullptr, q, scale, ldx, 0, 0, ldq, rows, d, -1.0f}, OPS_F32, s);
 }
 
 }  // namespace qasr

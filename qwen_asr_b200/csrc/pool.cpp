@@ -202,6 +202,19 @@ void qwen_asr_pool_set_decode_mode(QwenAsrPool* p, int32_t mode) {
   for (auto& w : p->workers) w->eng->ctx.eng.set_decode_mode(mode == 1 ? qasr::DECODE_BF16 : qasr::DECODE_INT8);
 }
 
+int32_t qwen_asr_pool_set_prefill_mode(QwenAsrPool* p, int32_t mode) {
+  if (!p || (mode != 0 && mode != 1)) return -1;
+  for (auto& w : p->workers) w->eng->ctx.eng.set_prefill_mode(mode == 1 ? qasr::PREFILL_INT8 : qasr::PREFILL_BF16);
+  return 0;
+}
+
+int32_t qwen_asr_pool_set_kv_mode(QwenAsrPool* p, int32_t mode) {
+  if (!p || (mode != 0 && mode != 1)) return -1;
+  for (auto& w : p->workers)
+    if (!w->eng->ctx.set_kv_mode(mode == 1 ? qasr::KV_INT8 : qasr::KV_F32)) return -1;
+  return 0;
+}
+
 void qwen_asr_pool_set_force_n_tokens(QwenAsrPool* p, int32_t n) {
   if (!p) return;
   for (auto& w : p->workers) w->eng->ctx.force_n_tokens = n > 0 ? n : 0;

@@ -62,6 +62,13 @@ int Ctx::stream_slot(StreamState& st, bool& owned) {
   return pick;
 }
 
+bool Ctx::set_kv_mode(KvMode m) {
+  if (m == eng.kv_mode()) return true;
+  if (!eng.set_kv_mode(m)) return false;
+  std::fill(slot_uid.begin(), slot_uid.end(), 0);
+  return true;
+}
+
 bool Ctx::load(const std::string& dir, int device) {
   model_dir = dir;
   const char* q = getenv("QASR_WEIGHT_QUANT");

@@ -104,6 +104,8 @@ class Ctx {
   std::vector<std::vector<int>> last_tokens;  // generated ids per segment / chunk of the last call
 
   bool load(const std::string& dir, int device);
+  // Engine::set_kv_mode; streams prefill from scratch on their next chunk (their rows are gone).
+  bool set_kv_mode(KvMode m);
   bool set_force_language(const std::string& lang);
   void set_prompt(const std::string& p) {
     prompt = p;
