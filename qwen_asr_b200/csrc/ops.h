@@ -38,7 +38,7 @@ cudaError_t linear_int8(const int8_t* xq, long long ldx, const float* xs, const 
 // int8 K/V of n_seq sequences: [n_seq][n_kv][capacity][head_dim] with an f32 scale for each
 // block of kKv8Block tokens of a head, [n_seq][n_kv][capacity / kKv8Block].
 constexpr int kKv8Block = 16;
-constexpr int kKv8Splits = 8;  // the engine's decode steps: a sequence's bits do not depend on the batch
+constexpr int kKv8Splits = 4;  // the engine's decode steps: a sequence's bits do not depend on the batch
 struct Kv8 {
   int8_t *k, *v;
   float *ks, *vs;
@@ -65,7 +65,7 @@ cudaError_t kv8_read(const Kv8& c, void* k_out, long long k_seq, long long k_row
 // q / out [n_seq][rows][heads * head_dim] (element strides). Rows from counts[b] on, and
 // sequences with a negative start, get zeros. max_len: an upper bound of the positions any row
 // sees (only the launch shape depends on it; <= 0: the capacity). splits: CTAs that share a
-// sequence's length when there are few query rows, 1, 2, 4 or 8 (0: by max_len and the sequences
+// sequence's length when there are few query rows, 1, 2, 4, 8 or 16 (0: by max_len and the sequences
 // at hand; a fixed number makes a sequence's result independent of the others).
 cudaError_t kv8_attention(const Kv8& c, const void* q, long long q_seq, long long q_row, void* out, long long o_seq,
                           long long o_row, OpsDtype dt, int rows, int heads, const int* starts, const int* counts,
@@ -86,17 +86,20 @@ inline int ops_sm_count() {
   return v;
 }
 
-// Raises a kernel's dynamic shared memory limit once a device (one object a kernel).
+// Raises a kernel's dynamic shared memory limit, and allows it clusters of 16 CTAs, once a device
+// (one object a kernel).
 struct OncePerDevice {
   std::atomic<unsigned long long> done{0};
   template <typename K>
-  cudaError_t smem(K kernel, int bytes) {
+  cudaError_t smem(K kernel, int bytes, bool clusters16 = false) {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
     if (done.load() & bit) return cudaSuccess;
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && clusters16)
+      e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e == cudaSuccess) done.fetch_or(bit);
     return e;
   }

@@ -17,10 +17,18 @@
 // product, and that of the output columns, are free as long as both operands agree. A thread takes
 // 16 contiguous bytes of a token for both products; V's token pairs are interleaved in registers.
 //
-// Step kernel (few query rows): one cluster per (KV head, row tile, sequence); its CTAs split the
-// sequence's actual length, their warps take tiles in turn, each with its own ring of asynchronous
-// copies and its own softmax state. States are merged in warp order, then in rank order over
-// distributed shared memory: no workspace, no atomics, the same bits every time.
+// Digit kernel (up to four query rows a KV head, so most single tokens): the products stay in
+// integers. A query row is held as three signed 7-bit digits of q / max|q| (2^-22 of the largest),
+// the probabilities as the three bytes of a 23-bit fraction (2^-24 of the largest, by V scale);
+// each digit is a column of its own in m16n8k32 products whose other operand is the cache's bytes:
+// K as it is, V with its 4 x 4 bytes transposed in registers. Two query rows fill eight columns
+// (three digits and one that is not looked at), and sums are exact, so 32 tokens take 16 products
+// and no conversion, against 64 and 350 conversions in f16.
+// Step kernel (few query rows, more than four): the f16 tiles above.
+// In both, one cluster per (KV head, row tile, sequence); its CTAs split the sequence's actual
+// length, their warps take tiles in turn, each with its own ring of asynchronous copies and its own
+// softmax state. States are merged in warp order, then in rank order over distributed shared
+// memory: no workspace, no atomics, the same bits every time.
 // Prompt kernel (many query rows): warps split the rows and share the CTA's ring of K/V tiles.
 //
 // Bound: step - DRAM (the cache is read once per KV head); prompt - the tensor pipe (mma.sync).
@@ -45,6 +53,7 @@ struct AttnArgs {
   const int *starts, *counts;
   int idx_stride, rows, heads, group, row_tiles;
   float scale;
+  int vec;  // q rows start on 16-byte boundaries
 };
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
@@ -68,6 +77,12 @@ __device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16816_zero(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 // Two bytes of w (already x + 128) as f16 values x.
 template <uint32_t SEL>
@@ -269,8 +284,8 @@ struct WarpState {
                               bytes_f16<0x4342>(b1)};
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        float o[4] = {0.f, 0.f, 0.f, 0.f};
-        mma16816(o, p, lo[k], hi[k]);
+        float o[4];
+        mma16816_zero(o, p, lo[k], hi[k]);
         float* d = acc[i * 4 + k];
         if (PL == 2) {
           d[0] = fmaf(o[0] + o[2], vr[0], d[0]);
@@ -437,6 +452,411 @@ __global__ void __launch_bounds__(kStepWarps * 32) step_kernel(const AttnArgs a)
   if (splits > 1) cluster_barrier();  // no CTA leaves while a peer reads its part
 }
 
+// 16 consecutive values of a query row.
+template <bool BF16>
+__device__ __forceinline__ void load16(const AttnArgs& a, long long at, float* f) {
+  if constexpr (BF16) {
+    const __nv_bfloat16* p = (const __nv_bfloat16*)a.q + at;
+    if (a.vec) {
+      bf16x8_to_f32(*reinterpret_cast<const uint4*>(p), f);
+      bf16x8_to_f32(*reinterpret_cast<const uint4*>(p + 8), f + 8);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) f[i] = __bfloat162float(p[i]);
+    }
+  } else {
+    const float* p = (const float*)a.q + at;
+    if (a.vec) {
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        const float4 v = *reinterpret_cast<const float4*>(p + i);
+        f[i] = v.x; f[i + 1] = v.y; f[i + 2] = v.z; f[i + 3] = v.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) f[i] = p[i];
+    }
+  }
+}
+
+// ------------------------------------------------------------------ digit kernel
+constexpr int kMaxSplits = 16;  // CTAs of a cluster (more than 8 need the kernel's leave)
+constexpr int kDigWarps = 4, kDigStages = 3;  // 32 tokens (two tiles) a step
+constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: float of a small int sum
+
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN when either is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// D = A B + C; with C = 1.5 * 2^23 as bits at first, D is the sum as a float, exact below 2^22
+// (128 dims * 127 * 128).
+__device__ __forceinline__ void mma_s8(int* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                       uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_s8u8(int* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// A unit in shared memory: two tiles' K, their V (16 tokens each, chunks permuted as in Tile), k scales, v scales.
+template <int HD>
+struct Unit {
+  static constexpr int kTile = kTok * HD;
+  static constexpr int kBytes = 4 * kTile + 16;
+  static constexpr int kIter = kTile / 512;  // 16-byte copies of a lane for one tile of K or V
+  // This lane's copies go to fixed places: byte lane * 16 + 512 i of a tile is row (lane * 16 + 512 i) / HD.
+  static __device__ void fetch(uint32_t st, const int8_t* k, const int8_t* v, const float* ks, const float* vs,
+                               int tile, int tiles, int lane) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (tile + h >= tiles) break;
+      const long long off = (long long)(tile + h) * kTile + lane * 16;
+#pragma unroll
+      for (int i = 0; i < kIter; ++i) {
+        const int row = i * (512 / HD) + lane / (HD / 16), ch = lane % (HD / 16);
+        cp16(st + h * kTile + Tile<HD>::k_at(row, ch), k + off + i * 512);
+        cp16(st + 2 * kTile + h * kTile + (Tile<HD>::v_at(row, ch) - kTok * HD), v + off + i * 512);
+      }
+      if (lane == 0) cp4(st + 4 * kTile + h * 4, ks + tile + h);
+      if (lane == 1) cp4(st + 4 * kTile + 8 + h * 4, vs + tile + h);
+    }
+  }
+};
+
+// grid (splits, n_kv * row_tiles, n_seq), cluster (splits, 1, 1). RH: pairs of query rows. As operand
+// column, lane (g, t) holds digit g % 4 of row g / 4 of a pair; as result, columns 2t and 2t + 1, so
+// digits 0, 1 (t even) or 2, 3 of row t / 2, whose softmax state it keeps.
+template <int HD, int RH, bool BF16>
+__global__ void __launch_bounds__(kDigWarps * 32, RH == 1 ? 3 : 2) digit_kernel(const AttnArgs a) {
+  constexpr int R = 2 * RH, kNt = HD / 8, kMt = HD / 16, kSteps = HD / 32, kWords = HD / 16;
+  using U = Unit<HD>;
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ float wm[kDigWarps][R], wl[kDigWarps][R], cm[R], cl[R];
+  __shared__ float part[R][HD];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int splits = gridDim.x, rank = blockIdx.x;
+  const int kvh = blockIdx.y / a.row_tiles, row0 = (blockIdx.y % a.row_tiles) * R, seq = blockIdx.z;
+  int start, count;
+  live_rows(a, seq, start, count);
+  const int s_last = min(count - 1, (row0 + R - 1) / a.group);
+  const int len = s_last >= row0 / a.group ? (int)min((long long)start + s_last + 1, (long long)a.c.capacity) : 0;
+  const int tiles = (len + kTok - 1) / kTok, units = (tiles + 1) / 2;
+  const int u0 = (int)((long long)units * rank / splits), u1 = (int)((long long)units * (rank + 1) / splits);
+  const long long blocks = a.c.capacity / kTok;
+  const int8_t* k = a.c.k + seq * a.c.seq_stride + (long long)kvh * a.c.capacity * HD;
+  const int8_t* v = a.c.v + seq * a.c.seq_stride + (long long)kvh * a.c.capacity * HD;
+  const float* ks = a.c.ks + seq * a.c.scale_stride + kvh * blocks;
+  const float* vs = a.c.vs + seq * a.c.scale_stride + kvh * blocks;
+  unsigned char* ring = smem + warp * kDigStages * U::kBytes;
+  const uint32_t ring_a = smem_u32(ring);
+  const int mine = u1 - u0 > warp ? (u1 - u0 - warp + kDigWarps - 1) / kDigWarps : 0;
+#pragma unroll
+  for (int i = 0; i < kDigStages - 1; ++i) {
+    if (i < mine) U::fetch(ring_a + i * U::kBytes, k, v, ks, vs, 2 * (u0 + warp + i * kDigWarps), tiles, lane);
+    cp_commit();
+  }
+
+  const int plane = g & 3, hrow = t >> 1;
+  uint32_t q[RH][kSteps][2];
+  float fac[RH], m[RH], l[RH], vref[RH], rv[RH];
+  int last[RH];
+  int all_see = 0x7FFFFFFF;  // every row of the warp sees up to here
+#pragma unroll
+  for (int h = 0; h < RH; ++h) {
+    const int rr = row0 + 2 * h + (g >> 2), s = rr / a.group;
+    const bool live = s < count;
+    float f[kWords / 4][16];  // 16 dims from t * 16 (+ 64)
+    float mx = 0.f;
+    const long long off = seq * a.q_seq + (long long)s * a.q_row + (long long)(kvh * a.group + rr % a.group) * HD;
+#pragma unroll
+    for (int c = 0; c < kWords / 4; ++c) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) f[c][i] = 0.f;
+      if (live) load16<BF16>(a, off + c * 64 + t * 16, f[c]);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = max_nan(mx, fabsf(f[c][i]));
+    }
+    mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+    mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+    constexpr float kTop = 127.f * 16384.f;
+    const bool fine = mx > 0.f && mx < __int_as_float(0x7F800000);
+    const float factor =
+        mx == 0.f ? 0.f : fine ? mx * (fabsf(a.scale) * (1.4426950408889634f / kTop)) : __int_as_float(0x7FFFFFFF);
+    fac[h] = __shfl_sync(0xffffffffu, factor, 16 * hrow);
+    const float up = mx < 1e-30f ? 1.2676506e30f : 1.f;  // 2^100: kTop / mx stays finite
+    const float inv = fine ? copysignf(__fdiv_rn(kTop, mx * up), a.scale) : 0.f;  // (the factor is positive)
+    // (z + 64 + 64 * 128) >> 14, >> 7, >> 0: the lower digits with 64 added
+    const int sh = plane == 0 ? 14 : plane == 1 ? 7 : 0, mask = plane == 0 ? -1 : 127, less = plane == 0 ? 0 : 64;
+#pragma unroll
+    for (int w = 0; w < kWords; ++w) {
+      uint32_t word = 0u;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int z = fine ? __float2int_rn(f[w >> 2][(w & 3) * 4 + i] * up * inv) : 0;
+        const int d = (((z + 64 + 64 * 128) >> sh) & mask) - less;
+        word |= ((uint32_t)d & 0xFFu) << (8 * i);
+      }
+      q[h][w >> 1][w & 1] = word;
+    }
+    const int sr = (row0 + 2 * h + hrow) / a.group;  // the row whose scores this lane gets
+    last[h] = sr < count ? min(start + sr, a.c.capacity - 1) : -1;
+    all_see = min(all_see, last[h]);
+    m[h] = kNone;
+    l[h] = vref[h] = rv[h] = 0.f;
+  }
+  all_see = __reduce_min_sync(0xffffffffu, all_see);
+  // weights of this lane's two result columns, for the scores and for the output
+  const float wa = t & 1 ? 1.f : 16384.f, wb = t & 1 ? 0.f : 128.f, ba = -kMagic * wa, bb = -kMagic * wb;
+  const float oa = t & 1 ? 1.f : 65536.f, ob = t & 1 ? 0.f : 256.f;
+  // the probabilities' bytes this lane hands out first: digit 0 (t even) or 1; digit 2 is the second
+  const uint32_t sel = t & 1 ? 0x0051u : 0x0062u;
+  const int from = 8 * t + 2 * (g >> 2) + (plane == 1 ? 1 : 0);  // tokens 2t: lane (2t, 2 row + digit)
+
+  // The output so far is sum * vref / (2^23 - 1) + acc: integer sums for the present maximum m and
+  // V scale vref (a power of two), f32 for what came before they last grew. So a step of 32 tokens
+  // neither converts nor rescales anything, unless its maximum or a V scale is a new record.
+  int sum[RH][kMt][4];
+  float acc[RH][kMt][2];
+#pragma unroll
+  for (int h = 0; h < RH; ++h)
+#pragma unroll
+    for (int j = 0; j < kMt; ++j) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum[h][j][i] = 0;
+      acc[h][j][0] = acc[h][j][1] = 0.f;
+    }
+  int since = 0;  // steps since the sums were emptied (2072 of 32 * 255 * 127 fit 31 bits)
+
+  for (int i = 0; i < mine; ++i) {
+    const int nx = i + kDigStages - 1;
+    if (nx < mine)
+      U::fetch(ring_a + nx % kDigStages * U::kBytes, k, v, ks, vs, 2 * (u0 + warp + nx * kDigWarps), tiles, lane);
+    cp_commit();
+    cp_wait<kDigStages - 1>();
+    __syncwarp();
+    const unsigned char* st = ring + i % kDigStages * U::kBytes;
+    const int pos0 = 2 * (u0 + warp + i * kDigWarps) * kTok;
+    const float4 sc = *reinterpret_cast<const float4*>(st + 4 * U::kTile);  // ks, ks, vs, vs
+    // ---- scores x[h][e]: token (e / 2) * 16 + (e % 2) * 8 + g
+    float x[RH][4];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      uint32_t w[2][kWords];
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int c = 0; c < kWords / 4; ++c) {
+          const uint4 w4 = *reinterpret_cast<const uint4*>(st + b * U::kTile + Tile<HD>::k_at(r * 8 + g, t + 4 * c));
+          w[r][4 * c] = w4.x; w[r][4 * c + 1] = w4.y; w[r][4 * c + 2] = w4.z; w[r][4 * c + 3] = w4.w;
+        }
+#pragma unroll
+      for (int h = 0; h < RH; ++h) {
+        int d[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) d[e] = __float_as_int(kMagic);
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j)
+          mma_s8(d, w[0][2 * j], w[1][2 * j], w[0][2 * j + 1], w[1][2 * j + 1], q[h][j][0], q[h][j][1]);
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          // (both products are exact)
+          const float y = fmaf(__int_as_float(d[2 * r]), wa, ba) + fmaf(__int_as_float(d[2 * r + 1]), wb, bb);
+          x[h][2 * b + r] = y + __shfl_xor_sync(0xffffffffu, y, 1);
+        }
+      }
+    }
+    // ---- softmax state
+    const bool partial = pos0 + 2 * kTok - 1 > all_see;
+    float f0[RH], f1[RH], v0[RH], v1[RH], mx[RH];
+    bool grew = ++since > 2048;
+#pragma unroll
+    for (int h = 0; h < RH; ++h) {
+      // a block that the row sees nothing of gives it nothing of its scales either (they may be NaN)
+      const bool see0 = pos0 <= last[h], see1 = pos0 + kTok <= last[h];
+      f0[h] = see0 ? fac[h] * sc.x : 0.f;
+      f1[h] = see1 ? fac[h] * sc.y : 0.f;
+      v0[h] = see0 ? sc.z : 0.f;
+      v1[h] = see1 ? sc.w : 0.f;
+      mx[h] = kNone;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (!partial || pos0 + (e >> 1) * 16 + (e & 1) * 8 + g <= last[h])
+          mx[h] = fmaxf(mx[h], x[h][e] * (e < 2 ? f0[h] : f1[h]));
+#pragma unroll
+      for (int o = 4; o < 32; o *= 2) mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], o));
+      grew |= mx[h] > m[h] || !(v0[h] <= vref[h]) || !(v1[h] <= vref[h]);
+    }
+    if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+      for (int h = 0; h < RH; ++h) {
+        const float mn = fmaxf(m[h], mx[h]), corr = ex2(m[h] - mn), to = vref[h] * (1.f / 8388607.f);
+#pragma unroll
+        for (int j = 0; j < kMt; ++j)
+#pragma unroll
+          for (int o = 0; o < 2; ++o) {
+            const float y = fmaf((float)sum[h][j][2 * o], oa, (float)sum[h][j][2 * o + 1] * ob);
+            acc[h][j][o] = fmaf(y, to, acc[h][j][o]) * corr;
+            sum[h][j][2 * o] = sum[h][j][2 * o + 1] = 0;
+          }
+        l[h] *= corr;
+        m[h] = mn;
+        const float vm = max_nan(v0[h], v1[h]);
+        if (!(vm <= vref[h]))  // to the power of two above it (2^-100 at least), or NaN
+          vref[h] = vm > 0.f ? fmaxf(__uint_as_float((__float_as_uint(vm) + 0x7FFFFFu) & 0xFF800000u), 7.888609e-31f) : vm;
+        rv[h] = vref[h] > 0.f ? __fdiv_rn(8388607.f, vref[h]) : 0.f;
+      }
+      since = 0;
+    }
+    // ---- probabilities as bytes: column (row g / 4, digit g % 4) of tokens 2t, 2t + 1, 2t + 8, 2t + 9 a tile
+    uint32_t pb[RH][2];
+#pragma unroll
+    for (int h = 0; h < RH; ++h) {
+      const float r0 = v0[h] * rv[h], r1 = v1[h] * rv[h];
+      uint32_t z[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float p = ex2(fmaf(x[h][e], e < 2 ? f0[h] : f1[h], -m[h]));
+        // (not by the score: a masked one times a zero scale is no number)
+        if (partial && pos0 + (e >> 1) * 16 + (e & 1) * 8 + g > last[h]) p = 0.f;
+        l[h] += p;
+        z[e] = __float_as_uint(fmaf(p, e < 2 ? r0 : r1, 8388608.f));
+      }
+      const uint32_t first = __byte_perm(__byte_perm(z[0], z[1], sel), __byte_perm(z[2], z[3], sel), 0x5410);
+      const uint32_t second = __byte_perm(__byte_perm(z[0], z[1], 0x0040), __byte_perm(z[2], z[3], 0x0040), 0x5410);
+      const uint32_t a0 = __shfl_sync(0xffffffffu, first, from), a1 = __shfl_sync(0xffffffffu, first, from + 4);
+      const uint32_t c0 = __shfl_sync(0xffffffffu, second, from), c1 = __shfl_sync(0xffffffffu, second, from + 4);
+      const uint32_t w0 = plane >= 2 ? c0 : a0, w1 = plane >= 2 ? c1 : a1;
+      pb[h][0] = __byte_perm(w0, w1, 0x5140);
+      pb[h][1] = __byte_perm(w0, w1, 0x7362);
+    }
+    // ---- V: per tile the same tokens, kNt dims from g * kNt, four at a time
+    constexpr int W = kNt / 4;
+    uint32_t vb[2][W][4];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      uint32_t r[4][W];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int row = 2 * t + (e & 1) + (e >> 1) * 8;
+        const unsigned char* p = st + 2 * U::kTile + b * U::kTile - kTok * HD;
+        if constexpr (HD == 128) {
+          const uint4 w = *reinterpret_cast<const uint4*>(p + Tile<HD>::v_at(row, g));
+          r[e][0] = w.x; r[e][1] = w.y; r[e][2] = w.z; r[e][3] = w.w;
+        } else {
+          const uint2 w = *reinterpret_cast<const uint2*>(p + Tile<HD>::v_at(row, g >> 1) + (g & 1) * 8);
+          r[e][0] = w.x; r[e][1] = w.y;
+        }
+      }
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        const uint32_t x0 = __byte_perm(r[0][w], r[1][w], 0x5140), x1 = __byte_perm(r[0][w], r[1][w], 0x7362);
+        const uint32_t y0 = __byte_perm(r[2][w], r[3][w], 0x5140), y1 = __byte_perm(r[2][w], r[3][w], 0x7362);
+        vb[b][w][0] = __byte_perm(x0, y0, 0x5410);
+        vb[b][w][1] = __byte_perm(x0, y0, 0x7632);
+        vb[b][w][2] = __byte_perm(x1, y1, 0x5410);
+        vb[b][w][3] = __byte_perm(x1, y1, 0x7632);
+      }
+    }
+    // rows g and g + 8 of product j: dims g * kNt + 2j and + 2j + 1
+#pragma unroll
+    for (int j = 0; j < kMt; ++j) {
+      const int e0 = 2 * j, e1 = 2 * j + 1;
+#pragma unroll
+      for (int h = 0; h < RH; ++h)
+        mma_s8u8(sum[h][j], vb[0][e0 >> 2][e0 & 3], vb[0][e1 >> 2][e1 & 3], vb[1][e0 >> 2][e0 & 3],
+                 vb[1][e1 >> 2][e1 & 3], pb[h][0], pb[h][1]);
+    }
+    __syncwarp();
+  }
+  cp_wait<0>();
+
+  // ---- the digits' sums joined, then the warps' states, then the cluster's
+  __syncthreads();  // every ring is idle: it holds the warps' outputs now
+  float* wo = reinterpret_cast<float*>(smem);  // [warp][R][HD]
+  static_assert(kDigWarps * R * HD * 4 <= kDigWarps * kDigStages * U::kBytes, "the warps' outputs reuse the rings");
+#pragma unroll
+  for (int h = 0; h < RH; ++h) {
+#pragma unroll
+    for (int o = 4; o < 32; o *= 2) l[h] += __shfl_xor_sync(0xffffffffu, l[h], o);
+    const int r = 2 * h + hrow;
+    if (g == 0 && !(t & 1)) {
+      wm[warp][r] = m[h];
+      wl[warp][r] = l[h];
+    }
+    const float to = vref[h] * (1.f / 8388607.f);
+#pragma unroll
+    for (int j = 0; j < kMt; ++j) {
+      float y[2];
+#pragma unroll
+      for (int o = 0; o < 2; ++o) {
+        y[o] = fmaf((float)sum[h][j][2 * o], oa, (float)sum[h][j][2 * o + 1] * ob);
+        y[o] = fmaf(y[o], to, acc[h][j][o]);
+        y[o] += __shfl_xor_sync(0xffffffffu, y[o], 1);
+      }
+      wo[(warp * R + r) * HD + g * kNt + 2 * j + (t & 1)] = t & 1 ? y[1] : y[0];
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < R * HD; i += kDigWarps * 32) {
+    const int r = i / HD, d = i % HD;
+    float mm = wm[0][r], ll = 0.f, o = 0.f;
+#pragma unroll
+    for (int w = 1; w < kDigWarps; ++w) mm = fmaxf(mm, wm[w][r]);
+#pragma unroll
+    for (int w = 0; w < kDigWarps; ++w) {
+      const float f = ex2(wm[w][r] - mm);
+      ll = fmaf(wl[w][r], f, ll);
+      o = fmaf(wo[(w * R + r) * HD + d], f, o);
+    }
+    part[r][d] = o;
+    if (d == 0) {
+      cm[r] = mm;
+      cl[r] = ll;
+    }
+  }
+  if (splits > 1)
+    cluster_barrier();
+  else
+    __syncthreads();
+  // warp r finishes query row r, this CTA a share of its dims: the peers' (max, sum) in the lanes
+  const int rr = row0 + warp;
+  if (warp < R && rr < a.rows * a.group) {
+    const bool peer = lane < splits;
+    const float pm = peer ? ld_peer(smem_u32(&cm[warp]), lane) : kNone;
+    const float pl = peer ? ld_peer(smem_u32(&cl[warp]), lane) : 0.f;
+    const float mm = warp_max(pm);
+    float f = ex2(pm - mm);
+    const float ll = warp_sum(pl * f);
+    f = ll == 0.f ? 0.f : __fdiv_rn(f, ll);
+    const int share = HD / splits;
+    for (int d0 = 0; d0 < share; d0 += 32) {
+      const int d = rank * share + d0 + lane;
+      const bool in = d0 + lane < share;
+      float o = 0.f;
+#pragma unroll
+      for (int p = 0; p < kMaxSplits; ++p) {
+        if (p >= splits) break;
+        const float y = in ? ld_peer(smem_u32(&part[warp][d]), p) : 0.f;
+        o = fmaf(y, __shfl_sync(0xffffffffu, f, p), o);
+      }
+      if (in)
+        put(a.out,
+            seq * a.o_seq + (long long)(rr / a.group) * a.o_row + (long long)(kvh * a.group + rr % a.group) * HD + d, o,
+            BF16);
+    }
+  }
+  __syncwarp();
+  if (splits > 1) cluster_barrier();  // no CTA leaves while a peer reads its part
+}
+
 // ------------------------------------------------------------------ prompt kernel
 constexpr int kPromptWarps = 8, kPromptTiles = 4, kPromptStages = 2;  // 64 tokens a stage
 template <int HD>
@@ -509,10 +929,39 @@ __global__ void __launch_bounds__(kPromptWarps * 32) prompt_kernel(const AttnArg
   }
 }
 
+// CTAs that share a sequence's length, for `ctas` CTAs unsplit: powers of two while all of them run
+// at once (two an SM) and each keeps 256 tokens; between one and two CTAs an SM two, because lengths
+// differ. 16 KV heads x tokens, measured (us) at 1 / 2 / 4 / 8 splits: 8 CTAs of 436 tokens 7.8 / 6.8 /
+// 6.2 / 6.8; 8 of 32000 186 / 96 / 51 / 30; 64 of 436 8.0 / 7.2 / 7.2 / 14.3; 256 of 0 to 8191 66 / 55 /
+// 61 / 91; 256 of 8191 91 / 89 / 98 / 122; 1024 of 1000 57 / 77 / 116 / 222.
+int auto_splits(long long ctas, int max_len) {
+  const long long room = 2LL * ops_sm_count();
+  int splits = 1;
+  while (splits < kMaxSplits && splits * 512 <= max_len && ctas * splits * 2 <= room) splits *= 2;
+  if (splits == 1 && ctas > room / 2 && ctas <= room && max_len >= 1024) splits = 2;
+  return splits;
+}
+
+template <int HD, int RH, bool BF16>
+cudaError_t launch_digit(AttnArgs a, int max_len, int splits, cudaStream_t s) {
+  constexpr int kSmem = kDigWarps * kDigStages * Unit<HD>::kBytes;
+  a.row_tiles = (a.rows * a.group + 2 * RH - 1) / (2 * RH);
+  const long long ctas = (long long)a.c.n_kv * a.row_tiles * a.c.n_seq;
+  if (splits < 1) splits = auto_splits(ctas, max_len);
+  static OncePerDevice once;
+  const cudaError_t e = once.smem(digit_kernel<HD, RH, BF16>, kSmem, true);
+  if (e != cudaSuccess) return e;
+  return ops_launch(digit_kernel<HD, RH, BF16>, dim3(splits, a.c.n_kv * a.row_tiles, a.c.n_seq), dim3(kDigWarps * 32),
+                    kSmem, s, splits, a);
+}
+
 template <int HD, int PL>
 cudaError_t launch(AttnArgs a, int max_len, int splits, cudaStream_t s) {
   constexpr int R = WarpState<HD, PL>::kRows;
   const int n_rows = a.rows * a.group;
+  if (n_rows <= 2) return launch_digit<HD, 1, PL == 1>(a, max_len, splits, s);
+  // (8 rows as two digit tiles: 170 us for 32 x 8191 tokens, one f16 tile 147 us)
+  if (n_rows <= 4) return launch_digit<HD, 2, PL == 1>(a, max_len, splits, s);
   if (n_rows > 8 * R) {
     const dim3 g((n_rows + R * kPromptWarps - 1) / (R * kPromptWarps), a.c.n_kv, a.c.n_seq);
     static OncePerDevice once;
@@ -522,13 +971,9 @@ cudaError_t launch(AttnArgs a, int max_len, int splits, cudaStream_t s) {
   }
   a.row_tiles = (n_rows + R - 1) / R;
   const long long ctas = (long long)a.c.n_kv * a.row_tiles * a.c.n_seq;
-  const int tiles = (max_len + kTok - 1) / kTok;
-  if (splits < 1) {
-    splits = 1;
-    while (splits < 8 && splits * 2 * kStepWarps <= tiles && ctas * splits < 6LL * ops_sm_count()) splits *= 2;
-  }
+  if (splits < 1) splits = auto_splits(ctas, max_len);
   static OncePerDevice once;
-  const cudaError_t e = once.smem(step_kernel<HD, PL>, step_smem<HD>());
+  const cudaError_t e = once.smem(step_kernel<HD, PL>, step_smem<HD>(), true);
   if (e != cudaSuccess) return e;
   return ops_launch(step_kernel<HD, PL>, dim3(splits, a.c.n_kv * a.row_tiles, a.c.n_seq), dim3(kStepWarps * 32),
                     step_smem<HD>(), s, splits, a);
@@ -540,7 +985,9 @@ cudaError_t kv8_attention(const Kv8& c, const void* q, long long q_seq, long lon
                           long long o_row, OpsDtype dt, int rows, int heads, const int* starts, const int* counts,
                           int idx_stride, float scale, int max_len, cudaStream_t s, int splits) {
   if (rows <= 0 || c.n_seq <= 0) return cudaSuccess;
-  AttnArgs a{c, q, out, q_seq, q_row, o_seq, o_row, starts, counts, idx_stride, rows, heads, heads / c.n_kv, 1, scale};
+  AttnArgs a{c, q, out, q_seq, q_row, o_seq, o_row, starts, counts, idx_stride, rows, heads, heads / c.n_kv, 1, scale, 0};
+  const int es = dt == OPS_BF16 ? 2 : 4;
+  a.vec = (uintptr_t)q % 16 == 0 && q_seq * es % 16 == 0 && q_row * es % 16 == 0;
   if (max_len <= 0 || max_len > c.capacity) max_len = c.capacity;
   if (c.head_dim == 128)
     return dt == OPS_BF16 ? launch<128, 1>(a, max_len, splits, s) : launch<128, 2>(a, max_len, splits, s);

@@ -332,11 +332,12 @@ def filled_cache(ops, n, n_kv, cap, hd, lens, seed=0, kstd=1.0):
 
 def attention_ref(q, c, starts, counts, scale, f32_planes):
     """(out, tolerance) in 64 bits. Tolerance of one output, relative to the head's largest |v|:
-      the scores' error d: q is held to 2^-25 of its row's largest value in each of two planes, and the
-        product, sum, factor and exponential of an f32 path are off by a few 2^-24 of sum |q k|: in all
-        under 2^-21 * (scale * max|q| * max_t sum |k_t|), and the probabilities by that much; twice, for
+      the scores' error d: q is held to 2^-25 of its row's largest value in each of two planes or to 2^-22
+        in digits, and the product, sum, factor and exponential of an f32 path are off by a few 2^-24 of
+        sum |q k|: in all under 2^-21 * (scale * max|q| * max_t sum |k_t|), and the probabilities by that much; twice, for
         numerator and denominator;
-      the probabilities' planes: 2^-25 of the largest for each key (len * 2^-25 / l), one plane: 2^-11 of each;
+      the probabilities: f16 planes hold them to 2^-25 of the largest, bytes of a 23-bit fraction to 2^-24,
+        for each key (len * 2^-24 / l); one f16 plane (bf16 rows): 2^-11 of each;
       the sums: 2^-23 for each tile of 16 tokens (f32 accumulation, rescaling), and 2^-22 for the end."""
     k, v, ks, vs = c
     n, rows, heads, hd = q.shape
@@ -357,7 +358,7 @@ def attention_ref(q, c, starts, counts, scale, f32_planes):
             l = p.sum(1)
             out[b, r] = (p[:, None] @ vv)[:, 0] / l[:, None]
             d = 2 * 2.0 ** -21 * scale * qq.abs().amax(1) * kk.abs().sum(2).amax(1)
-            planes = L * 2.0 ** -25 / l + (0 if f32_planes else 2.0 ** -11)
+            planes = L * 2.0 ** -24 / l + (0 if f32_planes else 2.0 ** -11)
             t = (d + planes + (L // 16 + 1) * 2.0 ** -23 + 2.0 ** -22) * vv.abs().amax((1, 2))
             tol[b, r] = t[:, None] + out[b, r].abs() * HALF[q.dtype]
     return out, tol
