@@ -105,7 +105,9 @@ struct OncePerDevice {
   }
 };
 
-// Launch, optionally in clusters of `cluster` CTAs along x.
+// Launch, optionally in clusters of `cluster` CTAs along x, with programmatic dependence on the
+// stream's previous kernel: the CTAs may start while it ends, so every kernel launched here waits
+// (pdl_wait) before it touches global memory, and lets its own successor start early in turn.
 template <typename K, typename... A>
 inline cudaError_t ops_launch(K kernel, dim3 grid, dim3 block, size_t smem, cudaStream_t s, int cluster,
                               const A&... args) {
@@ -114,14 +116,17 @@ inline cudaError_t ops_launch(K kernel, dim3 grid, dim3 block, size_t smem, cuda
   cfg.blockDim = block;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
   if (cluster > 1) {
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = cluster;
-    at[0].val.clusterDim.y = 1;
-    at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = cluster;
+    at[1].val.clusterDim.y = 1;
+    at[1].val.clusterDim.z = 1;
+    cfg.numAttrs = 2;
   }
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }

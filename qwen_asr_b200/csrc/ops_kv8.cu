@@ -16,6 +16,7 @@
 // Bound: latency for a token (one pass of 128 CTAs for 8 sequences of 8 heads), DRAM for prompts.
 #include <cuda_bf16.h>
 
+#include "bulk.cuh"
 #include "dev_util.cuh"
 #include "ops.h"
 
@@ -80,6 +81,8 @@ __global__ void __launch_bounds__(128) append_kernel(const AppendArgs a) {
   __shared__ unsigned red[4];
   const int seq = blockIdx.z, head = blockIdx.y >> 1;
   const bool is_v = blockIdx.y & 1;
+  pdl_launch_dependents();
+  pdl_wait();
   const int start = a.starts[(long long)seq * a.idx_stride];
   int count = a.rows;
   if (a.counts) count = min(max(a.counts[(long long)seq * a.idx_stride], 0), a.rows);
@@ -149,6 +152,8 @@ __global__ void __launch_bounds__(256) read_kernel(const ReadArgs a) {
   const bool is_v = blockIdx.y;
   void* out = is_v ? a.v : a.k;
   if (!out) return;
+  pdl_launch_dependents();
+  pdl_wait();
   const int start = a.starts[(long long)seq * a.idx_stride];
   int count = a.rows;
   if (a.counts) count = min(max(a.counts[(long long)seq * a.idx_stride], 0), a.rows);

@@ -325,8 +325,10 @@ __device__ __forceinline__ float ld_peer(uint32_t addr, int rank) {
   return v;
 }
 
-// A sequence's first position (at most the capacity) and live rows.
+// A sequence's first position (at most the capacity) and live rows: a kernel's first reads.
 __device__ __forceinline__ void live_rows(const AttnArgs& a, int seq, int& start, int& count) {
+  pdl_launch_dependents();
+  pdl_wait();
   start = a.starts[(long long)seq * a.idx_stride];
   count = a.rows;
   if (a.counts) count = min(max(a.counts[(long long)seq * a.idx_stride], 0), a.rows);

@@ -20,6 +20,7 @@
 // per-value conversions, @NORM_MANY@ so.
 #include <cuda_bf16.h>
 
+#include "bulk.cuh"
 #include "dev_util.cuh"
 #include "ops.h"
 
@@ -155,6 +156,8 @@ __global__ void __launch_bounds__(W * 32) norm_vec_kernel(const NormArgs a) {
   __shared__ unsigned low;  // ordered bits of the largest product's rounding error
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long row = blockIdx.x;
+  pdl_launch_dependents();
+  pdl_wait();
   const T* x = (const T*)a.x + row * a.ldx;
   uint4 raw[NV];
 #pragma unroll
@@ -298,6 +301,8 @@ __global__ void __launch_bounds__(512) norm_any_kernel(const NormArgs a) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long row = blockIdx.x;
   const T* x = (const T*)a.x + row * a.ldx;
+  pdl_launch_dependents();
+  pdl_wait();
   const T* r = a.r ? (const T*)a.r + row * a.ldr : nullptr;
   Stat st;
   for (int c = threadIdx.x; c < a.d; c += 512) {
