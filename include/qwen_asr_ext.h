@@ -296,8 +296,8 @@ int32_t qwen_asr_kv8_read(const QwenAsrKv8* cache, const QwenAsrRows* k_out, con
 int32_t qwen_asr_kv8_attention(const QwenAsrKv8* cache, const QwenAsrRows* q, const QwenAsrRows* out, int32_t dtype,
                                int32_t rows, int32_t heads, const int32_t* starts, const int32_t* counts,
                                int32_t index_stride, float scale, int32_t max_len, int32_t device, void* stream);
-/* Nonzero (and cleared) when a bounded wait inside qwen_asr_linear_int8 gave up on `device`: its
- * output is not to be used. Waits for the device. */
+/* Nonzero (and cleared) when a bounded wait inside qwen_asr_linear_int8 or qwen_asr_kv8_attention
+ * gave up on `device`: outputs since the last query are not to be used. Waits for the device. */
 int32_t qwen_asr_ops_error(int32_t device);
 
 #ifdef __cplusplus

@@ -675,6 +675,10 @@ bool Engine::gemm_stage_ok(long fallbacks_before) {
     set_error("int8 product: a device-side wait timed out (code " + std::to_string(e) + ")");
     return false;
   }
+  if (int e = kv_mode_ == KV_INT8 ? kv8_prompt_error() : 0) {
+    set_error("int8 KV attention: a device-side wait timed out (code " + std::to_string(e) + ")");
+    return false;
+  }
   if (int e = gemm_tc_error()) {
     set_error("tensor-core GEMM: a device-side wait timed out (code " + std::to_string(e) + ")");
     return false;

@@ -230,7 +230,9 @@ int32_t qwen_asr_kv8_attention(const QwenAsrKv8* cache, const QwenAsrRows* q, co
 
 int32_t qwen_asr_ops_error(int32_t device) {
   DeviceScope scope(device);
-  return scope.ok() ? linear_int8_error() : -1;
+  if (!scope.ok()) return -1;
+  const int e = linear_int8_error(), p = kv8_prompt_error();
+  return e ? e : p;
 }
 
 }  // extern "C"

@@ -29,9 +29,9 @@
 // length, their warps take tiles in turn, each with its own ring of asynchronous copies and its own
 // softmax state. States are merged in warp order, then in rank order over distributed shared
 // memory: no workspace, no atomics, the same bits every time.
-// Prompt kernel (many query rows): warps split the rows and share the CTA's ring of K/V tiles.
+// More than 64 rows a KV head take the tcgen05 kernel of ops_kv8_prompt.cu.
 //
-// Bound: step - DRAM (the cache is read once per KV head); prompt - the tensor pipe (mma.sync).
+// Bound: DRAM (the cache is read once per KV head and row tile) or, for short lengths, latency.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -43,6 +43,7 @@ namespace qasr {
 namespace {
 
 constexpr int kTok = kKv8Block;  // tokens of a tile
+constexpr int kStepRows = 64;    // query rows of a KV head up to which its length is split
 constexpr float kNone = -1.0e30f;  // running maximum before any key (finite: differences stay defined)
 
 struct AttnArgs {
@@ -859,78 +860,6 @@ __global__ void __launch_bounds__(kDigWarps * 32, RH == 1 ? 3 : 2) digit_kernel(
   if (splits > 1) cluster_barrier();  // no CTA leaves while a peer reads its part
 }
 
-// ------------------------------------------------------------------ prompt kernel
-constexpr int kPromptWarps = 8, kPromptTiles = 4, kPromptStages = 2;  // 64 tokens a stage
-template <int HD>
-constexpr int prompt_smem() {
-  return kPromptStages * kPromptTiles * Tile<HD>::kBytes;
-}
-
-// grid (row tiles of kPromptWarps * kRows, n_kv, n_seq)
-template <int HD, int PL>
-__global__ void __launch_bounds__(kPromptWarps * 32) prompt_kernel(const AttnArgs a) {
-  using S = WarpState<HD, PL>;
-  constexpr int R = S::kRows, CR = R * kPromptWarps, N = kPromptWarps * 32;
-  extern __shared__ __align__(128) unsigned char smem[];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int kvh = blockIdx.y, seq = blockIdx.z;
-  // the last rows see the most keys: they start first
-  const int base = (gridDim.x - 1 - blockIdx.x) * CR, row0 = base + warp * R;
-  int start, count;
-  live_rows(a, seq, start, count);
-  auto tokens = [&](int r_first, int r_last) {  // tokens that query rows r_first .. r_last see
-    const int s_last = min(count - 1, r_last / a.group);
-    return s_last >= r_first / a.group ? (int)min((long long)start + s_last + 1, (long long)a.c.capacity) : 0;
-  };
-  const int tiles = (tokens(base, base + CR - 1) + kTok - 1) / kTok;
-  const int own_tiles = (tokens(row0, row0 + R - 1) + kTok - 1) / kTok;
-  const long long blocks = a.c.capacity / kTok;
-  const int8_t* k = a.c.k + seq * a.c.seq_stride + (long long)kvh * a.c.capacity * HD;
-  const int8_t* v = a.c.v + seq * a.c.seq_stride + (long long)kvh * a.c.capacity * HD;
-  const float* ks = a.c.ks + seq * a.c.scale_stride + kvh * blocks;
-  const float* vs = a.c.vs + seq * a.c.scale_stride + kvh * blocks;
-  const uint32_t ring_a = smem_u32(smem);
-  constexpr int kStage = kPromptTiles * Tile<HD>::kBytes;
-  const int stages = (tiles + kPromptTiles - 1) / kPromptTiles;
-  auto fetch = [&](int i) {
-    for (int b = 0; b < kPromptTiles; ++b) {
-      const int tl = i * kPromptTiles + b;
-      if (tl < tiles)
-        Tile<HD>::fetch(ring_a + (i % kPromptStages) * kStage + b * Tile<HD>::kBytes, k, v, ks, vs, tl, threadIdx.x, N);
-    }
-  };
-  if (stages > 0) fetch(0);
-  cp_commit();
-  S st;
-  st.init(a, seq, kvh, row0, start, count, PL == 1);
-  for (int i = 0; i < stages; ++i) {
-    if (i + 1 < stages) fetch(i + 1);
-    cp_commit();
-    cp_wait<1>();
-    __syncthreads();
-    for (int b = 0; b < kPromptTiles; ++b) {
-      const int tl = i * kPromptTiles + b;
-      if (tl < own_tiles) st.tile(smem + (i % kPromptStages) * kStage + b * Tile<HD>::kBytes, tl * kTok);
-    }
-    __syncthreads();
-  }
-  st.finish_sum();
-  const int n_rows = a.rows * a.group;
-#pragma unroll
-  for (int h = 0; h < S::kR; ++h) {
-    const int rr = row0 + g + h * 8;
-    if (rr >= n_rows) continue;
-    const float inv = st.l[h] == 0.f ? 0.f : __fdiv_rn(1.0f, st.l[h]);
-    const long long o = seq * a.o_seq + (long long)(rr / a.group) * a.o_row +
-                        (long long)(kvh * a.group + rr % a.group) * HD;
-#pragma unroll
-    for (int j = 0; j < S::kNt; ++j)
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-        put(a.out, o + S::out_dim(2 * t + e, j), __fmul_rn(st.acc[j][2 * h + e], inv), PL == 1);
-  }
-}
-
 // CTAs that share a sequence's length, for `ctas` CTAs unsplit: powers of two while all of them run
 // at once (two an SM) and each keeps 256 tokens; between one and two CTAs an SM two, because lengths
 // differ. 16 KV heads x tokens, measured (us) at 1 / 2 / 4 / 8 splits: 8 CTAs of 436 tokens 7.8 / 6.8 /
@@ -964,13 +893,6 @@ cudaError_t launch(AttnArgs a, int max_len, int splits, cudaStream_t s) {
   if (n_rows <= 2) return launch_digit<HD, 1, PL == 1>(a, max_len, splits, s);
   // (8 rows as two digit tiles: 170 us for 32 x 8191 tokens, one f16 tile 147 us)
   if (n_rows <= 4) return launch_digit<HD, 2, PL == 1>(a, max_len, splits, s);
-  if (n_rows > 8 * R) {
-    const dim3 g((n_rows + R * kPromptWarps - 1) / (R * kPromptWarps), a.c.n_kv, a.c.n_seq);
-    static OncePerDevice once;
-    const cudaError_t e = once.smem(prompt_kernel<HD, PL>, prompt_smem<HD>());
-    if (e != cudaSuccess) return e;
-    return ops_launch(prompt_kernel<HD, PL>, g, dim3(kPromptWarps * 32), prompt_smem<HD>(), s, 1, a);
-  }
   a.row_tiles = (n_rows + R - 1) / R;
   const long long ctas = (long long)a.c.n_kv * a.row_tiles * a.c.n_seq;
   if (splits < 1) splits = auto_splits(ctas, max_len);
@@ -987,6 +909,9 @@ cudaError_t kv8_attention(const Kv8& c, const void* q, long long q_seq, long lon
                           long long o_row, OpsDtype dt, int rows, int heads, const int* starts, const int* counts,
                           int idx_stride, float scale, int max_len, cudaStream_t s, int splits) {
   if (rows <= 0 || c.n_seq <= 0) return cudaSuccess;
+  if ((long long)rows * (heads / c.n_kv) > kStepRows)
+    return kv8_prompt_attention(c, q, q_seq, q_row, out, o_seq, o_row, dt, rows, heads, starts, counts, idx_stride,
+                                scale, s);
   AttnArgs a{c, q, out, q_seq, q_row, o_seq, o_row, starts, counts, idx_stride, rows, heads, heads / c.n_kv, 1, scale, 0};
   const int es = dt == OPS_BF16 ? 2 : 4;
   a.vec = (uintptr_t)q % 16 == 0 && q_seq * es % 16 == 0 && q_row * es % 16 == 0;

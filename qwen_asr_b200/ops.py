@@ -298,9 +298,9 @@ def kv8_attention(q, cache: Kv8Cache, starts, counts=None, scale: float | None =
 
 
 def check(device=None) -> None:
-    """Raises RuntimeError when a bounded wait inside linear_int8 gave up since the last check (its
-    output is then not to be used). Waits for the device."""
+    """Raises RuntimeError when a bounded wait inside linear_int8 or kv8_attention gave up since the
+    last check (outputs since then are not to be used). Waits for the device."""
     index = torch.cuda.current_device() if device is None else torch.device(device).index
     e = lib().qwen_asr_ops_error(-1 if index is None else index)
     if e:
-        raise RuntimeError(f"linear_int8: a device-side wait timed out (code {e})")
+        raise RuntimeError(f"8-bit operators: a device-side wait timed out (code {e})")
