@@ -177,11 +177,14 @@ struct WarpState {
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
       int e = 0;
       if (mx > 0.f && mx < __int_as_float(0x7F800000)) frexpf(mx, &e);
-      fac[h] = scalbnf(a.scale * 1.4426950408889634f, e);
+      // 2^-e and 2^e as two exact factors each (one alone can leave f32's normal range)
+      const int e1 = e / 2, e2 = e - e1;
+      const float d1 = __int_as_float((127 - e1) << 23), d2 = __int_as_float((127 - e2) << 23);
+      fac[h] = a.scale * 1.4426950408889634f * __int_as_float((127 + e1) << 23) * __int_as_float((127 + e2) << 23);
 #pragma unroll
       for (int j = 0; j < kSteps; ++j) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) f[j][i] = scalbnf(f[j][i], -e);
+        for (int i = 0; i < 4; ++i) f[j][i] = f[j][i] * d1 * d2;
         const uint32_t h0 = pack_f16(f[j][0], f[j][1]), h1 = pack_f16(f[j][2], f[j][3]);
         q[j][h] = h0;
         q[j][2 + h] = h1;

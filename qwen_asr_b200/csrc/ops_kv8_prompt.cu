@@ -16,10 +16,13 @@
 // m is only raised when a score exceeds it by 2^8 (p up to 256 is as exact in f16): O is then
 // rescaled in TMEM, which the first blocks of a row do and later ones hardly ever.
 //
-// Roles (288 threads, two CTAs an SM, so that one's softmax runs beside the other's products):
-// warps 0-3 softmax, a thread a row; warps 4-7 bring K and V from global memory as int8, one block
-// ahead in registers, and write them as f16 rows of a token in the 128-byte-swizzle layout, which is
-// K-major for Q K^T and MN-major for P V; one thread of warp 8 issues the products: Q K^T of the next block before P V of this one.
+// Roles (256 threads, two CTAs an SM, so that one's softmax runs beside the other's products): warps
+// 0-3 softmax, a thread a row; warps 4-6 bring K and V from global memory as int8, one block ahead in
+// registers, and write them as f16 rows of a token in the 128-byte-swizzle layout, which is K-major for
+// Q K^T and MN-major for P V; one thread of warp 7 issues the products, Q K^T of the next block before
+// P V of this one. (Issuing takes as long as the products do, 48 cycles each at N = 64 and 64 at N = 128,
+// so a softmax thread that did it kept its warp waiting: 3.1 us a block instead of 1.8.) K has two
+// buffers, so that its conversion runs beside the products of the block before.
 //
 // Bound: f32 rows - the tensor pipe (four products of 128 x 64 x head_dim a block), bf16 rows - exp2
 // and the conversions around it.
@@ -33,7 +36,7 @@
 namespace qasr {
 namespace {
 
-constexpr int kRows = 128, kKeys = 64, kThreads = 288;
+constexpr int kRows = 128, kKeys = 64, kThreads = 256, kFill = 96;  // (threads that bring K and V)
 constexpr float kNone = -1.0e30f;
 constexpr uint32_t kColS = 0, kColP = 64, kColO = 128, kCols = 256;  // TMEM columns
 
@@ -53,7 +56,8 @@ struct PromptArgs {
 template <int HD, int PL>
 struct Smem {
   static constexpr int kPlane = kRows * HD * 2, kK = kKeys * HD * 2, kV = kK;
-  static constexpr int kBytes = 1024 + PL * kPlane + kK + kV + 256;
+  // Q, two K, V, then 1024 bytes of rows' factors, V scales and barriers: two f32 CTAs fill an SM
+  static constexpr int kBytes = PL * kPlane + 2 * kK + kV + 1024;
 };
 
 // 128-byte swizzle, 8-row groups 1024 bytes apart; lead: bytes from 64 columns to the next (MN-major)
@@ -196,74 +200,104 @@ __device__ __forceinline__ uint32_t bytes_f16(uint32_t w) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Bounded wait of a whole warp, which leaves it converged (and of one mind).
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int code) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, &g_prompt_err, code));
+// Bounded wait. Once one gave up nobody waits any more: the warps run through what is left of their
+// loops, with the barriers between them, and leave an output that the error code disowns.
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile int* gave_up, int code) {
+  if (*gave_up) return false;
+  if (mbar_wait(bar, parity, &g_prompt_err, code)) return true;
+  *gave_up = 1;
+  return false;
 }
 
-// 8 values of a query row.
-template <bool BF16>
-__device__ __forceinline__ void load8(const PromptArgs& a, long long at, float* f) {
-  if constexpr (BF16) {
-    const __nv_bfloat16* p = (const __nv_bfloat16*)a.q + at;
-    if (a.q_vec) {
-      bf16x8_to_f32(*reinterpret_cast<const uint4*>(p), f);
-    } else {
+// N (4 or 2) neighbouring values of a query row, as loaded: converted later, so that no load waits for
+// the one before.
+template <bool BF16, int N>
+struct LaneValues {
+  uint32_t w[BF16 ? N / 2 : N];
+  __device__ __forceinline__ void load(const PromptArgs& a, long long at) {
+    if constexpr (BF16) {
+      const uint16_t* p = (const uint16_t*)a.q + at;
+      if (a.q_vec) {
+        if constexpr (N == 4) {
+          const uint2 v = *reinterpret_cast<const uint2*>(p);
+          w[0] = v.x; w[1] = v.y;
+        } else {
+          w[0] = *reinterpret_cast<const uint32_t*>(p);
+        }
+      } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = __bfloat162float(p[i]);
-    }
-  } else {
-    const float* p = (const float*)a.q + at;
-    if (a.q_vec) {
-      const float4 x = *reinterpret_cast<const float4*>(p), y = *reinterpret_cast<const float4*>(p + 4);
-      f[0] = x.x; f[1] = x.y; f[2] = x.z; f[3] = x.w;
-      f[4] = y.x; f[5] = y.y; f[6] = y.z; f[7] = y.w;
+        for (int i = 0; i < N / 2; ++i) w[i] = (uint32_t)p[2 * i] | (uint32_t)p[2 * i + 1] << 16;
+      }
     } else {
+      const uint32_t* p = (const uint32_t*)a.q + at;
+      if (a.q_vec) {
+        if constexpr (N == 4) {
+          const uint4 v = *reinterpret_cast<const uint4*>(p);
+          w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+        } else {
+          const uint2 v = *reinterpret_cast<const uint2*>(p);
+          w[0] = v.x; w[1] = v.y;
+        }
+      } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = p[i];
+        for (int i = 0; i < N; ++i) w[i] = p[i];
+      }
     }
   }
-}
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (uint32_t& x : w) x = 0u;
+  }
+  __device__ __forceinline__ float get(int i) const {
+    if constexpr (BF16) return __uint_as_float(i & 1 ? w[i >> 1] & 0xFFFF0000u : w[i >> 1] << 16);
+    else return __uint_as_float(w[i]);
+  }
+};
 
-// grid (row tiles, n_kv, n_seq). PL: planes of q and P; bf16 rows have one.
+// grid: row tiles x sequences x KV heads. PL: planes of q and P; bf16 rows have one.
 template <int HD, int PL>
 __global__ void __launch_bounds__(kThreads, 2) prompt_tc_kernel(const PromptArgs a) {
   using L = Smem<HD, PL>;
   constexpr bool BF16 = PL == 1;
-  extern __shared__ unsigned char smem_raw[];
-  __shared__ float red[4];
-  unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  unsigned char *sq = smem, *sk = smem + PL * L::kPlane, *sv = sk + L::kK;
-  uint64_t* q_full = reinterpret_cast<uint64_t*>(sv + L::kV);
-  uint64_t *k_full = q_full + 1, *v_full = q_full + 2, *s_full = q_full + 3, *s_free = q_full + 4, *p_full = q_full + 5,
-           *o_done = q_full + 6;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_full + 7);
+  extern __shared__ __align__(1024) unsigned char smem[];
+  unsigned char *sq = smem, *sk = smem + PL * L::kPlane, *sv = sk + 2 * L::kK;
+  float* row_fac = reinterpret_cast<float*>(sv + L::kV);  // each row's factor
+  float* red = row_fac + kRows;                           // the largest V scale of each warp's tiles
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(red + 8);
+  uint64_t *k_free = k_full + 2, *v_full = k_full + 4, *s_full = k_full + 5, *s_free = k_full + 6, *p_full = k_full + 7,
+           *o_done = k_full + 8;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(k_full + 9);
+  volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (smem_u32(smem) & 1023) {  // the swizzle's rows would not fit (never seen: no static shared memory)
+    if (tid == 0) atomicExch(&g_prompt_err, 40);
+    return;
+  }
   if (tid == 0) {
-    mbar_init(q_full, kRows);
-    mbar_init(k_full, 128);
-    mbar_init(v_full, 128);
-    mbar_init(s_full, 1);   // Q K^T of a block is done: S may be read, K overwritten
+    mbar_init(&k_full[0], kFill);
+    mbar_init(&k_full[1], kFill);
+    mbar_init(&k_free[0], 1);  // Q K^T of a block is done: its K may be overwritten
+    mbar_init(&k_free[1], 1);
+    mbar_init(v_full, kFill);
+    mbar_init(s_full, 1);   // and S may be read
     mbar_init(s_free, kRows);
     mbar_init(p_full, kRows);
     mbar_init(o_done, 1);   // P V of a block is done: P and V may be overwritten, O rescaled
+    *gave_up = 0;
     fence_mbar_init();
   }
-  if (warp == 8) {
+  if (warp == 7) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
                  "r"(kCols));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
-  before_sync();
-  __syncthreads();
-  after_sync();
-  const uint32_t tmem = *tmem_slot;
   pdl_launch_dependents();
   pdl_wait();
 
-  const int kvh = blockIdx.y, seq = blockIdx.z;
-  // the last rows see the most keys: they start first
-  const int row0 = (gridDim.x - 1 - blockIdx.x) * kRows;
+  // all (sequence, KV head) of a row tile in turn, and the last tiles, which see the most keys, first
+  const int heads = a.c.n_kv * a.c.n_seq, row_tile = (int)(gridDim.x / heads) - 1 - (int)(blockIdx.x / heads);
+  const int kvh = blockIdx.x % heads % a.c.n_kv, seq = blockIdx.x % heads / a.c.n_kv;
+  const int row0 = row_tile * kRows;
   int start = a.starts[(long long)seq * a.idx_stride], count = a.rows;
   if (a.counts) count = min(max(a.counts[(long long)seq * a.idx_stride], 0), a.rows);
   if (start < 0) count = 0;
@@ -276,58 +310,87 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_tc_kernel(const PromptArgs
   const float* ks = a.c.ks + seq * a.c.scale_stride + kvh * blocks;
   const float* vs = a.c.vs + seq * a.c.scale_stride + kvh * blocks;
 
+  // ---- Q: every warp brings 16 rows, all of them in flight, a lane HD / 32 neighbouring values
+  if (nb > 0) {
+    constexpr int N = HD / 32;
+    float top = 0.f;
+    {
+      const int r0 = warp * 16;
+      // lane i knows where row i is (a division a row, not one for each of its values)
+      const int lr = row0 + r0 + (lane & 15), ls = lr / a.group;
+      const long long loff =
+          ls < count ? seq * a.q_seq + (long long)ls * a.q_row + (long long)(kvh * a.group + lr - ls * a.group) * HD : -1;
+      LaneValues<BF16, N> raw[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const long long off = __shfl_sync(0xffffffffu, loff, i);
+        raw[i].zero();
+        if (off >= 0) raw[i].load(a, off + lane * N);
+      }
+      // the largest V scale among the tiles (a NaN one only spoils the rows that see it)
+      for (int i = tid; i < tiles; i += kThreads) top = fmaxf(top, __ldg(vs + i));
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int r = r0 + i;
+        float f[N], mx = 0.f;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          f[e] = raw[i].get(e);
+          mx = fmaxf(mx, fabsf(f[e]));
+        }
+        mx = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mx)));
+        // 2^-e and 2^e for the exponent that puts the largest value into [1/2, 1): exact factors, two
+        // of them where one would leave f32's normal range
+        const int top_e = (int)(__float_as_uint(mx) >> 23);  // (0: zero or subnormal, 255: no number)
+        const int e = top_e == 255 ? 0 : max(top_e, 1) - 126;
+        const int e1 = e / 2, e2 = e - e1;
+        // (a negative scale turns the query round, so that larger scores stay larger)
+        const float d1 = copysignf(__int_as_float((127 - e1) << 23), a.scale), d2 = __int_as_float((127 - e2) << 23);
+        if (lane == 0)
+          row_fac[r] = fabsf(a.scale) * 1.4426950408889634f * __int_as_float((127 + e1) << 23) * __int_as_float((127 + e2) << 23);
+        uint32_t hi[N / 2], lo[N / 2];
+#pragma unroll
+        for (int p = 0; p < N / 2; ++p) {
+          const float x = f[2 * p] * d1 * d2, y = f[2 * p + 1] * d1 * d2;
+          hi[p] = pack_f16(x, y);
+          if (PL == 2) lo[p] = pack_rest(x, y, hi[p]);
+        }
+        const int col = lane * N;
+        unsigned char* at = sq + (col >> 6) * (kRows * 128) + r * 128 + ((((col & 63) >> 3) ^ (r & 7)) << 4) + (col & 7) * 2;
+        if constexpr (N == 4) {
+          *reinterpret_cast<uint2*>(at) = make_uint2(hi[0], hi[1]);
+          if (PL == 2) *reinterpret_cast<uint2*>(at + L::kPlane) = make_uint2(lo[0], lo[1]);
+        } else {
+          *reinterpret_cast<uint32_t*>(at) = hi[0];
+          if (PL == 2) *reinterpret_cast<uint32_t*>(at + L::kPlane) = lo[0];
+        }
+      }
+    }
+    fence_async_smem();
+    top = warp_max(top);
+    if (lane == 0) red[warp] = top;
+  }
+  before_sync();
+  __syncthreads();
+  after_sync();
+  const uint32_t tmem = *tmem_slot;
+
   if (warp < 4) {
     // ---------------------------------------------------------------- softmax: thread = query row = TMEM lane
     const int rr = row0 + tid, s = rr / a.group;
     const bool live = s < count;
     const int last = live ? min(start + s, a.c.capacity - 1) : -1;
-    const long long qoff = seq * a.q_seq + (long long)s * a.q_row + (long long)(kvh * a.group + rr % a.group) * HD;
-    float fac = 0.f, vref = 0.f;
-    {
-      float mx = 0.f;
-      if (live)
-        for (int c = 0; c < HD; c += 8) {
-          float f[8];
-          load8<BF16>(a, qoff + c, f);
+    const float fac = nb > 0 ? row_fac[tid] : 0.f;
+    float top = 0.f, vref = 0.f;
+    if (nb > 0)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) mx = fmaxf(mx, fabsf(f[i]));
-        }
-      int e = 0;
-      if (mx > 0.f && mx < __int_as_float(0x7F800000)) frexpf(mx, &e);
-      fac = scalbnf(fabsf(a.scale) * 1.4426950408889634f, e);
-      // (a negative scale turns the query round, so that larger scores stay larger)
-      const float sign = a.scale < 0.f ? -1.f : 1.f;
-      for (int c = 0; c < HD; c += 8) {
-        float f[8] = {};
-        if (live) load8<BF16>(a, qoff + c, f);
-        uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float x = scalbnf(f[2 * i], -e) * sign, y = scalbnf(f[2 * i + 1], -e) * sign;
-          hi[i] = pack_f16(x, y);
-          if (PL == 2) lo[i] = pack_rest(x, y, hi[i]);
-        }
-        const uint32_t at = (uint32_t)((c >> 6) * (kRows * 128) + tid * 128 + ((((c & 63) >> 3) ^ (tid & 7)) << 4));
-        *reinterpret_cast<uint4*>(sq + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        if (PL == 2) *reinterpret_cast<uint4*>(sq + L::kPlane + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-      }
-      fence_async_smem();
-      mbar_arrive(q_full);
-      // the largest V scale among the tiles (a NaN one only spoils the rows that see it)
-      float top = 0.f;
-      for (int i = tid; i < tiles; i += kRows) top = fmaxf(top, __ldg(vs + i));
-      top = warp_max(top);
-      if (lane == 0) red[warp] = top;
-      asm volatile("bar.sync 1, 128;" ::: "memory");
-      top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-      if (top > 0.f)  // the power of two above it, 2^-100 at least
-        vref = fmaxf(__uint_as_float((__float_as_uint(top) + 0x7FFFFFu) & 0xFF800000u), 7.888609e-31f);
-    }
+      for (int i = 0; i < 8; ++i) top = fmaxf(top, red[i]);
+    if (top > 0.f)  // the power of two above it, 2^-100 at least
+      vref = fmaxf(__uint_as_float((__float_as_uint(top) + 0x7FFFFFu) & 0xFF800000u), 7.888609e-31f);
     const float rvref = vref > 0.f ? __fdiv_rn(1.0f, vref) : 0.f;
     const uint32_t trow = tmem + ((uint32_t)(warp * 32) << 16);
     float m = kNone;
     f32x2 l = 0;  // two partial sums
-    bool ok = true;
     float kn[4], vn[4];  // the next block's scales
     auto scales = [&](int j) {
 #pragma unroll
@@ -350,10 +413,8 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_tc_kernel(const PromptArgs
         if (partial && pos0 + b * kKv8Block > last) w[b] = 0.f;
       }
       if (j + 1 < nb) scales(j + 1);
-      if (!warp_wait(s_full, (uint32_t)j & 1u, 41)) {
-        ok = false;
-        break;
-      }
+      wait(s_full, (uint32_t)j & 1u, gave_up, 43);
+      __syncwarp();
       after_sync();
       float x[kKeys];
       tmem_ld32(trow + kColS, reinterpret_cast<uint32_t*>(x));
@@ -378,10 +439,8 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_tc_kernel(const PromptArgs
       const float corr = grow ? ex2(m - mx) : 1.f;
       if (grow) m = mx;
       if (j > 0) {
-        if (!warp_wait(o_done, (uint32_t)(j - 1) & 1u, 42)) {
-          ok = false;
-          break;
-        }
+        wait(o_done, (uint32_t)(j - 1) & 1u, gave_up, 44);
+        __syncwarp();
         after_sync();
         if (__any_sync(0xffffffffu, grow)) {
           l = mul2(l, pair(corr, corr));
@@ -412,73 +471,98 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_tc_kernel(const PromptArgs
       mbar_arrive(p_full);
     }
     // ---- O * vref / l
-    if (ok && nb > 0) ok = warp_wait(o_done, (uint32_t)(nb - 1) & 1u, 43);
+    if (nb > 0) wait(o_done, (uint32_t)(nb - 1) & 1u, gave_up, 45);
+    __syncwarp();
     after_sync();
     const float2 sums = split(l);
     const float total = sums.x + sums.y;
     const float inv = total == 0.f ? 0.f : __fdiv_rn(vref, total);
-    const long long ooff = seq * a.o_seq + (long long)s * a.o_row + (long long)(kvh * a.group + rr % a.group) * HD;
+    // through shared memory (operands are idle now, 32 rows a warp), so that a row's stores are contiguous
+    constexpr int kPitch = HD + 4;  // floats; eight rows' 16-byte pieces hit distinct banks
+    static_assert(kRows * kPitch * 4 <= PL * L::kPlane + 2 * L::kK + L::kV, "the output reuses the operands");
+    float* stage = reinterpret_cast<float*>(smem);
 #pragma unroll 1
-    for (int c = 0; c < HD; c += 16) {
-      float o[16];
+    for (int c = 0; c < HD; c += 32) {
+      float o[32];
       if (nb > 0) {
-        tmem_ld16(trow + kColO + c, reinterpret_cast<uint32_t*>(o));
+        tmem_ld32(trow + kColO + c, reinterpret_cast<uint32_t*>(o));
         tmem_ld_wait();
       }
 #pragma unroll
-      for (int i = 0; i < 16; ++i) o[i] = nb > 0 ? o[i] * inv : 0.f;
-      if (rr >= a.rows * a.group) {
-        // a row behind the last: nothing to write
-      } else if constexpr (BF16) {
-        __nv_bfloat16* p = (__nv_bfloat16*)a.out + ooff + c;
-        __nv_bfloat162 v[8];
+      for (int i = 0; i < 32; i += 4)
+        *reinterpret_cast<float4*>(stage + tid * kPitch + c + i) =
+            nb > 0 ? make_float4(o[i] * inv, o[i + 1] * inv, o[i + 2] * inv, o[i + 3] * inv)
+                   : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    __syncwarp();
+    constexpr int kLanes = HD / 4, kPer = 32 / kLanes;  // lanes of a row, rows at a time
+    // (this lane's own row: s, rr)
+    const long long mine = rr < a.rows * a.group
+                               ? seq * a.o_seq + (long long)s * a.o_row + (long long)(kvh * a.group + rr - s * a.group) * HD
+                               : -1;
+    const int col = lane % kLanes * 4;
+#pragma unroll 1
+    for (int i0 = 0; i0 < 32; i0 += 8 * kPer) {
+      float4 o[8];  // (all read before the first store, which might alias them for all the compiler knows)
+      long long off[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = __floats2bfloat162_rn(o[2 * i], o[2 * i + 1]);
-        if (a.o_vec) {
-          reinterpret_cast<uint4*>(p)[0] = reinterpret_cast<uint4*>(v)[0];
-          reinterpret_cast<uint4*>(p)[1] = reinterpret_cast<uint4*>(v)[1];
+      for (int i = 0; i < 8; ++i) {
+        const int r = i0 + i * kPer + lane / kLanes;
+        o[i] = *reinterpret_cast<const float4*>(stage + (warp * 32 + r) * kPitch + col);
+        off[i] = __shfl_sync(0xffffffffu, mine, r);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (off[i] < 0) continue;
+        const long long at = off[i] + col;
+        if constexpr (BF16) {
+          __nv_bfloat16* p = (__nv_bfloat16*)a.out + at;
+          __nv_bfloat162 v[2] = {__floats2bfloat162_rn(o[i].x, o[i].y), __floats2bfloat162_rn(o[i].z, o[i].w)};
+          if (a.o_vec) {
+            *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(v);
+          } else {
+            p[0] = v[0].x; p[1] = v[0].y; p[2] = v[1].x; p[3] = v[1].y;
+          }
         } else {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) p[i] = i & 1 ? v[i >> 1].y : v[i >> 1].x;
-        }
-      } else {
-        float* p = (float*)a.out + ooff + c;
-        if (a.o_vec) {
-#pragma unroll
-          for (int i = 0; i < 16; i += 4)
-            *reinterpret_cast<float4*>(p + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) p[i] = o[i];
+          float* p = (float*)a.out + at;
+          if (a.o_vec) {
+            *reinterpret_cast<float4*>(p) = o[i];
+          } else {
+            p[0] = o[i].x; p[1] = o[i].y; p[2] = o[i].z; p[3] = o[i].w;
+          }
         }
       }
-      __syncwarp();
     }
-  } else if (warp < 8) {
+  } else if (warp < 7) {
     // ---------------------------------------------------------------- K and V: int8 -> f16 operands
     const int ct = tid - 128;
     const int8_t* k = a.c.k + seq * a.c.seq_stride + (long long)kvh * a.c.capacity * HD;
     const int8_t* v = a.c.v + seq * a.c.seq_stride + (long long)kvh * a.c.capacity * HD;
     const int end = tiles * kKv8Block;  // tokens past it are zeros
-    constexpr int kN = kKeys * HD / 16 / 128;  // 16-byte pieces of a block's K or V a thread
+    constexpr int kPieces = kKeys * HD / 16, kN = (kPieces + kFill - 1) / kFill;  // 16 bytes of K or V, a thread's
     uint4 kr[kN], vr[kN];
     auto load = [&](const int8_t* src, int j, uint4* r) {
 #pragma unroll
       for (int i = 0; i < kN; ++i) {
-        const int id = ct + i * 128, tok = j * kKeys + id / (HD / 16);
+        const int id = ct + i * kFill, tok = j * kKeys + id / (HD / 16);
         r[i] = make_uint4(0, 0, 0, 0);
-        if (tok < end) r[i] = __ldg(reinterpret_cast<const uint4*>(src + (long long)tok * HD + id % (HD / 16) * 16));
+        if (id < kPieces && tok < end)
+          r[i] = __ldg(reinterpret_cast<const uint4*>(src + (long long)tok * HD + id % (HD / 16) * 16));
       }
     };
     auto store = [&](unsigned char* dst, const uint4* r) {
 #pragma unroll
       for (int i = 0; i < kN; ++i) {
-        const int id = ct + i * 128, row = id / (HD / 16), c = id % (HD / 16) * 2;  // 16-byte f16 chunks c, c + 1
-        const uint32_t w[4] = {r[i].x ^ 0x80808080u, r[i].y ^ 0x80808080u, r[i].z ^ 0x80808080u, r[i].w ^ 0x80808080u};
+        const int id = ct + i * kFill, row = id / (HD / 16), c = id % (HD / 16) * 2;  // 16-byte f16 chunks c, c + 1
+        if (id >= kPieces) break;
+        // lanes of the second 64 columns begin with their second chunk, so that eight lanes hit distinct banks
+        const bool swap = c & 8;
+        const uint32_t w[4] = {(swap ? r[i].z : r[i].x) ^ 0x80808080u, (swap ? r[i].w : r[i].y) ^ 0x80808080u,
+                               (swap ? r[i].x : r[i].z) ^ 0x80808080u, (swap ? r[i].y : r[i].w) ^ 0x80808080u};
         unsigned char* p = dst + (c >> 3) * (kKeys * 128) + row * 128;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
-          *reinterpret_cast<uint4*>(p + ((((c & 7) + h) ^ (row & 7)) << 4)) =
+          *reinterpret_cast<uint4*>(p + ((((c & 7) + (h ^ (int)swap)) ^ (row & 7)) << 4)) =
               make_uint4(bytes_f16<0x4140>(w[2 * h]), bytes_f16<0x4342>(w[2 * h]), bytes_f16<0x4140>(w[2 * h + 1]),
                          bytes_f16<0x4342>(w[2 * h + 1]));
       }
@@ -486,12 +570,20 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_tc_kernel(const PromptArgs
     };
     load(k, 0, kr);
     load(v, 0, vr);
-    for (int j = 0; j < nb; ++j) {
-      if (j > 0 && !mbar_wait(s_full, (uint32_t)(j - 1) & 1u, &g_prompt_err, 44)) break;
-      store(sk, kr);
-      mbar_arrive(k_full);
+    auto put_k = [&](int j) {  // into its buffer, then the next block's loads
+      store(sk + (j & 1) * L::kK, kr);
+      mbar_arrive(&k_full[j & 1]);
       if (j + 1 < nb) load(k, j + 1, kr);
-      if (j > 0 && !mbar_wait(o_done, (uint32_t)(j - 1) & 1u, &g_prompt_err, 45)) break;
+    };
+    if (nb > 0) put_k(0);
+    for (int j = 0; j < nb; ++j) {
+      // K of block j + 1 goes where that of j - 1 was
+      if (j + 1 < nb) {
+        // (a barrier of its own: that of S may be two phases on by now)
+        if (j > 0 && !wait(&k_free[(j - 1) & 1], (uint32_t)((j - 1) >> 1) & 1u, gave_up, 46)) break;
+        put_k(j + 1);
+      }
+      if (j > 0 && !wait(o_done, (uint32_t)(j - 1) & 1u, gave_up, 47)) break;
       store(sv, vr);
       mbar_arrive(v_full);
       if (j + 1 < nb) load(v, j + 1, vr);
@@ -499,48 +591,41 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_tc_kernel(const PromptArgs
   } else if (lane == 0 && nb > 0) {
     // ---------------------------------------------------------------- products
     const uint32_t qa = smem_u32(sq), ka = smem_u32(sk), va = smem_u32(sv);
-    auto qk = [&]() {
-      bool first = true;
+    auto qk = [&](int j) {
+      if (!wait(&k_full[j & 1], (uint32_t)(j >> 1) & 1u, gave_up, 41)) return;
+      after_sync();
+      const uint32_t kb = ka + (uint32_t)(j & 1) * L::kK;
 #pragma unroll
       for (int pl = 0; pl < PL; ++pl)
 #pragma unroll
-        for (int kk = 0; kk < HD / 16; ++kk) {
+        for (int kk = 0; kk < HD / 16; ++kk)
           mma_ss(tmem + kColS, sw128_desc(qa + pl * L::kPlane + (kk >> 2) * (kRows * 128) + (kk & 3) * 32),
-                 sw128_desc(ka + (kk >> 2) * (kKeys * 128) + (kk & 3) * 32), idesc_f16(kKeys, false), first ? 0u : 1u);
-          first = false;
-        }
+                 sw128_desc(kb + (kk >> 2) * (kKeys * 128) + (kk & 3) * 32), idesc_f16(kKeys, false),
+                 (pl > 0 || kk > 0) ? 1u : 0u);
       commit(s_full);
+      commit(&k_free[j & 1]);
     };
-    bool ok = mbar_wait(q_full, 0, &g_prompt_err, 46) && mbar_wait(k_full, 0, &g_prompt_err, 47);
-    if (ok) {
-      after_sync();
-      qk();
-    }
-    for (int j = 0; j < nb && ok; ++j) {
+    qk(0);
+    for (int j = 0; j < nb && !*gave_up; ++j) {
       if (j + 1 < nb) {
-        ok = mbar_wait(k_full, (uint32_t)(j + 1) & 1u, &g_prompt_err, 48) &&
-             mbar_wait(s_free, (uint32_t)j & 1u, &g_prompt_err, 49);
-        if (!ok) break;
-        after_sync();
-        qk();
+        if (!wait(s_free, (uint32_t)j & 1u, gave_up, 48)) break;
+        qk(j + 1);
       }
-      ok = mbar_wait(v_full, (uint32_t)j & 1u, &g_prompt_err, 50) && mbar_wait(p_full, (uint32_t)j & 1u, &g_prompt_err, 51);
-      if (!ok) break;
+      if (!wait(v_full, (uint32_t)j & 1u, gave_up, 42) || !wait(p_full, (uint32_t)j & 1u, gave_up, 49)) break;
       after_sync();
 #pragma unroll
       for (int pl = 0; pl < PL; ++pl)
 #pragma unroll
         for (int kk = 0; kk < kKeys / 16; ++kk)
           mma_ts(tmem + kColO, tmem + kColP + pl * 32 + kk * 8, sw128_desc(va + kk * 2048, kKeys * 128),
-                 idesc_f16(HD, true),
-                 (j > 0 || pl > 0 || kk > 0) ? 1u : 0u);
+                 idesc_f16(HD, true), (j > 0 || pl > 0 || kk > 0) ? 1u : 0u);
       commit(o_done);
     }
   }
   __syncwarp();
   before_sync();
   __syncthreads();
-  if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols));
+  if (warp == 7) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols));
 }
 
 template <int HD, int PL>
@@ -548,7 +633,9 @@ cudaError_t launch(const PromptArgs& a, cudaStream_t s) {
   static OncePerDevice once;
   const cudaError_t e = once.smem(prompt_tc_kernel<HD, PL>, Smem<HD, PL>::kBytes);
   if (e != cudaSuccess) return e;
-  const dim3 g((a.rows * a.group + kRows - 1) / kRows, a.c.n_kv, a.c.n_seq);
+  const long long ctas = ((long long)a.rows * a.group + kRows - 1) / kRows * a.c.n_kv * a.c.n_seq;
+  if (ctas > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
+  const dim3 g((unsigned)ctas);
   return ops_launch(prompt_tc_kernel<HD, PL>, g, dim3(kThreads), Smem<HD, PL>::kBytes, s, 1, a);
 }
 
