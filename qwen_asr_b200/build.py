@@ -1,4 +1,5 @@
-"""Builds libqwen_asr.so in-tree: CUDA sources with nvcc for sm_100a, host C++ with g++.
+"""Builds libqwen_asr.so in-tree (CUDA sources with nvcc for sm_100a, host C++ with g++), and the
+torch binding of the 8-bit operators, _ops_fast.so.
 
 Usage: python -m qwen_asr_b200.build [--force]
 """
@@ -53,7 +54,7 @@ def build(force: bool = False, verbose: bool = True) -> str:
     with cf.ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 4)) as ex:
         objs = list(ex.map(lambda s: _compile(s, hm, force), srcs))
     if force or not os.path.exists(LIB) or os.path.getmtime(LIB) < _newest(objs):
-        cmd = [NVCC] + ARCH + ["-shared", "-o", LIB] + objs + ["-cudart", "static", "-lpthread", "-ldl", "-lrt"]
+        cmd = [NVCC] + ARCH + ["-shared", "-Xlinker", "-soname=libqwen_asr.so", "-o", LIB] + objs + ["-cudart", "static", "-lpthread", "-ldl", "-lrt"]
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
@@ -62,5 +63,30 @@ def build(force: bool = False, verbose: bool = True) -> str:
     return LIB
 
 
+def build_binding(force: bool = False, verbose: bool = True) -> str:
+    """_ops_fast.so: the C++ binding of the 8-bit operators (ops.py) against the installed torch."""
+    import sysconfig
+    import torch
+    from torch.utils import cpp_extension
+    src = os.path.join(CSRC, "binding", "ops_fast.cpp")
+    out = os.path.join(HERE, "_ops_fast.so")
+    newest = _newest([src, LIB] + glob.glob(os.path.join(INC, "*.h")))
+    if not force and os.path.exists(out) and os.path.getmtime(out) >= newest:
+        return out
+    torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-I" + INC, "-I" + sysconfig.get_path("include"), "-I/usr/local/cuda/include"]
+    cmd += ["-isystem" + p for p in cpp_extension.include_paths()]
+    cmd += [src, "-o", out, LIB, "-L" + torch_lib, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda",
+            "-Wl,-rpath,$ORIGIN", "-Wl,-rpath," + torch_lib]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"compile failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+    if verbose:
+        print(f"built {out}")
+    return out
+
+
 if __name__ == "__main__":
     build(force="--force" in sys.argv)
+    build_binding(force="--force" in sys.argv)

@@ -23,6 +23,11 @@ import torch
 
 from . import last_error, lib
 
+try:
+    from . import _ops_fast as _fast  # the same calls made in C++ (binding/ops_fast.cpp)
+except ImportError:  # not built, or for another torch: every call takes the ctypes path below
+    _fast = None
+
 BLOCK = 16  # cache tokens that share a scale
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
@@ -51,9 +56,8 @@ def kv8_cache(n_seq: int, n_kv: int, capacity: int, head_dim: int = 128, device=
     return Kv8Cache(*q, *s)
 
 
-# A call of a few microseconds has no time for a check of its arguments one by one: each operator asks
-# whether everything is as it should be in one expression, and only where it is not does the slow
-# form below look for the argument to name.
+# An ordinary call is checked and made in C++, which answers None to any other: unusual strides and
+# sizes, which ctypes handles here, and arguments that do not fit, which are named here.
 def _tensor(t, name, dims, dtypes, device=None, shape=None):
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor, not {type(t).__name__}")
@@ -94,6 +98,10 @@ def rms_norm_int8(x, weight, eps: float = 1e-6, residual=None):
     """(q, scale, h) of x [rows, d] (f32 or bf16): h = x + residual in x's type (x itself without a
     residual), q int8 [rows, d] and scale f32 [rows] with q * scale[:, None] the RMS-normalised
     rows times weight (f32 [d]). q's row stride is d rounded up to 16, as linear_int8 wants it."""
+    if _fast is not None:
+        out = _fast.rms_norm_int8(x, weight, eps, residual)
+        if out is not None:
+            return out
     _x = isinstance(x, torch.Tensor)
     code = _DTYPES.get(x.dtype) if _x else None
     if code is None or x.dim() != 2 or not x.is_cuda or (x.requires_grad and _grad()):
@@ -129,6 +137,10 @@ def linear_int8(xq, xs, wq, ws, residual=None, swiglu: bool = False, dtype=torch
     (f32 or bf16), with exact integer sums. residual [m, n] (in dtype) is added; swiglu takes the
     rows of wq as gate0, up0, gate1, ... and returns silu(gate) * up, [m, n / 2]. Rows of xq and wq
     start on 16-byte boundaries (row strides that are multiples of 16)."""
+    if _fast is not None and dtype in _DTYPES:
+        out = _fast.linear_int8(xq, xs, wq, ws, residual, bool(swiglu), dtype is torch.bfloat16)
+        if out is not None:
+            return out
     if not (isinstance(xq, torch.Tensor) and xq.dtype is _INT8 and xq.is_cuda and xq.dim() == 2):
         _tensor(xq, "xq", 2, (_INT8,))
     dev, (m, k) = xq.get_device(), xq.shape
@@ -235,6 +247,8 @@ def kv8_append(cache: Kv8Cache, k, v, starts, counts=None) -> None:
     (int32, on the device) of each sequence; counts[b] says how many of the rows it has (default
     all). The scale of a block of 16 tokens only grows while it fills, and what it holds is
     re-coded; rows past the capacity are dropped, and a negative start skips the sequence."""
+    if _fast is not None and _fast.kv8_append(cache, k, v, starts, counts):
+        return
     desc, dev, n, h, hd = _cache(cache)
     code = _DTYPES.get(k.dtype) if isinstance(k, torch.Tensor) else None
     if code is None or k.dim() != 4:
@@ -253,6 +267,10 @@ def kv8_append(cache: Kv8Cache, k, v, starts, counts=None) -> None:
 def kv8_read(cache: Kv8Cache, starts, rows: int, counts=None, dtype=torch.float32):
     """(k, v) [n_seq, rows, n_kv, head_dim]: the values of positions starts[b] + r, zeros from row
     counts[b] and from the capacity on."""
+    if _fast is not None and dtype in _DTYPES:
+        out = _fast.kv8_read(cache, starts, rows, counts, dtype is torch.bfloat16)
+        if out is not None:
+            return out
     desc, dev, n, h, hd = _cache(cache)
     code = _DTYPES.get(dtype)
     if code is None:
@@ -275,6 +293,10 @@ def kv8_attention(q, cache: Kv8Cache, starts, counts=None, scale: float | None =
     the cache: row r of sequence b attends positions 0 .. starts[b] + r; rows from counts[b] on get
     zeros. scale defaults to 1 / sqrt(head_dim). max_len, an upper bound of starts + rows when the
     caller knows one, only shapes the launch."""
+    if _fast is not None:
+        out = _fast.kv8_attention(q, cache, starts, counts, scale, max_len)
+        if out is not None:
+            return out
     desc, dev, n, h, hd = _cache(cache)
     code = _DTYPES.get(q.dtype) if isinstance(q, torch.Tensor) else None
     if code is None or q.dim() != 4:

@@ -15,10 +15,32 @@ F32, BF16 = torch.float32, torch.bfloat16
 HALF = {F32: 2.0 ** -24, BF16: 2.0 ** -8}  # largest relative error of a rounding
 
 
-@pytest.fixture(scope="module")
-def ops():
+@pytest.fixture(params=["binding", "ctypes"])
+def ops(request, monkeypatch):
+    """The operators through the C++ binding, and through ctypes as where it is not built."""
     from qwen_asr_b200 import ops
+    if request.param == "ctypes":
+        monkeypatch.setattr(ops, "_fast", None)
     return ops
+
+
+def test_binding_is_built_and_takes_ordinary_calls():
+    from qwen_asr_b200 import ops
+    x, w = rand(3, 64), rand(64)
+    q, s, _ = ops._fast.rms_norm_int8(x, w, 1e-6, x)
+    assert ops._fast.linear_int8(q, s, q, s, None, False, True).dtype == BF16
+    c = ops.kv8_cache(2, 2, 32, 64)
+    z = torch.zeros(2, dtype=torch.int32, device="cuda")
+    assert ops._fast.kv8_append(c, rand(2, 1, 2, 64), rand(2, 1, 2, 64), z, None) is True
+    assert ops._fast.kv8_attention(rand(2, 1, 4, 64), c, z, None, None, 0).shape == (2, 1, 4, 64)
+    assert len(ops._fast.kv8_read(c, z, 1, None, False)) == 2
+    # and leaves the others, with their errors, to the caller
+    assert ops._fast.rms_norm_int8(x.half(), w, 1e-6, None) is None
+    assert ops._fast.rms_norm_int8(x.clone().requires_grad_(), w, 1e-6, None) is None
+    assert ops._fast.linear_int8(q, s, q[:, :32], s, None, False, False) is None
+    assert ops._fast.kv8_append(c, rand(2, 1, 2, 64), rand(2, 1, 2, 64).to(BF16), z, None) is None
+    assert ops._fast.kv8_attention(rand(2, 1, 3, 64), c, z, None, None, 0) is None
+    assert ops._fast.kv8_read(c, z.cpu(), 1, None, False) is None
 
 
 def rand(*shape, seed=0, std=1.0):
