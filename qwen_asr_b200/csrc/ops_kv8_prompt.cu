@@ -2,30 +2,31 @@
 //
 // One CTA owns 128 query rows of one KV head (row = query position x head of the group) and walks
 // the keys they see in blocks of 64. Per block
-//   S = Q K^T          M = 128, N = 64, K = head_dim                 -> TMEM columns 0 .. 63
+//   S = Q K^T          M = 128, N = 64, K = head_dim   -> TMEM
 //   p = exp2(S f - m)  f = scale * log2(e) * K scale of 16 tokens; running maximum m and sum l
-//   O += P V           P = p * V scale / vref, from TMEM; N = head_dim -> TMEM columns 128 ..
+//   O += P V           P = p * V scale / vref, an operand in TMEM; N = head_dim
 // and at the end O * vref / l.
 //
 // Precision. int8 is exact in f16, so K and V enter the products as they are; their scales stay
 // outside, in f32 (vref, a power of two above every V scale the rows see, keeps P in f16's range).
-// A query row is scaled by a power of two to [1/2, 1). With PL = 2 (f32 rows) q and P are two f16
-// planes, hi + lo, held to 2^-25 of the row's largest; both planes add into the same f32
-// accumulator. With PL = 1 (bf16 rows) one plane: 2^-11 of a probability, an eighth of the output's
-// own rounding.
-// m is only raised when a score exceeds it by 2^8 (p up to 256 is as exact in f16): O is then
-// rescaled in TMEM, which the first blocks of a row do and later ones hardly ever.
+// A query row is scaled by a power of two to [1/2, 1). For f32 rows q and P are two f16 planes,
+// hi + lo, held to 2^-25 of the row's largest; both planes add into the same f32 accumulator. For bf16
+// rows one plane: 2^-11 of a probability, an eighth of the output's own rounding.
+// m is only raised when a score exceeds it by 2^8 (p up to 256 is as exact in f16): what has been summed
+// is then rescaled, which the first blocks of a row do and later ones hardly ever.
 //
-// Roles (256 threads, two CTAs an SM, so that one's softmax runs beside the other's products): warps
-// 0-3 softmax, a thread a row; warps 4-6 bring K and V from global memory as int8, one block ahead in
-// registers, and write them as f16 rows of a token in the 128-byte-swizzle layout, which is K-major for
-// Q K^T and MN-major for P V; one thread of warp 7 issues the products, Q K^T of the next block before
-// P V of this one. (Issuing takes as long as the products do, 48 cycles each at N = 64 and 64 at N = 128,
-// so a softmax thread that did it kept its warp waiting: 3.1 us a block instead of 1.8.) K has two
-// buffers, so that its conversion runs beside the products of the block before.
-//
-// Bound: f32 rows - the tensor pipe (four products of 128 x 64 x head_dim a block), bf16 rows - exp2
-// and the conversions around it.
+// Two kernels. In both some warps do the softmax; others bring K and V from global memory as int8, a block
+// or two ahead in registers, and write them as f16 rows of a token in the 128-byte-swizzle layout, which is
+// K-major for Q K^T and MN-major for P V; the last warp issues the products, Q K^T of the next block
+// before P V of this one. (One thread that did this was the longest chain of all: the operands of a product
+// are uniform registers, and a branch of one lane has to fill them anew each time. A whole warp that waits
+// and counts together, with an elected lane to issue, took 64 rows over 8064 f32 keys from 197 to 149 us.)
+//   bf16 rows: 256 threads, a softmax thread a row; two CTAs an SM, one's softmax beside the other's
+//   products. O stays in TMEM. 8 x 381 rows over up to 1403 keys, 8 KV heads of 2 x 128: 52 us; 2048 rows
+//   over 8048 keys, 4 KV heads of 4 x 64: 143 us; 592 heads' rows over 8064 keys: 205 us, 755 TFLOP/s.
+//   f32 rows: see below. The same shapes: 77, 209 and 335 us (a block has four times the products' bytes).
+// Bound: bf16 rows - exp2 and the conversions around it, f32 rows - the chain of a block's steps in its
+// one CTA an SM, 1.2 us of which the products take 0.7.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -53,11 +54,12 @@ struct PromptArgs {
   int q_vec, o_vec;  // rows start on 16-byte boundaries
 };
 
-template <int HD, int PL>
+template <int HD>
 struct Smem {
-  static constexpr int kPlane = kRows * HD * 2, kK = kKeys * HD * 2, kV = kK;
-  // Q, two K, V, then 1024 bytes of rows' factors, V scales and barriers: two f32 CTAs fill an SM
-  static constexpr int kBytes = PL * kPlane + 2 * kK + kV + 1024;
+  static constexpr int kPlane = kRows * HD * 2, kK = kKeys * HD * 2;
+  // bf16 rows: Q, two K, a V; f32 rows: two planes of Q, two K, two V; then rows' factors, V scales, barriers
+  static constexpr int kBytes1 = kPlane + 3 * kK + 1024;
+  static constexpr int kBytes2 = 2 * kPlane + 4 * kK + 4096;
 };
 
 // 128-byte swizzle, 8-row groups 1024 bytes apart; lead: bytes from 64 columns to the next (MN-major)
@@ -76,19 +78,21 @@ __device__ __forceinline__ constexpr uint32_t idesc_f16(int n, bool b_mn) {
 }
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accum) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "{\n .reg .pred e, p;\n elect.sync _|e, 0xffffffff;\n setp.ne.b32 p, %4, 0;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
       "l"(a), "l"(b), "r"(idesc), "r"(accum));
 }
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accum) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "{\n .reg .pred e, p;\n elect.sync _|e, 0xffffffff;\n setp.ne.b32 p, %4, 0;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
       "r"(a), "l"(b), "r"(idesc), "r"(accum));
 }
 __device__ __forceinline__ void commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-               : "memory");
+  asm volatile(
+      "{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n"
+      " @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(bar))
+      : "memory");
 }
 __device__ __forceinline__ void before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -203,10 +207,25 @@ __device__ __forceinline__ uint32_t bytes_f16(uint32_t w) {
 // Bounded wait. Once one gave up nobody waits any more: the warps run through what is left of their
 // loops, with the barriers between them, and leave an output that the error code disowns.
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile int* gave_up, int code) {
-  if (*gave_up) return false;
-  if (mbar_wait(bar, parity, &g_prompt_err, code)) return true;
-  *gave_up = 1;
-  return false;
+  if (mbar_try_wait(bar, parity)) return true;
+  uint64_t t0 = 0;
+  for (uint32_t i = 1;; ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if (i & 15) continue;  // (the timer is slow to read: never on a wait that soon ends)
+    if (*gave_up) return false;
+    const uint64_t now = global_timer_ns();
+    if (t0 == 0) t0 = now;
+    if (now - t0 > 2000000000ull) {
+      atomicExch(&g_prompt_err, code);
+      *gave_up = 1;
+      return false;
+    }
+  }
+}
+
+// The same for a whole warp, as one answer: what follows stays uniform to the compiler.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* gave_up, int code) {
+  return __all_sync(0xffffffffu, wait(bar, parity, gave_up, code));
 }
 
 // N (4 or 2) neighbouring values of a query row, as loaded: converted later, so that no load waits for
@@ -254,21 +273,206 @@ struct LaneValues {
   }
 };
 
-// grid: row tiles x sequences x KV heads. PL: planes of q and P; bf16 rows have one.
-template <int HD, int PL>
-__global__ void __launch_bounds__(kThreads, 2) prompt_tc_kernel(const PromptArgs a) {
-  using L = Smem<HD, PL>;
-  constexpr bool BF16 = PL == 1;
+// What a CTA works on.
+struct Work {
+  int kvh, seq, row0, start, count, tiles, nb;  // tiles of 16 keys (a scale each), blocks of 64
+  const float *ks, *vs;
+  const int8_t *k, *v;
+};
+__device__ __forceinline__ Work work_of(const PromptArgs& a) {
+  Work t;
+  // all (sequence, KV head) of a row tile in turn, and the last tiles, which see the most keys, first
+  const int heads = a.c.n_kv * a.c.n_seq;
+  t.kvh = blockIdx.x % heads % a.c.n_kv;
+  t.seq = blockIdx.x % heads / a.c.n_kv;
+  t.row0 = ((int)(gridDim.x / heads) - 1 - (int)(blockIdx.x / heads)) * kRows;
+  t.start = a.starts[(long long)t.seq * a.idx_stride];
+  t.count = a.rows;
+  if (a.counts) t.count = min(max(a.counts[(long long)t.seq * a.idx_stride], 0), a.rows);
+  if (t.start < 0) t.count = 0;
+  t.start = min(t.start, a.c.capacity);
+  // keys any row of the tile sees
+  const int s_last = min(t.count - 1, (t.row0 + kRows - 1) / a.group);
+  const int len = s_last >= t.row0 / a.group ? (int)min((long long)t.start + s_last + 1, (long long)a.c.capacity) : 0;
+  t.tiles = (len + kKv8Block - 1) / kKv8Block;
+  t.nb = (len + kKeys - 1) / kKeys;
+  const long long blocks = a.c.capacity / kKv8Block, head = (long long)t.kvh * a.c.capacity * a.c.head_dim;
+  t.ks = a.c.ks + t.seq * a.c.scale_stride + t.kvh * blocks;
+  t.vs = a.c.vs + t.seq * a.c.scale_stride + t.kvh * blocks;
+  t.k = a.c.k + t.seq * a.c.seq_stride + head;
+  t.v = a.c.v + t.seq * a.c.seq_stride + head;
+  return t;
+}
+
+// Q as operand planes: each of eight warps brings 16 rows, all of them in flight, a lane HD / 32
+// neighbouring values. Also the rows' factors and the warps' largest V scales.
+template <int HD, int PL, bool BF16>
+__device__ __forceinline__ void bring_q(const PromptArgs& a, const Work& t, unsigned char* sq, float* row_fac, float* red,
+                                        int warp, int lane) {
+  constexpr int N = HD / 32, kPlane = kRows * HD * 2;
+  float top = 0.f;
+  const int r0 = warp * 16;
+  // lane i knows where row i is (a division a row, not one for each of its values)
+  const int lr = t.row0 + r0 + (lane & 15), ls = lr / a.group;
+  const long long loff = ls < t.count ? t.seq * a.q_seq + (long long)ls * a.q_row +
+                                            (long long)(t.kvh * a.group + lr - ls * a.group) * HD
+                                      : -1;
+  LaneValues<BF16, N> raw[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const long long off = __shfl_sync(0xffffffffu, loff, i);
+    raw[i].zero();
+    if (off >= 0) raw[i].load(a, off + lane * N);
+  }
+  // (a NaN V scale only spoils the rows that see it)
+  for (int i = warp * 32 + lane; i < t.tiles; i += 256) top = fmaxf(top, __ldg(t.vs + i));
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int r = r0 + i;
+    float f[N], mx = 0.f;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      f[e] = raw[i].get(e);
+      mx = fmaxf(mx, fabsf(f[e]));
+    }
+    mx = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mx)));
+    // 2^-e and 2^e for the exponent that puts the largest value into [1/2, 1): exact factors, two
+    // of them where one would leave f32's normal range
+    const int top_e = (int)(__float_as_uint(mx) >> 23);  // (0: zero or subnormal, 255: no number)
+    const int e = top_e == 255 ? 0 : max(top_e, 1) - 126;
+    const int e1 = e / 2, e2 = e - e1;
+    // (a negative scale turns the query round, so that larger scores stay larger)
+    const float d1 = copysignf(__int_as_float((127 - e1) << 23), a.scale), d2 = __int_as_float((127 - e2) << 23);
+    if (lane == 0)
+      row_fac[r] = fabsf(a.scale) * 1.4426950408889634f * __int_as_float((127 + e1) << 23) * __int_as_float((127 + e2) << 23);
+    uint32_t hi[N / 2], lo[N / 2];
+#pragma unroll
+    for (int p = 0; p < N / 2; ++p) {
+      const float x = f[2 * p] * d1 * d2, y = f[2 * p + 1] * d1 * d2;
+      hi[p] = pack_f16(x, y);
+      if (PL == 2) lo[p] = pack_rest(x, y, hi[p]);
+    }
+    const int col = lane * N;
+    unsigned char* at = sq + (col >> 6) * (kRows * 128) + r * 128 + ((((col & 63) >> 3) ^ (r & 7)) << 4) + (col & 7) * 2;
+    if constexpr (N == 4) {
+      *reinterpret_cast<uint2*>(at) = make_uint2(hi[0], hi[1]);
+      if (PL == 2) *reinterpret_cast<uint2*>(at + kPlane) = make_uint2(lo[0], lo[1]);
+    } else {
+      *reinterpret_cast<uint32_t*>(at) = hi[0];
+      if (PL == 2) *reinterpret_cast<uint32_t*>(at + kPlane) = lo[0];
+    }
+  }
+  fence_async_smem();
+  top = warp_max(top);
+  if (lane == 0) red[warp] = top;
+}
+
+// Where a query row's output starts (negative behind the last row).
+__device__ __forceinline__ long long out_row(const PromptArgs& a, const Work& t, int rr, int hd) {
+  if (rr >= a.rows * a.group) return -1;
+  const int s = rr / a.group;
+  return t.seq * a.o_seq + (long long)s * a.o_row + (long long)(t.kvh * a.group + rr - s * a.group) * hd;
+}
+
+// The power of two above every V scale the tile sees (2^-100 at least), 0 for none.
+__device__ __forceinline__ float vref_of(const float* red) {
+  float top = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = fmaxf(top, red[i]);
+  return top > 0.f ? fmaxf(__uint_as_float((__float_as_uint(top) + 0x7FFFFFu) & 0xFF800000u), 7.888609e-31f) : 0.f;
+}
+
+// A thread's pieces of one block of K or V: int8 in registers, then f16 rows of a token in shared memory.
+template <int HD, int FILL>  // FILL: threads that share a block
+struct Pieces {
+  static constexpr int kAll = kKeys * HD / 16, kN = (kAll + FILL - 1) / FILL;
+  uint4 r[kN];
+  __device__ __forceinline__ void load(const int8_t* src, int j, int end, int ct) {  // tokens from end on are zeros
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      const int id = ct + i * FILL, tok = j * kKeys + id / (HD / 16);
+      r[i] = make_uint4(0, 0, 0, 0);
+      if (id < kAll && tok < end)
+        r[i] = __ldg(reinterpret_cast<const uint4*>(src + (long long)tok * HD + id % (HD / 16) * 16));
+    }
+  }
+  __device__ __forceinline__ void store(unsigned char* dst, int ct) const {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      const int id = ct + i * FILL, row = id / (HD / 16), c = id % (HD / 16) * 2;  // 16-byte f16 chunks c, c + 1
+      if (id >= kAll) break;
+      // lanes of the second 64 columns begin with their second chunk, so that eight lanes hit distinct banks
+      const bool swap = c & 8;
+      const uint32_t w[4] = {(swap ? r[i].z : r[i].x) ^ 0x80808080u, (swap ? r[i].w : r[i].y) ^ 0x80808080u,
+                             (swap ? r[i].x : r[i].z) ^ 0x80808080u, (swap ? r[i].y : r[i].w) ^ 0x80808080u};
+      unsigned char* p = dst + (c >> 3) * (kKeys * 128) + row * 128;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        *reinterpret_cast<uint4*>(p + ((((c & 7) + (h ^ (int)swap)) ^ (row & 7)) << 4)) =
+            make_uint4(bytes_f16<0x4140>(w[2 * h]), bytes_f16<0x4342>(w[2 * h]), bytes_f16<0x4140>(w[2 * h + 1]),
+                       bytes_f16<0x4342>(w[2 * h + 1]));
+    }
+    fence_async_smem();
+  }
+};
+
+// Stores 32 / PARTS rows of a warp's 32 staged rows (pitch kPitch floats), the part-th share; `mine`: the
+// output offset of this lane's row, negative for none.
+template <int HD>
+constexpr int kPitch = HD + 4;  // floats; eight rows' 16-byte pieces hit distinct banks
+template <int HD, bool BF16, int PARTS>
+__device__ __forceinline__ void write_rows(const PromptArgs& a, const float* stage, long long mine, int part, int lane) {
+  constexpr int kLanes = HD / 4, kPer = 32 / kLanes, kRowsEach = 32 / PARTS;  // lanes of a row, rows at a time
+  const int col = lane % kLanes * 4;
+#pragma unroll 1
+  for (int i0 = part * kRowsEach; i0 < (part + 1) * kRowsEach; i0 += 8 * kPer) {
+    float4 o[8];  // (all read before the first store, which might alias them for all the compiler knows)
+    long long off[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = i0 + i * kPer + lane / kLanes;
+      o[i] = *reinterpret_cast<const float4*>(stage + r * kPitch<HD> + col);
+      off[i] = __shfl_sync(0xffffffffu, mine, r);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (off[i] < 0) continue;
+      const long long at = off[i] + col;
+      if constexpr (BF16) {
+        __nv_bfloat16* p = (__nv_bfloat16*)a.out + at;
+        __nv_bfloat162 v[2] = {__floats2bfloat162_rn(o[i].x, o[i].y), __floats2bfloat162_rn(o[i].z, o[i].w)};
+        if (a.o_vec) {
+          *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(v);
+        } else {
+          p[0] = v[0].x; p[1] = v[0].y; p[2] = v[1].x; p[3] = v[1].y;
+        }
+      } else {
+        float* p = (float*)a.out + at;
+        if (a.o_vec) {
+          *reinterpret_cast<float4*>(p) = o[i];
+        } else {
+          p[0] = o[i].x; p[1] = o[i].y; p[2] = o[i].z; p[3] = o[i].w;
+        }
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------ bf16 rows: one plane, two CTAs an SM
+// grid: row tiles x sequences x KV heads
+template <int HD>
+__global__ void __launch_bounds__(kThreads, 2) prompt_bf16_kernel(const PromptArgs a) {
+  using L = Smem<HD>;
   extern __shared__ __align__(1024) unsigned char smem[];
-  unsigned char *sq = smem, *sk = smem + PL * L::kPlane, *sv = sk + 2 * L::kK;
-  float* row_fac = reinterpret_cast<float*>(sv + L::kV);  // each row's factor
+  unsigned char *sq = smem, *sk = smem + L::kPlane, *sv = sk + 2 * L::kK;
+  float* row_fac = reinterpret_cast<float*>(sv + L::kK);  // each row's factor
   float* red = row_fac + kRows;                           // the largest V scale of each warp's tiles
   uint64_t* k_full = reinterpret_cast<uint64_t*>(red + 8);
   uint64_t *k_free = k_full + 2, *v_full = k_full + 4, *s_full = k_full + 5, *s_free = k_full + 6, *p_full = k_full + 7,
            *o_done = k_full + 8;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(k_full + 9);
   volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;  // (uniform)
   if (smem_u32(smem) & 1023) {  // the swizzle's rows would not fit (never seen: no static shared memory)
     if (tid == 0) atomicExch(&g_prompt_err, 40);
     return;
@@ -294,86 +498,13 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_tc_kernel(const PromptArgs
   pdl_launch_dependents();
   pdl_wait();
 
-  // all (sequence, KV head) of a row tile in turn, and the last tiles, which see the most keys, first
-  const int heads = a.c.n_kv * a.c.n_seq, row_tile = (int)(gridDim.x / heads) - 1 - (int)(blockIdx.x / heads);
-  const int kvh = blockIdx.x % heads % a.c.n_kv, seq = blockIdx.x % heads / a.c.n_kv;
-  const int row0 = row_tile * kRows;
-  int start = a.starts[(long long)seq * a.idx_stride], count = a.rows;
-  if (a.counts) count = min(max(a.counts[(long long)seq * a.idx_stride], 0), a.rows);
-  if (start < 0) count = 0;
-  start = min(start, a.c.capacity);
-  // keys any row of the tile sees, in tiles of 16 (a scale each) and blocks of 64
-  const int s_last = min(count - 1, (row0 + kRows - 1) / a.group);
-  const int len = s_last >= row0 / a.group ? (int)min((long long)start + s_last + 1, (long long)a.c.capacity) : 0;
-  const int tiles = (len + kKv8Block - 1) / kKv8Block, nb = (len + kKeys - 1) / kKeys;
-  const long long blocks = a.c.capacity / kKv8Block;
-  const float* ks = a.c.ks + seq * a.c.scale_stride + kvh * blocks;
-  const float* vs = a.c.vs + seq * a.c.scale_stride + kvh * blocks;
-
-  // ---- Q: every warp brings 16 rows, all of them in flight, a lane HD / 32 neighbouring values
-  if (nb > 0) {
-    constexpr int N = HD / 32;
-    float top = 0.f;
-    {
-      const int r0 = warp * 16;
-      // lane i knows where row i is (a division a row, not one for each of its values)
-      const int lr = row0 + r0 + (lane & 15), ls = lr / a.group;
-      const long long loff =
-          ls < count ? seq * a.q_seq + (long long)ls * a.q_row + (long long)(kvh * a.group + lr - ls * a.group) * HD : -1;
-      LaneValues<BF16, N> raw[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const long long off = __shfl_sync(0xffffffffu, loff, i);
-        raw[i].zero();
-        if (off >= 0) raw[i].load(a, off + lane * N);
-      }
-      // the largest V scale among the tiles (a NaN one only spoils the rows that see it)
-      for (int i = tid; i < tiles; i += kThreads) top = fmaxf(top, __ldg(vs + i));
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int r = r0 + i;
-        float f[N], mx = 0.f;
-#pragma unroll
-        for (int e = 0; e < N; ++e) {
-          f[e] = raw[i].get(e);
-          mx = fmaxf(mx, fabsf(f[e]));
-        }
-        mx = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mx)));
-        // 2^-e and 2^e for the exponent that puts the largest value into [1/2, 1): exact factors, two
-        // of them where one would leave f32's normal range
-        const int top_e = (int)(__float_as_uint(mx) >> 23);  // (0: zero or subnormal, 255: no number)
-        const int e = top_e == 255 ? 0 : max(top_e, 1) - 126;
-        const int e1 = e / 2, e2 = e - e1;
-        // (a negative scale turns the query round, so that larger scores stay larger)
-        const float d1 = copysignf(__int_as_float((127 - e1) << 23), a.scale), d2 = __int_as_float((127 - e2) << 23);
-        if (lane == 0)
-          row_fac[r] = fabsf(a.scale) * 1.4426950408889634f * __int_as_float((127 + e1) << 23) * __int_as_float((127 + e2) << 23);
-        uint32_t hi[N / 2], lo[N / 2];
-#pragma unroll
-        for (int p = 0; p < N / 2; ++p) {
-          const float x = f[2 * p] * d1 * d2, y = f[2 * p + 1] * d1 * d2;
-          hi[p] = pack_f16(x, y);
-          if (PL == 2) lo[p] = pack_rest(x, y, hi[p]);
-        }
-        const int col = lane * N;
-        unsigned char* at = sq + (col >> 6) * (kRows * 128) + r * 128 + ((((col & 63) >> 3) ^ (r & 7)) << 4) + (col & 7) * 2;
-        if constexpr (N == 4) {
-          *reinterpret_cast<uint2*>(at) = make_uint2(hi[0], hi[1]);
-          if (PL == 2) *reinterpret_cast<uint2*>(at + L::kPlane) = make_uint2(lo[0], lo[1]);
-        } else {
-          *reinterpret_cast<uint32_t*>(at) = hi[0];
-          if (PL == 2) *reinterpret_cast<uint32_t*>(at + L::kPlane) = lo[0];
-        }
-      }
-    }
-    fence_async_smem();
-    top = warp_max(top);
-    if (lane == 0) red[warp] = top;
-  }
+  const Work t = work_of(a);
+  const int row0 = t.row0, start = t.start, count = t.count, tiles = t.tiles, nb = t.nb;
+  if (nb > 0) bring_q<HD, 1, true>(a, t, sq, row_fac, red, warp, lane);
   before_sync();
   __syncthreads();
   after_sync();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
   if (warp < 4) {
     // ---------------------------------------------------------------- softmax: thread = query row = TMEM lane
@@ -381,12 +512,7 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_tc_kernel(const PromptArgs
     const bool live = s < count;
     const int last = live ? min(start + s, a.c.capacity - 1) : -1;
     const float fac = nb > 0 ? row_fac[tid] : 0.f;
-    float top = 0.f, vref = 0.f;
-    if (nb > 0)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) top = fmaxf(top, red[i]);
-    if (top > 0.f)  // the power of two above it, 2^-100 at least
-      vref = fmaxf(__uint_as_float((__float_as_uint(top) + 0x7FFFFFu) & 0xFF800000u), 7.888609e-31f);
+    const float vref = nb > 0 ? vref_of(red) : 0.f;
     const float rvref = vref > 0.f ? __fdiv_rn(1.0f, vref) : 0.f;
     const uint32_t trow = tmem + ((uint32_t)(warp * 32) << 16);
     float m = kNone;
@@ -396,8 +522,8 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_tc_kernel(const PromptArgs
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
         const int tl = j * 4 + b;
-        kn[b] = tl < tiles ? __ldg(ks + tl) : 0.f;
-        vn[b] = tl < tiles ? __ldg(vs + tl) : 0.f;
+        kn[b] = tl < tiles ? __ldg(t.ks + tl) : 0.f;
+        vn[b] = tl < tiles ? __ldg(t.vs + tl) : 0.f;
       }
     };
     scales(0);
@@ -458,13 +584,12 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_tc_kernel(const PromptArgs
       }
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
-        uint32_t hi[8], lo[8];
+        uint32_t hi[8];
         if (partial)
-          weigh<PL, true>(x + 16 * b, f[b], m, w[b], last + 1 - pos0 - 16 * b, l, hi, lo);
+          weigh<1, true>(x + 16 * b, f[b], m, w[b], last + 1 - pos0 - 16 * b, l, hi, nullptr);
         else
-          weigh<PL, false>(x + 16 * b, f[b], m, w[b], 16, l, hi, lo);
+          weigh<1, false>(x + 16 * b, f[b], m, w[b], 16, l, hi, nullptr);
         tmem_st8(trow + kColP + 8 * b, hi);
-        if (PL == 2) tmem_st8(trow + kColP + 32 + 8 * b, lo);
       }
       tmem_st_wait();
       before_sync();
@@ -478,8 +603,7 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_tc_kernel(const PromptArgs
     const float total = sums.x + sums.y;
     const float inv = total == 0.f ? 0.f : __fdiv_rn(vref, total);
     // through shared memory (operands are idle now, 32 rows a warp), so that a row's stores are contiguous
-    constexpr int kPitch = HD + 4;  // floats; eight rows' 16-byte pieces hit distinct banks
-    static_assert(kRows * kPitch * 4 <= PL * L::kPlane + 2 * L::kK + L::kV, "the output reuses the operands");
+    static_assert(kRows * kPitch<HD> * 4 <= L::kPlane + 3 * L::kK, "the output reuses the operands");
     float* stage = reinterpret_cast<float*>(smem);
 #pragma unroll 1
     for (int c = 0; c < HD; c += 32) {
@@ -490,90 +614,22 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_tc_kernel(const PromptArgs
       }
 #pragma unroll
       for (int i = 0; i < 32; i += 4)
-        *reinterpret_cast<float4*>(stage + tid * kPitch + c + i) =
+        *reinterpret_cast<float4*>(stage + tid * kPitch<HD> + c + i) =
             nb > 0 ? make_float4(o[i] * inv, o[i + 1] * inv, o[i + 2] * inv, o[i + 3] * inv)
                    : make_float4(0.f, 0.f, 0.f, 0.f);
     }
     __syncwarp();
-    constexpr int kLanes = HD / 4, kPer = 32 / kLanes;  // lanes of a row, rows at a time
-    // (this lane's own row: s, rr)
-    const long long mine = rr < a.rows * a.group
-                               ? seq * a.o_seq + (long long)s * a.o_row + (long long)(kvh * a.group + rr - s * a.group) * HD
-                               : -1;
-    const int col = lane % kLanes * 4;
-#pragma unroll 1
-    for (int i0 = 0; i0 < 32; i0 += 8 * kPer) {
-      float4 o[8];  // (all read before the first store, which might alias them for all the compiler knows)
-      long long off[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int r = i0 + i * kPer + lane / kLanes;
-        o[i] = *reinterpret_cast<const float4*>(stage + (warp * 32 + r) * kPitch + col);
-        off[i] = __shfl_sync(0xffffffffu, mine, r);
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (off[i] < 0) continue;
-        const long long at = off[i] + col;
-        if constexpr (BF16) {
-          __nv_bfloat16* p = (__nv_bfloat16*)a.out + at;
-          __nv_bfloat162 v[2] = {__floats2bfloat162_rn(o[i].x, o[i].y), __floats2bfloat162_rn(o[i].z, o[i].w)};
-          if (a.o_vec) {
-            *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(v);
-          } else {
-            p[0] = v[0].x; p[1] = v[0].y; p[2] = v[1].x; p[3] = v[1].y;
-          }
-        } else {
-          float* p = (float*)a.out + at;
-          if (a.o_vec) {
-            *reinterpret_cast<float4*>(p) = o[i];
-          } else {
-            p[0] = o[i].x; p[1] = o[i].y; p[2] = o[i].z; p[3] = o[i].w;
-          }
-        }
-      }
-    }
+    write_rows<HD, true, 1>(a, stage + warp * 32 * kPitch<HD>, out_row(a, t, rr, HD), 0, lane);
   } else if (warp < 7) {
     // ---------------------------------------------------------------- K and V: int8 -> f16 operands
-    const int ct = tid - 128;
-    const int8_t* k = a.c.k + seq * a.c.seq_stride + (long long)kvh * a.c.capacity * HD;
-    const int8_t* v = a.c.v + seq * a.c.seq_stride + (long long)kvh * a.c.capacity * HD;
-    const int end = tiles * kKv8Block;  // tokens past it are zeros
-    constexpr int kPieces = kKeys * HD / 16, kN = (kPieces + kFill - 1) / kFill;  // 16 bytes of K or V, a thread's
-    uint4 kr[kN], vr[kN];
-    auto load = [&](const int8_t* src, int j, uint4* r) {
-#pragma unroll
-      for (int i = 0; i < kN; ++i) {
-        const int id = ct + i * kFill, tok = j * kKeys + id / (HD / 16);
-        r[i] = make_uint4(0, 0, 0, 0);
-        if (id < kPieces && tok < end)
-          r[i] = __ldg(reinterpret_cast<const uint4*>(src + (long long)tok * HD + id % (HD / 16) * 16));
-      }
-    };
-    auto store = [&](unsigned char* dst, const uint4* r) {
-#pragma unroll
-      for (int i = 0; i < kN; ++i) {
-        const int id = ct + i * kFill, row = id / (HD / 16), c = id % (HD / 16) * 2;  // 16-byte f16 chunks c, c + 1
-        if (id >= kPieces) break;
-        // lanes of the second 64 columns begin with their second chunk, so that eight lanes hit distinct banks
-        const bool swap = c & 8;
-        const uint32_t w[4] = {(swap ? r[i].z : r[i].x) ^ 0x80808080u, (swap ? r[i].w : r[i].y) ^ 0x80808080u,
-                               (swap ? r[i].x : r[i].z) ^ 0x80808080u, (swap ? r[i].y : r[i].w) ^ 0x80808080u};
-        unsigned char* p = dst + (c >> 3) * (kKeys * 128) + row * 128;
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          *reinterpret_cast<uint4*>(p + ((((c & 7) + (h ^ (int)swap)) ^ (row & 7)) << 4)) =
-              make_uint4(bytes_f16<0x4140>(w[2 * h]), bytes_f16<0x4342>(w[2 * h]), bytes_f16<0x4140>(w[2 * h + 1]),
-                         bytes_f16<0x4342>(w[2 * h + 1]));
-      }
-      fence_async_smem();
-    };
-    load(k, 0, kr);
-    load(v, 0, vr);
+    const int ct = tid - 128, end = tiles * kKv8Block;
+    Pieces<HD, kFill> kr, vr;
+    kr.load(t.k, 0, end, ct);
+    vr.load(t.v, 0, end, ct);
     auto put_k = [&](int j) {  // into its buffer, then the next block's loads
-      store(sk + (j & 1) * L::kK, kr);
+      kr.store(sk + (j & 1) * L::kK, ct);
       mbar_arrive(&k_full[j & 1]);
-      if (j + 1 < nb) load(k, j + 1, kr);
+      if (j + 1 < nb) kr.load(t.k, j + 1, end, ct);
     };
     if (nb > 0) put_k(0);
     for (int j = 0; j < nb; ++j) {
@@ -584,41 +640,36 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_tc_kernel(const PromptArgs
         put_k(j + 1);
       }
       if (j > 0 && !wait(o_done, (uint32_t)(j - 1) & 1u, gave_up, 47)) break;
-      store(sv, vr);
+      vr.store(sv, ct);
       mbar_arrive(v_full);
-      if (j + 1 < nb) load(v, j + 1, vr);
+      if (j + 1 < nb) vr.load(t.v, j + 1, end, ct);
     }
-  } else if (lane == 0 && nb > 0) {
+  } else if (nb > 0) {
     // ---------------------------------------------------------------- products
     const uint32_t qa = smem_u32(sq), ka = smem_u32(sk), va = smem_u32(sv);
     auto qk = [&](int j) {
-      if (!wait(&k_full[j & 1], (uint32_t)(j >> 1) & 1u, gave_up, 41)) return;
+      if (!warp_wait(&k_full[j & 1], (uint32_t)(j >> 1) & 1u, gave_up, 41)) return;
       after_sync();
       const uint32_t kb = ka + (uint32_t)(j & 1) * L::kK;
 #pragma unroll
-      for (int pl = 0; pl < PL; ++pl)
-#pragma unroll
-        for (int kk = 0; kk < HD / 16; ++kk)
-          mma_ss(tmem + kColS, sw128_desc(qa + pl * L::kPlane + (kk >> 2) * (kRows * 128) + (kk & 3) * 32),
-                 sw128_desc(kb + (kk >> 2) * (kKeys * 128) + (kk & 3) * 32), idesc_f16(kKeys, false),
-                 (pl > 0 || kk > 0) ? 1u : 0u);
+      for (int kk = 0; kk < HD / 16; ++kk)
+        mma_ss(tmem + kColS, sw128_desc(qa + (kk >> 2) * (kRows * 128) + (kk & 3) * 32),
+               sw128_desc(kb + (kk >> 2) * (kKeys * 128) + (kk & 3) * 32), idesc_f16(kKeys, false), kk > 0 ? 1u : 0u);
       commit(s_full);
       commit(&k_free[j & 1]);
     };
     qk(0);
-    for (int j = 0; j < nb && !*gave_up; ++j) {
+    for (int j = 0; j < nb; ++j) {
       if (j + 1 < nb) {
-        if (!wait(s_free, (uint32_t)j & 1u, gave_up, 48)) break;
+        if (!warp_wait(s_free, (uint32_t)j & 1u, gave_up, 48)) break;
         qk(j + 1);
       }
-      if (!wait(v_full, (uint32_t)j & 1u, gave_up, 42) || !wait(p_full, (uint32_t)j & 1u, gave_up, 49)) break;
+      if (!warp_wait(v_full, (uint32_t)j & 1u, gave_up, 42) || !warp_wait(p_full, (uint32_t)j & 1u, gave_up, 49)) break;
       after_sync();
 #pragma unroll
-      for (int pl = 0; pl < PL; ++pl)
-#pragma unroll
-        for (int kk = 0; kk < kKeys / 16; ++kk)
-          mma_ts(tmem + kColO, tmem + kColP + pl * 32 + kk * 8, sw128_desc(va + kk * 2048, kKeys * 128),
-                 idesc_f16(HD, true), (j > 0 || pl > 0 || kk > 0) ? 1u : 0u);
+      for (int kk = 0; kk < kKeys / 16; ++kk)
+        mma_ts(tmem + kColO, tmem + kColP + kk * 8, sw128_desc(va + kk * 2048, kKeys * 128), idesc_f16(HD, true),
+               (j > 0 || kk > 0) ? 1u : 0u);
       commit(o_done);
     }
   }
@@ -628,15 +679,282 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_tc_kernel(const PromptArgs
   if (warp == 7) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols));
 }
 
-template <int HD, int PL>
+// ------------------------------------------------------------------ f32 rows: two planes, one CTA an SM
+constexpr int kThreads2 = 512, kFillV = 96;
+// TMEM columns: S, P's planes and O of two blocks each
+constexpr uint32_t kS2 = 0, kP2 = 128, kO2 = 256, kCols2 = 512;
+
+// Warps 0-7 softmax: two threads a row, each half the block's keys and half the output's dims, whose sums
+// it keeps in f32 registers: every block's product starts from zero and is added there. (Accumulated in
+// TMEM over all blocks, the tensor core's rounding towards zero shrank the output by 4e-8 a product:
+// 1.7e-6 at 1400 keys, and growing.) Warps 8-11 bring K and 12-14 V, two blocks ahead in registers, one
+// thread of warp 15 issues the products. The softmax warps take the registers that the others leave:
+// 256 x (168 + 88) = 512 x 128.
+template <int HD>
+__global__ void __launch_bounds__(kThreads2, 1) prompt_f32_kernel(const PromptArgs a) {
+  using L = Smem<HD>;
+  extern __shared__ __align__(1024) unsigned char smem[];
+  unsigned char *sq = smem, *sk = smem + 2 * L::kPlane, *sv = sk + 2 * L::kK;
+  float* row_fac = reinterpret_cast<float*>(sv + 2 * L::kK);  // each row's factor
+  float* row_max = row_fac + kRows;                           // [block parity][half][row]
+  float* row_sum = row_max + 4 * kRows;                       // [row] the second half's sum
+  float* red = row_sum + kRows;                               // the largest V scale of each warp's tiles
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(red + 8);
+  uint64_t *k_free = k_full + 2, *v_full = k_full + 4, *v_free = k_full + 6, *s_full = k_full + 8, *s_free = k_full + 10,
+           *o_full = k_full + 12, *o_free = k_full + 14, *p_full = k_full + 16;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(k_full + 18);
+  volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;  // (uniform)
+  if (smem_u32(smem) & 1023) {
+    if (tid == 0) atomicExch(&g_prompt_err, 40);
+    return;
+  }
+  if (tid == 0) {
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&k_full[b], 128);
+      mbar_init(&k_free[b], 1);
+      mbar_init(&v_full[b], kFillV);
+      mbar_init(&v_free[b], 1);
+      mbar_init(&s_full[b], 1);
+      mbar_init(&s_free[b], 256);
+      mbar_init(&o_full[b], 1);  // P V of a block is done: its O may be read, P overwritten
+      mbar_init(&o_free[b], 256);
+      mbar_init(&p_full[b], 256);
+    }
+    *gave_up = 0;
+    fence_mbar_init();
+  }
+  if (warp == 15) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(kCols2));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  pdl_launch_dependents();
+  pdl_wait();
+  const Work t = work_of(a);
+  const int nb = t.nb;
+  if (nb > 0 && warp < 8) bring_q<HD, 2, false>(a, t, sq, row_fac, red, warp, lane);
+  before_sync();
+  __syncthreads();
+  after_sync();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+
+  if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+    // ---------------------------------------------------------------- softmax: row = TMEM lane
+    constexpr int kDims = HD / 2;
+    const int half = warp >> 2, row = (warp & 3) * 32 + lane, rr = t.row0 + row, s = rr / a.group;
+    const int last = s < t.count ? min(t.start + s, a.c.capacity - 1) : -1;
+    const float fac = nb > 0 ? row_fac[row] : 0.f, vref = nb > 0 ? vref_of(red) : 0.f;
+    const float rvref = vref > 0.f ? __fdiv_rn(1.0f, vref) : 0.f;
+    const uint32_t trow = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    float m = kNone;
+    f32x2 l = 0, acc[kDims / 2];
+#pragma unroll
+    for (f32x2& x : acc) x = 0;
+    float kn[2], vn[2];  // the next block's scales, of this half's two tiles
+    auto scales = [&](int j) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const int tl = j * 4 + half * 2 + b;
+        kn[b] = tl < t.tiles ? __ldg(t.ks + tl) : 0.f;
+        vn[b] = tl < t.tiles ? __ldg(t.vs + tl) : 0.f;
+      }
+    };
+    auto add_o = [&](int j) {  // acc += O of block j, whose buffer is free then
+      const uint32_t col = trow + kO2 + (uint32_t)((j & 1) * HD + half * kDims);
+#pragma unroll
+      for (int c = 0; c < kDims; c += 32) {
+        float o[32];
+        tmem_ld32(col + c, reinterpret_cast<uint32_t*>(o));
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[c / 2 + i] = add2(acc[c / 2 + i], pair(o[2 * i], o[2 * i + 1]));
+      }
+      before_sync();
+      mbar_arrive(&o_free[j & 1]);
+    };
+    scales(0);
+    for (int j = 0; j < nb; ++j) {
+      float f[2], w[2];
+      const int pos0 = j * kKeys + half * 32;
+      const bool partial = __any_sync(0xffffffffu, pos0 + 31 > last);
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        f[b] = fac * kn[b];
+        w[b] = vn[b] * rvref;
+        // a row that sees nothing of a tile takes nothing of its scale either
+        if (partial && pos0 + b * kKv8Block > last) w[b] = 0.f;
+      }
+      if (j + 1 < nb) scales(j + 1);
+      wait(&s_full[j & 1], (uint32_t)(j >> 1) & 1u, gave_up, 51);
+      __syncwarp();
+      after_sync();
+      float x[32];
+      tmem_ld32(trow + kS2 + (uint32_t)((j & 1) * kKeys + half * 32), reinterpret_cast<uint32_t*>(x));
+      tmem_ld_wait();
+      before_sync();
+      mbar_arrive(&s_free[j & 1]);
+      if (partial) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (pos0 + i > last) x[i] = -__int_as_float(0x7F800000);
+      }
+      float mx = kNone;
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        float top = x[16 * b];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) top = fmaxf(top, x[16 * b + i]);
+        mx = fmaxf(mx, top * f[b]);  // (a masked tile's -inf, or no number: ignored)
+      }
+      // the row's maximum over both halves (two buffers: the next block's barrier keeps them apart)
+      float* shared_max = row_max + (j & 1) * 2 * kRows;
+      shared_max[half * kRows + row] = mx;
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      mx = fmaxf(mx, shared_max[(half ^ 1) * kRows + row]);
+      const bool grow = mx > m + 8.f;
+      const float corr = grow ? ex2(m - mx) : 1.f;
+      const bool rescale = __any_sync(0xffffffffu, grow);
+      if (grow) m = mx;
+      if (rescale) l = mul2(l, pair(corr, corr));
+      // (P of block j - 2 has been read: its O was added in the last round)
+      const uint32_t pcol = trow + kP2 + (uint32_t)((j & 1) * 64 + half * 16);
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        uint32_t hi[8], lo[8];
+        if (partial)
+          weigh<2, true>(x + 16 * b, f[b], m, w[b], last + 1 - pos0 - 16 * b, l, hi, lo);
+        else
+          weigh<2, false>(x + 16 * b, f[b], m, w[b], 16, l, hi, lo);
+        tmem_st8(pcol + 8 * b, hi);
+        tmem_st8(pcol + 32 + 8 * b, lo);
+      }
+      tmem_st_wait();
+      before_sync();
+      mbar_arrive(&p_full[j & 1]);
+      if (j > 0) {  // beside this block's product
+        wait(&o_full[(j - 1) & 1], (uint32_t)((j - 1) >> 1) & 1u, gave_up, 52);
+        __syncwarp();
+        after_sync();
+        add_o(j - 1);
+      }
+      if (rescale) {
+#pragma unroll
+        for (f32x2& y : acc) y = mul2(y, pair(corr, corr));
+      }
+    }
+    if (nb > 0) {
+      wait(&o_full[(nb - 1) & 1], (uint32_t)((nb - 1) >> 1) & 1u, gave_up, 53);
+      __syncwarp();
+      after_sync();
+      add_o(nb - 1);
+    }
+    // ---- O * vref / l, through shared memory, so that a row's stores are contiguous
+    const float2 sums = split(l);
+    float total = sums.x + sums.y;
+    if (half == 1) row_sum[row] = total;
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    if (half == 0) row_sum[row] += total;
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    total = row_sum[row];
+    const float inv = total == 0.f ? 0.f : __fdiv_rn(vref, total);
+    static_assert(kRows * kPitch<HD> * 4 <= 2 * L::kPlane + 4 * L::kK, "the output reuses the operands");
+    float* stage = reinterpret_cast<float*>(smem);
+#pragma unroll
+    for (int i = 0; i < kDims / 2; i += 2) {
+      const float2 p = split(acc[i]), q = split(acc[i + 1]);
+      *reinterpret_cast<float4*>(stage + row * kPitch<HD> + half * kDims + 2 * i) =
+          make_float4(p.x * inv, p.y * inv, q.x * inv, q.y * inv);
+    }
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    write_rows<HD, false, 2>(a, stage + (warp & 3) * 32 * kPitch<HD>, out_row(a, t, rr, HD), half, lane);
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    const int end = t.tiles * kKv8Block;
+    // one operand's blocks in turn: two in registers, each stored when its buffer is free
+    auto fill = [&](auto& even, auto& odd, const int8_t* src, unsigned char* dst, uint64_t* full, uint64_t* free, int ct) {
+      even.load(src, 0, end, ct);
+      if (nb > 1) odd.load(src, 1, end, ct);
+      for (int j = 0; j < nb; j += 2) {
+        const uint32_t before = (uint32_t)((j >> 1) - 1) & 1u;  // the phase in which block j - 2 left the buffer
+        if (j >= 2 && !wait(&free[0], before, gave_up, 54)) break;
+        even.store(dst, ct);
+        mbar_arrive(&full[0]);
+        if (j + 2 < nb) even.load(src, j + 2, end, ct);
+        if (j + 1 >= nb) break;
+        if (j >= 2 && !wait(&free[1], before, gave_up, 55)) break;
+        odd.store(dst + L::kK, ct);
+        mbar_arrive(&full[1]);
+        if (j + 3 < nb) odd.load(src, j + 3, end, ct);
+      }
+    };
+    if (warp < 12) {
+      // -------------------------------------------------------------- K: int8 -> f16 operand
+      Pieces<HD, 128> even, odd;
+      fill(even, odd, t.k, sk, k_full, k_free, tid - 256);
+    } else if (warp < 15) {
+      // -------------------------------------------------------------- V
+      Pieces<HD, kFillV> even, odd;
+      fill(even, odd, t.v, sv, v_full, v_free, tid - 384);
+    } else if (nb > 0) {
+    // ---------------------------------------------------------------- products
+    const uint32_t qa = smem_u32(sq), ka = smem_u32(sk), va = smem_u32(sv);
+    auto qk = [&](int j) {
+      const int b = j & 1;
+      if (j >= 2 && !warp_wait(&s_free[b], (uint32_t)((j - 2) >> 1) & 1u, gave_up, 56)) return;
+      if (!warp_wait(&k_full[b], (uint32_t)(j >> 1) & 1u, gave_up, 57)) return;
+      after_sync();
+#pragma unroll
+      for (int pl = 0; pl < 2; ++pl)
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; ++kk)
+          mma_ss(tmem + kS2 + (uint32_t)(b * kKeys),
+                 sw128_desc(qa + pl * L::kPlane + (kk >> 2) * (kRows * 128) + (kk & 3) * 32),
+                 sw128_desc(ka + b * L::kK + (kk >> 2) * (kKeys * 128) + (kk & 3) * 32), idesc_f16(kKeys, false),
+                 (pl > 0 || kk > 0) ? 1u : 0u);
+      commit(&s_full[b]);
+      commit(&k_free[b]);
+    };
+    qk(0);
+    for (int j = 0; j < nb; ++j) {
+      const int b = j & 1;
+      if (j + 1 < nb) qk(j + 1);
+      if (!warp_wait(&v_full[b], (uint32_t)(j >> 1) & 1u, gave_up, 58) || !warp_wait(&p_full[b], (uint32_t)(j >> 1) & 1u, gave_up, 59)) break;
+      if (j >= 2 && !warp_wait(&o_free[b], (uint32_t)((j - 2) >> 1) & 1u, gave_up, 60)) break;
+      after_sync();
+#pragma unroll
+      for (int pl = 0; pl < 2; ++pl)
+#pragma unroll
+        for (int kk = 0; kk < kKeys / 16; ++kk)
+          mma_ts(tmem + kO2 + (uint32_t)(b * HD), tmem + kP2 + (uint32_t)(b * 64) + pl * 32 + kk * 8,
+                 sw128_desc(va + b * L::kK + kk * 2048, kKeys * 128), idesc_f16(HD, true), (pl > 0 || kk > 0) ? 1u : 0u);
+      commit(&o_full[b]);
+      commit(&v_free[b]);
+    }
+    }
+  }
+  __syncwarp();
+  before_sync();
+  __syncthreads();
+  if (warp == 15) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols2));
+}
+
+template <int HD, bool BF16>
 cudaError_t launch(const PromptArgs& a, cudaStream_t s) {
-  static OncePerDevice once;
-  const cudaError_t e = once.smem(prompt_tc_kernel<HD, PL>, Smem<HD, PL>::kBytes);
-  if (e != cudaSuccess) return e;
   const long long ctas = ((long long)a.rows * a.group + kRows - 1) / kRows * a.c.n_kv * a.c.n_seq;
   if (ctas > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
   const dim3 g((unsigned)ctas);
-  return ops_launch(prompt_tc_kernel<HD, PL>, g, dim3(kThreads), Smem<HD, PL>::kBytes, s, 1, a);
+  static OncePerDevice once;
+  if constexpr (BF16) {
+    const cudaError_t e = once.smem(prompt_bf16_kernel<HD>, Smem<HD>::kBytes1);
+    if (e != cudaSuccess) return e;
+    return ops_launch(prompt_bf16_kernel<HD>, g, dim3(kThreads), Smem<HD>::kBytes1, s, 1, a);
+  } else {
+    const cudaError_t e = once.smem(prompt_f32_kernel<HD>, Smem<HD>::kBytes2);
+    if (e != cudaSuccess) return e;
+    return ops_launch(prompt_f32_kernel<HD>, g, dim3(kThreads2), Smem<HD>::kBytes2, s, 1, a);
+  }
 }
 
 }  // namespace
@@ -650,8 +968,8 @@ cudaError_t kv8_prompt_attention(const Kv8& c, const void* q, long long q_seq, l
   };
   const PromptArgs a{c, q, out, q_seq, q_row, o_seq, o_row, starts, counts, idx_stride, rows, heads / c.n_kv, scale,
                      vec(q, q_seq, q_row), vec(out, o_seq, o_row)};
-  if (c.head_dim == 128) return dt == OPS_BF16 ? launch<128, 1>(a, s) : launch<128, 2>(a, s);
-  return dt == OPS_BF16 ? launch<64, 1>(a, s) : launch<64, 2>(a, s);
+  if (c.head_dim == 128) return dt == OPS_BF16 ? launch<128, true>(a, s) : launch<128, false>(a, s);
+  return dt == OPS_BF16 ? launch<64, true>(a, s) : launch<64, false>(a, s);
 }
 
 int kv8_prompt_error() {
