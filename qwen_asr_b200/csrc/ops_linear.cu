@@ -74,24 +74,40 @@ __device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr) {
   return d;
 }
 
-__device__ __forceinline__ void tma_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+// The copies and products are issued by an elected lane of a warp that waits and counts together: their
+// operands are uniform registers, which a branch of one lane would have to fill anew each time (8 x 12288
+// x 2048 7.2 us so, 5.2 now; 64 tokens 9.1 and 7.4; 381 x 4096 x 2048 11.2 and 9.5).
+// Both tiles of a stage, which are `bytes` together.
+__device__ __forceinline__ void tma_pair(void* dst_w, const CUtensorMap* map_w, int ch, void* dst_x, const CUtensorMap* map_x,
+                                         int m, int k, uint32_t bytes, uint64_t* bar) {
   asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
-          smem_u32(dst)),
-      "l"((uint64_t)map), "r"(x), "r"(y), "r"(smem_u32(bar))
+      "{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n"
+      " @e mbarrier.arrive.expect_tx.shared::cta.b64 _, [%7], %8;\n"
+      " @e cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%6, %2}], [%7];\n"
+      " @e cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%3], [%4, {%6, %5}], [%7];\n}\n" ::"r"(
+          smem_u32(dst_w)),
+      "l"((uint64_t)map_w), "r"(ch), "r"(smem_u32(dst_x)), "l"((uint64_t)map_x), "r"(m), "r"(k), "r"(smem_u32(bar)),
+      "r"(bytes)
       : "memory");
 }
 
 __device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accum) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "{\n .reg .pred e, p;\n elect.sync _|e, 0xffffffff;\n setp.ne.b32 p, %4, 0;\n"
+      " @e tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
       "l"(a), "l"(b), "r"(idesc), "r"(accum));
 }
 
 __device__ __forceinline__ void commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-               : "memory");
+  asm volatile(
+      "{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n"
+      " @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(bar))
+      : "memory");
+}
+
+// A wait of a whole warp, as one answer.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int code) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, &g_wait_err, code));
 }
 
 #define QASR_R8(r, i) "=r"((r)[i]), "=r"((r)[i + 1]), "=r"((r)[i + 2]), "=r"((r)[i + 3]), "=r"((r)[i + 4]), \
@@ -227,7 +243,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
   uint64_t* acc_empty = acc_full + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const int rank = a.split > 1 ? blockIdx.x % a.split : 0;
   const int unit0 = a.split > 1 ? blockIdx.x / a.split : blockIdx.x;
   const int step = a.split > 1 ? a.tiles : gridDim.x;  // a split tile's CTAs have one unit each
@@ -253,60 +269,54 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
   asm volatile("tcgen05.fence::before_thread_sync;");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;");
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   pdl_launch_dependents();
   pdl_wait();
 
   if (warp == 0) {
-    if (lane == 0) {
-      int it = 0;
-      for (int u = unit0; u < a.tiles && !*abort_flag; u += step) {
-        const int ch0 = u % a.ct * kCh, m0 = u / a.ct * a.nt;
-        for (int kt = k0; kt < k1; ++kt, ++it) {
-          const int st = it % ST;
-          if (it >= ST && !mbar_wait(&empty[st], (uint32_t)((it / ST) - 1) & 1u, &g_wait_err, 31)) {
-            *abort_flag = 1;
-            break;
-          }
-          unsigned char* sp = smem + st * S::kStage;
-          mbar_expect_tx(&full[st], kCh * kKb + a.nt * kKb);
-          tma_2d(sp, &map_w, kt * kKb, ch0, &full[st]);
-          tma_2d(sp + kCh * kKb, &map_x, kt * kKb, m0, &full[st]);
+    int it = 0;
+    for (int u = unit0; u < a.tiles && !__any_sync(0xffffffffu, *abort_flag); u += step) {
+      const int ch0 = u % a.ct * kCh, m0 = u / a.ct * a.nt;
+      for (int kt = k0; kt < k1; ++kt, ++it) {
+        const int st = it % ST;
+        if (it >= ST && !warp_wait(&empty[st], (uint32_t)((it / ST) - 1) & 1u, 31)) {
+          *abort_flag = 1;
+          break;
         }
+        unsigned char* sp = smem + st * S::kStage;
+        tma_pair(sp, &map_w, ch0, sp + kCh * kKb, &map_x, m0, kt * kKb, kCh * kKb + a.nt * kKb, &full[st]);
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      const uint32_t idesc = idesc_i8(a.nt);
-      int it = 0, lt = 0;
-      for (int u = unit0; u < a.tiles && !*abort_flag; u += step, ++lt) {
-        const int ab = lt & 1;
-        if (lt >= 2 && !mbar_wait(&acc_empty[ab], (uint32_t)((lt >> 1) - 1) & 1u, &g_wait_err, 32)) {
-          *abort_flag = 1;
+    const uint32_t idesc = idesc_i8(a.nt);
+    int it = 0, lt = 0;
+    for (int u = unit0; u < a.tiles && !__any_sync(0xffffffffu, *abort_flag); u += step, ++lt) {
+      const int ab = lt & 1;
+      if (lt >= 2 && !warp_wait(&acc_empty[ab], (uint32_t)((lt >> 1) - 1) & 1u, 32)) {
+        *abort_flag = 1;
+        break;
+      }
+      asm volatile("tcgen05.fence::after_thread_sync;");
+      const uint32_t acc = tmem + (uint32_t)(ab * NT);
+      bool ok = true;
+      for (int kt = k0; kt < k1; ++kt, ++it) {
+        const int st = it % ST;
+        if (!warp_wait(&full[st], (uint32_t)(it / ST) & 1u, 33)) {
+          ok = false;
           break;
         }
         asm volatile("tcgen05.fence::after_thread_sync;");
-        const uint32_t acc = tmem + (uint32_t)(ab * NT);
-        bool ok = true;
-        for (int kt = k0; kt < k1; ++kt, ++it) {
-          const int st = it % ST;
-          if (!mbar_wait(&full[st], (uint32_t)(it / ST) & 1u, &g_wait_err, 33)) {
-            ok = false;
-            break;
-          }
-          asm volatile("tcgen05.fence::after_thread_sync;");
-          const uint32_t sw = smem_u32(smem + st * S::kStage), sx = sw + kCh * kKb;
+        const uint32_t sw = smem_u32(smem + st * S::kStage), sx = sw + kCh * kKb;
 #pragma unroll
-          for (int kk = 0; kk < kKb / 32; ++kk)
-            mma_i8(acc, sw128_desc(sw + kk * 32), sw128_desc(sx + kk * 32), idesc, (kt > k0 || kk > 0) ? 1u : 0u);
-          commit(&empty[st]);
-        }
-        if (!ok) {
-          *abort_flag = 1;
-          break;
-        }
-        commit(&acc_full[ab]);
+        for (int kk = 0; kk < kKb / 32; ++kk)
+          mma_i8(acc, sw128_desc(sw + kk * 32), sw128_desc(sx + kk * 32), idesc, (kt > k0 || kk > 0) ? 1u : 0u);
+        commit(&empty[st]);
       }
+      if (!ok) {
+        *abort_flag = 1;
+        break;
+      }
+      commit(&acc_full[ab]);
     }
   } else {
     const int q = warp & 3, half = (warp - 2) >> 2;  // TMEM lane quarter and token half of this warp
@@ -463,10 +473,10 @@ cudaError_t linear_int8(const int8_t* xq, long long ldx, const float* xs, const 
   // Tile width and K split with the least estimated time in cycles. A step of 128 bytes of K takes 2
   // for each of the 128 + nt rows it brings from L2 (64 bytes a cycle and SM; the products take 2
   // nt), a tile's epilogue about 8 nt beside the next tile's products, and a split's join 2000.
-  // Measured against all widths and splits at 16 shapes, the choice is within 6 % of the best
-  // (9 % at 32 x 4096 x 2048); e.g. 8191 x 2048 x 6144: 224 tokens 93 us (592 tiles, four full
-  // waves), 256 tokens 101 us, 128 tokens 118 us; 381 x 2048 x 6144: 192 tokens in 4 splits 13.3
-  // us, 96 in 2 15.7 us, 128 unsplit 22 us; 8 x 2048 x 6144: 8 splits 7.7 us, 1 split 17 us.
+  // Measured against all widths and splits at 16 shapes, the choice is within 8 % of the best
+  // (12 % at 32 x 4096 x 2048); e.g. 8191 x 2048 x 6144: 224 tokens 90 us (592 tiles, four full
+  // waves), 256 or 128 tokens 94 us, 160 107 us; 381 x 2048 x 6144: 192 tokens in 4 splits 11.9 us,
+  // 96 in 2 11.2 us, the worst 32 us; 8 x 2048 x 6144: 8 splits 5.2 us, 4 4.9 us, the worst 9.4 us.
   long long best = -1;
   static const int widths[] = {16, 32, 64, 96, 128, 160, 192, 224, 256};
   for (int nt : widths) {
