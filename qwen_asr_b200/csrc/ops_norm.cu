@@ -17,7 +17,7 @@
 // value, rounding by the 1.5 * 2^23 trick whose low byte is the int8 value, and a warp that adds up
 // the squares behind the barrier while the others quantise (they do not need the norm). 16411
 // rows of 2048 bf16 values with a residual: 89 us with a shuffled (f64, u64) reduction and
-// per-value conversions, @NORM_MANY@ so.
+// per-value conversions, 46 us so (alone on the GPU; 68 us in a row, 3.5 TB/s; f32 67 us, 6.6 TB/s).
 #include <cuda_bf16.h>
 
 #include "bulk.cuh"
