@@ -16,8 +16,7 @@
 // Bound: DRAM for many rows. What it took to get near: a bf16 sum as packed adds, one fmax a
 // value, rounding by the 1.5 * 2^23 trick whose low byte is the int8 value, and a warp that adds up
 // the squares behind the barrier while the others quantise (they do not need the norm). 16411
-// rows of 2048 bf16 values with a residual: 89 us with a shuffled (f64, u64) reduction and
-// per-value conversions, 46 us so (alone on the GPU; 68 us in a row, 3.5 TB/s; f32 67 us, 6.6 TB/s).
+// rows of 2048 bf16 values with a residual, call after call: 44 us, 5.3 TB/s; f32 67 us, 6.6 TB/s.
 #include <cuda_bf16.h>
 
 #include "bulk.cuh"
@@ -146,11 +145,31 @@ __device__ __forceinline__ float max_nan(float a, float b) {  // NaN when either
 
 constexpr float kRound = 12582912.f;  // 1.5 * 2^23: adding it rounds to an integer, in the low bits
 
+// A thread's int8 values whose bit is set once more, from the exact products; its vectors of V are `step`
+// vectors apart. (The value is read back from memory: an index into the registers would push them all to the
+// stack. One row in eight has such a value: a thread that did all of its own again, one after the other, cost
+// 16411 bf16 rows of 2048 68 us, finding them by a second look 47 to 51, this 44.)
+template <bool BF16, int V>
+__device__ __forceinline__ void fix_near(const NormArgs& a, long long row, double top64, int step, uint32_t mask) {
+  using T = typename Elem<BF16>::T;
+  const T* src = a.h ? (const T*)a.h + row * a.ldh : (const T*)a.x + row * a.ldx;
+  int8_t* q = a.q + row * a.ldq;
+  while (mask) {
+    const int b = __ffs((int)mask) - 1;
+    mask &= mask - 1;
+    const int c = ((int)threadIdx.x + b / V * step) * V + b % V;
+    if (c >= a.d) break;
+    const double w = a.w ? (double)a.w[c] : 1.0;
+    q[c] = (int8_t)__double2int_rn((double)Elem<BF16>::load(src + c) * w * 127.0 / top64);
+  }
+}
+
 // One row by W warps, its values in registers: NV vectors a thread.
 template <bool BF16, int W, int NV>
 __global__ void __launch_bounds__(W * 32) norm_vec_kernel(const NormArgs a) {
   using T = typename Elem<BF16>::T;
   constexpr int V = Elem<BF16>::kVec, N = W * 32;
+  static_assert(NV * V <= 32, "a bit a value");
   __shared__ double parts[N];
   __shared__ unsigned tops[W];
   __shared__ unsigned low;  // ordered bits of the largest product's rounding error
@@ -236,7 +255,7 @@ __global__ void __launch_bounds__(W * 32) norm_vec_kernel(const NormArgs a) {
     }
   }
   const float r127 = finite && top ? __fdiv_rn(127.0f, __uint_as_float(top)) : 0.f;
-  bool near = r127 > 3e38f;  // 127 / top overflowed: a row of subnormals takes the exact path
+  uint32_t near = r127 > 3e38f ? ~0u : 0u;  // 127 / top overflowed: a row of subnormals takes the exact path
   int8_t* q = a.q + row * a.ldq;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
@@ -250,7 +269,7 @@ __global__ void __launch_bounds__(W * 32) norm_vec_kernel(const NormArgs a) {
         const float v = __fmul_rn(u[j][i + k], r127);
         const float t = __fadd_rn(v, kRound);
         b[k] = __float_as_uint(t);
-        near |= fabsf(__fsub_rn(v, __fsub_rn(t, kRound))) > 0.5f - 3.2e-5f;
+        if (fabsf(__fsub_rn(v, __fsub_rn(t, kRound))) > 0.5f - 3.2e-5f) near |= 1u << (j * V + i + k);
       }
       o[i / 4] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
       if (!finite) o[i / 4] = 0u;
@@ -264,20 +283,7 @@ __global__ void __launch_bounds__(W * 32) norm_vec_kernel(const NormArgs a) {
   }
   __syncthreads();  // `low` is complete
   const double top64 = (double)__uint_as_float(top) + (double)ordered_to_float((int)(low ^ 0x80000000u));
-  if (near && finite) {
-#pragma unroll 1
-    for (int j = 0; j < NV; ++j) {
-      const int c = (threadIdx.x + j * N) * V;
-      if (c < a.d)
-#pragma unroll 1
-        for (int i = 0; i < V; ++i) {
-          // (the row again from memory: an index into the registers would push them all to the stack)
-          const T* src = a.h ? (const T*)a.h + row * a.ldh : x;
-          const double w = a.w ? (double)a.w[c + i] : 1.0;
-          q[c + i] = (int8_t)__double2int_rn((double)Elem<BF16>::load(src + c + i) * w * 127.0 / top64);
-        }
-    }
-  }
+  if (near && finite) fix_near<BF16, V>(a, row, top64, N, near);
   if (warp == 0) {
     double sum = 0.0;
 #pragma unroll
