@@ -14,14 +14,17 @@
 // Schedule. Warp 0 issues TMA into a ring, warp 1 issues four MMAs (K = 32 each) a stage, warps
 // 2-9 drain the accumulator (two warps a TMEM lane quarter, half the tokens each; the residual's
 // loads run one chunk ahead). Many tiles: a persistent grid with two accumulators, so that one
-// tile's epilogue runs behind the next one's products. Few tiles (fewer than the SMs): a cluster
+// tile's epilogue runs behind the next one's products; for a long K by pairs of CTAs, whose tensor
+// cores share the tokens' rows (256 channels a tile). Few tiles (fewer than the SMs): a cluster
 // of 2 to 8 CTAs splits K, each leaves its int32 partial tile in its own shared memory, and after
 // one cluster barrier every CTA adds up its share of the tokens over distributed shared memory.
 // No workspace, no atomics.
 //
-// Bound: weight bytes from DRAM up to some 100 tokens, the tensor cores beyond.
+// Bound: weight bytes from DRAM up to some 100 tokens; beyond, the operands' way from L2 for single CTAs, the
+// tensor cores for pairs (8192^3: 2850 TOP/s, bf16 out 3060).
 #include <cuda.h>
 
+#include <algorithm>
 #include <mutex>
 
 #include "bulk.cuh"
@@ -40,18 +43,18 @@ constexpr int kMaxCluster = 8;
 
 __device__ int g_wait_err;  // nonzero once a bounded wait gave up
 
-template <int NT>
+template <int NT, bool PAIR = false>
 struct Shape {
-  static constexpr int kStage = kCh * kKb + NT * kKb;
-  static constexpr int kStages = NT >= 256 ? 4 : NT >= 128 ? 6 : NT >= 64 ? 4 : NT >= 32 ? 5 : 6;
+  static constexpr int kStage = kCh * kKb + (PAIR ? NT / 2 : NT) * kKb;
+  static constexpr int kStages = PAIR ? 6 : NT >= 256 ? 4 : NT >= 128 ? 6 : NT >= 64 ? 4 : NT >= 32 ? 5 : 6;
   static constexpr int kHalf = NT / 2;                       // tokens of an epilogue warp
   static constexpr int kSmem = 1024 + kStages * kStage + kEpiWarps * kHalf * 4 + 256;
   static_assert(kStages * kStage >= NT * kCh * 4, "the partial tile reuses the ring");
 };
 
-// Instruction descriptor: int32 accumulator, signed 8-bit A and B, both K-major, M = 128, N = nt.
-__device__ __forceinline__ uint32_t idesc_i8(int nt) {
-  return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(nt >> 3) << 17) | ((uint32_t)(kCh >> 4) << 24);
+// Instruction descriptor: int32 accumulator, signed 8-bit A and B, both K-major, M = channels, N = nt.
+__device__ __forceinline__ uint32_t idesc_i8(int nt, int channels) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(nt >> 3) << 17) | ((uint32_t)(channels >> 4) << 24);
 }
 
 struct LinArgs {
@@ -91,15 +94,48 @@ __device__ __forceinline__ void tma_pair(void* dst_w, const CUtensorMap* map_w, 
       : "memory");
 }
 
-__device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accum) {
+// The same for one CTA of a pair, whose shares all complete on the first CTA's barrier (`bar`, as a cluster
+// address); that CTA expects the bytes of both (0: the second CTA).
+__device__ __forceinline__ void tma_pair2(void* dst_w, const CUtensorMap* map_w, int ch, void* dst_x,
+                                          const CUtensorMap* map_x, int m, int k, uint32_t bytes, uint64_t* own,
+                                          uint32_t bar) {
   asm volatile(
+      "{\n .reg .pred e, f;\n elect.sync _|e, 0xffffffff;\n setp.ne.and.u32 f, %8, 0, e;\n"
+      " @f mbarrier.arrive.expect_tx.shared::cta.b64 _, [%9], %8;\n"
+      " @e cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%6, %2}], [%7];\n"
+      " @e cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%3], [%4, {%6, %5}], [%7];\n}\n" ::"r"(
+          smem_u32(dst_w)),
+      "l"((uint64_t)map_w), "r"(ch), "r"(smem_u32(dst_x)), "l"((uint64_t)map_x), "r"(m), "r"(k), "r"(bar), "r"(bytes),
+      "r"(smem_u32(own))
+      : "memory");
+}
+
+template <bool PAIR>
+__device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accum) {
+  if constexpr (PAIR)
+    asm volatile(
+        "{\n .reg .pred e, p;\n elect.sync _|e, 0xffffffff;\n setp.ne.b32 p, %4, 0;\n"
+        " @e tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accum));
+  else
+    asm volatile(
       "{\n .reg .pred e, p;\n elect.sync _|e, 0xffffffff;\n setp.ne.b32 p, %4, 0;\n"
       " @e tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
       "l"(a), "l"(b), "r"(idesc), "r"(accum));
 }
 
+// On `bar` of this CTA, or of both CTAs of the pair.
+template <bool PAIR>
 __device__ __forceinline__ void commit(uint64_t* bar) {
-  asm volatile(
+  if constexpr (PAIR)
+    asm volatile(
+        "{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n"
+        " @e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n}\n" ::"r"(
+            smem_u32(bar)),
+        "h"((uint16_t)3)
+        : "memory");
+  else
+    asm volatile(
       "{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n"
       " @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(bar))
       : "memory");
@@ -138,6 +174,9 @@ __device__ __forceinline__ uint32_t map_rank(uint32_t addr, int rank) {
   uint32_t r;
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
   return r;
+}
+__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ int ld_cluster(uint32_t addr) {
   int v;
@@ -228,11 +267,11 @@ __device__ __forceinline__ void join(const LinArgs& a, uint32_t part, const floa
   }
 }
 
-template <int NT, int EPI, bool BF16>
+template <int NT, int EPI, bool BF16, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_constant__ CUtensorMap map_w,
                                                              const __grid_constant__ CUtensorMap map_x,
                                                              const LinArgs a) {
-  using S = Shape<NT>;
+  using S = Shape<NT, PAIR>;
   constexpr int ST = S::kStages;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -244,10 +283,14 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
-  const int rank = a.split > 1 ? blockIdx.x % a.split : 0;
-  const int unit0 = a.split > 1 ? blockIdx.x / a.split : blockIdx.x;
-  const int step = a.split > 1 ? a.tiles : gridDim.x;  // a split tile's CTAs have one unit each
-  const int k0 = (int)((long long)rank * a.nk / a.split), k1 = (int)((long long)(rank + 1) * a.nk / a.split);
+  const int cluster = PAIR ? 2 : a.split;
+  const int rank = cluster > 1 ? blockIdx.x % cluster : 0;
+  const int unit0 = cluster > 1 ? blockIdx.x / cluster : blockIdx.x;
+  // (a split tile's CTAs have one unit each)
+  const int step = PAIR ? gridDim.x / 2 : a.split > 1 ? a.tiles : gridDim.x;
+  const int k0 = PAIR ? 0 : (int)((long long)rank * a.nk / a.split);
+  const int k1 = PAIR ? a.nk : (int)((long long)(rank + 1) * a.nk / a.split);
+  constexpr int kTileCh = PAIR ? 2 * kCh : kCh;  // channels of a unit, this CTA's the rank-th 128
 
   if (tid == 0) {
     for (int s = 0; s < ST; ++s) {
@@ -256,18 +299,25 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], kEpiWarps);
+      mbar_init(&acc_empty[b], PAIR ? 2 * kEpiWarps : kEpiWarps);
     }
     *abort_flag = 0;
     fence_mbar_init();
   }
   if (warp == 0) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
-                 "r"(2 * NT));
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    if constexpr (PAIR) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                   "r"(2 * NT));
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                   "r"(2 * NT));
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
   }
   asm volatile("tcgen05.fence::before_thread_sync;");
   __syncthreads();
+  if constexpr (PAIR) cluster_barrier();  // both CTAs' barriers are set up
   asm volatile("tcgen05.fence::after_thread_sync;");
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   pdl_launch_dependents();
@@ -276,7 +326,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
   if (warp == 0) {
     int it = 0;
     for (int u = unit0; u < a.tiles && !__any_sync(0xffffffffu, *abort_flag); u += step) {
-      const int ch0 = u % a.ct * kCh, m0 = u / a.ct * a.nt;
+      const int ch0 = u % a.ct * kTileCh + (PAIR ? rank * kCh : 0), m0 = u / a.ct * a.nt + (PAIR ? rank * (a.nt / 2) : 0);
       for (int kt = k0; kt < k1; ++kt, ++it) {
         const int st = it % ST;
         if (it >= ST && !warp_wait(&empty[st], (uint32_t)((it / ST) - 1) & 1u, 31)) {
@@ -284,13 +334,18 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
           break;
         }
         unsigned char* sp = smem + st * S::kStage;
-        tma_pair(sp, &map_w, ch0, sp + kCh * kKb, &map_x, m0, kt * kKb, kCh * kKb + a.nt * kKb, &full[st]);
+        if constexpr (PAIR)
+          tma_pair2(sp, &map_w, ch0, sp + kCh * kKb, &map_x, m0, kt * kKb,
+                    rank == 0 ? (uint32_t)(2 * kCh * kKb + a.nt * kKb) : 0u, &full[st], map_rank(smem_u32(&full[st]), 0));
+        else
+          tma_pair(sp, &map_w, ch0, sp + kCh * kKb, &map_x, m0, kt * kKb, kCh * kKb + a.nt * kKb, &full[st]);
       }
     }
   } else if (warp == 1) {
-    const uint32_t idesc = idesc_i8(a.nt);
+    const uint32_t idesc = idesc_i8(a.nt, kTileCh);
     int it = 0, lt = 0;
-    for (int u = unit0; u < a.tiles && !__any_sync(0xffffffffu, *abort_flag); u += step, ++lt) {
+    // (a pair's first CTA issues for both)
+    for (int u = PAIR && rank > 0 ? a.tiles : unit0; u < a.tiles && !__any_sync(0xffffffffu, *abort_flag); u += step, ++lt) {
       const int ab = lt & 1;
       if (lt >= 2 && !warp_wait(&acc_empty[ab], (uint32_t)((lt >> 1) - 1) & 1u, 32)) {
         *abort_flag = 1;
@@ -309,14 +364,14 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
         const uint32_t sw = smem_u32(smem + st * S::kStage), sx = sw + kCh * kKb;
 #pragma unroll
         for (int kk = 0; kk < kKb / 32; ++kk)
-          mma_i8(acc, sw128_desc(sw + kk * 32), sw128_desc(sx + kk * 32), idesc, (kt > k0 || kk > 0) ? 1u : 0u);
-        commit(&empty[st]);
+          mma_i8<PAIR>(acc, sw128_desc(sw + kk * 32), sw128_desc(sx + kk * 32), idesc, (kt > k0 || kk > 0) ? 1u : 0u);
+        commit<PAIR>(&empty[st]);
       }
       if (!ok) {
         *abort_flag = 1;
         break;
       }
-      commit(&acc_full[ab]);
+      commit<PAIR>(&acc_full[ab]);
     }
   } else {
     const int q = warp & 3, half = (warp - 2) >> 2;  // TMEM lane quarter and token half of this warp
@@ -327,7 +382,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
     int lt = 0;
     for (int u = unit0; u < a.tiles; u += step, ++lt) {
       const int ab = lt & 1;
-      const int ch = u % a.ct * kCh + q * 32 + lane;
+      const int ch = u % a.ct * kTileCh + (PAIR ? rank * kCh : 0) + q * 32 + lane;
       const long long m0 = (long long)(u / a.ct) * a.nt + half * H;
       const float wsc = ch < a.n ? __ldg(a.ws + ch) : 0.f;
       __syncwarp();
@@ -365,7 +420,10 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
         }
       }
       asm volatile("tcgen05.fence::before_thread_sync;");
-      if (lane == 0) mbar_arrive(&acc_empty[ab]);
+      if (lane == 0) {
+        if (PAIR && rank > 0) arrive_cluster(map_rank(smem_u32(&acc_empty[ab]), 0));
+        else mbar_arrive(&acc_empty[ab]);
+      }
     }
   }
   if (a.split > 1) {
@@ -394,7 +452,12 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
   }
   asm volatile("tcgen05.fence::before_thread_sync;");
   __syncthreads();
-  if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * NT));
+  if constexpr (PAIR) {
+    cluster_barrier();  // neither CTA leaves while the other's products read its operands or signal its barriers
+    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * NT));
+  } else {
+    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * NT));
+  }
 }
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
@@ -434,28 +497,28 @@ struct LinCall {
   bool bf16;
 };
 
-template <int NT, int EPI, bool BF16>
-cudaError_t launch_as(const LinCall& c, const LinArgs& a, const CUtensorMap& mw, const CUtensorMap& mx, int grid,
-                      cudaStream_t s) {
+template <int NT, int EPI, bool BF16, bool PAIR>
+cudaError_t launch_as(const LinArgs& a, const CUtensorMap& mw, const CUtensorMap& mx, int grid, cudaStream_t s) {
   static OncePerDevice once;
-  const cudaError_t e = once.smem(linear_kernel<NT, EPI, BF16>, Shape<NT>::kSmem);
+  constexpr int kSmem = Shape<NT, PAIR>::kSmem;
+  const cudaError_t e = once.smem(linear_kernel<NT, EPI, BF16, PAIR>, kSmem);
   if (e != cudaSuccess) return e;
-  return ops_launch(linear_kernel<NT, EPI, BF16>, dim3(grid), dim3(kThreads), Shape<NT>::kSmem, s, a.split, mw, mx, a);
+  return ops_launch(linear_kernel<NT, EPI, BF16, PAIR>, dim3(grid), dim3(kThreads), kSmem, s, PAIR ? 2 : a.split, mw, mx, a);
 }
 
-template <int NT>
+template <int NT, bool PAIR = false>
 cudaError_t launch(const LinCall& c, const LinArgs& a, int grid, cudaStream_t s) {
   CUtensorMap mw, mx;
-  if (!byte_map(&mw, c.wq, a.n, c.k, c.ldw, kCh) || !byte_map(&mx, c.xq, a.m, c.k, c.ldx, a.nt))
+  if (!byte_map(&mw, c.wq, a.n, c.k, c.ldw, kCh) || !byte_map(&mx, c.xq, a.m, c.k, c.ldx, PAIR ? a.nt / 2 : a.nt))
     return cudaErrorInvalidValue;
   if (c.epi == LINEAR_SWIGLU)
-    return c.bf16 ? launch_as<NT, LINEAR_SWIGLU, true>(c, a, mw, mx, grid, s)
-                  : launch_as<NT, LINEAR_SWIGLU, false>(c, a, mw, mx, grid, s);
+    return c.bf16 ? launch_as<NT, LINEAR_SWIGLU, true, PAIR>(a, mw, mx, grid, s)
+                  : launch_as<NT, LINEAR_SWIGLU, false, PAIR>(a, mw, mx, grid, s);
   if (c.epi == LINEAR_RESID)
-    return c.bf16 ? launch_as<NT, LINEAR_RESID, true>(c, a, mw, mx, grid, s)
-                  : launch_as<NT, LINEAR_RESID, false>(c, a, mw, mx, grid, s);
-  return c.bf16 ? launch_as<NT, LINEAR_STORE, true>(c, a, mw, mx, grid, s)
-                : launch_as<NT, LINEAR_STORE, false>(c, a, mw, mx, grid, s);
+    return c.bf16 ? launch_as<NT, LINEAR_RESID, true, PAIR>(a, mw, mx, grid, s)
+                  : launch_as<NT, LINEAR_RESID, false, PAIR>(a, mw, mx, grid, s);
+  return c.bf16 ? launch_as<NT, LINEAR_STORE, true, PAIR>(a, mw, mx, grid, s)
+                : launch_as<NT, LINEAR_STORE, false, PAIR>(a, mw, mx, grid, s);
 }
 
 }  // namespace
@@ -497,6 +560,30 @@ cudaError_t linear_int8(const int8_t* xq, long long ldx, const float* xs, const 
     }
   }
   if (best < 0) return cudaErrorInvalidValue;
+  // A pair of CTAs (cta_group::2) works on 256 channels, each CTA with its 128 and half the tokens: it brings
+  // 128 + nt / 2 rows a step, and the products of a step, 2 nt, weigh as much. For a long K and a full grid:
+  // 8191 x 2048 x 6144 90 us without and 80 with pairs, 3048 x 2048 x 6144 40 and 34, 8192^3 430 and 385. At
+  // K = 2048, where a tile's epilogue weighs as much as its products, the two are alike with a full grid (8191
+  // x 4096: 68 and 69 us) and pairs are worse with a small one (381 x 12288: 15.6 and 18.7).
+  bool pair = false;
+  for (int nt = 160; nt <= 256 && a.nk >= 32; nt += 32) {
+    const long long tiles = (long long)ceil_div(n, 2 * kCh) * ((m + nt - 1) / nt);
+    if (tiles > 0x7FFFFFFF / 16 || tiles < sms / 2) continue;
+    const long long waves = (tiles + sms / 2 - 1) / (sms / 2);
+    const long long step = 2 * std::max(128 + nt / 2, nt), loop = a.nk * step, epi = 8 * nt;
+    const long long cost = waves * (loop > epi ? loop : epi) + epi;
+    if (cost < best) {
+      best = cost;
+      pair = true;
+      a.nt = nt;
+      a.split = 1;
+      a.tiles = (int)tiles;
+    }
+  }
+  if (pair) {
+    a.ct = ceil_div(n, 2 * kCh);
+    return launch<256, true>(c, a, 2 * std::min(a.tiles, sms / 2), s);
+  }
   const int grid = a.split > 1 ? a.tiles * a.split : (a.tiles < sms ? a.tiles : sms);
   if (a.nt <= 16) return launch<16>(c, a, grid, s);
   if (a.nt <= 32) return launch<32>(c, a, grid, s);

@@ -185,6 +185,26 @@ def test_linear_residual_and_swiglu(ops, dt, m, n, k):
     assert ((s.double() - want).abs() <= tol).all()
 
 
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("m,n,k", [(2999, 1900, 4100), (20001, 130, 3970), (4100, 1794, 5000)])
+def test_linear_many_rows_long_k(ops, dt, m, n, k):
+    """The tiles of CTA pairs: a second CTA without channels, with two of them, odd rows and widths."""
+    xq, wq = ints(m, k, 15), ints(n, k, 16)
+    xs, ws = rand(m, seed=17).abs() * 0.01, rand(n, seed=18).abs() * (0.5 / k ** 0.5)
+    ref = linear_ref(xq, xs, wq, ws)
+    assert torch.equal(ops.linear_int8(xq, xs, wq, ws, dtype=dt), ref.to(dt))
+    r = rand(m, n, seed=19).to(dt)
+    assert torch.equal(ops.linear_int8(xq, xs, wq, ws, residual=r, dtype=dt), (ref + r.float()).to(dt))
+    assert torch.equal(ops.linear_int8(xq[:100], xs[:100], wq, ws, dtype=dt), ref[:100].to(dt))
+    s = ops.linear_int8(xq, xs, wq, ws, swiglu=True, dtype=dt)
+    g, u = ref[:, 0::2].double(), ref[:, 1::2].double()
+    want = g / (1 + torch.exp(-g)) * u
+    # as in the test before
+    tol = want.abs() * (8 * 2.0 ** -24 + HALF[dt]) + 2.0 ** -126
+    assert ((s.double() - want).abs() <= tol).all()
+    ops.check()
+
+
 def test_linear_in_place_residual_and_rows_independent(ops):
     """out may be the residual (C call), and a row has the same bits whatever rows share its call."""
     from qwen_asr_b200 import lib
