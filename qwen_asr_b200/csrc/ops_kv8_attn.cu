@@ -54,7 +54,8 @@ struct AttnArgs {
   const int *starts, *counts;
   int idx_stride, rows, heads, group, row_tiles;
   float scale;
-  int vec;  // q rows start on 16-byte boundaries
+  int vec;            // q rows start on 16-byte boundaries
+  int longest_first;  // more CTAs than run at once
 };
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
@@ -329,15 +330,40 @@ __device__ __forceinline__ float ld_peer(uint32_t addr, int rank) {
   return v;
 }
 
-// A sequence's first position (at most the capacity) and live rows: a kernel's first reads.
-__device__ __forceinline__ void live_rows(const AttnArgs& a, int seq, int& start, int& count) {
-  pdl_launch_dependents();
-  pdl_wait();
+// A sequence's first position (at most the capacity) and live rows.
+__device__ __forceinline__ void rows_of(const AttnArgs& a, int seq, int& start, int& count) {
   start = a.starts[(long long)seq * a.idx_stride];
   count = a.rows;
   if (a.counts) count = min(max(a.counts[(long long)seq * a.idx_stride], 0), a.rows);
   if (start < 0) count = 0;
   start = min(start, a.c.capacity);
+}
+
+// The CTA's sequence and its rows: a kernel's first reads. Where not all CTAs run at once, the longest of
+// every 32 sequences go first, so that none of them is left for the end (32 sequences of 0 to 8191 tokens in
+// ascending order: 61 us as they come, 49 so). All 32 lanes call it.
+__device__ __forceinline__ int live_rows(const AttnArgs& a, int& start, int& count) {
+  pdl_launch_dependents();
+  pdl_wait();
+  int seq = blockIdx.z;
+  if (a.longest_first) {
+    const int lane = threadIdx.x & 31, base = seq & ~31, i = base + lane;
+    int len = -1;
+    if (i < a.c.n_seq) {
+      rows_of(a, i, start, count);
+      len = count > 0 ? start + count : 0;
+    }
+    int rank = 0;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      const int other = __shfl_sync(0xffffffffu, len, j);
+      rank += other > len || (other == len && j < lane);
+    }
+    const unsigned mine = __ballot_sync(0xffffffffu, rank == (seq & 31));  // (one lane)
+    seq = base + __ffs((int)mine) - 1;
+  }
+  rows_of(a, seq, start, count);
+  return seq;
 }
 
 // ------------------------------------------------------------------ step kernel
@@ -357,9 +383,9 @@ __global__ void __launch_bounds__(kStepWarps * 32) step_kernel(const AttnArgs a)
   __shared__ float part[R][HD];  // the CTA's merged output
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int splits = gridDim.x, rank = blockIdx.x;
-  const int kvh = blockIdx.y / a.row_tiles, row0 = (blockIdx.y % a.row_tiles) * R, seq = blockIdx.z;
+  const int kvh = blockIdx.y / a.row_tiles, row0 = (blockIdx.y % a.row_tiles) * R;
   int start, count;
-  live_rows(a, seq, start, count);
+  const int seq = live_rows(a, start, count);
   // tokens any row of the tile sees
   const int s_last = min(count - 1, (row0 + R - 1) / a.group);
   const int len = s_last >= row0 / a.group ? (int)min((long long)start + s_last + 1, (long long)a.c.capacity) : 0;
@@ -549,9 +575,9 @@ __global__ void __launch_bounds__(kDigWarps * 32, RH == 1 ? 3 : 2) digit_kernel(
   __shared__ float part[R][HD];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int splits = gridDim.x, rank = blockIdx.x;
-  const int kvh = blockIdx.y / a.row_tiles, row0 = (blockIdx.y % a.row_tiles) * R, seq = blockIdx.z;
+  const int kvh = blockIdx.y / a.row_tiles, row0 = (blockIdx.y % a.row_tiles) * R;
   int start, count;
-  live_rows(a, seq, start, count);
+  const int seq = live_rows(a, start, count);
   const int s_last = min(count - 1, (row0 + R - 1) / a.group);
   const int len = s_last >= row0 / a.group ? (int)min((long long)start + s_last + 1, (long long)a.c.capacity) : 0;
   const int tiles = (len + kTok - 1) / kTok, units = (tiles + 1) / 2;
@@ -864,15 +890,17 @@ __global__ void __launch_bounds__(kDigWarps * 32, RH == 1 ? 3 : 2) digit_kernel(
 }
 
 // CTAs that share a sequence's length, for `ctas` CTAs unsplit: powers of two while all of them run
-// at once (two an SM) and each keeps 256 tokens; between one and two CTAs an SM two, because lengths
-// differ. 16 KV heads x tokens, measured (us) at 1 / 2 / 4 / 8 splits: 8 CTAs of 436 tokens 7.8 / 6.8 /
-// 6.2 / 6.8; 8 of 32000 186 / 96 / 51 / 30; 64 of 436 8.0 / 7.2 / 7.2 / 14.3; 256 of 0 to 8191 66 / 55 /
-// 61 / 91; 256 of 8191 91 / 89 / 98 / 122; 1024 of 1000 57 / 77 / 116 / 222.
+// at once (two an SM; one an SM for 16, which wait long for room) and each keeps 256 tokens; between one and
+// two CTAs an SM two where sequences may be long, because lengths differ. 16 query heads on 8 x 128, measured
+// (us) at 1 / 2 / 4 / 8 / 16 splits: 8 CTAs of 436 tokens 7.5 / 6.6 / 5.7 / 6.3 / 8.2; 8 of 8000 49 / 28 / 17 /
+// 12.4 / 12.5; 16 of 0 to 8000 49 / 28 / 17 / 14 / 18; 64 of 0 to 8000 49 / 28 / 21 / 24 / 51; 256 of 0 to 8000
+// 63 / 48 / 62 / 93, of 8000 92 / 88 / 101 / 134, of 1000 15 / 22 / 33 / 61; 1024 of 0 to 1000 40 / 65 / 109.
 int auto_splits(long long ctas, int max_len) {
-  const long long room = 2LL * ops_sm_count();
+  const int sms = ops_sm_count();
+  const long long room = 2LL * sms;
   int splits = 1;
-  while (splits < kMaxSplits && splits * 512 <= max_len && ctas * splits * 2 <= room) splits *= 2;
-  if (splits == 1 && ctas > room / 2 && ctas <= room && max_len >= 1024) splits = 2;
+  while (splits < kMaxSplits && splits * 512 <= max_len && ctas * splits * 2 <= (splits < 8 ? room : sms)) splits *= 2;
+  if (splits == 1 && ctas > sms && ctas <= room && max_len >= 4096) splits = 2;
   return splits;
 }
 
@@ -882,6 +910,7 @@ cudaError_t launch_digit(AttnArgs a, int max_len, int splits, cudaStream_t s) {
   a.row_tiles = (a.rows * a.group + 2 * RH - 1) / (2 * RH);
   const long long ctas = (long long)a.c.n_kv * a.row_tiles * a.c.n_seq;
   if (splits < 1) splits = auto_splits(ctas, max_len);
+  a.longest_first = a.c.n_seq > 1 && ctas * splits > 2LL * ops_sm_count();
   static OncePerDevice once;
   const cudaError_t e = once.smem(digit_kernel<HD, RH, BF16>, kSmem, true);
   if (e != cudaSuccess) return e;
@@ -899,6 +928,7 @@ cudaError_t launch(AttnArgs a, int max_len, int splits, cudaStream_t s) {
   a.row_tiles = (n_rows + R - 1) / R;
   const long long ctas = (long long)a.c.n_kv * a.row_tiles * a.c.n_seq;
   if (splits < 1) splits = auto_splits(ctas, max_len);
+  a.longest_first = a.c.n_seq > 1 && ctas * splits > 2LL * ops_sm_count();
   static OncePerDevice once;
   const cudaError_t e = once.smem(step_kernel<HD, PL>, step_smem<HD>(), true);
   if (e != cudaSuccess) return e;
@@ -915,7 +945,7 @@ cudaError_t kv8_attention(const Kv8& c, const void* q, long long q_seq, long lon
   if ((long long)rows * (heads / c.n_kv) > kStepRows)
     return kv8_prompt_attention(c, q, q_seq, q_row, out, o_seq, o_row, dt, rows, heads, starts, counts, idx_stride,
                                 scale, s);
-  AttnArgs a{c, q, out, q_seq, q_row, o_seq, o_row, starts, counts, idx_stride, rows, heads, heads / c.n_kv, 1, scale, 0};
+  AttnArgs a{c, q, out, q_seq, q_row, o_seq, o_row, starts, counts, idx_stride, rows, heads, heads / c.n_kv, 1, scale, 0, 0};
   const int es = dt == OPS_BF16 ? 2 : 4;
   a.vec = (uintptr_t)q % 16 == 0 && q_seq * es % 16 == 0 && q_row * es % 16 == 0;
   if (max_len <= 0 || max_len > c.capacity) max_len = c.capacity;

@@ -429,6 +429,22 @@ def test_attention_tokens(ops, dt, hd, heads, n_kv):
     attend_and_check(ops, q, c, [L - 1 for L in lens], [1, 0, 1, -5, 1, 1, 9, 1, 1], scale=0.05, max_len=16)
 
 
+@pytest.mark.parametrize("rows,heads", [(1, 16), (2, 16), (5, 32)])
+def test_attention_many_sequences_of_any_order(ops, rows, heads):
+    """More sequences than run at once, which are taken up by length: equal ones, empty ones, a last group of 7."""
+    n, n_kv = 71, 8
+    g = torch.Generator().manual_seed(rows)
+    starts = torch.randint(0, 120, (n,), generator=g).tolist()
+    starts[3], starts[40:44], starts[70] = -1, [77] * 4, 0
+    counts = torch.randint(0, rows + 1, (n,), generator=g).tolist()
+    c = filled_cache(ops, n, n_kv, 128, 64, [max(s, 0) + k for s, k in zip(starts, counts)], seed=rows)
+    q = rand(n, rows, heads, 64, seed=5, std=1.5)
+    live = [k if s >= 0 else 0 for s, k in zip(starts, counts)]
+    want = attend_and_check(ops, q, c, [max(s, 0) for s in starts], live)
+    st, ct = (torch.tensor(v, dtype=torch.int32, device="cuda") for v in (starts, counts))
+    assert torch.equal(ops.kv8_attention(q, ops.Kv8Cache(*c), st, ct), want)
+
+
 @pytest.mark.parametrize("dt", [F32, BF16])
 @pytest.mark.parametrize("hd,heads,n_kv,rows", [(128, 16, 8, 3), (128, 4, 2, 32), (128, 4, 2, 33), (64, 8, 2, 50),
                                                 (128, 2, 2, 150), (64, 12, 4, 101)])
