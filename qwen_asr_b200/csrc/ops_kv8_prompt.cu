@@ -22,11 +22,12 @@
 // are uniform registers, and a branch of one lane has to fill them anew each time. A whole warp that waits
 // and counts together, with an elected lane to issue, took 64 rows over 8064 f32 keys from 197 to 149 us.)
 //   bf16 rows: 256 threads, a softmax thread a row; two CTAs an SM, one's softmax beside the other's
-//   products. O stays in TMEM. 8 x 381 rows over up to 1403 keys, 8 KV heads of 2 x 128: 52 us; 2048 rows
+//   products. O stays in TMEM. 8 x 381 rows over up to 1403 keys, 8 KV heads of 2 x 128: 44 us; 2048 rows
 //   over 8048 keys, 4 KV heads of 4 x 64: 143 us; 592 heads' rows over 8064 keys: 205 us, 755 TFLOP/s.
-//   f32 rows: see below. The same shapes: 77, 209 and 335 us (a block has four times the products' bytes).
-// Bound: bf16 rows - exp2 and the conversions around it, f32 rows - the chain of a block's steps in its
-// one CTA an SM, 1.2 us of which the products take 0.7.
+//   f32 rows: see below. The same shapes: 69, 213 and 335 us.
+// Bound: the chain of a block's steps (scores, maximum, exp2, P V). bf16 rows: 1.0 us a block and CTA, two
+// CTAs an SM, in which exp2 takes 0.27 us an SM and the products 0.3 to 0.35 (a quarter of the exp2 as
+// polynomials on the FMA units was slower: 51 -> 55 us); f32 rows: 1.2 us, the products 0.7 of them.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -279,18 +280,63 @@ struct Work {
   const float *ks, *vs;
   const int8_t *k, *v;
 };
+// A sequence's first position (at most the capacity) and live rows.
+__device__ __forceinline__ void rows_of(const PromptArgs& a, int seq, int& start, int& count) {
+  start = a.starts[(long long)seq * a.idx_stride];
+  count = a.rows;
+  if (a.counts) count = min(max(a.counts[(long long)seq * a.idx_stride], 0), a.rows);
+  if (start < 0) count = 0;
+  start = min(start, a.c.capacity);
+}
+// All 32 lanes call it. The row tiles of up to 32 sequences are taken up by the keys they see, most first, so
+// that no long one is left for the end: lane i counts those of sequence i that see at least K tiles' worth of
+// keys, and a search over K finds the CTA's (8 x 381 f32 rows behind 0 to 1024 tokens 77 us with the last rows
+// of all sequences as they come, 69 so; 4 x 1024 behind 6000, 0, 1000, 3000 291 and 229; where all begin alike,
+// which needs no search, 37 and 39).
 __device__ __forceinline__ Work work_of(const PromptArgs& a) {
   Work t;
-  // all (sequence, KV head) of a row tile in turn, and the last tiles, which see the most keys, first
-  const int heads = a.c.n_kv * a.c.n_seq;
-  t.kvh = blockIdx.x % heads % a.c.n_kv;
-  t.seq = blockIdx.x % heads / a.c.n_kv;
-  t.row0 = ((int)(gridDim.x / heads) - 1 - (int)(blockIdx.x / heads)) * kRows;
-  t.start = a.starts[(long long)t.seq * a.idx_stride];
-  t.count = a.rows;
-  if (a.counts) t.count = min(max(a.counts[(long long)t.seq * a.idx_stride], 0), a.rows);
-  if (t.start < 0) t.count = 0;
-  t.start = min(t.start, a.c.capacity);
+  const int row_tiles = (int)(((long long)a.rows * a.group + kRows - 1) / kRows), item = blockIdx.x / a.c.n_kv;
+  t.kvh = blockIdx.x % a.c.n_kv;
+  if (a.c.n_seq == 1) {
+    t.seq = 0;
+    t.row0 = (row_tiles - 1 - item) * kRows;
+    rows_of(a, 0, t.start, t.count);
+  } else {
+    const int lane = threadIdx.x & 31, base = item / (32 * row_tiles) * 32, p = item % (32 * row_tiles);
+    const int n = min(a.c.n_seq - base, 32), i = base + min(lane, n - 1);  // (lanes behind the last repeat it)
+    int start, count;
+    rows_of(a, i, start, count);
+    // row tiles with live rows, and what the first sees, in rows of a tile
+    int live = (int)(((long long)count * a.group + kRows - 1) / kRows);
+    const int first = min(start / max(kRows / a.group, 1), 1 << 30);
+    int who, tile;
+    if (__all_sync(0xffffffffu, first == __shfl_sync(0xffffffffu, first, 0) && live == row_tiles)) {
+      who = p % n;
+      tile = row_tiles - 1 - p / n;
+    } else {
+      const int all = lane < n ? row_tiles : 0;
+      if (lane >= n) live = 0;
+      // tile x's key: first + x, or -1 - x without live rows; how many have K at least
+      auto upto = [&](int K) {
+        return K >= 0 ? min(max(live - max(K - first, 0), 0), live) : live + max(min(all - 1, -1 - K) - live + 1, 0);
+      };
+      int lo = -row_tiles, hi = __reduce_max_sync(0xffffffffu, first + live);  // more than p at lo, none at hi
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (__reduce_add_sync(0xffffffffu, upto(mid)) > p) lo = mid;
+        else hi = mid;
+      }
+      const int above = __reduce_add_sync(0xffffffffu, upto(lo + 1));
+      const unsigned same = __ballot_sync(0xffffffffu, upto(lo) > upto(lo + 1));
+      const bool me = (same >> lane & 1u) && __popc(same & ((1u << lane) - 1u)) == p - above;
+      who = __ffs((int)__ballot_sync(0xffffffffu, me)) - 1;
+      tile = lo >= 0 ? lo - __shfl_sync(0xffffffffu, first, who) : -1 - lo;
+    }
+    t.seq = base + who;
+    t.row0 = tile * kRows;
+    t.start = __shfl_sync(0xffffffffu, start, who);
+    t.count = __shfl_sync(0xffffffffu, count, who);
+  }
   // keys any row of the tile sees
   const int s_last = min(t.count - 1, (t.row0 + kRows - 1) / a.group);
   const int len = s_last >= t.row0 / a.group ? (int)min((long long)t.start + s_last + 1, (long long)a.c.capacity) : 0;
