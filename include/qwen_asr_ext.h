@@ -216,7 +216,7 @@ void qwen_asr_pool_set_segment_sec(QwenAsrPool* pool, float sec);
 int32_t qwen_asr_pool_set_language(QwenAsrPool* pool, const char* language);
 void qwen_asr_pool_set_decode_mode(QwenAsrPool* pool, int32_t mode); /* 0 int8, 1 bf16 */
 int32_t qwen_asr_pool_set_prefill_mode(QwenAsrPool* pool, int32_t mode); /* 0 bf16, 1 int8 */
-int32_t qwen_asr_pool_set_kv_mode(QwenAsrPool* pool, int32_t mode);      /* 0 f32, 1 int8 */
+int32_t qwen_asr_pool_set_kv_mode(QwenAsrPool* pool, int32_t mode);      /* 0 f32, 1 int8; -1: not every worker has it */
 void qwen_asr_pool_set_force_n_tokens(QwenAsrPool* pool, int32_t n);
 void qwen_asr_pool_stream_set_max_new_tokens(QwenAsrPool* pool, int32_t n);
 /* Like qwen_asr_transcribe_pcm, the segments spread over the pool's GPUs. */

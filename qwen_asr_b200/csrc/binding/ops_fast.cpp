@@ -12,6 +12,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
+#include <cstring>
 
 #include "qwen_asr_ext.h"
 
@@ -35,8 +36,11 @@ bool is(const at::Tensor* t, at::ScalarType type, int device, int dims) {
 
 void* stream_of(int device) { return c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream(); }
 
+// As ops.py does: RuntimeError where CUDA refused, ValueError for the arguments.
 PyObject* failed() {
-  PyErr_SetString(PyExc_RuntimeError, qwen_asr_last_error());
+  const char* why = qwen_asr_last_error();
+  const bool cuda = !why || std::strstr(why, "launch failed") || std::strstr(why, "cannot use device");
+  PyErr_SetString(cuda ? PyExc_RuntimeError : PyExc_ValueError, why ? why : "unknown");
   return nullptr;
 }
 

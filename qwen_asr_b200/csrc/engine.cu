@@ -402,6 +402,13 @@ Kv8 Engine::kv8_at(int slot, int layer, int n_seq) const {
 
 bool Engine::set_kv_mode(KvMode m) {
   if (m == kv_mode_) return true;
+  struct Back {  // a setting leaves the caller's current device as it was
+    int prev = -1;
+    Back() { cudaGetDevice(&prev); }
+    ~Back() {
+      if (prev >= 0) cudaSetDevice(prev);
+    }
+  } back;
   cudaSetDevice(device_);
   CUDA_OK(cudaStreamSynchronize(stream_), false);
   if (max_seq_ > 0) {

@@ -566,7 +566,7 @@ cudaError_t linear_int8(const int8_t* xq, long long ldx, const float* xs, const 
   // K = 2048, where a tile's epilogue weighs as much as its products, the two are alike with a full grid (8191
   // x 4096: 68 and 69 us) and pairs are worse with a small one (381 x 12288: 15.6 and 18.7).
   bool pair = false;
-  for (int nt = 160; nt <= 256 && a.nk >= 32; nt += 32) {
+  for (int nt = 160; nt <= 256 && a.nk >= 32 && sms > 1; nt += 32) {
     const long long tiles = (long long)ceil_div(n, 2 * kCh) * ((m + nt - 1) / nt);
     if (tiles > 0x7FFFFFFF / 16 || tiles < sms / 2) continue;
     const long long waves = (tiles + sms / 2 - 1) / (sms / 2);

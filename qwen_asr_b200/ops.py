@@ -91,7 +91,9 @@ def _pitch(t, name):
 
 
 def _failed():
-    raise RuntimeError(last_error())
+    """Raises what the library refused: RuntimeError where CUDA did, ValueError for the arguments."""
+    why = last_error()
+    raise (RuntimeError if "launch failed" in why or "cannot use device" in why else ValueError)(why)
 
 
 def rms_norm_int8(x, weight, eps: float = 1e-6, residual=None):

@@ -429,6 +429,24 @@ def test_attention_tokens(ops, dt, hd, heads, n_kv):
     attend_and_check(ops, q, c, [L - 1 for L in lens], [1, 0, 1, -5, 1, 1, 9, 1, 1], scale=0.05, max_len=16)
 
 
+def test_refusals_of_the_library_are_value_errors(ops):
+    """Arguments that pass the first checks and fail in the library: a cache whose sequences share memory, more
+    rows than a call takes."""
+    c = ops.kv8_cache(1, 2, 32, 64)
+    both = ops.Kv8Cache(*[t.expand(2, *t.shape[1:]) for t in c])
+    z = torch.zeros(2, dtype=torch.int32, device="cuda")
+    k = rand(2, 1, 2, 64)
+    with pytest.raises(ValueError, match="seq_stride"):
+        ops.kv8_append(both, k, k, z)
+    with pytest.raises(ValueError, match="seq_stride"):
+        ops.kv8_attention(k, both, z)
+    with pytest.raises(ValueError, match="seq_stride"):
+        ops.kv8_read(both, z, 1)
+    one = ops.kv8_cache(1, 1, 16, 64)
+    with pytest.raises(ValueError, match="rows"):
+        ops.kv8_attention(rand(1, 1, 1, 64).to(BF16).expand(1, (1 << 22) + 1, 1, 64), one, z[:1])
+
+
 @pytest.mark.parametrize("rows,heads", [(1, 16), (2, 16), (5, 32)])
 def test_attention_many_sequences_of_any_order(ops, rows, heads):
     """More sequences than run at once, which are taken up by length: equal ones, empty ones, a last group of 7."""

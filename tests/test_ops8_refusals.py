@@ -100,3 +100,11 @@ def test_tensors_off_the_gpu_are_refused():
     with pytest.raises(ValueError, match="CUDA"):
         ops.kv8_cache(1, 1, 16, 64, device="cpu") and ops.kv8_read(
             ops.kv8_cache(1, 1, 16, 64, device="cpu"), torch.zeros(1, dtype=torch.int32), 1)
+
+
+def test_library_refusals_are_value_errors():
+    pytest.importorskip("torch")
+    from qwen_asr_b200 import ops
+    assert append(n=-1) == -1
+    with pytest.raises(ValueError, match="row count"):
+        ops._failed()
