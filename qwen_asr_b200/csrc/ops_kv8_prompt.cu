@@ -15,18 +15,18 @@
 // m is only raised when a score exceeds it by 2^8 (p up to 256 is as exact in f16): what has been summed
 // is then rescaled, which the first blocks of a row do and later ones hardly ever.
 //
-// Two kernels. In both some warps do the softmax; others bring K and V from global memory as int8, a block
-// or two ahead in registers, and write them as f16 rows of a token in the 128-byte-swizzle layout, which is
+// Two kernels. In both some warps do the softmax; others bring K and V from global memory as int8, two
+// blocks ahead in registers, and write them as f16 rows of a token in the 128-byte-swizzle layout, which is
 // K-major for Q K^T and MN-major for P V; the last warp issues the products, Q K^T of the next block
 // before P V of this one. (One thread that did this was the longest chain of all: the operands of a product
 // are uniform registers, and a branch of one lane has to fill them anew each time. A whole warp that waits
 // and counts together, with an elected lane to issue, took 64 rows over 8064 f32 keys from 197 to 149 us.)
 //   bf16 rows: 256 threads, a softmax thread a row; two CTAs an SM, one's softmax beside the other's
 //   products. O stays in TMEM. 8 x 381 rows over up to 1403 keys, 8 KV heads of 2 x 128: 44 us; 2048 rows
-//   over 8048 keys, 4 KV heads of 4 x 64: 143 us; 592 heads' rows over 8064 keys: 205 us, 755 TFLOP/s.
-//   f32 rows: see below. The same shapes: 69, 213 and 335 us.
-// Bound: the chain of a block's steps (scores, maximum, exp2, P V). bf16 rows: 1.0 us a block and CTA, two
-// CTAs an SM, in which exp2 takes 0.27 us an SM and the products 0.3 to 0.35 (a quarter of the exp2 as
+//   over 8048 keys, 4 KV heads of 4 x 64: 143 us; 592 heads' rows over 8064 keys: 198 us, 785 TFLOP/s.
+//   f32 rows: see below. The same shapes: 67, 213 and 310 us.
+// Bound: the chain of a block's steps (scores, maximum, exp2, P V). bf16 rows: 0.9 us a block and CTA alone
+// on its SM, two CTAs an SM, in which exp2 takes 0.27 us an SM and the products 0.3 to 0.35 (a quarter of the exp2 as
 // polynomials on the FMA units was slower: 51 -> 55 us); f32 rows: 1.2 us, the products 0.7 of them.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -428,33 +428,46 @@ __device__ __forceinline__ float vref_of(const float* red) {
   return top > 0.f ? fmaxf(__uint_as_float((__float_as_uint(top) + 0x7FFFFFu) & 0xFF800000u), 7.888609e-31f) : 0.f;
 }
 
-// A thread's pieces of one block of K or V: int8 in registers, then f16 rows of a token in shared memory.
-template <int HD, int FILL>  // FILL: threads that share a block
+// 16 bytes, or zeros.
+__device__ __forceinline__ uint4 ld_if(const int8_t* p, bool there) {
+  uint4 v;
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %5, 0;\n mov.b32 %0, 0;\n mov.b32 %1, 0;\n mov.b32 %2, 0;\n mov.b32 %3, 0;\n"
+      " @p ld.global.nc.v4.b32 {%0,%1,%2,%3}, [%4];\n}\n"
+      : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w)
+      : "l"(p), "r"((int)there));
+  return v;
+}
+
+// What one of FILL threads brings of a block of K or V: 16-byte pieces of rows (tokens) kStep apart, as int8 in
+// registers, then f16 rows in shared memory. All addresses are a thread's own constants plus immediates.
+template <int HD, int FILL>
 struct Pieces {
-  static constexpr int kAll = kKeys * HD / 16, kN = (kAll + FILL - 1) / FILL;
+  static constexpr int kRow = HD / 16, kStep = FILL / kRow, kN = (kKeys + kStep - 1) / kStep;
+  static_assert(FILL % kRow == 0 && kStep % 4 == 0, "whole rows; their swizzle is one of two");
   uint4 r[kN];
-  __device__ __forceinline__ void load(const int8_t* src, int j, int end, int ct) {  // tokens from end on are zeros
+  // tokens from end on are zeros
+  __device__ __forceinline__ void load(const int8_t* src, int j, int end, int ct) {
+    const int row = ct / kRow, left = min(end - j * kKeys, kKeys) - row;
+    const int8_t* p = src + (long long)j * (kKeys * HD) + ct * 16;
 #pragma unroll
-    for (int i = 0; i < kN; ++i) {
-      const int id = ct + i * FILL, tok = j * kKeys + id / (HD / 16);
-      r[i] = make_uint4(0, 0, 0, 0);
-      if (id < kAll && tok < end)
-        r[i] = __ldg(reinterpret_cast<const uint4*>(src + (long long)tok * HD + id % (HD / 16) * 16));
-    }
+    for (int i = 0; i < kN; ++i) r[i] = ld_if(p + i * (kStep * HD), i * kStep < left);
   }
   __device__ __forceinline__ void store(unsigned char* dst, int ct) const {
+    const int row = ct / kRow, c = ct % kRow * 2;  // 16-byte f16 chunks c, c + 1
+    // lanes of the second 64 columns begin with their second chunk, so that eight lanes hit distinct banks
+    const bool swap = c & 8;
+    unsigned char* p = dst + (c >> 3) * (kKeys * 128) + row * 128;
+    const uint32_t at0 = (((c & 7) + (int)swap) ^ (row & 7)) << 4, at1 = at0 ^ 16;
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
-      const int id = ct + i * FILL, row = id / (HD / 16), c = id % (HD / 16) * 2;  // 16-byte f16 chunks c, c + 1
-      if (id >= kAll) break;
-      // lanes of the second 64 columns begin with their second chunk, so that eight lanes hit distinct banks
-      const bool swap = c & 8;
+      if (kKeys % kStep && i == kN - 1 && row + i * kStep >= kKeys) break;
+      const uint32_t flip = (i * kStep & 4) << 4;
       const uint32_t w[4] = {(swap ? r[i].z : r[i].x) ^ 0x80808080u, (swap ? r[i].w : r[i].y) ^ 0x80808080u,
                              (swap ? r[i].x : r[i].z) ^ 0x80808080u, (swap ? r[i].y : r[i].w) ^ 0x80808080u};
-      unsigned char* p = dst + (c >> 3) * (kKeys * 128) + row * 128;
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        *reinterpret_cast<uint4*>(p + ((((c & 7) + (h ^ (int)swap)) ^ (row & 7)) << 4)) =
+        *reinterpret_cast<uint4*>(p + i * (kStep * 128) + ((h ? at1 : at0) ^ flip)) =
             make_uint4(bytes_f16<0x4140>(w[2 * h]), bytes_f16<0x4342>(w[2 * h]), bytes_f16<0x4140>(w[2 * h + 1]),
                        bytes_f16<0x4342>(w[2 * h + 1]));
     }
@@ -540,8 +553,8 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_bf16_kernel(const PromptAr
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
                  "r"(kCols));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    pdl_launch_dependents();  // (not before: the next kernel's blocks may want TMEM too, and wait for this one's end)
   }
-  pdl_launch_dependents();
   pdl_wait();
 
   const Work t = work_of(a);
@@ -669,27 +682,34 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_bf16_kernel(const PromptAr
   } else if (warp < 7) {
     // ---------------------------------------------------------------- K and V: int8 -> f16 operands
     const int ct = tid - 128, end = tiles * kKv8Block;
-    Pieces<HD, kFill> kr, vr;
-    kr.load(t.k, 0, end, ct);
-    vr.load(t.v, 0, end, ct);
-    auto put_k = [&](int j) {  // into its buffer, then the next block's loads
-      kr.store(sk + (j & 1) * L::kK, ct);
+    // two blocks ahead in registers (memory takes 1.2 us, a block 1.0 to 1.3; one ahead: 592 heads' rows over
+    // 8064 tokens 240 us, two 198)
+    Pieces<HD, kFill> k0, k1, v0, v1;  // of even and of odd blocks
+    k0.load(t.k, 0, end, ct);
+    k1.load(t.k, 1, end, ct);
+    v0.load(t.v, 0, end, ct);
+    v1.load(t.v, 1, end, ct);
+    auto put_k = [&](int j, Pieces<HD, kFill>& k) {  // into its buffer, then the loads of the block after the next
+      k.store(sk + (j & 1) * L::kK, ct);
       mbar_arrive(&k_full[j & 1]);
-      if (j + 1 < nb) kr.load(t.k, j + 1, end, ct);
+      k.load(t.k, j + 2, end, ct);
     };
-    if (nb > 0) put_k(0);
-    for (int j = 0; j < nb; ++j) {
+    auto block = [&](int j, Pieces<HD, kFill>& k, Pieces<HD, kFill>& v) {
       // K of block j + 1 goes where that of j - 1 was
       if (j + 1 < nb) {
         // (a barrier of its own: that of S may be two phases on by now)
-        if (j > 0 && !wait(&k_free[(j - 1) & 1], (uint32_t)((j - 1) >> 1) & 1u, gave_up, 46)) break;
-        put_k(j + 1);
+        if (j > 0 && !wait(&k_free[(j - 1) & 1], (uint32_t)((j - 1) >> 1) & 1u, gave_up, 46)) return false;
+        put_k(j + 1, k);
       }
-      if (j > 0 && !wait(o_done, (uint32_t)(j - 1) & 1u, gave_up, 47)) break;
-      vr.store(sv, ct);
+      if (j > 0 && !wait(o_done, (uint32_t)(j - 1) & 1u, gave_up, 47)) return false;
+      v.store(sv, ct);
       mbar_arrive(v_full);
-      if (j + 1 < nb) vr.load(t.v, j + 1, end, ct);
-    }
+      v.load(t.v, j + 2, end, ct);
+      return true;
+    };
+    if (nb > 0) put_k(0, k0);
+    for (int j = 0; j < nb; j += 2)
+      if (!block(j, k1, v0) || (j + 1 < nb && !block(j + 1, k0, v1))) break;
   } else if (nb > 0) {
     // ---------------------------------------------------------------- products
     const uint32_t qa = smem_u32(sq), ka = smem_u32(sk), va = smem_u32(sv);
@@ -774,8 +794,8 @@ __global__ void __launch_bounds__(kThreads2, 1) prompt_f32_kernel(const PromptAr
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
                  "r"(kCols2));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    pdl_launch_dependents();  // (not before: the next kernel's blocks may want TMEM too, and wait for this one's end)
   }
-  pdl_launch_dependents();
   pdl_wait();
   const Work t = work_of(a);
   const int nb = t.nb;
@@ -921,18 +941,18 @@ __global__ void __launch_bounds__(kThreads2, 1) prompt_f32_kernel(const PromptAr
     // one operand's blocks in turn: two in registers, each stored when its buffer is free
     auto fill = [&](auto& even, auto& odd, const int8_t* src, unsigned char* dst, uint64_t* full, uint64_t* free, int ct) {
       even.load(src, 0, end, ct);
-      if (nb > 1) odd.load(src, 1, end, ct);
+      odd.load(src, 1, end, ct);
       for (int j = 0; j < nb; j += 2) {
         const uint32_t before = (uint32_t)((j >> 1) - 1) & 1u;  // the phase in which block j - 2 left the buffer
         if (j >= 2 && !wait(&free[0], before, gave_up, 54)) break;
         even.store(dst, ct);
         mbar_arrive(&full[0]);
-        if (j + 2 < nb) even.load(src, j + 2, end, ct);
+        even.load(src, j + 2, end, ct);
         if (j + 1 >= nb) break;
         if (j >= 2 && !wait(&free[1], before, gave_up, 55)) break;
         odd.store(dst + L::kK, ct);
         mbar_arrive(&full[1]);
-        if (j + 3 < nb) odd.load(src, j + 3, end, ct);
+        odd.load(src, j + 3, end, ct);
       }
     };
     if (warp < 12) {

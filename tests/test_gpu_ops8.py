@@ -475,6 +475,21 @@ def test_attention_prompt_rows(ops, dt, hd, heads, n_kv, rows):
     assert not got[2].any() and not got[3, 1:].any()  # rows not in use are zeros
 
 
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("n,rows", [(2, 150), (33, 70), (40, 200)])
+def test_attention_prompts_of_any_order(ops, dt, n, rows):
+    """Row tiles of many sequences, taken up by the keys they see: any lengths, empty and equal sequences."""
+    g = torch.Generator().manual_seed(n)
+    starts = torch.randint(0, 300, (n,), generator=g).tolist()
+    counts = torch.randint(0, rows + 1, (n,), generator=g).tolist()
+    starts[0], counts[1], starts[n // 2], counts[n // 2] = 0, rows, starts[-1], counts[-1]
+    c = filled_cache(ops, n, 2, 512, 64, [s + k for s, k in zip(starts, counts)], seed=n)
+    q = rand(n, rows, 4, 64, seed=6, std=1.5).to(dt)
+    attend_and_check(ops, q, c, starts, counts)
+    c = filled_cache(ops, n, 2, 512, 64, [17 + rows] * n, seed=n)
+    attend_and_check(ops, q, c, [17] * n, None)
+
+
 @pytest.mark.parametrize("rows", [1, 40])
 def test_attention_ignores_what_is_masked(ops, rows):
     """NaN blocks behind a row's last position do not touch it; a NaN it does see reaches its head."""
