@@ -164,11 +164,13 @@ __device__ __forceinline__ void fix_near(const NormArgs& a, long long row, doubl
   }
 }
 
-// One row by W warps, its values in registers: NV vectors a thread.
-template <bool BF16, int W, int NV>
+// One row by W warps, its values in registers: NV vectors of V a thread. V = 1: rows of any length, stride and
+// alignment (16411 x 2045 bf16 with residual 184 us by the kernel below, 92 so).
+template <bool BF16, int V, int W, int NV>
 __global__ void __launch_bounds__(W * 32) norm_vec_kernel(const NormArgs a) {
-  using T = typename Elem<BF16>::T;
-  constexpr int V = Elem<BF16>::kVec, N = W * 32;
+  using E = Elem<BF16>;
+  using T = typename E::T;
+  constexpr int N = W * 32;
   static_assert(NV * V <= 32, "a bit a value");
   __shared__ double parts[N];
   __shared__ unsigned tops[W];
@@ -178,43 +180,62 @@ __global__ void __launch_bounds__(W * 32) norm_vec_kernel(const NormArgs a) {
   pdl_launch_dependents();
   pdl_wait();
   const T* x = (const T*)a.x + row * a.ldx;
-  uint4 raw[NV];
-#pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int c = (threadIdx.x + j * N) * V;
-    raw[j] = make_uint4(0, 0, 0, 0);
-    if (c < a.d) raw[j] = *reinterpret_cast<const uint4*>(x + c);
-  }
-  if (a.r) {
-    const T* r = (const T*)a.r + row * a.ldr;
-    uint4 add[NV];
+  float h[NV][V], u[NV][V];
+  uint4 raw[V > 1 ? NV : 1];
+  if constexpr (V > 1) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = (threadIdx.x + j * N) * V;
-      add[j] = make_uint4(0, 0, 0, 0);
-      if (c < a.d) add[j] = *reinterpret_cast<const uint4*>(r + c);
+      raw[j] = make_uint4(0, 0, 0, 0);
+      if (c < a.d) raw[j] = *reinterpret_cast<const uint4*>(x + c);
     }
+    if (a.r) {
+      const T* r = (const T*)a.r + row * a.ldr;
+      uint4 add[NV];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) raw[j] = add_packed<BF16>(raw[j], add[j]);
+      for (int j = 0; j < NV; ++j) {
+        const int c = (threadIdx.x + j * N) * V;
+        add[j] = make_uint4(0, 0, 0, 0);
+        if (c < a.d) add[j] = *reinterpret_cast<const uint4*>(r + c);
+      }
+#pragma unroll
+      for (int j = 0; j < NV; ++j) raw[j] = add_packed<BF16>(raw[j], add[j]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) h[j][0] = threadIdx.x + j * N < a.d ? E::load(x + threadIdx.x + j * N) : 0.f;
+    if (a.r) {
+      const T* r = (const T*)a.r + row * a.ldr;
+      float add[NV];
+#pragma unroll
+      for (int j = 0; j < NV; ++j) add[j] = threadIdx.x + j * N < a.d ? E::load(r + threadIdx.x + j * N) : 0.f;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) h[j][0] = E::round(__fadd_rn(h[j][0], add[j]));
+    }
   }
-  float h[NV][V], u[NV][V];
   float mx = 0.f;
   double ss = 0.0;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const int c = (threadIdx.x + j * N) * V;
-    if constexpr (BF16) {
+    if constexpr (V == 8) {
       bf16x8_to_f32(raw[j], h[j]);
-    } else {
+    } else if constexpr (V == 4) {
       h[j][0] = __uint_as_float(raw[j].x);
       h[j][1] = __uint_as_float(raw[j].y);
       h[j][2] = __uint_as_float(raw[j].z);
       h[j][3] = __uint_as_float(raw[j].w);
     }
-    if (c < a.d) {
-      if (a.h) *reinterpret_cast<uint4*>((T*)a.h + row * a.ldh + c) = raw[j];
+    if (V == 1) {
+      u[j][0] = 0.f;
+      if (c < a.d) {
+        if (a.h) E::store((T*)a.h + row * a.ldh + c, h[j][0]);
+        u[j][0] = __fmul_rn(h[j][0], a.w ? __ldg(a.w + c) : 1.f);
+      }
+    } else if (c < a.d) {
+      if (a.h) *reinterpret_cast<uint4*>((T*)a.h + row * a.ldh + c) = raw[V > 1 ? j : 0];
 #pragma unroll
-      for (int i = 0; i < V; i += 4) {
+      for (int i = 0; i + 3 < V; i += 4) {
         const float4 w = a.w ? __ldg(reinterpret_cast<const float4*>(a.w + c + i)) : make_float4(1.f, 1.f, 1.f, 1.f);
         u[j][i] = __fmul_rn(h[j][i], w.x);
         u[j][i + 1] = __fmul_rn(h[j][i + 1], w.y);
@@ -260,25 +281,24 @@ __global__ void __launch_bounds__(W * 32) norm_vec_kernel(const NormArgs a) {
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const int c = (threadIdx.x + j * N) * V;
-    uint32_t o[V / 4];
+    uint32_t b[V];
 #pragma unroll
-    for (int i = 0; i < V; i += 4) {
-      uint32_t b[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float v = __fmul_rn(u[j][i + k], r127);
-        const float t = __fadd_rn(v, kRound);
-        b[k] = __float_as_uint(t);
-        if (fabsf(__fsub_rn(v, __fsub_rn(t, kRound))) > 0.5f - 3.2e-5f) near |= 1u << (j * V + i + k);
-      }
-      o[i / 4] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
-      if (!finite) o[i / 4] = 0u;
+    for (int i = 0; i < V; ++i) {
+      const float v = __fmul_rn(u[j][i], r127);
+      const float t = __fadd_rn(v, kRound);
+      b[i] = finite ? __float_as_uint(t) : 0u;
+      if (fabsf(__fsub_rn(v, __fsub_rn(t, kRound))) > 0.5f - 3.2e-5f) near |= 1u << (j * V + i);
     }
     if (c < a.d) {
+      auto word = [&](int i) {
+        return __byte_perm(__byte_perm(b[i], b[i + 1], 0x0040), __byte_perm(b[i + 2], b[i + 3], 0x0040), 0x5410);
+      };
       if constexpr (V == 8)
-        *reinterpret_cast<uint2*>(q + c) = make_uint2(o[0], o[1]);
+        *reinterpret_cast<uint2*>(q + c) = make_uint2(word(0), word(4));
+      else if constexpr (V == 4)
+        *reinterpret_cast<uint32_t*>(q + c) = word(0);
       else
-        *reinterpret_cast<uint32_t*>(q + c) = o[0];
+        q[c] = (int8_t)b[0];
     }
   }
   __syncthreads();  // `low` is complete
@@ -297,7 +317,7 @@ __global__ void __launch_bounds__(W * 32) norm_vec_kernel(const NormArgs a) {
   }
 }
 
-// Any d, stride and alignment: the row is staged in shared memory, one element a thread at a time.
+// Any d, stride and alignment, for the longest rows: the row is staged in shared memory, one element a thread at a time.
 template <bool BF16>
 __global__ void __launch_bounds__(512) norm_any_kernel(const NormArgs a) {
   using E = Elem<BF16>;
@@ -334,17 +354,21 @@ __global__ void __launch_bounds__(512) norm_any_kernel(const NormArgs a) {
 template <bool BF16>
 cudaError_t launch(const NormArgs& a, bool vec, cudaStream_t s) {
   constexpr int V = Elem<BF16>::kVec;
-  const int nv = a.d / V;  // vectors of a row
+  const int nv = vec ? a.d / V : a.d;  // vectors of a row, or single values
   const dim3 g((unsigned)a.rows);
   if (vec) {
     // two vectors a thread where rows fill the GPU anyway, one where a row's latency counts
     const bool many = a.rows >= 4 * ops_sm_count();
-    if (nv <= 128) return ops_launch(norm_vec_kernel<BF16, 4, 1>, g, dim3(128), 0, s, 1, a);
-    if (nv <= 256 && many) return ops_launch(norm_vec_kernel<BF16, 4, 2>, g, dim3(128), 0, s, 1, a);
-    if (nv <= 256) return ops_launch(norm_vec_kernel<BF16, 8, 1>, g, dim3(256), 0, s, 1, a);
-    if (nv <= 512) return ops_launch(norm_vec_kernel<BF16, 8, 2>, g, dim3(256), 0, s, 1, a);
-    if (nv <= 1024) return ops_launch(norm_vec_kernel<BF16, 8, 4>, g, dim3(256), 0, s, 1, a);
-    if (nv <= 2048) return ops_launch(norm_vec_kernel<BF16, 16, 4>, g, dim3(512), 0, s, 1, a);
+    if (nv <= 128) return ops_launch(norm_vec_kernel<BF16, V, 4, 1>, g, dim3(128), 0, s, 1, a);
+    if (nv <= 256 && many) return ops_launch(norm_vec_kernel<BF16, V, 4, 2>, g, dim3(128), 0, s, 1, a);
+    if (nv <= 256) return ops_launch(norm_vec_kernel<BF16, V, 8, 1>, g, dim3(256), 0, s, 1, a);
+    if (nv <= 512) return ops_launch(norm_vec_kernel<BF16, V, 8, 2>, g, dim3(256), 0, s, 1, a);
+    if (nv <= 1024) return ops_launch(norm_vec_kernel<BF16, V, 8, 4>, g, dim3(256), 0, s, 1, a);
+    if (nv <= 2048) return ops_launch(norm_vec_kernel<BF16, V, 16, 4>, g, dim3(512), 0, s, 1, a);
+  } else {
+    if (nv <= 512) return ops_launch(norm_vec_kernel<BF16, 1, 4, 4>, g, dim3(128), 0, s, 1, a);
+    if (nv <= 2048) return ops_launch(norm_vec_kernel<BF16, 1, 8, 8>, g, dim3(256), 0, s, 1, a);
+    if (nv <= 8192) return ops_launch(norm_vec_kernel<BF16, 1, 16, 16>, g, dim3(512), 0, s, 1, a);
   }
   const size_t smem = (size_t)a.d * sizeof(float);
   if (smem > 40 * 1024) {

@@ -78,6 +78,41 @@ def test_norm_rows(ops, dt, rows, d, residual):
     assert ((scale.double() - rs).abs() <= rs * 2 ** -23).all()
 
 
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("rows,d", [(3, 5), (9, 513), (1000, 2047), (5, 2049), (7, 8191), (3, 8193)])
+@pytest.mark.parametrize("residual", [False, True])
+def test_norm_rows_of_odd_lengths(ops, dt, rows, d, residual):
+    """Rows without a common alignment, read value by value; also those of a wider matrix."""
+    wide = rand(rows, d + 3, seed=31).to(dt)
+    w = 1 + rand(d, seed=32, std=0.1)
+    r = rand(rows, d, seed=33).to(dt) if residual else None
+    for x in (wide[:, 1:d + 1].contiguous(), wide[:, 1:d + 1]):
+        q, scale, h = ops.rms_norm_int8(x, w, 1e-6, residual=r)
+        rh, rq, rs = norm_ref(x, w, 1e-6, r)
+        assert torch.equal(h, rh) and torch.equal(q.double(), rq)
+        assert ((scale.double() - rs).abs() <= rs * 2 ** -23).all()  # as above
+
+
+def test_norm_special_rows_of_odd_length(ops):
+    """As the special rows below, on the path that reads value by value, in bf16 too."""
+    d = 1023
+    for dt in (F32, BF16):
+        x = rand(7, d, seed=34)
+        x[1], x[2, 5], x[3, d - 1], x[6, 0] = 0, math.nan, math.inf, -math.inf
+        x[4] *= 1e-39
+        x[5] *= 1e30
+        x, w = x.to(dt), torch.ones(d, device="cuda")
+        q, scale, h = ops.rms_norm_int8(x, w, 1e-6)
+        _, rq, rs = norm_ref(x, w, 1e-6, None)
+        for i in (0, 1, 4, 5):
+            assert torch.equal(q[i].double(), rq[i]), i
+            # (a subnormal scale is rounded to 2^-149)
+            assert abs(scale[i].double() - rs[i]) <= rs[i] * 2 ** -23 + 2.0 ** -149, i
+        assert scale[1] == 1 and not q[1].any()
+        for i in (2, 3, 6):
+            assert torch.isnan(scale[i]) and not q[i].any()
+
+
 def test_norm_exact_ties(ops):
     """Values whose quotient is exactly a half round to even, as in 64 bits."""
     x = torch.zeros(2, 256, device="cuda")
