@@ -71,10 +71,11 @@ cudaError_t kv8_attention(const Kv8& c, const void* q, long long q_seq, long lon
                           long long o_row, OpsDtype dt, int rows, int heads, const int* starts, const int* counts,
                           int idx_stride, float scale, int max_len, cudaStream_t s, int splits = 0);
 
-// The same for many query rows, on tcgen05 (kv8_attention calls it for more than 64 a KV head).
+// The same for many query rows, on tcgen05 (kv8_attention calls it for more than 64 a KV head). splits: CTAs
+// that share a row tile's keys, 1, 2 or 4 (0: by max_len and the CTAs at hand).
 cudaError_t kv8_prompt_attention(const Kv8& c, const void* q, long long q_seq, long long q_row, void* out,
                                  long long o_seq, long long o_row, OpsDtype dt, int rows, int heads, const int* starts,
-                                 const int* counts, int idx_stride, float scale, cudaStream_t s);
+                                 const int* counts, int idx_stride, float scale, int max_len, int splits, cudaStream_t s);
 // Nonzero once a bounded wait inside kv8_prompt_attention gave up on the current device (clears it).
 int kv8_prompt_error();
 // Nonzero once a bounded wait inside linear_int8 gave up on the current device (clears it).

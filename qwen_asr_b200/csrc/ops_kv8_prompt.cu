@@ -38,6 +38,7 @@
 namespace qasr {
 namespace {
 
+constexpr int kMaxParts = 4;  // CTAs that share a row tile's keys
 constexpr int kRows = 128, kKeys = 64, kThreads = 256, kFill = 96;  // (threads that bring K and V)
 constexpr float kNone = -1.0e30f;
 constexpr uint32_t kColS = 0, kColP = 64, kColO = 128, kCols = 256;  // TMEM columns
@@ -53,13 +54,14 @@ struct PromptArgs {
   int idx_stride, rows, group;
   float scale;
   int q_vec, o_vec;  // rows start on 16-byte boundaries
+  int splits;        // CTAs of a cluster that share a row tile's keys
 };
 
 template <int HD>
 struct Smem {
   static constexpr int kPlane = kRows * HD * 2, kK = kKeys * HD * 2;
   // bf16 rows: Q, two K, a V; f32 rows: two planes of Q, two K, two V; then rows' factors, V scales, barriers
-  static constexpr int kBytes1 = kPlane + 3 * kK + 1024;
+  static constexpr int kBytes1 = kPlane + 3 * kK + 2048;
   static constexpr int kBytes2 = 2 * kPlane + 4 * kK + 4096;
 };
 
@@ -277,6 +279,7 @@ struct LaneValues {
 // What a CTA works on.
 struct Work {
   int kvh, seq, row0, start, count, tiles, nb;  // tiles of 16 keys (a scale each), blocks of 64
+  int first;                                    // the first key; scales, keys and tiles count from there
   const float *ks, *vs;
   const int8_t *k, *v;
 };
@@ -295,8 +298,9 @@ __device__ __forceinline__ void rows_of(const PromptArgs& a, int seq, int& start
 // which needs no search, 37 and 39).
 __device__ __forceinline__ Work work_of(const PromptArgs& a) {
   Work t;
-  const int row_tiles = (int)(((long long)a.rows * a.group + kRows - 1) / kRows), item = blockIdx.x / a.c.n_kv;
-  t.kvh = blockIdx.x % a.c.n_kv;
+  const int row_tiles = (int)(((long long)a.rows * a.group + kRows - 1) / kRows), id = blockIdx.x / a.splits;
+  const int item = id / a.c.n_kv;
+  t.kvh = id % a.c.n_kv;
   if (a.c.n_seq == 1) {
     t.seq = 0;
     t.row0 = (row_tiles - 1 - item) * kRows;
@@ -340,11 +344,16 @@ __device__ __forceinline__ Work work_of(const PromptArgs& a) {
   // keys any row of the tile sees
   const int s_last = min(t.count - 1, (t.row0 + kRows - 1) / a.group);
   const int len = s_last >= t.row0 / a.group ? (int)min((long long)t.start + s_last + 1, (long long)a.c.capacity) : 0;
-  t.tiles = (len + kKv8Block - 1) / kKv8Block;
-  t.nb = (len + kKeys - 1) / kKeys;
-  const long long blocks = a.c.capacity / kKv8Block, head = (long long)t.kvh * a.c.capacity * a.c.head_dim;
-  t.ks = a.c.ks + t.seq * a.c.scale_stride + t.kvh * blocks;
-  t.vs = a.c.vs + t.seq * a.c.scale_stride + t.kvh * blocks;
+  // this CTA's share of their blocks
+  const int all = (len + kKeys - 1) / kKeys, part = blockIdx.x % a.splits;
+  const int b0 = (int)((long long)all * part / a.splits), b1 = (int)((long long)all * (part + 1) / a.splits);
+  t.nb = b1 - b0;
+  t.first = b0 * kKeys;
+  t.tiles = (min(len, b1 * kKeys) - t.first + kKv8Block - 1) / kKv8Block;
+  const long long blocks = a.c.capacity / kKv8Block;
+  const long long head = ((long long)t.kvh * a.c.capacity + t.first) * a.c.head_dim;
+  t.ks = a.c.ks + t.seq * a.c.scale_stride + t.kvh * blocks + t.first / kKv8Block;
+  t.vs = a.c.vs + t.seq * a.c.scale_stride + t.kvh * blocks + t.first / kKv8Block;
   t.k = a.c.k + t.seq * a.c.seq_stride + head;
   t.v = a.c.v + t.seq * a.c.seq_stride + head;
   return t;
@@ -475,6 +484,49 @@ struct Pieces {
   }
 };
 
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t map_rank(uint32_t addr, int rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float peer1(uint32_t addr, int rank) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(map_rank(addr, rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 peer4(uint32_t addr, int rank) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(map_rank(addr, rank))
+               : "memory");
+  return v;
+}
+
+// Four values of an output row.
+template <bool BF16>
+__device__ __forceinline__ void put4(const PromptArgs& a, long long at, float4 o) {
+  if constexpr (BF16) {
+    __nv_bfloat16* p = (__nv_bfloat16*)a.out + at;
+    __nv_bfloat162 v[2] = {__floats2bfloat162_rn(o.x, o.y), __floats2bfloat162_rn(o.z, o.w)};
+    if (a.o_vec) {
+      *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(v);
+    } else {
+      p[0] = v[0].x; p[1] = v[0].y; p[2] = v[1].x; p[3] = v[1].y;
+    }
+  } else {
+    float* p = (float*)a.out + at;
+    if (a.o_vec) {
+      *reinterpret_cast<float4*>(p) = o;
+    } else {
+      p[0] = o.x; p[1] = o.y; p[2] = o.z; p[3] = o.w;
+    }
+  }
+}
+
 // Stores 32 / PARTS rows of a warp's 32 staged rows (pitch kPitch floats), the part-th share; `mine`: the
 // output offset of this lane's row, negative for none.
 template <int HD>
@@ -495,25 +547,43 @@ __device__ __forceinline__ void write_rows(const PromptArgs& a, const float* sta
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      if (off[i] < 0) continue;
-      const long long at = off[i] + col;
-      if constexpr (BF16) {
-        __nv_bfloat16* p = (__nv_bfloat16*)a.out + at;
-        __nv_bfloat162 v[2] = {__floats2bfloat162_rn(o[i].x, o[i].y), __floats2bfloat162_rn(o[i].z, o[i].w)};
-        if (a.o_vec) {
-          *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(v);
-        } else {
-          p[0] = v[0].x; p[1] = v[0].y; p[2] = v[1].x; p[3] = v[1].y;
-        }
-      } else {
-        float* p = (float*)a.out + at;
-        if (a.o_vec) {
-          *reinterpret_cast<float4*>(p) = o[i];
-        } else {
-          p[0] = o[i].x; p[1] = o[i].y; p[2] = o[i].z; p[3] = o[i].w;
-        }
-      }
+      if (off[i] >= 0) put4<BF16>(a, off[i] + col, o[i]);
     }
+  }
+}
+
+// A cluster's parts of the output rows (staged: each by itself, with its maximum and sum of p), joined by 256
+// threads: a CTA finishes 128 / splits of the rows. First the weights of each row's parts, a thread each, ...
+__device__ __forceinline__ void join_weights(const PromptArgs& a, uint32_t maxima, uint32_t sums, float* weights, int tid) {
+  if (tid >= kRows) return;
+  const int p = tid % a.splits, r = (int)(blockIdx.x % a.splits) * (kRows / a.splits) + tid / a.splits;
+  const float m = peer1(maxima + r * 4, p), l = peer1(sums + r * 4, p);
+  float top = m;
+  for (int o = 1; o < a.splits; o *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const float part = l * ex2(m - top);
+  float total = part;
+  for (int o = 1; o < a.splits; o *= 2) total += __shfl_xor_sync(0xffffffffu, total, o);
+  weights[tid] = total == 0.f ? 0.f : __fdiv_rn(part, total);
+}
+// ... then the rows.
+template <int HD, bool BF16>
+__device__ __forceinline__ void join_rows(const PromptArgs& a, const Work& t, uint32_t stage, const float* weights,
+                                          int warp, int lane) {
+  constexpr int kLanes = HD / 4, kPer = 32 / kLanes;
+  const int each = kRows / a.splits, r0 = (int)(blockIdx.x % a.splits) * each, col = lane % kLanes * 4;
+  for (int i = warp * kPer + lane / kLanes; i < each; i += 8 * kPer) {
+    const uint32_t at = stage + ((r0 + i) * kPitch<HD> + col) * 4;
+    const long long off = out_row(a, t, t.row0 + r0 + i, HD);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](const float4& v, float w) {
+      o.x = fmaf(v.x, w, o.x); o.y = fmaf(v.y, w, o.y); o.z = fmaf(v.z, w, o.z); o.w = fmaf(v.w, w, o.w);
+    };
+    for (int p = 0; p < a.splits; p += 2) {
+      const float4 v0 = peer4(at, p), v1 = peer4(at, p + 1);
+      add(v0, weights[i * a.splits + p]);
+      add(v1, weights[i * a.splits + p + 1]);
+    }
+    if (off >= 0) put4<BF16>(a, off + col, o);
   }
 }
 
@@ -525,7 +595,9 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_bf16_kernel(const PromptAr
   extern __shared__ __align__(1024) unsigned char smem[];
   unsigned char *sq = smem, *sk = smem + L::kPlane, *sv = sk + 2 * L::kK;
   float* row_fac = reinterpret_cast<float*>(sv + L::kK);  // each row's factor
-  float* red = row_fac + kRows;                           // the largest V scale of each warp's tiles
+  float* row_sum = row_fac + kRows;                       // (a part's) each row's sum
+  float* weights = row_sum + kRows;                       // the joined parts'
+  float* red = weights + kRows;                           // the largest V scale of each warp's tiles
   uint64_t* k_full = reinterpret_cast<uint64_t*>(red + 8);
   uint64_t *k_free = k_full + 2, *v_full = k_full + 4, *s_full = k_full + 5, *s_free = k_full + 6, *p_full = k_full + 7,
            *o_done = k_full + 8;
@@ -569,7 +641,7 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_bf16_kernel(const PromptAr
     // ---------------------------------------------------------------- softmax: thread = query row = TMEM lane
     const int rr = row0 + tid, s = rr / a.group;
     const bool live = s < count;
-    const int last = live ? min(start + s, a.c.capacity - 1) : -1;
+    const int last = (live ? min(start + s, a.c.capacity - 1) : -1) - t.first;
     const float fac = nb > 0 ? row_fac[tid] : 0.f;
     const float vref = nb > 0 ? vref_of(red) : 0.f;
     const float rvref = vref > 0.f ? __fdiv_rn(1.0f, vref) : 0.f;
@@ -661,6 +733,10 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_bf16_kernel(const PromptAr
     const float2 sums = split(l);
     const float total = sums.x + sums.y;
     const float inv = total == 0.f ? 0.f : __fdiv_rn(vref, total);
+    if (a.splits > 1) {  // (joined below)
+      row_fac[tid] = m;
+      row_sum[tid] = total;
+    }
     // through shared memory (operands are idle now, 32 rows a warp), so that a row's stores are contiguous
     static_assert(kRows * kPitch<HD> * 4 <= L::kPlane + 3 * L::kK, "the output reuses the operands");
     float* stage = reinterpret_cast<float*>(smem);
@@ -678,7 +754,8 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_bf16_kernel(const PromptAr
                    : make_float4(0.f, 0.f, 0.f, 0.f);
     }
     __syncwarp();
-    write_rows<HD, true, 1>(a, stage + warp * 32 * kPitch<HD>, out_row(a, t, rr, HD), 0, lane);
+    if (a.splits == 1)
+      write_rows<HD, true, 1>(a, stage + warp * 32 * kPitch<HD>, out_row(a, t, rr, HD), 0, lane);
   } else if (warp < 7) {
     // ---------------------------------------------------------------- K and V: int8 -> f16 operands
     const int ct = tid - 128, end = tiles * kKv8Block;
@@ -738,6 +815,15 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_bf16_kernel(const PromptAr
                (j > 0 || kk > 0) ? 1u : 0u);
       commit(o_done);
     }
+  }
+  if (a.splits > 1) {
+    __syncwarp();
+    cluster_barrier();  // every part is staged
+    join_weights(a, smem_u32(row_fac), smem_u32(row_sum), weights, tid);
+    __syncthreads();
+    join_rows<HD, true>(a, t, smem_u32(smem), weights, warp, lane);
+    __syncwarp();
+    cluster_barrier();  // no CTA leaves while a peer reads its part
   }
   __syncwarp();
   before_sync();
@@ -810,7 +896,7 @@ __global__ void __launch_bounds__(kThreads2, 1) prompt_f32_kernel(const PromptAr
     // ---------------------------------------------------------------- softmax: row = TMEM lane
     constexpr int kDims = HD / 2;
     const int half = warp >> 2, row = (warp & 3) * 32 + lane, rr = t.row0 + row, s = rr / a.group;
-    const int last = s < t.count ? min(t.start + s, a.c.capacity - 1) : -1;
+    const int last = (s < t.count ? min(t.start + s, a.c.capacity - 1) : -1) - t.first;
     const float fac = nb > 0 ? row_fac[row] : 0.f, vref = nb > 0 ? vref_of(red) : 0.f;
     const float rvref = vref > 0.f ? __fdiv_rn(1.0f, vref) : 0.f;
     const uint32_t trow = tmem + ((uint32_t)((warp & 3) * 32) << 16);
@@ -925,6 +1011,7 @@ __global__ void __launch_bounds__(kThreads2, 1) prompt_f32_kernel(const PromptAr
     asm volatile("bar.sync 1, 256;" ::: "memory");
     total = row_sum[row];
     const float inv = total == 0.f ? 0.f : __fdiv_rn(vref, total);
+    if (a.splits > 1 && half == 0) row_fac[row] = m;  // (joined below)
     static_assert(kRows * kPitch<HD> * 4 <= 2 * L::kPlane + 4 * L::kK, "the output reuses the operands");
     float* stage = reinterpret_cast<float*>(smem);
 #pragma unroll
@@ -934,7 +1021,16 @@ __global__ void __launch_bounds__(kThreads2, 1) prompt_f32_kernel(const PromptAr
           make_float4(p.x * inv, p.y * inv, q.x * inv, q.y * inv);
     }
     asm volatile("bar.sync 1, 256;" ::: "memory");
-    write_rows<HD, false, 2>(a, stage + (warp & 3) * 32 * kPitch<HD>, out_row(a, t, rr, HD), half, lane);
+    if (a.splits == 1) {
+      write_rows<HD, false, 2>(a, stage + (warp & 3) * 32 * kPitch<HD>, out_row(a, t, rr, HD), half, lane);
+    } else {
+      cluster_barrier();  // every part is staged
+      join_weights(a, smem_u32(row_fac), smem_u32(row_sum), row_max, tid);
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      join_rows<HD, false>(a, t, smem_u32(smem), row_max, warp, lane);
+      __syncwarp();
+      cluster_barrier();  // no CTA leaves while a peer reads its part
+    }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     const int end = t.tiles * kKv8Block;
@@ -964,40 +1060,45 @@ __global__ void __launch_bounds__(kThreads2, 1) prompt_f32_kernel(const PromptAr
       Pieces<HD, kFillV> even, odd;
       fill(even, odd, t.v, sv, v_full, v_free, tid - 384);
     } else if (nb > 0) {
-    // ---------------------------------------------------------------- products
-    const uint32_t qa = smem_u32(sq), ka = smem_u32(sk), va = smem_u32(sv);
-    auto qk = [&](int j) {
-      const int b = j & 1;
-      if (j >= 2 && !warp_wait(&s_free[b], (uint32_t)((j - 2) >> 1) & 1u, gave_up, 56)) return;
-      if (!warp_wait(&k_full[b], (uint32_t)(j >> 1) & 1u, gave_up, 57)) return;
-      after_sync();
+      // ---------------------------------------------------------------- products
+      const uint32_t qa = smem_u32(sq), ka = smem_u32(sk), va = smem_u32(sv);
+      auto qk = [&](int j) {
+        const int b = j & 1;
+        if (j >= 2 && !warp_wait(&s_free[b], (uint32_t)((j - 2) >> 1) & 1u, gave_up, 56)) return;
+        if (!warp_wait(&k_full[b], (uint32_t)(j >> 1) & 1u, gave_up, 57)) return;
+        after_sync();
 #pragma unroll
-      for (int pl = 0; pl < 2; ++pl)
+        for (int pl = 0; pl < 2; ++pl)
 #pragma unroll
-        for (int kk = 0; kk < HD / 16; ++kk)
-          mma_ss(tmem + kS2 + (uint32_t)(b * kKeys),
-                 sw128_desc(qa + pl * L::kPlane + (kk >> 2) * (kRows * 128) + (kk & 3) * 32),
-                 sw128_desc(ka + b * L::kK + (kk >> 2) * (kKeys * 128) + (kk & 3) * 32), idesc_f16(kKeys, false),
-                 (pl > 0 || kk > 0) ? 1u : 0u);
-      commit(&s_full[b]);
-      commit(&k_free[b]);
-    };
-    qk(0);
-    for (int j = 0; j < nb; ++j) {
-      const int b = j & 1;
-      if (j + 1 < nb) qk(j + 1);
-      if (!warp_wait(&v_full[b], (uint32_t)(j >> 1) & 1u, gave_up, 58) || !warp_wait(&p_full[b], (uint32_t)(j >> 1) & 1u, gave_up, 59)) break;
-      if (j >= 2 && !warp_wait(&o_free[b], (uint32_t)((j - 2) >> 1) & 1u, gave_up, 60)) break;
-      after_sync();
+          for (int kk = 0; kk < HD / 16; ++kk)
+            mma_ss(tmem + kS2 + (uint32_t)(b * kKeys),
+                   sw128_desc(qa + pl * L::kPlane + (kk >> 2) * (kRows * 128) + (kk & 3) * 32),
+                   sw128_desc(ka + b * L::kK + (kk >> 2) * (kKeys * 128) + (kk & 3) * 32), idesc_f16(kKeys, false),
+                   (pl > 0 || kk > 0) ? 1u : 0u);
+        commit(&s_full[b]);
+        commit(&k_free[b]);
+      };
+      qk(0);
+      for (int j = 0; j < nb; ++j) {
+        const int b = j & 1;
+        if (j + 1 < nb) qk(j + 1);
+        if (!warp_wait(&v_full[b], (uint32_t)(j >> 1) & 1u, gave_up, 58) || !warp_wait(&p_full[b], (uint32_t)(j >> 1) & 1u, gave_up, 59)) break;
+        if (j >= 2 && !warp_wait(&o_free[b], (uint32_t)((j - 2) >> 1) & 1u, gave_up, 60)) break;
+        after_sync();
 #pragma unroll
-      for (int pl = 0; pl < 2; ++pl)
+        for (int pl = 0; pl < 2; ++pl)
 #pragma unroll
-        for (int kk = 0; kk < kKeys / 16; ++kk)
-          mma_ts(tmem + kO2 + (uint32_t)(b * HD), tmem + kP2 + (uint32_t)(b * 64) + pl * 32 + kk * 8,
-                 sw128_desc(va + b * L::kK + kk * 2048, kKeys * 128), idesc_f16(HD, true), (pl > 0 || kk > 0) ? 1u : 0u);
-      commit(&o_full[b]);
-      commit(&v_free[b]);
+          for (int kk = 0; kk < kKeys / 16; ++kk)
+            mma_ts(tmem + kO2 + (uint32_t)(b * HD), tmem + kP2 + (uint32_t)(b * 64) + pl * 32 + kk * 8,
+                   sw128_desc(va + b * L::kK + kk * 2048, kKeys * 128), idesc_f16(HD, true), (pl > 0 || kk > 0) ? 1u : 0u);
+        commit(&o_full[b]);
+        commit(&v_free[b]);
+      }
     }
+    if (a.splits > 1) {  // (with the softmax warps)
+      __syncwarp();
+      cluster_barrier();
+      cluster_barrier();
     }
   }
   __syncwarp();
@@ -1006,20 +1107,31 @@ __global__ void __launch_bounds__(kThreads2, 1) prompt_f32_kernel(const PromptAr
   if (warp == 15) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols2));
 }
 
+// CTAs of a row tile: 2 or 4 while all of them run at once and each keeps 256 keys; a cluster joins their parts
+// through shared memory. 16 heads on 8 x 128, measured (us) at 1 / 2 / 4 / 8: 128 rows behind 8000 bf16 116 / 66 /
+// 39 / 33, f32 148 / 82 / 46 / 57 (eight CTAs wait for a place), behind 900 22 / 19 / 15 / 16 and 27 / 22 / 16 /
+// 26; 512 rows behind 7000 bf16 127 / 85 / 53 / 68, f32 139 / 79 / 87; 381 rows from 0 bf16 14 / 16 / 16 / 30.
+int auto_splits(long long ctas, int room, int max_len) {
+  int splits = 1;
+  while (splits < kMaxParts && ctas * splits * 2 <= room && splits * 512 <= max_len) splits *= 2;
+  return splits;
+}
+
 template <int HD, bool BF16>
-cudaError_t launch(const PromptArgs& a, cudaStream_t s) {
+cudaError_t launch(PromptArgs a, int max_len, cudaStream_t s) {
   const long long ctas = ((long long)a.rows * a.group + kRows - 1) / kRows * a.c.n_kv * a.c.n_seq;
   if (ctas > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
-  const dim3 g((unsigned)ctas);
+  if (a.splits < 1) a.splits = auto_splits(ctas, ops_sm_count() * (BF16 ? 2 : 1), max_len);
+  const dim3 g((unsigned)ctas * a.splits);
   static OncePerDevice once;
   if constexpr (BF16) {
     const cudaError_t e = once.smem(prompt_bf16_kernel<HD>, Smem<HD>::kBytes1);
     if (e != cudaSuccess) return e;
-    return ops_launch(prompt_bf16_kernel<HD>, g, dim3(kThreads), Smem<HD>::kBytes1, s, 1, a);
+    return ops_launch(prompt_bf16_kernel<HD>, g, dim3(kThreads), Smem<HD>::kBytes1, s, a.splits, a);
   } else {
     const cudaError_t e = once.smem(prompt_f32_kernel<HD>, Smem<HD>::kBytes2);
     if (e != cudaSuccess) return e;
-    return ops_launch(prompt_f32_kernel<HD>, g, dim3(kThreads2), Smem<HD>::kBytes2, s, 1, a);
+    return ops_launch(prompt_f32_kernel<HD>, g, dim3(kThreads2), Smem<HD>::kBytes2, s, a.splits, a);
   }
 }
 
@@ -1027,15 +1139,16 @@ cudaError_t launch(const PromptArgs& a, cudaStream_t s) {
 
 cudaError_t kv8_prompt_attention(const Kv8& c, const void* q, long long q_seq, long long q_row, void* out,
                                  long long o_seq, long long o_row, OpsDtype dt, int rows, int heads, const int* starts,
-                                 const int* counts, int idx_stride, float scale, cudaStream_t s) {
+                                 const int* counts, int idx_stride, float scale, int max_len,
+                                 int splits, cudaStream_t s) {
   auto vec = [&](const void* p, long long seq, long long row) {
     const int es = dt == OPS_BF16 ? 2 : 4;
     return (uintptr_t)p % 16 == 0 && seq * es % 16 == 0 && row * es % 16 == 0;
   };
   const PromptArgs a{c, q, out, q_seq, q_row, o_seq, o_row, starts, counts, idx_stride, rows, heads / c.n_kv, scale,
-                     vec(q, q_seq, q_row), vec(out, o_seq, o_row)};
-  if (c.head_dim == 128) return dt == OPS_BF16 ? launch<128, true>(a, s) : launch<128, false>(a, s);
-  return dt == OPS_BF16 ? launch<64, true>(a, s) : launch<64, false>(a, s);
+                     vec(q, q_seq, q_row), vec(out, o_seq, o_row), splits};
+  if (c.head_dim == 128) return dt == OPS_BF16 ? launch<128, true>(a, max_len, s) : launch<128, false>(a, max_len, s);
+  return dt == OPS_BF16 ? launch<64, true>(a, max_len, s) : launch<64, false>(a, max_len, s);
 }
 
 int kv8_prompt_error() {

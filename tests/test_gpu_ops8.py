@@ -525,6 +525,20 @@ def test_attention_prompts_of_any_order(ops, dt, n, rows):
     attend_and_check(ops, q, c, [17] * n, None)
 
 
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("hd,heads,n_kv,rows", [(128, 2, 1, 65), (64, 8, 2, 140), (128, 6, 3, 300)])
+def test_attention_few_rows_behind_many(ops, dt, hd, heads, n_kv, rows):
+    """Few row tiles, whose keys several blocks share: long and short histories, parts that see nothing."""
+    starts, counts = [3700, 0, 130], [rows, rows, rows // 3]
+    c = filled_cache(ops, 3, n_kv, 4096, hd, [s + k for s, k in zip(starts, counts)], seed=rows)
+    q = rand(3, rows, heads, hd, seed=7, std=1.5).to(dt)
+    got = attend_and_check(ops, q, c, starts, counts)
+    assert not got[2, rows // 3:].any()
+    attend_and_check(ops, q[:1], [t[:1] for t in c], starts[:1], None)
+    attend_and_check(ops, q[:1], [t[:1] for t in c], [600], None, max_len=600 + rows)
+    attend_and_check(ops, q[:1], [t[:1] for t in c], starts[:1], [0])
+
+
 @pytest.mark.parametrize("rows", [1, 40])
 def test_attention_ignores_what_is_masked(ops, rows):
     """NaN blocks behind a row's last position do not touch it; a NaN it does see reaches its head."""
