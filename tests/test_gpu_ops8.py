@@ -559,6 +559,71 @@ def test_attention_ignores_what_is_masked(ops, rows):
         assert torch.isnan(got[0, seen:, 2:]).all()
 
 
+@pytest.mark.parametrize("dt", [F32, BF16])
+def test_attention_shared_keys_with_bad_and_extreme_blocks(ops, dt):
+    """Keys that several blocks share: NaN scales behind the last position, NaN in a block that only later rows
+    see, one key far above all others."""
+    rows, start, hd, cap = 100, 2990, 128, 4096
+    c = filled_cache(ops, 1, 1, cap, hd, [cap], seed=12)
+    q = rand(1, rows, 2, hd, seed=13).to(dt)
+    st = torch.tensor([start], dtype=torch.int32, device="cuda")
+    want = ops.kv8_attention(q, ops.Kv8Cache(*c), st)
+    for t in c[2:]:
+        t[:, :, (start + rows - 1) // 16 + 1:] = math.nan
+    assert torch.equal(ops.kv8_attention(q, ops.Kv8Cache(*c), st), want)
+    for t in c[2:]:  # K, then V
+        keep = t[0, 0, (start + 50) // 16].clone()
+        t[0, 0, (start + 50) // 16] = math.nan
+        got = ops.kv8_attention(q, ops.Kv8Cache(*c), st)
+        seen = (start + 50) // 16 * 16 - start
+        assert torch.equal(got[:, :seen], want[:, :seen])
+        assert torch.isnan(got[:, seen:]).all()
+        t[0, 0, (start + 50) // 16] = keep
+    c[2][0, 0, 70] *= 60  # (16 keys of the second part)
+    attend_and_check(ops, q, c, [start], None)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("rows,cap", [(3, 64), (20, 64), (90, 128), (90, 2048)])
+def test_attention_rows_without_alignment(ops, dt, rows, cap):
+    """Query rows that start anywhere in a wider matrix: the bits of aligned ones."""
+    heads, hd = 4, 64
+    c = filled_cache(ops, 2, 2, cap, hd, [rows + 7, rows], seed=51)
+    wide = rand(2, rows, heads * hd + 3, seed=52).to(dt)
+    q = wide[:, :, 1:heads * hd + 1].unflatten(2, (heads, hd))
+    st = torch.tensor([7, 0], dtype=torch.int32, device="cuda")
+    assert torch.equal(ops.kv8_attention(q, ops.Kv8Cache(*c), st), ops.kv8_attention(q.contiguous(), ops.Kv8Cache(*c), st))
+
+
+def test_two_streams_at_once(ops):
+    """Calls that fill the GPU, on two streams at the same time, give the bits of calls one after the other."""
+    m, n, k = 2999, 1900, 4100
+    xq, wq = ints(m, k, 41), ints(n, k, 42)
+    xs, ws = rand(m, seed=43).abs() * 0.01, rand(n, seed=44).abs() * 0.01
+    c = filled_cache(ops, 2, 2, 4096, 128, [4096, 4096], seed=45)
+    q = rand(2, 150, 4, 128, seed=46)
+    st = torch.tensor([3900, 1000], dtype=torch.int32, device="cuda")
+    one = rand(2, 1, 4, 128, seed=47)
+    calls = (lambda: ops.linear_int8(xq, xs, wq, ws), lambda: ops.kv8_attention(q, ops.Kv8Cache(*c), st),
+             lambda: ops.kv8_attention(q.to(BF16), ops.Kv8Cache(*c), st), lambda: ops.linear_int8(xq[:9], xs[:9], wq, ws),
+             lambda: ops.kv8_attention(one, ops.Kv8Cache(*c), st))
+    want = [f() for f in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for turn in range(3):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                order = calls if i == 0 else calls[::-1]
+                got[i].append([f() for f in order])
+    torch.cuda.synchronize()
+    for i in range(2):
+        for r in got[i]:
+            for a, b in zip(r if i == 0 else r[::-1], want):
+                assert torch.equal(a, b)
+    ops.check()
+
+
 def test_attention_extreme_scores(ops):
     """One key far above the rest, queries of very different size, zero queries and zero blocks."""
     n_kv, hd, cap = 1, 128, 64
