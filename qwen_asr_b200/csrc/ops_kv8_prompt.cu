@@ -31,6 +31,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
+
 #include "bulk.cuh"
 #include "dev_util.cuh"
 #include "ops.h"
@@ -1107,14 +1109,24 @@ __global__ void __launch_bounds__(kThreads2, 1) prompt_f32_kernel(const PromptAr
   if (warp == 15) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols2));
 }
 
-// CTAs of a row tile: 2 or 4 while all of them run at once and each keeps 256 keys; a cluster joins their parts
-// through shared memory. 16 heads on 8 x 128, measured (us) at 1 / 2 / 4 / 8: 128 rows behind 8000 bf16 116 / 66 /
-// 39 / 33, f32 148 / 82 / 46 / 57 (eight CTAs wait for a place), behind 900 22 / 19 / 15 / 16 and 27 / 22 / 16 /
-// 26; 512 rows behind 7000 bf16 127 / 85 / 53 / 68, f32 139 / 79 / 87; 381 rows from 0 bf16 14 / 16 / 16 / 30.
+// CTAs of a row tile, 1, 2 or 4, whose parts a cluster joins through shared memory: the number with the least
+// estimated time in blocks of keys, of which a CTA's prologue and output cost 8 and a joined one's 11; `room` CTAs
+// run at once. (Eight wait long for a place.) 16 heads on 8 x 128, measured (us) at 1 / 2 / 4: 128 rows behind 8000
+// bf16 116 / 66 / 39, f32 148 / 82 / 46, behind 900 22 / 19 / 15 and 27 / 22 / 16; 512 rows behind 7000 bf16 127 /
+// 85 / 53; 1500 rows behind 6000 bf16 181 / 137 / 146; 4 x 512 behind 1000 to 7000 bf16 163 / 112 / 141, f32 166 /
+// 186 / 245; 8 x 381 behind 0 to 1022 bf16 46 / 68 / 108.
 int auto_splits(long long ctas, int room, int max_len) {
-  int splits = 1;
-  while (splits < kMaxParts && ctas * splits * 2 <= room && splits * 512 <= max_len) splits *= 2;
-  return splits;
+  const long long blocks = (max_len + kKeys - 1) / kKeys;
+  int best = 1;
+  long long least = 0;
+  for (int s = 1; s <= kMaxParts; s *= 2) {
+    const long long cost = std::max<long long>(room, ctas * s) * ((blocks + s - 1) / s + (s > 1 ? 11 : 8));
+    if (s == 1 || cost < least) {
+      best = s;
+      least = cost;
+    }
+  }
+  return best;
 }
 
 template <int HD, bool BF16>

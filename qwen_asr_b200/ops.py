@@ -294,7 +294,8 @@ def kv8_attention(q, cache: Kv8Cache, starts, counts=None, scale: float | None =
     """softmax(scale * q k^T) v of query rows q [n_seq, rows, heads, head_dim] (f32 or bf16) over
     the cache: row r of sequence b attends positions 0 .. starts[b] + r; rows from counts[b] on get
     zeros. scale defaults to 1 / sqrt(head_dim). max_len, an upper bound of starts + rows when the
-    caller knows one, only shapes the launch."""
+    caller knows one, only shapes the launch: worth giving where the capacity is far larger (f32: 381
+    rows from 0 in a cache of 2048 take 24 us without it, 16 with)."""
     if _fast is not None:
         out = _fast.kv8_attention(q, cache, starts, counts, scale, max_len)
         if out is not None:
