@@ -23,8 +23,8 @@
 // and counts together, with an elected lane to issue, took 64 rows over 8064 f32 keys from 197 to 149 us.)
 //   bf16 rows: 256 threads, a softmax thread a row; two CTAs an SM, one's softmax beside the other's
 //   products. O stays in TMEM. 8 x 381 rows over up to 1403 keys, 8 KV heads of 2 x 128: 44 us; 2048 rows
-//   over 8048 keys, 4 KV heads of 4 x 64: 143 us; 592 heads' rows over 8064 keys: 198 us, 785 TFLOP/s.
-//   f32 rows: see below. The same shapes: 67, 213 and 310 us.
+//   over 8048 keys, 4 KV heads of 4 x 64: 140 us; 592 heads' rows over 8064 keys: 198 us, 785 TFLOP/s.
+//   f32 rows: see below. The same shapes: 67, 208 and 310 us.
 // Bound: the chain of a block's steps (scores, maximum, exp2, P V). bf16 rows: 0.9 us a block and CTA alone
 // on its SM, two CTAs an SM, in which exp2 takes 0.27 us an SM and the products 0.3 to 0.35 (a quarter of the exp2 as
 // polynomials on the FMA units was slower: 51 -> 55 us); f32 rows: 1.2 us, the products 0.7 of them.
