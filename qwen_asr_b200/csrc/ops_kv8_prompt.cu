@@ -285,13 +285,14 @@ struct Work {
   const float *ks, *vs;
   const int8_t *k, *v;
 };
-// A sequence's first position (at most the capacity) and live rows.
+// A sequence's first position (0 to the capacity) and live rows. (A skipped one's start must not be negative
+// either: the order below counts from it, and would find no tile for a CTA.)
 __device__ __forceinline__ void rows_of(const PromptArgs& a, int seq, int& start, int& count) {
   start = a.starts[(long long)seq * a.idx_stride];
   count = a.rows;
   if (a.counts) count = min(max(a.counts[(long long)seq * a.idx_stride], 0), a.rows);
   if (start < 0) count = 0;
-  start = min(start, a.c.capacity);
+  start = min(max(start, 0), a.c.capacity);
 }
 // All 32 lanes call it. The row tiles of up to 32 sequences are taken up by the keys they see, most first, so
 // that no long one is left for the end: lane i counts those of sequence i that see at least K tiles' worth of
