@@ -4,16 +4,23 @@
 // the keys they see in blocks of 64. Per block
 //   S = Q K^T          M = 128, N = 64, K = head_dim   -> TMEM
 //   p = exp2(S f - m)  f = scale * log2(e) * K scale of 16 tokens; running maximum m and sum l
-//   O += P V           P = p * V scale / vref, an operand in TMEM; N = head_dim
-// and at the end O * vref / l.
+//   O += P V           P = p * V scale * 2^(kTop - r), an operand in TMEM; N = head_dim
+// and at the end O * 2^(r - kTop) / l.
 //
 // Precision. int8 is exact in f16, so K and V enter the products as they are; their scales stay
-// outside, in f32 (vref, a power of two above every V scale the rows see, keeps P in f16's range).
-// A query row is scaled by a power of two to [1/2, 1). For f32 rows q and P are two f16 planes,
-// hi + lo, held to 2^-25 of the row's largest; both planes add into the same f32 accumulator. For bf16
+// outside, in f32. A query row is scaled by a power of two to [1/2, 1). For f32 rows q and P are two f16
+// planes, hi + lo, which hold a value to 2^-22 of itself (q, or 2^-25 of the row's largest); both planes add into the same f32 accumulator. For bf16
 // rows one plane: 2^-11 of a probability, an eighth of the output's own rounding.
-// m is only raised when a score exceeds it by 2^8 (p up to 256 is as exact in f16): what has been summed
-// is then rescaled, which the first blocks of a row do and later ones hardly ever.
+// f16 has no step below 2^-24, so a row's weights p * V scale are held as fractions of about the largest of them,
+// 2^r, in the upper part of its range: none is off by more than 2^-30 of the row's largest so far (bf16 rows) or
+// 2^-37 of the block's (f32 rows, whose blocks are added outside TMEM, each with an r of its own). Not as fractions
+// of the largest V scale: a block of large values that a row gives no weight, or does not see, would cost it the
+// others' bits (1e-3 of the output behind a scale 1e4 times as large); and thousands of keys that have 2^-25 of the
+// weight each add up. (Against the largest V scale of the row tile, looked at once: 4 x 512 bf16 rows behind 1000 to
+// 7000 113 -> 117 us, f32 166 -> 170. Looking at a block's weights only where its V scales leave a window below 2^r,
+// in a branch of the warp: 121 and 182.)
+// m is only raised when a score exceeds it by 2^kLag, and r of bf16 rows when a weight exceeds 2^(r + kLag): what has
+// been summed is then rescaled, which the first blocks of a row do and later ones hardly ever.
 //
 // Two kernels. In both some warps do the softmax; others bring K and V from global memory as int8, two
 // blocks ahead in registers, and write them as f16 rows of a token in the 128-byte-swizzle layout, which is
@@ -43,6 +50,9 @@ namespace {
 constexpr int kMaxParts = 4;  // CTAs that share a row tile's keys
 constexpr int kRows = 128, kKeys = 64, kThreads = 256, kFill = 96;  // (threads that bring K and V)
 constexpr float kNone = -1.0e30f;
+constexpr float kLag = 8.f;  // what a score may exceed m by, and a bf16 row's weight 2^r (log2)
+constexpr int kTop1 = 7, kTop2 = 14;  // log2 of 2^r in P: 2^(kTop1 + kLag) and 2^kTop2 are in f16's range (to 65504)
+constexpr float kFaint = 80.f;  // probabilities under 2^-80 count as 2^-80 for r: P's factor stays finite
 constexpr uint32_t kColS = 0, kColP = 64, kColO = 128, kCols = 256;  // TMEM columns
 
 __device__ int g_prompt_err;  // nonzero once a bounded wait gave up
@@ -64,7 +74,7 @@ struct Smem {
   static constexpr int kPlane = kRows * HD * 2, kK = kKeys * HD * 2;
   // bf16 rows: Q, two K, a V; f32 rows: two planes of Q, two K, two V; then rows' factors, V scales, barriers
   static constexpr int kBytes1 = kPlane + 3 * kK + 2048;
-  static constexpr int kBytes2 = 2 * kPlane + 4 * kK + 4096;
+  static constexpr int kBytes2 = 2 * kPlane + 4 * kK + 6144;
 };
 
 // 128-byte swizzle, 8-row groups 1024 bytes apart; lead: bytes from 64 columns to the next (MN-major)
@@ -140,6 +150,23 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float lg2(float x) {  // (-inf for 0 and, flushed, for what is below 2^-126)
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// (NaN when a is)
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// r for weights of up to 2^e: the whole number 1/2 to 3/2 above it, within what leaves 2^r, and a V scale times
+// 2^-r, in f32's range. (By 1.5 * 2^23, whose low bits are then the number.)
+__device__ __forceinline__ int exponent_of(float e) {
+  return __float_as_int(fminf(fmaxf(e, -100.f), 121.f) + 12582912.f) - 0x4B400000 + 1;
+}
+__device__ __forceinline__ float power(int r) { return __int_as_float((127 + r) << 23); }
 // Two f32 in one register pair.
 typedef unsigned long long f32x2;
 __device__ __forceinline__ f32x2 pair(float a, float b) {
@@ -363,12 +390,11 @@ __device__ __forceinline__ Work work_of(const PromptArgs& a) {
 }
 
 // Q as operand planes: each of eight warps brings 16 rows, all of them in flight, a lane HD / 32
-// neighbouring values. Also the rows' factors and the warps' largest V scales.
+// neighbouring values. Also the rows' factors.
 template <int HD, int PL, bool BF16>
-__device__ __forceinline__ void bring_q(const PromptArgs& a, const Work& t, unsigned char* sq, float* row_fac, float* red,
-                                        int warp, int lane) {
+__device__ __forceinline__ void bring_q(const PromptArgs& a, const Work& t, unsigned char* sq, float* row_fac, int warp,
+                                        int lane) {
   constexpr int N = HD / 32, kPlane = kRows * HD * 2;
-  float top = 0.f;
   const int r0 = warp * 16;
   // lane i knows where row i is (a division a row, not one for each of its values)
   const int lr = t.row0 + r0 + (lane & 15), ls = lr / a.group;
@@ -382,8 +408,6 @@ __device__ __forceinline__ void bring_q(const PromptArgs& a, const Work& t, unsi
     raw[i].zero();
     if (off >= 0) raw[i].load(a, off + lane * N);
   }
-  // (a NaN V scale only spoils the rows that see it)
-  for (int i = warp * 32 + lane; i < t.tiles; i += 256) top = fmaxf(top, __ldg(t.vs + i));
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     const int r = r0 + i;
@@ -421,8 +445,6 @@ __device__ __forceinline__ void bring_q(const PromptArgs& a, const Work& t, unsi
     }
   }
   fence_async_smem();
-  top = warp_max(top);
-  if (lane == 0) red[warp] = top;
 }
 
 // Where a query row's output starts (negative behind the last row).
@@ -430,14 +452,6 @@ __device__ __forceinline__ long long out_row(const PromptArgs& a, const Work& t,
   if (rr >= a.rows * a.group) return -1;
   const int s = rr / a.group;
   return t.seq * a.o_seq + (long long)s * a.o_row + (long long)(t.kvh * a.group + rr - s * a.group) * hd;
-}
-
-// The power of two above every V scale the tile sees (2^-100 at least), 0 for none.
-__device__ __forceinline__ float vref_of(const float* red) {
-  float top = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) top = fmaxf(top, red[i]);
-  return top > 0.f ? fmaxf(__uint_as_float((__float_as_uint(top) + 0x7FFFFFu) & 0xFF800000u), 7.888609e-31f) : 0.f;
 }
 
 // 16 bytes, or zeros.
@@ -600,8 +614,7 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_bf16_kernel(const PromptAr
   float* row_fac = reinterpret_cast<float*>(sv + L::kK);  // each row's factor
   float* row_sum = row_fac + kRows;                       // (a part's) each row's sum
   float* weights = row_sum + kRows;                       // the joined parts'
-  float* red = weights + kRows;                           // the largest V scale of each warp's tiles
-  uint64_t* k_full = reinterpret_cast<uint64_t*>(red + 8);
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(weights + kRows);
   uint64_t *k_free = k_full + 2, *v_full = k_full + 4, *s_full = k_full + 5, *s_free = k_full + 6, *p_full = k_full + 7,
            *o_done = k_full + 8;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(k_full + 9);
@@ -634,7 +647,7 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_bf16_kernel(const PromptAr
 
   const Work t = work_of(a);
   const int row0 = t.row0, start = t.start, count = t.count, tiles = t.tiles, nb = t.nb;
-  if (nb > 0) bring_q<HD, 1, true>(a, t, sq, row_fac, red, warp, lane);
+  if (nb > 0) bring_q<HD, 1, true>(a, t, sq, row_fac, warp, lane);
   before_sync();
   __syncthreads();
   after_sync();
@@ -646,10 +659,9 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_bf16_kernel(const PromptAr
     const bool live = s < count;
     const int last = (live ? min(start + s, a.c.capacity - 1) : -1) - t.first;
     const float fac = nb > 0 ? row_fac[tid] : 0.f;
-    const float vref = nb > 0 ? vref_of(red) : 0.f;
-    const float rvref = vref > 0.f ? __fdiv_rn(1.0f, vref) : 0.f;
     const uint32_t trow = tmem + ((uint32_t)(warp * 32) << 16);
-    float m = kNone;
+    // log2 of the largest weight so far; r + kLag, and 2^(kTop1 - r)
+    float m = kNone, most = -__int_as_float(0x7F800000), full = -__int_as_float(0x7F800000), up = 1.f;
     f32x2 l = 0;  // two partial sums
     float kn[4], vn[4];  // the next block's scales
     auto scales = [&](int j) {
@@ -665,13 +677,16 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_bf16_kernel(const PromptAr
       float f[4], w[4];
       const int pos0 = j * kKeys;
       const bool partial = __any_sync(0xffffffffu, pos0 + kKeys - 1 > last);
+      float wl[4];
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
         f[b] = fac * kn[b];
-        w[b] = vn[b] * rvref;
+        w[b] = vn[b];
         // a row that sees nothing of a tile takes nothing of its scale either
         if (partial && pos0 + b * kKv8Block > last) w[b] = 0.f;
+        wl[b] = lg2(w[b]);
       }
+      const float faint = fmaxf(fmaxf(wl[0], wl[1]), fmaxf(wl[2], wl[3])) - kFaint;
       if (j + 1 < nb) scales(j + 1);
       wait(s_full, (uint32_t)j & 1u, gave_up, 43);
       __syncwarp();
@@ -687,22 +702,35 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_bf16_kernel(const PromptAr
         for (int i = 0; i < kKeys; ++i)
           if (pos0 + i > last) x[i] = -__int_as_float(0x7F800000);
       }
-      float mx = kNone;
+      float mx = kNone, e = -__int_as_float(0x7F800000);  // the largest score, and log2 of the largest weight
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
         float t = x[16 * b];
 #pragma unroll
         for (int i = 1; i < 16; ++i) t = fmaxf(t, x[16 * b + i]);
-        mx = fmaxf(mx, t * f[b]);  // (a masked tile's -inf, or no number: ignored)
+        t *= f[b];
+        mx = fmaxf(mx, t);  // (a masked tile's -inf, or no number: ignored)
+        e = fmaxf(e, t + wl[b]);
       }
-      const bool grow = mx > m + 8.f;
-      const float corr = grow ? ex2(m - mx) : 1.f;
-      if (grow) m = mx;
+      const bool grow = mx > m + kLag || fmaxf(e - m, faint) > full, rescale = __any_sync(0xffffffffu, grow);
+      float corr = 1.f, corr_o = 1.f;
+      if (grow) {
+        const float m1 = mx > m + kLag ? mx : m;
+        most = fmaxf(most, e);
+        const int r = exponent_of(fmaxf(most - m1, faint));
+        corr = ex2(m - m1);
+        corr_o = ex2(m - m1 + (full - (kLag + (float)r)));
+        m = m1;
+        full = kLag + (float)r;
+        up = power(kTop1 - r);
+      }
+#pragma unroll
+      for (int b = 0; b < 4; ++b) w[b] *= up;
       if (j > 0) {
         wait(o_done, (uint32_t)(j - 1) & 1u, gave_up, 44);
         __syncwarp();
         after_sync();
-        if (__any_sync(0xffffffffu, grow)) {
+        if (rescale) {
           l = mul2(l, pair(corr, corr));
 #pragma unroll 1
           for (int c = 0; c < HD; c += 16) {
@@ -710,7 +738,7 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_bf16_kernel(const PromptAr
             tmem_ld16(trow + kColO + c, o);
             tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr_o);
             tmem_st16(trow + kColO + c, o);
           }
           tmem_st_wait();
@@ -729,13 +757,13 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_bf16_kernel(const PromptAr
       before_sync();
       mbar_arrive(p_full);
     }
-    // ---- O * vref / l
+    // ---- O * 2^(r - kTop1) / l
     if (nb > 0) wait(o_done, (uint32_t)(nb - 1) & 1u, gave_up, 45);
     __syncwarp();
     after_sync();
     const float2 sums = split(l);
     const float total = sums.x + sums.y;
-    const float inv = total == 0.f ? 0.f : __fdiv_rn(vref, total);
+    const float inv = total == 0.f ? 0.f : __fdiv_rn(1.0f, up * total);
     if (a.splits > 1) {  // (joined below)
       row_fac[tid] = m;
       row_sum[tid] = total;
@@ -842,8 +870,8 @@ constexpr uint32_t kS2 = 0, kP2 = 128, kO2 = 256, kCols2 = 512;
 // Warps 0-7 softmax: two threads a row, each half the block's keys and half the output's dims, whose sums
 // it keeps in f32 registers: every block's product starts from zero and is added there. (Accumulated in
 // TMEM over all blocks, the tensor core's rounding towards zero shrank the output by 4e-8 a product:
-// 1.7e-6 at 1400 keys, and growing.) Warps 8-11 bring K and 12-14 V, two blocks ahead in registers, one
-// thread of warp 15 issues the products. The softmax warps take the registers that the others leave:
+// 1.7e-6 at 1400 keys, and growing.) Warps 8-11 bring K and 12-14 V, two blocks ahead in registers,
+// warp 15 issues the products. The softmax warps take the registers that the others leave:
 // 256 x (168 + 88) = 512 x 128.
 template <int HD>
 __global__ void __launch_bounds__(kThreads2, 1) prompt_f32_kernel(const PromptArgs a) {
@@ -851,10 +879,9 @@ __global__ void __launch_bounds__(kThreads2, 1) prompt_f32_kernel(const PromptAr
   extern __shared__ __align__(1024) unsigned char smem[];
   unsigned char *sq = smem, *sk = smem + 2 * L::kPlane, *sv = sk + 2 * L::kK;
   float* row_fac = reinterpret_cast<float*>(sv + 2 * L::kK);  // each row's factor
-  float* row_max = row_fac + kRows;                           // [block parity][half][row]
-  float* row_sum = row_max + 4 * kRows;                       // [row] the second half's sum
-  float* red = row_sum + kRows;                               // the largest V scale of each warp's tiles
-  uint64_t* k_full = reinterpret_cast<uint64_t*>(red + 8);
+  float* row_max = row_fac + kRows;                           // [block parity][half][row] (largest score, weight)
+  float* row_sum = row_max + 8 * kRows;                       // [row] the second half's sum
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(row_sum + kRows);
   uint64_t *k_free = k_full + 2, *v_full = k_full + 4, *v_free = k_full + 6, *s_full = k_full + 8, *s_free = k_full + 10,
            *o_full = k_full + 12, *o_free = k_full + 14, *p_full = k_full + 16;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(k_full + 18);
@@ -888,7 +915,7 @@ __global__ void __launch_bounds__(kThreads2, 1) prompt_f32_kernel(const PromptAr
   pdl_wait();
   const Work t = work_of(a);
   const int nb = t.nb;
-  if (nb > 0 && warp < 8) bring_q<HD, 2, false>(a, t, sq, row_fac, red, warp, lane);
+  if (nb > 0 && warp < 8) bring_q<HD, 2, false>(a, t, sq, row_fac, warp, lane);
   before_sync();
   __syncthreads();
   after_sync();
@@ -900,8 +927,7 @@ __global__ void __launch_bounds__(kThreads2, 1) prompt_f32_kernel(const PromptAr
     constexpr int kDims = HD / 2;
     const int half = warp >> 2, row = (warp & 3) * 32 + lane, rr = t.row0 + row, s = rr / a.group;
     const int last = (s < t.count ? min(t.start + s, a.c.capacity - 1) : -1) - t.first;
-    const float fac = nb > 0 ? row_fac[row] : 0.f, vref = nb > 0 ? vref_of(red) : 0.f;
-    const float rvref = vref > 0.f ? __fdiv_rn(1.0f, vref) : 0.f;
+    const float fac = nb > 0 ? row_fac[row] : 0.f;
     const uint32_t trow = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     float m = kNone;
     f32x2 l = 0, acc[kDims / 2];
@@ -916,7 +942,9 @@ __global__ void __launch_bounds__(kThreads2, 1) prompt_f32_kernel(const PromptAr
         vn[b] = tl < t.tiles ? __ldg(t.vs + tl) : 0.f;
       }
     };
+    float down = 0.f;          // 2^(r - kTop2) of the last block
     auto add_o = [&](int j) {  // acc += O of block j, whose buffer is free then
+      const f32x2 d2 = pair(down, down);
       const uint32_t col = trow + kO2 + (uint32_t)((j & 1) * HD + half * kDims);
 #pragma unroll
       for (int c = 0; c < kDims; c += 32) {
@@ -924,22 +952,23 @@ __global__ void __launch_bounds__(kThreads2, 1) prompt_f32_kernel(const PromptAr
         tmem_ld32(col + c, reinterpret_cast<uint32_t*>(o));
         tmem_ld_wait();
 #pragma unroll
-        for (int i = 0; i < 16; ++i) acc[c / 2 + i] = add2(acc[c / 2 + i], pair(o[2 * i], o[2 * i + 1]));
+        for (int i = 0; i < 16; ++i) acc[c / 2 + i] = fma2(pair(o[2 * i], o[2 * i + 1]), d2, acc[c / 2 + i]);
       }
       before_sync();
       mbar_arrive(&o_free[j & 1]);
     };
     scales(0);
     for (int j = 0; j < nb; ++j) {
-      float f[2], w[2];
+      float f[2], w[2], wl[2];
       const int pos0 = j * kKeys + half * 32;
       const bool partial = __any_sync(0xffffffffu, pos0 + 31 > last);
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
         f[b] = fac * kn[b];
-        w[b] = vn[b] * rvref;
+        w[b] = vn[b];
         // a row that sees nothing of a tile takes nothing of its scale either
         if (partial && pos0 + b * kKv8Block > last) w[b] = 0.f;
+        wl[b] = lg2(w[b]);
       }
       if (j + 1 < nb) scales(j + 1);
       wait(&s_full[j & 1], (uint32_t)(j >> 1) & 1u, gave_up, 51);
@@ -955,24 +984,31 @@ __global__ void __launch_bounds__(kThreads2, 1) prompt_f32_kernel(const PromptAr
         for (int i = 0; i < 32; ++i)
           if (pos0 + i > last) x[i] = -__int_as_float(0x7F800000);
       }
-      float mx = kNone;
+      float mx = kNone, e = -__int_as_float(0x7F800000);  // the largest score, and log2 of the largest weight
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
-        float top = x[16 * b];
+        float t = x[16 * b];
 #pragma unroll
-        for (int i = 1; i < 16; ++i) top = fmaxf(top, x[16 * b + i]);
-        mx = fmaxf(mx, top * f[b]);  // (a masked tile's -inf, or no number: ignored)
+        for (int i = 1; i < 16; ++i) t = fmaxf(t, x[16 * b + i]);
+        t *= f[b];
+        mx = fmaxf(mx, t);  // (a masked tile's -inf, or no number: ignored)
+        e = fmaxf(e, t + wl[b]);
       }
-      // the row's maximum over both halves (two buffers: the next block's barrier keeps them apart)
-      float* shared_max = row_max + (j & 1) * 2 * kRows;
-      shared_max[half * kRows + row] = mx;
+      e = fmaxf(e, mx - kFaint + fmaxf(wl[0], wl[1]));
+      // over both halves of the row (two buffers: the next block's barrier keeps them apart)
+      float2* shared_max = reinterpret_cast<float2*>(row_max) + (j & 1) * 2 * kRows;
+      shared_max[half * kRows + row] = make_float2(mx, e);
       asm volatile("bar.sync 1, 256;" ::: "memory");
-      mx = fmaxf(mx, shared_max[(half ^ 1) * kRows + row]);
-      const bool grow = mx > m + 8.f;
+      const float2 other = shared_max[(half ^ 1) * kRows + row];
+      mx = fmaxf(mx, other.x);
+      const bool grow = mx > m + kLag;
       const float corr = grow ? ex2(m - mx) : 1.f;
       const bool rescale = __any_sync(0xffffffffu, grow);
       if (grow) m = mx;
       if (rescale) l = mul2(l, pair(corr, corr));
+      const int r = exponent_of(fmaxf(e, other.y) - m);
+#pragma unroll
+      for (int b = 0; b < 2; ++b) w[b] = min_nan(w[b] * power(kTop2 - r), 1e37f);
       // (P of block j - 2 has been read: its O was added in the last round)
       const uint32_t pcol = trow + kP2 + (uint32_t)((j & 1) * 64 + half * 16);
 #pragma unroll
@@ -994,6 +1030,7 @@ __global__ void __launch_bounds__(kThreads2, 1) prompt_f32_kernel(const PromptAr
         after_sync();
         add_o(j - 1);
       }
+      down = power(r - kTop2);
       if (rescale) {
 #pragma unroll
         for (f32x2& y : acc) y = mul2(y, pair(corr, corr));
@@ -1005,7 +1042,7 @@ __global__ void __launch_bounds__(kThreads2, 1) prompt_f32_kernel(const PromptAr
       after_sync();
       add_o(nb - 1);
     }
-    // ---- O * vref / l, through shared memory, so that a row's stores are contiguous
+    // ---- O / l, through shared memory, so that a row's stores are contiguous
     const float2 sums = split(l);
     float total = sums.x + sums.y;
     if (half == 1) row_sum[row] = total;
@@ -1013,7 +1050,7 @@ __global__ void __launch_bounds__(kThreads2, 1) prompt_f32_kernel(const PromptAr
     if (half == 0) row_sum[row] += total;
     asm volatile("bar.sync 1, 256;" ::: "memory");
     total = row_sum[row];
-    const float inv = total == 0.f ? 0.f : __fdiv_rn(vref, total);
+    const float inv = total == 0.f ? 0.f : __fdiv_rn(1.0f, total);
     if (a.splits > 1 && half == 0) row_fac[row] = m;  // (joined below)
     static_assert(kRows * kPitch<HD> * 4 <= 2 * L::kPlane + 4 * L::kK, "the output reuses the operands");
     float* stage = reinterpret_cast<float*>(smem);

@@ -47,3 +47,115 @@ def test_prompt_rows_of_skipped_sequences_are_zeros(ops, dt, n, live, group, row
     attend_into(ops, out.transpose(0, 1), q, c, [s if i < live else -1000 for i, s in enumerate(starts)], counts)
     assert torch.equal(out.transpose(0, 1), want)
     ops.check()
+
+
+# ------------------------------------------------------------------ blocks of very different V scales, long tails
+def weighed_ref(q, c, starts, scale):
+    """(out, tolerance) in 64 bits, the tolerance relative to what a row weighs: with weights w = p vscale of its
+    keys, W the largest of them and l the sum of p,
+      the scores' error d of a key, under 2^-21 scale max|q| sum|k| (q held to 2^-22 of its largest value or better,
+        product, factor and exponential of an f32 path), once in the numerator and once in l;
+      the weights: two f16 planes hold each to 2^-22, one to 2^-11, and none is off by more than 2^-29 of W (half of
+        f16's smallest step, 2^-24, under a largest value of 2^4 and up) or half of 2^-32 of 8 W (digits), with int8
+        values up to 127;
+      the sums: 2^-23 for each tile of 16 tokens, and 2^-22 for the end, of sum w |v|; half a step of the output."""
+    k, v, ks, vs = c
+    n, rows, heads, hd = q.shape
+    g = heads // k.shape[1]
+    out = torch.zeros_like(q, dtype=torch.float64)
+    tol = torch.zeros_like(out)
+    plane = 2.0 ** -22 if q.dtype == F32 else 2.0 ** -11
+    for b in range(n):
+        for r in range(rows):
+            L = starts[b] + r + 1
+            kk = k[b, :, :L].double() * ks[b].repeat_interleave(16, 1)[:, :L, None].double()
+            sv = vs[b].repeat_interleave(16, 1)[:, :L].double()
+            vv = v[b, :, :L].double() * sv[:, :, None]
+            kk, vv, sv = kk.repeat_interleave(g, 0), vv.repeat_interleave(g, 0), sv.repeat_interleave(g, 0)
+            qq = q[b, r].double()
+            x = (kk @ qq[:, :, None])[..., 0] * scale
+            p = torch.exp(x - x.amax(1, keepdim=True))
+            l = p.sum(1, keepdim=True)
+            out[b, r] = (p[:, None] @ vv)[:, 0] / l
+            d = 2.0 ** -21 * scale * qq.abs().amax(1, keepdim=True) * kk.abs().sum(2)
+            size = (p[:, None] @ vv.abs())[:, 0] / l
+            t = ((p * d)[:, None] @ vv.abs())[:, 0] / l + out[b, r].abs() * (p * d).sum(1, keepdim=True) / l
+            t += size * (plane + (L // 16 + 1) * 2.0 ** -23 + 2.0 ** -22)
+            t += L * 2.0 ** -29 * 127 * (p * sv).amax(1, keepdim=True) / l
+            tol[b, r] = t + out[b, r].abs() * HALF[q.dtype]
+    return out, tol
+
+
+def weighed_check(ops, q, c, starts, rows=None):
+    st = torch.tensor(starts, dtype=torch.int32, device="cuda")
+    got = ops.kv8_attention(q, ops.Kv8Cache(*c), st)
+    rows = q.shape[1] if rows is None else rows
+    want, tol = weighed_ref(q[:, :rows], c, starts, 1 / math.sqrt(q.shape[3]))
+    err = (got[:, :rows].double() - want).abs()
+    assert (err <= tol).all(), (err / tol.clamp_min(1e-300)).max()
+
+
+PROMPT, STEP, DIGITS = [(70, 2), (40, 4)], [(6, 2), (1, 16), (20, 3)], [(1, 1), (1, 2), (2, 2), (1, 4)]
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("times", [1e3, 1e5, 1e8, 1e30])
+@pytest.mark.parametrize("hd,start,cap", [(64, 100, 256), (128, 100, 256), (128, 3000, 4096), (64, 3000, 4096)])
+def test_a_large_block_that_a_row_does_not_see_leaves_it_alone(ops, dt, times, hd, start, cap):
+    """Rows before the block, in the same tile as rows that see it (with and without keys shared by a cluster)."""
+    rows, group = 70, 2
+    c = filled_cache(ops, 1, 1, cap, hd, [start + rows], seed=71)
+    q = rand(1, rows, group, hd, seed=72).to(dt)
+    big = (start + 40) // 16
+    c[3][0, 0, big] *= times
+    weighed_check(ops, q, c, [start], big * 16 - start)
+    weighed_check(ops, q, c, [start])
+
+
+def weightless_cache(ops, rows, group, hd, L, cap, at, times, seed):
+    """A cache of L tokens whose block `at` has V scales `times` as large, and keys with some e^-30 of the weight."""
+    c = filled_cache(ops, 1, 1, cap, hd, [L], seed=seed, kstd=0.3)
+    q = rand(1, rows, group, hd, seed=seed + 3, std=0.3) + 1
+    k = torch.full((1, 16, 1, hd), -30 / math.sqrt(hd), device="cuda")
+    end = min(16, L - at * 16)
+    z = torch.full((1,), at * 16, dtype=torch.int32, device="cuda")
+    v = rand(1, 16, 1, hd, seed=seed + 4, std=0.5)
+    ops.kv8_append(ops.Kv8Cache(*c), k[:, :end], v[:, :end], z)
+    c[3][0, 0, at] *= times
+    return c, q
+
+
+def weightless(ops, dt, times, rows, group, hd, long):
+    L = (3000 if long else 437) + rows
+    cap = 4096 if long else 512
+    for i, at in enumerate((0, 1, L // 32, (L - rows) // 16 - 1)):
+        c, q = weightless_cache(ops, rows, group, hd, L, cap, at, times, 80 + i)
+        weighed_check(ops, q.to(dt), c, [L - rows])
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("times", [1e2, 1e3, 1e5, 1e8])
+@pytest.mark.parametrize("hd,long", [(64, False), (128, False), (128, True)])
+@pytest.mark.parametrize("rows,group", PROMPT)
+def test_a_large_block_without_weight_prompts(ops, dt, times, hd, long, rows, group):
+    weightless(ops, dt, times, rows, group, hd, long)
+
+
+def tails(ops, dt, rows, group, hd, bits):
+    """One key holds nearly all of the weight and has no value; the others, 2^-bits each, are the output."""
+    L, cap = 3500 + rows, 4096
+    c = filled_cache(ops, 1, 1, cap, hd, [L], seed=91, kstd=0.02)
+    q = rand(1, rows, group, hd, seed=92, std=0.1) + 1
+    z = torch.full((1,), 1700, dtype=torch.int32, device="cuda")
+    k = torch.full((1, 1, 1, hd), bits * math.log(2) / math.sqrt(hd), device="cuda")
+    ops.kv8_append(ops.Kv8Cache(*c), k, torch.zeros_like(k), z)
+    c[1].abs_()  # (values of one sign, whose loss adds up)
+    weighed_check(ops, q.to(dt), c, [L - rows])
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("bits", [20, 24, 25, 27])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("rows,group", PROMPT)
+def test_many_keys_of_little_weight_prompts(ops, dt, bits, hd, rows, group):
+    tails(ops, dt, rows, group, hd, bits)
