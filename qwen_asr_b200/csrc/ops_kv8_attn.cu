@@ -19,10 +19,12 @@
 //
 // Digit kernel (up to four query rows a KV head, so most single tokens): the products stay in
 // integers. A query row is held as three signed 7-bit digits of q / max|q| (2^-22 of the largest),
-// the probabilities as the three bytes of a 23-bit fraction (2^-24 of the largest, by V scale);
+// the weights (probability x V scale) as the four bytes of a 32-bit fraction of about the largest weight so far
+// (2^-30 of it at most; not of the largest V scale, which may have no weight at all: a block 1000 times as large
+// cost a row 4e-4 of its output so, and thousands of keys of 2^-25 each were lost with the three bytes of 23 bits);
 // each digit is a column of its own in m16n8k32 products whose other operand is the cache's bytes:
 // K as it is, V with its 4 x 4 bytes transposed in registers. Two query rows fill eight columns
-// (three digits and one that is not looked at), and sums are exact, so 32 tokens take 16 products
+// (q's fourth is not looked at), and sums are exact, so 32 tokens take 16 products
 // and no conversion, against 64 and 350 conversions in f16.
 // Step kernel (few query rows, more than four): the f16 tiles above.
 // In both, one cluster per (KV head, row tile, sequence); its CTAs split the sequence's actual
@@ -598,7 +600,7 @@ __global__ void __launch_bounds__(kDigWarps * 32, RH == 1 ? 3 : 2) digit_kernel(
 
   const int plane = g & 3, hrow = t >> 1;
   uint32_t q[RH][kSteps][2];
-  float fac[RH], m[RH], l[RH], vref[RH], rv[RH];
+  float fac[RH], m[RH], l[RH], top[RH], vref[RH], rv[RH];
   int last[RH];
   int all_see = 0x7FFFFFFF;  // every row of the warp sees up to here
 #pragma unroll
@@ -642,19 +644,19 @@ __global__ void __launch_bounds__(kDigWarps * 32, RH == 1 ? 3 : 2) digit_kernel(
     last[h] = sr < count ? min(start + sr, a.c.capacity - 1) : -1;
     all_see = min(all_see, last[h]);
     m[h] = kNone;
-    l[h] = vref[h] = rv[h] = 0.f;
+    l[h] = top[h] = vref[h] = rv[h] = 0.f;
   }
   all_see = __reduce_min_sync(0xffffffffu, all_see);
   // weights of this lane's two result columns, for the scores and for the output
   const float wa = t & 1 ? 1.f : 16384.f, wb = t & 1 ? 0.f : 128.f, ba = -kMagic * wa, bb = -kMagic * wb;
-  const float oa = t & 1 ? 1.f : 65536.f, ob = t & 1 ? 0.f : 256.f;
-  // the probabilities' bytes this lane hands out first: digit 0 (t even) or 1; digit 2 is the second
-  const uint32_t sel = t & 1 ? 0x0051u : 0x0062u;
-  const int from = 8 * t + 2 * (g >> 2) + (plane == 1 ? 1 : 0);  // tokens 2t: lane (2t, 2 row + digit)
+  const float oa = t & 1 ? 0x1p-24f : 0x1p-8f, ob = t & 1 ? 0x1p-32f : 0x1p-16f;
+  // the weights' bytes this lane hands out: digits 0 and 2 (t even), or 1 and 3
+  const uint32_t sel = t & 1 ? 0x0062u : 0x0073u, sel2 = t & 1 ? 0x0040u : 0x0051u;
+  const int from = 8 * t + 2 * (g >> 2) + (plane & 1);  // tokens 2t: lane (2t, 2 row + digit's parity)
 
-  // The output so far is sum * vref / (2^23 - 1) + acc: integer sums for the present maximum m and
-  // V scale vref (a power of two), f32 for what came before they last grew. So a step of 32 tokens
-  // neither converts nor rescales anything, unless its maximum or a V scale is a new record.
+  // The output so far is sum * vref / 2^32 + acc: integer sums for the present maximum m and the
+  // power of two vref above the largest weight (about `top`), f32 for what came before they last grew. So a
+  // step of 32 tokens neither converts nor rescales anything, unless its maximum or a weight is a new record.
   int sum[RH][kMt][4];
   float acc[RH][kMt][2];
 #pragma unroll
@@ -707,8 +709,11 @@ __global__ void __launch_bounds__(kDigWarps * 32, RH == 1 ? 3 : 2) digit_kernel(
     }
     // ---- softmax state
     const bool partial = pos0 + 2 * kTok - 1 > all_see;
-    float f0[RH], f1[RH], v0[RH], v1[RH], mx[RH];
+    float f0[RH], f1[RH], v0[RH], v1[RH], mx[RH], most[RH];
     bool grew = ++since > 2048;
+    // the step's largest weight, within 4 times: its largest probability times its larger V scale, unless these are
+    // further apart
+    const bool apart = !(fmaxf(sc.z, sc.w) <= 4.f * fminf(sc.z, sc.w));
 #pragma unroll
     for (int h = 0; h < RH; ++h) {
       // a block that the row sees nothing of gives it nothing of its scales either (they may be NaN)
@@ -717,41 +722,56 @@ __global__ void __launch_bounds__(kDigWarps * 32, RH == 1 ? 3 : 2) digit_kernel(
       f1[h] = see1 ? fac[h] * sc.y : 0.f;
       v0[h] = see0 ? sc.z : 0.f;
       v1[h] = see1 ? sc.w : 0.f;
-      mx[h] = kNone;
+      float t0 = kNone, t1 = kNone;
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (!partial || pos0 + (e >> 1) * 16 + (e & 1) * 8 + g <= last[h])
-          mx[h] = fmaxf(mx[h], x[h][e] * (e < 2 ? f0[h] : f1[h]));
+        if (!partial || pos0 + (e >> 1) * 16 + (e & 1) * 8 + g <= last[h]) {
+          if (e < 2) t0 = fmaxf(t0, x[h][e] * f0[h]);
+          else t1 = fmaxf(t1, x[h][e] * f1[h]);
+        }
+      mx[h] = fmaxf(t0, t1);
 #pragma unroll
       for (int o = 4; o < 32; o *= 2) mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], o));
-      grew |= mx[h] > m[h] || !(v0[h] <= vref[h]) || !(v1[h] <= vref[h]);
+      const float mn = fmaxf(m[h], mx[h]);
+      // (2^-80 at least, so that rv times a V scale stays finite)
+      if (apart) {
+#pragma unroll
+        for (int o = 4; o < 32; o *= 2) {
+          t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, o));
+          t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, o));
+        }
+        most[h] = max_nan(ex2(fmaxf(t0 - mn, -80.f)) * v0[h], ex2(fmaxf(t1 - mn, -80.f)) * v1[h]);
+      } else {
+        most[h] = ex2(fmaxf(mx[h] - mn, -80.f)) * max_nan(v0[h], v1[h]);
+      }
+      grew |= mx[h] > m[h] || !(most[h] <= vref[h]);
     }
     if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
       for (int h = 0; h < RH; ++h) {
-        const float mn = fmaxf(m[h], mx[h]), corr = ex2(m[h] - mn), to = vref[h] * (1.f / 8388607.f);
+        const float mn = fmaxf(m[h], mx[h]), corr = ex2(m[h] - mn);
 #pragma unroll
         for (int j = 0; j < kMt; ++j)
 #pragma unroll
           for (int o = 0; o < 2; ++o) {
             const float y = fmaf((float)sum[h][j][2 * o], oa, (float)sum[h][j][2 * o + 1] * ob);
-            acc[h][j][o] = fmaf(y, to, acc[h][j][o]) * corr;
+            acc[h][j][o] = fmaf(y, vref[h], acc[h][j][o]) * corr;
             sum[h][j][2 * o] = sum[h][j][2 * o + 1] = 0;
           }
         l[h] *= corr;
         m[h] = mn;
-        const float vm = max_nan(v0[h], v1[h]);
-        if (!(vm <= vref[h]))  // to the power of two above it (2^-100 at least), or NaN
-          vref[h] = vm > 0.f ? fmaxf(__uint_as_float((__float_as_uint(vm) + 0x7FFFFFu) & 0xFF800000u), 7.888609e-31f) : vm;
-        rv[h] = vref[h] > 0.f ? __fdiv_rn(8388607.f, vref[h]) : 0.f;
+        // the weights so far count less where the maximum grew; the power of two above them (2^-120 at least), or NaN
+        const float w = top[h] = max_nan(top[h] * corr, most[h]);
+        vref[h] = w > 0.f ? fmaxf(__uint_as_float((__float_as_uint(w) + 0x7FFFFFu) & 0xFF800000u), 0x1p-120f) : w;
+        rv[h] = vref[h] > 0.f ? __fdiv_rn(1.f, vref[h]) : 0.f;
       }
       since = 0;
     }
-    // ---- probabilities as bytes: column (row g / 4, digit g % 4) of tokens 2t, 2t + 1, 2t + 8, 2t + 9 a tile
+    // ---- weights as bytes: column (row g / 4, digit g % 4) of tokens 2t, 2t + 1, 2t + 8, 2t + 9 a tile
     uint32_t pb[RH][2];
 #pragma unroll
     for (int h = 0; h < RH; ++h) {
-      const float r0 = v0[h] * rv[h], r1 = v1[h] * rv[h];
+      const float r0 = v0[h] * rv[h] * 0x1p32f, r1 = v1[h] * rv[h] * 0x1p32f;
       uint32_t z[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -759,10 +779,10 @@ __global__ void __launch_bounds__(kDigWarps * 32, RH == 1 ? 3 : 2) digit_kernel(
         // (not by the score: a masked one times a zero scale is no number)
         if (partial && pos0 + (e >> 1) * 16 + (e & 1) * 8 + g > last[h]) p = 0.f;
         l[h] += p;
-        z[e] = __float_as_uint(fmaf(p, e < 2 ? r0 : r1, 8388608.f));
+        z[e] = __float2uint_rn(p * (e < 2 ? r0 : r1));  // (saturates: 1 becomes 1 - 2^-32)
       }
       const uint32_t first = __byte_perm(__byte_perm(z[0], z[1], sel), __byte_perm(z[2], z[3], sel), 0x5410);
-      const uint32_t second = __byte_perm(__byte_perm(z[0], z[1], 0x0040), __byte_perm(z[2], z[3], 0x0040), 0x5410);
+      const uint32_t second = __byte_perm(__byte_perm(z[0], z[1], sel2), __byte_perm(z[2], z[3], sel2), 0x5410);
       const uint32_t a0 = __shfl_sync(0xffffffffu, first, from), a1 = __shfl_sync(0xffffffffu, first, from + 4);
       const uint32_t c0 = __shfl_sync(0xffffffffu, second, from), c1 = __shfl_sync(0xffffffffu, second, from + 4);
       const uint32_t w0 = plane >= 2 ? c0 : a0, w1 = plane >= 2 ? c1 : a1;
@@ -823,14 +843,13 @@ __global__ void __launch_bounds__(kDigWarps * 32, RH == 1 ? 3 : 2) digit_kernel(
       wm[warp][r] = m[h];
       wl[warp][r] = l[h];
     }
-    const float to = vref[h] * (1.f / 8388607.f);
 #pragma unroll
     for (int j = 0; j < kMt; ++j) {
       float y[2];
 #pragma unroll
       for (int o = 0; o < 2; ++o) {
         y[o] = fmaf((float)sum[h][j][2 * o], oa, (float)sum[h][j][2 * o + 1] * ob);
-        y[o] = fmaf(y[o], to, acc[h][j][o]);
+        y[o] = fmaf(y[o], vref[h], acc[h][j][o]);
         y[o] += __shfl_xor_sync(0xffffffffu, y[o], 1);
       }
       wo[(warp * R + r) * HD + g * kNt + 2 * j + (t & 1)] = t & 1 ? y[1] : y[0];

@@ -159,3 +159,36 @@ def tails(ops, dt, rows, group, hd, bits):
 @pytest.mark.parametrize("rows,group", PROMPT)
 def test_many_keys_of_little_weight_prompts(ops, dt, bits, hd, rows, group):
     tails(ops, dt, rows, group, hd, bits)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("times", [1e2, 1e3, 1e5, 1e8])
+@pytest.mark.parametrize("hd,long", [(64, False), (128, False), (128, True)])
+@pytest.mark.parametrize("rows,group", DIGITS)
+def test_a_large_block_without_weight_tokens(ops, dt, times, hd, long, rows, group):
+    weightless(ops, dt, times, rows, group, hd, long)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("bits", [20, 24, 25, 27])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("rows,group", DIGITS)
+def test_many_keys_of_little_weight_tokens(ops, dt, bits, hd, rows, group):
+    tails(ops, dt, rows, group, hd, bits)
+
+
+def test_tokens_over_scales_of_every_size(ops):
+    """V scales from the smallest normal numbers to the largest, in any order, alone and side by side; a NaN among
+    them reaches the rows that see it."""
+    hd, cap = 128, 512
+    q = rand(1, 1, 2, hd, seed=95)
+    for seed in range(4):
+        c = filled_cache(ops, 1, 1, cap, hd, [cap], seed=96)
+        g = torch.Generator().manual_seed(seed)
+        c[3][0, 0] = torch.exp2(torch.randint(-120, 110, (cap // 16,), generator=g).float()).cuda()
+        for L in (1, 16, 17, 300, 512):
+            weighed_check(ops, q, c, [L - 1])
+        c[3][0, 0, 20] = math.nan
+        st = torch.tensor([500], dtype=torch.int32, device="cuda")
+        assert torch.isnan(ops.kv8_attention(q, ops.Kv8Cache(*c), st)).all()
+        assert not torch.isnan(ops.kv8_attention(q, ops.Kv8Cache(*c), st - 181)).any()
