@@ -7,10 +7,12 @@
 // scale the tile's product. A query row is first scaled by a power of two that puts its largest
 // value into [1/2, 1).
 //   f32 rows: q and the probabilities enter as two f16 planes, v = hi + lo, which holds them to
-//     2^-25 of the row's largest (below f32's own rounding of it). The two planes are rows r and
-//     r + 8 of the same 16-row operand: a tile holds 8 query rows and both planes cost one product.
+//     2^-22 of themselves (q: or 2^-25 of the row's largest, below f32's own rounding of it). The two planes are
+//     rows r and r + 8 of the same 16-row operand: a tile holds 8 query rows and both planes cost one product.
 //   bf16 rows: one plane (a bf16 value is exact in f16 down to 2^-14 of the row's largest, and
 //     the probabilities' 2^-11 is an eighth of the output's own 2^-8), 16 rows a tile.
+//   The probabilities of a tile are relative to the largest of the tile, 2^15 (f16 has no step below 2^-24, and
+//     thousands of keys of 2^-25 each add up): what it is of the row's is in the tile's V scale.
 // Scores, the running maximum and sum and the output stay in f32 registers.
 //
 // Fragments straight from the cache's layout: the order of the head's dimensions within the score
@@ -204,9 +206,7 @@ struct WarpState {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const float ks = *reinterpret_cast<const float*>(st + 2 * kTok * HD);
     const float vs = *reinterpret_cast<const float*>(st + 2 * kTok * HD + 4);
-    float vr[kR];  // a row that sees nothing of the tile takes nothing of its scale either (it may be NaN)
-#pragma unroll
-    for (int h = 0; h < kR; ++h) vr[h] = pos0 <= last[h] ? vs : 0.f;
+    float vr[kR];
     float s[2][4];
 #pragma unroll
     for (int nt = 0; nt < 2; ++nt) {
@@ -245,13 +245,16 @@ struct WarpState {
       corr[h] = ex2(m[h] - mn);
       grew |= mn > m[h];
       m[h] = mn;
+      const float part = ex2(mx - mn);  // the tile's largest
+      // a row that sees nothing of the tile takes nothing of its scale either (it may be NaN)
+      vr[h] = pos0 <= last[h] ? vs * part : 0.f;
       float sum = 0.f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        x[i] = ex2(x[i] - mn);
+        x[i] = ex2(x[i] - mx + 15.f);
         sum += x[i];
       }
-      l[h] = l[h] * corr[h] + sum;
+      l[h] = fmaf(sum, part, l[h] * corr[h]);
       p[h] = pack_f16(x[0], x[1]);
       p[2 + h] = pack_f16(x[2], x[3]);
       if (PL == 2) {

@@ -744,15 +744,17 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_bf16_kernel(const PromptAr
           tmem_st_wait();
         }
       }
+      f32x2 sum = 0;  // (a block's own: one by one, small probabilities would not move a large l)
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
         uint32_t hi[8];
         if (partial)
-          weigh<1, true>(x + 16 * b, f[b], m, w[b], last + 1 - pos0 - 16 * b, l, hi, nullptr);
+          weigh<1, true>(x + 16 * b, f[b], m, w[b], last + 1 - pos0 - 16 * b, sum, hi, nullptr);
         else
-          weigh<1, false>(x + 16 * b, f[b], m, w[b], 16, l, hi, nullptr);
+          weigh<1, false>(x + 16 * b, f[b], m, w[b], 16, sum, hi, nullptr);
         tmem_st8(trow + kColP + 8 * b, hi);
       }
+      l = add2(l, sum);
       tmem_st_wait();
       before_sync();
       mbar_arrive(p_full);
@@ -1011,16 +1013,18 @@ __global__ void __launch_bounds__(kThreads2, 1) prompt_f32_kernel(const PromptAr
       for (int b = 0; b < 2; ++b) w[b] = min_nan(w[b] * power(kTop2 - r), 1e37f);
       // (P of block j - 2 has been read: its O was added in the last round)
       const uint32_t pcol = trow + kP2 + (uint32_t)((j & 1) * 64 + half * 16);
+      f32x2 sum = 0;  // (a block's own: one by one, small probabilities would not move a large l)
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
         uint32_t hi[8], lo[8];
         if (partial)
-          weigh<2, true>(x + 16 * b, f[b], m, w[b], last + 1 - pos0 - 16 * b, l, hi, lo);
+          weigh<2, true>(x + 16 * b, f[b], m, w[b], last + 1 - pos0 - 16 * b, sum, hi, lo);
         else
-          weigh<2, false>(x + 16 * b, f[b], m, w[b], 16, l, hi, lo);
+          weigh<2, false>(x + 16 * b, f[b], m, w[b], 16, sum, hi, lo);
         tmem_st8(pcol + 8 * b, hi);
         tmem_st8(pcol + 32 + 8 * b, lo);
       }
+      l = add2(l, sum);
       tmem_st_wait();
       before_sync();
       mbar_arrive(&p_full[j & 1]);

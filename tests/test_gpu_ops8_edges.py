@@ -50,7 +50,7 @@ def test_prompt_rows_of_skipped_sequences_are_zeros(ops, dt, n, live, group, row
 
 
 # ------------------------------------------------------------------ blocks of very different V scales, long tails
-def weighed_ref(q, c, starts, scale):
+def weighed_ref(q, c, starts, scale, held=29):
     """(out, tolerance) in 64 bits, the tolerance relative to what a row weighs: with weights w = p vscale of its
     keys, W the largest of them and l the sum of p,
       the scores' error d of a key, under 2^-21 scale max|q| sum|k| (q held to 2^-22 of its largest value or better,
@@ -81,16 +81,16 @@ def weighed_ref(q, c, starts, scale):
             size = (p[:, None] @ vv.abs())[:, 0] / l
             t = ((p * d)[:, None] @ vv.abs())[:, 0] / l + out[b, r].abs() * (p * d).sum(1, keepdim=True) / l
             t += size * (plane + (L // 16 + 1) * 2.0 ** -23 + 2.0 ** -22)
-            t += L * 2.0 ** -29 * 127 * (p * sv).amax(1, keepdim=True) / l
+            t += L * 2.0 ** -held * 127 * (p * sv).amax(1, keepdim=True) / l
             tol[b, r] = t + out[b, r].abs() * HALF[q.dtype]
     return out, tol
 
 
-def weighed_check(ops, q, c, starts, rows=None):
+def weighed_check(ops, q, c, starts, rows=None, held=29, max_len=0):
     st = torch.tensor(starts, dtype=torch.int32, device="cuda")
-    got = ops.kv8_attention(q, ops.Kv8Cache(*c), st)
+    got = ops.kv8_attention(q, ops.Kv8Cache(*c), st, max_len=max_len)
     rows = q.shape[1] if rows is None else rows
-    want, tol = weighed_ref(q[:, :rows], c, starts, 1 / math.sqrt(q.shape[3]))
+    want, tol = weighed_ref(q[:, :rows], c, starts, 1 / math.sqrt(q.shape[3]), held)
     err = (got[:, :rows].double() - want).abs()
     assert (err <= tol).all(), (err / tol.clamp_min(1e-300)).max()
 
@@ -141,16 +141,20 @@ def test_a_large_block_without_weight_prompts(ops, dt, times, hd, long, rows, gr
     weightless(ops, dt, times, rows, group, hd, long)
 
 
-def tails(ops, dt, rows, group, hd, bits):
-    """One key holds nearly all of the weight and has no value; the others, 2^-bits each, are the output."""
+def tails(ops, dt, rows, group, hd, bits, held):
+    """The first key holds nearly all of the weight and has no value; the others, 2^-bits each, are the output. The
+    V scales are alike here, so a weight is off by no more than 2^-held of the largest. (Unsplit: a warp that does not
+    meet the first key holds its weights by its own.)"""
     L, cap = 3500 + rows, 4096
     c = filled_cache(ops, 1, 1, cap, hd, [L], seed=91, kstd=0.02)
     q = rand(1, rows, group, hd, seed=92, std=0.1) + 1
-    z = torch.full((1,), 1700, dtype=torch.int32, device="cuda")
+    z = torch.zeros(1, dtype=torch.int32, device="cuda")
     k = torch.full((1, 1, 1, hd), bits * math.log(2) / math.sqrt(hd), device="cuda")
     ops.kv8_append(ops.Kv8Cache(*c), k, torch.zeros_like(k), z)
     c[1].abs_()  # (values of one sign, whose loss adds up)
-    weighed_check(ops, q.to(dt), c, [L - rows])
+    for first in (0.0, c[3][0, 0, 1].item()):
+        c[3][0, 0, 0] = first
+        weighed_check(ops, q.to(dt), c, [L - rows], held=held, max_len=16)
 
 
 @pytest.mark.parametrize("dt", [F32, BF16])
@@ -158,7 +162,7 @@ def tails(ops, dt, rows, group, hd, bits):
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("rows,group", PROMPT)
 def test_many_keys_of_little_weight_prompts(ops, dt, bits, hd, rows, group):
-    tails(ops, dt, rows, group, hd, bits)
+    tails(ops, dt, rows, group, hd, bits, 36 if dt == F32 else 30)
 
 
 @pytest.mark.parametrize("dt", [F32, BF16])
@@ -174,7 +178,7 @@ def test_a_large_block_without_weight_tokens(ops, dt, times, hd, long, rows, gro
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("rows,group", DIGITS)
 def test_many_keys_of_little_weight_tokens(ops, dt, bits, hd, rows, group):
-    tails(ops, dt, rows, group, hd, bits)
+    tails(ops, dt, rows, group, hd, bits, 32)
 
 
 def test_tokens_over_scales_of_every_size(ops):
@@ -192,3 +196,19 @@ def test_tokens_over_scales_of_every_size(ops):
         st = torch.tensor([500], dtype=torch.int32, device="cuda")
         assert torch.isnan(ops.kv8_attention(q, ops.Kv8Cache(*c), st)).all()
         assert not torch.isnan(ops.kv8_attention(q, ops.Kv8Cache(*c), st - 181)).any()
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("times", [1e2, 1e3, 1e5, 1e8])
+@pytest.mark.parametrize("hd,long", [(64, False), (128, False), (128, True)])
+@pytest.mark.parametrize("rows,group", STEP)
+def test_a_large_block_without_weight_steps(ops, dt, times, hd, long, rows, group):
+    weightless(ops, dt, times, rows, group, hd, long)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("bits", [20, 24, 25, 27])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("rows,group", STEP)
+def test_many_keys_of_little_weight_steps(ops, dt, bits, hd, rows, group):
+    tails(ops, dt, rows, group, hd, bits, 39)
