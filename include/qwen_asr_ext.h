@@ -297,7 +297,8 @@ int32_t qwen_asr_kv8_attention(const QwenAsrKv8* cache, const QwenAsrRows* q, co
                                int32_t rows, int32_t heads, const int32_t* starts, const int32_t* counts,
                                int32_t index_stride, float scale, int32_t max_len, int32_t device, void* stream);
 /* Nonzero (and cleared) when a bounded wait inside qwen_asr_linear_int8 or qwen_asr_kv8_attention
- * gave up on `device`: outputs since the last query are not to be used. Waits for the device. */
+ * gave up on `device`: outputs since the last query are not to be used. Waits for all of the device's streams.
+ * Negative, with the reason in qwen_asr_last_error(), where the device cannot be waited for or asked. */
 int32_t qwen_asr_ops_error(int32_t device);
 
 #ifdef __cplusplus

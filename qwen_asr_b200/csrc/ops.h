@@ -76,9 +76,10 @@ cudaError_t kv8_attention(const Kv8& c, const void* q, long long q_seq, long lon
 cudaError_t kv8_prompt_attention(const Kv8& c, const void* q, long long q_seq, long long q_row, void* out,
                                  long long o_seq, long long o_row, OpsDtype dt, int rows, int heads, const int* starts,
                                  const int* counts, int idx_stride, float scale, int max_len, int splits, cudaStream_t s);
-// Nonzero once a bounded wait inside kv8_prompt_attention gave up on the current device (clears it).
+// Positive once a bounded wait inside kv8_prompt_attention gave up on the current device (clears it), -1 where that
+// cannot be read.
 int kv8_prompt_error();
-// Nonzero once a bounded wait inside linear_int8 gave up on the current device (clears it).
+// The same of linear_int8.
 int linear_int8_error();
 
 // The current device's SM count (queried once a device).

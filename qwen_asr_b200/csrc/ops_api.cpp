@@ -229,10 +229,21 @@ int32_t qwen_asr_kv8_attention(const QwenAsrKv8* cache, const QwenAsrRows* q, co
 }
 
 int32_t qwen_asr_ops_error(int32_t device) {
-  DeviceScope scope(device);
-  if (!scope.ok()) return -1;
-  const int e = linear_int8_error(), p = kv8_prompt_error();
-  return e ? e : p;
+  const char* op = "ops_error";
+  try {
+    DeviceScope scope(device);
+    if (!scope.ok()) return fail(op, "cannot use device " + std::to_string(device));
+    // (reading the flags waits for the default stream alone)
+    if (const cudaError_t s = cudaDeviceSynchronize()) {
+      cudaGetLastError();
+      return fail(op, std::string("cannot wait for the device: ") + cudaGetErrorString(s));
+    }
+    const int e = linear_int8_error(), p = kv8_prompt_error();
+    if (e < 0 || p < 0) return fail(op, "cannot read the device's error flags");
+    return e ? e : p;
+  } catch (const std::exception& ex) {
+    return fail(op, ex.what());
+  }
 }
 
 }  // extern "C"

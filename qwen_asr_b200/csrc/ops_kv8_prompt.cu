@@ -1207,7 +1207,10 @@ cudaError_t kv8_prompt_attention(const Kv8& c, const void* q, long long q_seq, l
 
 int kv8_prompt_error() {
   int e = 0;
-  if (cudaMemcpyFromSymbol(&e, g_prompt_err, sizeof(int)) != cudaSuccess) return 0;
+  if (cudaMemcpyFromSymbol(&e, g_prompt_err, sizeof(int)) != cudaSuccess) {
+    cudaGetLastError();
+    return -1;
+  }
   if (e) {
     const int zero = 0;
     cudaMemcpyToSymbol(g_prompt_err, &zero, sizeof(int));

@@ -594,7 +594,10 @@ cudaError_t linear_int8(const int8_t* xq, long long ldx, const float* xs, const 
 
 int linear_int8_error() {
   int e = 0;
-  if (cudaMemcpyFromSymbol(&e, g_wait_err, sizeof(int)) != cudaSuccess) return 0;
+  if (cudaMemcpyFromSymbol(&e, g_wait_err, sizeof(int)) != cudaSuccess) {
+    cudaGetLastError();
+    return -1;
+  }
   if (e) {
     const int zero = 0;
     cudaMemcpyToSymbol(g_wait_err, &zero, sizeof(int));

@@ -324,8 +324,11 @@ def kv8_attention(q, cache: Kv8Cache, starts, counts=None, scale: float | None =
 
 def check(device=None) -> None:
     """Raises RuntimeError when a bounded wait inside linear_int8 or kv8_attention gave up since the
-    last check (outputs since then are not to be used). Waits for the device."""
+    last check (outputs since then are not to be used), or when the device cannot be asked. Waits
+    for all of the device's streams."""
     index = torch.cuda.current_device() if device is None else torch.device(device).index
     e = lib().qwen_asr_ops_error(-1 if index is None else index)
+    if e < 0:
+        raise RuntimeError(f"8-bit operators: {last_error()}")
     if e:
         raise RuntimeError(f"8-bit operators: a device-side wait timed out (code {e})")

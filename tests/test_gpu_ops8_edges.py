@@ -212,3 +212,15 @@ def test_a_large_block_without_weight_steps(ops, dt, times, hd, long, rows, grou
 @pytest.mark.parametrize("rows,group", STEP)
 def test_many_keys_of_little_weight_steps(ops, dt, bits, hd, rows, group):
     tails(ops, dt, rows, group, hd, bits, 39)
+
+
+# ------------------------------------------------------------------ errors of the device
+def test_check_waits_for_every_stream(ops):
+    """A call still running on a stream that does not wait for the default one could give up after the check."""
+    ops.check()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)
+    assert not side.query()
+    ops.check()
+    assert side.query()
