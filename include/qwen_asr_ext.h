@@ -139,6 +139,9 @@ int64_t qwen_asr_gemm_fallbacks(void);
 /* KV cache (decoder.rs:185-253) of one slot and layer: k, v [kv_heads][n_pos][128] f32 for
  * positions 0..n_pos-1 (slot 0 = the offline path). Returns 0 or -1. */
 int32_t qwen_asr_debug_kv(QwenAsrEngine* engine, int32_t slot, int32_t layer, int32_t n_pos, float* k, float* v);
+/* Reports `code` as an 8-bit kernel does whose bounded wait gives up: one of this engine's, or (engine NULL) of the
+ * operators below on the current device. Returns 0 or -1. For tests. */
+int32_t qwen_asr_debug_report_ops_error(QwenAsrEngine* engine, int32_t code);
 /* Current KV capacity in positions (KvCache::max_seq). */
 int32_t qwen_asr_debug_kv_capacity(QwenAsrEngine* engine);
 /* Grows the KV cache to hold `needed` positions by doubling, keeping the rows already

@@ -91,6 +91,7 @@ SIGNATURES = {
                                               C.POINTER(C.c_float), C.POINTER(C.c_uint64)]),
     "qwen_asr_debug_valid_utf8": (C.c_int32, [C.c_char_p]),
     "qwen_asr_debug_kv": (C.c_int32, [_VP, C.c_int32, C.c_int32, C.c_int32, _F32P, _F32P]),
+    "qwen_asr_debug_report_ops_error": (C.c_int32, [_VP, C.c_int32]),
     "qwen_asr_debug_kv_capacity": (C.c_int32, [_VP]),
     "qwen_asr_debug_grow_kv": (C.c_int32, [_VP, C.c_int32]),
     "qwen_asr_debug_quant": (C.c_int64, [_VP, C.c_int32, C.c_int32, C.POINTER(C.c_int8), _F32P, C.c_int64]),

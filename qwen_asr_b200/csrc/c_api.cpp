@@ -490,6 +490,11 @@ int32_t qwen_asr_debug_kv(QwenAsrEngine* e, int32_t slot, int32_t layer, int32_t
   return e->ctx.eng.copy_kv(slot, layer, n_pos, k, v) ? 0 : -1;
 }
 
+int32_t qwen_asr_debug_report_ops_error(QwenAsrEngine* e, int32_t code) {
+  if (e) return e->ctx.eng.report_ops_error(code) ? 0 : -1;
+  return qasr::ops_report(qasr::ops_api_errors(), code) == cudaSuccess ? 0 : -1;
+}
+
 int32_t qwen_asr_debug_kv_capacity(QwenAsrEngine* e) { return e ? e->ctx.eng.kv_capacity() : -1; }
 
 int32_t qwen_asr_debug_grow_kv(QwenAsrEngine* e, int32_t needed) {

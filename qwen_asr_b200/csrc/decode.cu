@@ -1851,7 +1851,7 @@ bool decode_step(const DecodeArgs& a, cudaStream_t s) {
       const float* k = a.qkv + (size_t)a.q_heads * kHd;
       launched(kv8_append(c, k, nqkv, nqkv, k + (size_t)a.kv_heads * kHd, nqkv, nqkv, OPS_F32, 1, pos, nullptr, kStride, s));
       launched(kv8_attention(c, a.qkv, nqkv, nqkv, a.attn, qd, qd, OPS_F32, 1, a.q_heads, pos, nullptr, kStride,
-                             1.0f / sqrtf((float)kHd), 0, s, kKv8Splits));
+                             1.0f / sqrtf((float)kHd), 0, a.ops_err, s, kKv8Splits));
       if (a.on_launch) a.on_launch(a.hook_ctx, 1);
       check("kv8_attention", l);
     } else {

@@ -288,12 +288,13 @@ bool Engine::load(const std::string& dir, int device, bool trunc_quant) {
   if (!dx_.alloc((size_t)kMaxSlots * h) || !dqkv_.alloc((size_t)mb * (qd + 2 * kvd)) || !dattn_.alloc((size_t)mb * qd) ||
       !dffn_.alloc((size_t)mb * inter) || !dpart_.alloc((size_t)c.dec_heads * 16 * 130) ||
       !dticket_.alloc(c.dec_kv_heads) || !dam_ticket_.alloc(1) || !dam_part_.alloc((size_t)mb * 1024) ||
-      !dstate_.alloc(kMaxSlots) || !dlogits_.alloc(c.vocab_size) || !derr_.alloc(1) ||
+      !dstate_.alloc(kMaxSlots) || !dlogits_.alloc(c.vocab_size) || !derr_.alloc(1) || !ops_err_.alloc(1) ||
       !dstaged_.alloc(decode_staged_bytes(h, qd, inter)))
     return false;
   CUDA_OK(cudaMemset(dticket_.p, 0, c.dec_kv_heads * sizeof(int)), false);
   CUDA_OK(cudaMemset(dam_ticket_.p, 0, sizeof(int)), false);
   CUDA_OK(cudaMemset(derr_.p, 0, sizeof(int)), false);
+  CUDA_OK(cudaMemset(ops_err_.p, 0, sizeof(OpsErrors)), false);
   for (auto& L : dec_layers_) {
     pn1_.push_back(L.n1);
     pn2_.push_back(L.n2);
@@ -678,12 +679,10 @@ bool Engine::gemm_stage_ok(long fallbacks_before) {
     set_error("tensor-core attention: a device-side wait timed out (code " + std::to_string(e) + ")");
     return false;
   }
-  if (int e = prefill_mode_ == PREFILL_INT8 ? linear_int8_error() : 0) {
-    set_error("int8 product: a device-side wait timed out (code " + std::to_string(e) + ")");
-    return false;
-  }
-  if (int e = kv_mode_ == KV_INT8 ? kv8_prompt_error() : 0) {
-    set_error("int8 KV attention: a device-side wait timed out (code " + std::to_string(e) + ")");
+  const bool ops = prefill_mode_ == PREFILL_INT8 || kv_mode_ == KV_INT8;
+  if (int e = ops ? ops_errors(ops_err_.p, ops_seen_) : 0) {
+    set_error(e < 0 ? std::string("8-bit operators: cannot read the error word")
+                    : "int8 product or KV attention: a device-side wait timed out (code " + std::to_string(e) + ")");
     return false;
   }
   if (int e = gemm_tc_error()) {
@@ -740,7 +739,7 @@ bool Engine::prefill_layers(float* x, int R, const std::vector<RowBlock>& blocks
                             stream_),
               false);
       CUDA_OK(linear_int8(q8_.p, h, q8s_.p, L.qqkv, h, L.sqkv, R, ldq, h, LINEAR_STORE, nullptr, 0, pqkv_.p, ldq,
-                          OPS_F32, stream_),
+                          OPS_F32, ops_err_.p, stream_),
               false);
     } else {
     rms_norm_rows(x, pxn_.p, R, h, L.n1, c.dec_rms_norm_eps, stream_, pl_a_.p, plH);
@@ -766,7 +765,7 @@ bool Engine::prefill_layers(float* x, int R, const std::vector<RowBlock>& blocks
         CUDA_OK(kv8_append(cache, q + qd, 0, ldq, q + qd + kvd, 0, ldq, OPS_F32, bk.S, start, nullptr, 1, stream_),
                 false);
         CUDA_OK(kv8_attention(cache, q, 0, ldq, patt_.p + (size_t)bk.off * qd, 0, qd, OPS_F32, bk.S, c.dec_heads,
-                              start, nullptr, 1, scale, 0, stream_, kKv8Splits),
+                              start, nullptr, 1, scale, 0, ops_err_.p, stream_, kKv8Splits),
                 false);
         launches += 2;
       }
@@ -802,16 +801,16 @@ bool Engine::prefill_layers(float* x, int R, const std::vector<RowBlock>& blocks
       // attention rows -> int8 -> o projection; its sum with x is the next norm's; gate/up; down
       CUDA_OK(quant_rows_int8(patt_.p, qd, R, qd, q8_.p, qd, q8s_.p, stream_), false);
       CUDA_OK(linear_int8(q8_.p, qd, q8s_.p, L.qo, qd, L.so, R, h, qd, LINEAR_STORE, nullptr, 0, pxn_.p, h, OPS_F32,
-                          stream_),
+                          ops_err_.p, stream_),
               false);
       CUDA_OK(rms_norm_int8(x, h, pxn_.p, h, L.n2, c.dec_rms_norm_eps, OPS_F32, R, h, q8_.p, h, q8s_.p, x, h, stream_),
               false);
       CUDA_OK(linear_int8(q8_.p, h, q8s_.p, L.qgu, h, L.sgu, R, 2 * inter, h, LINEAR_SWIGLU, nullptr, 0, pmid_.p,
-                          inter, OPS_F32, stream_),
+                          inter, OPS_F32, ops_err_.p, stream_),
               false);
       CUDA_OK(quant_rows_int8(pmid_.p, inter, R, inter, q8_.p, inter, q8s_.p, stream_), false);
       CUDA_OK(linear_int8(q8_.p, inter, q8s_.p, L.qdown, inter, L.sdown, R, h, inter, LINEAR_RESID, x, h, x, h,
-                          OPS_F32, stream_),
+                          OPS_F32, ops_err_.p, stream_),
               false);
       launches += 8;
       continue;
@@ -1040,6 +1039,12 @@ bool Engine::compact_silence(const float* h_in, long n, std::vector<float>& out)
   return true;
 }
 
+bool Engine::report_ops_error(int code) {
+  cudaSetDevice(device_);
+  CUDA_OK(ops_report(ops_err_.p, code), false);
+  return true;
+}
+
 bool Engine::copy_kv(int slot, int layer, int n_pos, float* k, float* v) {
   cudaSetDevice(device_);
   const Config& c = cfg_;
@@ -1141,6 +1146,7 @@ DecodeArgs Engine::dargs(const int* forced, float* logits, int slot) {
   if (kv_mode_ == KV_INT8) {
     a.kv8 = kv8_at(slot, 0, 1);
     a.kv8_layer_stride = (size_t)c.dec_kv_heads * max_seq_ * 128;
+    a.ops_err = ops_err_.p;
   }
   a.x = dx_.p; a.qkv = dqkv_.p; a.attn = dattn_.p; a.ffn = dffn_.p; a.part = dpart_.p; a.ticket = dticket_.p;
   a.am_ticket = dam_ticket_.p; a.am_part = dam_part_.p; a.st = dstate_.p; a.tokens = dtokens_.p;

@@ -148,6 +148,7 @@ class Engine {
   // the kept samples, equal to the reference's compact_silence.
   bool compact_silence(const float* h_in, long n, std::vector<float>& out);
   // Debug: K and V rows [kv_heads][n_pos][128] of positions 0..n_pos-1 of one slot and layer.
+  bool report_ops_error(int code);  // as if one of this engine's 8-bit kernels had given up waiting (for tests)
   bool copy_kv(int slot, int layer, int n_pos, float* k, float* v);
   int kv_capacity() const { return max_seq_; }
   // Debug: grow the KV cache to hold `needed` positions (the doubling path of KvCache::grow).
@@ -199,6 +200,8 @@ class Engine {
   DevBuf<int> ids_;
   DevBuf<int8_t> q8_;           // int8 prefill: rows of the next product, and their scales
   DevBuf<float> q8s_;
+  DevBuf<OpsErrors> ops_err_;  // this engine's own
+  int ops_seen_ = 0;
   DevBuf<float> mel_keep_, cls_x_, cls_xn_, cls_logits_;
   DevBuf<int> cls_ids_, cls_out_;
   // KV cache [slot][layers][kv][max_seq][128] f32

@@ -252,6 +252,7 @@ struct DecodeArgs {
   // layer 0; a layer is layer_stride further, its scales layer_stride / (16 * 128).
   Kv8 kv8{};
   size_t kv8_layer_stride = 0;
+  OpsErrors* ops_err = nullptr;
   // Batched steps: device buffer of decode_staged_bytes() where each matvec's inputs are
   // staged once (stage_kernel) instead of by every CTA; null stages in every CTA.
   void* staged = nullptr;

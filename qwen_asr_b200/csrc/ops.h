@@ -11,6 +11,22 @@ namespace qasr {
 
 enum OpsDtype { OPS_F32 = 0, OPS_BF16 = 1 };
 
+// Where kernels report a bounded wait that gave up: how many did, and the last one's code. Each user of the operators
+// has a word of its own (an engine its buffer, the C entry points one a device) and compares the count with the one
+// it saw last, so nobody takes or clears another's error.
+struct OpsErrors {
+  int count, code;
+};
+OpsErrors* ops_api_errors();                       // the C entry points' on the current device; null: not to be had
+int ops_errors(const OpsErrors* word, int& seen);  // the code of errors since `seen`, 0: none, -1: unreadable
+cudaError_t ops_report(OpsErrors* word, int code); // as a kernel does (for tests), and waits for it
+#ifdef __CUDACC__
+__device__ __forceinline__ void ops_gave_up(OpsErrors* word, int code) {
+  atomicExch(&word->code, code);
+  atomicAdd(&word->count, 1);
+}
+#endif
+
 constexpr int kNormMaxD = 32768;  // the row is staged in shared memory as f32
 
 // rows r < rows of x (row pitch ldx elements): h = x + residual rounded to the type (h = x
@@ -33,7 +49,7 @@ enum LinearEpi { LINEAR_STORE = 0, LINEAR_RESID = 1, LINEAR_SWIGLU = 2 };
 // aligned with row pitches that are multiples of 16 bytes. out may be residual.
 cudaError_t linear_int8(const int8_t* xq, long long ldx, const float* xs, const int8_t* wq, long long ldw,
                         const float* ws, long long m, int n, int k, LinearEpi epi, const void* residual, long long ldr,
-                        void* out, long long ldo, OpsDtype dt, cudaStream_t s);
+                        void* out, long long ldo, OpsDtype dt, OpsErrors* err, cudaStream_t s);
 
 // int8 K/V of n_seq sequences: [n_seq][n_kv][capacity][head_dim] with an f32 scale for each
 // block of kKv8Block tokens of a head, [n_seq][n_kv][capacity / kKv8Block].
@@ -69,18 +85,14 @@ cudaError_t kv8_read(const Kv8& c, void* k_out, long long k_seq, long long k_row
 // at hand; a fixed number makes a sequence's result independent of the others).
 cudaError_t kv8_attention(const Kv8& c, const void* q, long long q_seq, long long q_row, void* out, long long o_seq,
                           long long o_row, OpsDtype dt, int rows, int heads, const int* starts, const int* counts,
-                          int idx_stride, float scale, int max_len, cudaStream_t s, int splits = 0);
+                          int idx_stride, float scale, int max_len, OpsErrors* err, cudaStream_t s, int splits = 0);
 
 // The same for many query rows, on tcgen05 (kv8_attention calls it for more than 64 a KV head). splits: CTAs
 // that share a row tile's keys, 1, 2 or 4 (0: by max_len and the CTAs at hand).
 cudaError_t kv8_prompt_attention(const Kv8& c, const void* q, long long q_seq, long long q_row, void* out,
                                  long long o_seq, long long o_row, OpsDtype dt, int rows, int heads, const int* starts,
-                                 const int* counts, int idx_stride, float scale, int max_len, int splits, cudaStream_t s);
-// Positive once a bounded wait inside kv8_prompt_attention gave up on the current device (clears it), -1 where that
-// cannot be read.
-int kv8_prompt_error();
-// The same of linear_int8.
-int linear_int8_error();
+                                 const int* counts, int idx_stride, float scale, int max_len, int splits,
+                                 OpsErrors* err, cudaStream_t s);
 
 // The current device's SM count (queried once a device).
 inline int ops_sm_count() {

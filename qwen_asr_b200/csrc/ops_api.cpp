@@ -3,6 +3,7 @@
 #include <cuda.h>
 
 #include <exception>
+#include <mutex>
 #include <string>
 
 #include "../../include/qwen_asr_ext.h"
@@ -160,7 +161,7 @@ int32_t qwen_asr_linear_int8(const int8_t* xq, int64_t ldx, const float* xs, con
     return fail(op, "a misaligned pointer");
   return run(op, device, [&] {
     return linear_int8(xq, ldx, xs, wq, ldw, ws, m, n, k, (LinearEpi)epilogue, residual, ldr, out, ldo,
-                       (OpsDtype)dtype, (cudaStream_t)stream);
+                       (OpsDtype)dtype, ops_api_errors(), (cudaStream_t)stream);
   });
 }
 
@@ -224,7 +225,7 @@ int32_t qwen_asr_kv8_attention(const QwenAsrKv8* cache, const QwenAsrRows* q, co
   return run(op, device, [&] {
     return kv8_attention(cache_of(cache), q->data, q->seq_stride, q->row_stride, out->data, out->seq_stride,
                          out->row_stride, (OpsDtype)dtype, rows, heads, starts, counts, index_stride, scale, max_len,
-                         (cudaStream_t)stream);
+                         ops_api_errors(), (cudaStream_t)stream);
   });
 }
 
@@ -238,9 +239,13 @@ int32_t qwen_asr_ops_error(int32_t device) {
       cudaGetLastError();
       return fail(op, std::string("cannot wait for the device: ") + cudaGetErrorString(s));
     }
-    const int e = linear_int8_error(), p = kv8_prompt_error();
-    if (e < 0 || p < 0) return fail(op, "cannot read the device's error flags");
-    return e ? e : p;
+    static std::mutex mutex;
+    static int seen[64];  // errors of each device that an earlier call returned
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return fail(op, "cannot use the current device");
+    const std::lock_guard<std::mutex> lock(mutex);
+    const int e = ops_errors(ops_api_errors(), seen[dev]);
+    return e < 0 ? fail(op, "cannot read the device's error word") : e;
   } catch (const std::exception& ex) {
     return fail(op, ex.what());
   }

@@ -962,12 +962,12 @@ cudaError_t launch(AttnArgs a, int max_len, int splits, cudaStream_t s) {
 
 cudaError_t kv8_attention(const Kv8& c, const void* q, long long q_seq, long long q_row, void* out, long long o_seq,
                           long long o_row, OpsDtype dt, int rows, int heads, const int* starts, const int* counts,
-                          int idx_stride, float scale, int max_len, cudaStream_t s, int splits) {
+                          int idx_stride, float scale, int max_len, OpsErrors* err, cudaStream_t s, int splits) {
   if (rows <= 0 || c.n_seq <= 0) return cudaSuccess;
   if ((long long)rows * (heads / c.n_kv) > kStepRows)
     return kv8_prompt_attention(c, q, q_seq, q_row, out, o_seq, o_row, dt, rows, heads, starts, counts, idx_stride,
                                 scale, max_len <= 0 || max_len > c.capacity ? c.capacity : max_len, splits > 0 ? 1 : 0,
-                                s);
+                                err, s);
   AttnArgs a{c, q, out, q_seq, q_row, o_seq, o_row, starts, counts, idx_stride, rows, heads, heads / c.n_kv, 1, scale, 0, 0};
   const int es = dt == OPS_BF16 ? 2 : 4;
   a.vec = (uintptr_t)q % 16 == 0 && q_seq * es % 16 == 0 && q_row * es % 16 == 0;

@@ -55,8 +55,6 @@ constexpr int kTop1 = 7, kTop2 = 14;  // log2 of 2^r in P: 2^(kTop1 + kLag) and 
 constexpr float kFaint = 80.f;  // probabilities under 2^-80 count as 2^-80 for r: P's factor stays finite
 constexpr uint32_t kColS = 0, kColP = 64, kColO = 128, kCols = 256;  // TMEM columns
 
-__device__ int g_prompt_err;  // nonzero once a bounded wait gave up
-
 struct PromptArgs {
   Kv8 c;
   const void* q;
@@ -67,6 +65,7 @@ struct PromptArgs {
   float scale;
   int q_vec, o_vec;  // rows start on 16-byte boundaries
   int splits;        // CTAs of a cluster that share a row tile's keys
+  OpsErrors* err;
 };
 
 template <int HD>
@@ -237,7 +236,7 @@ __device__ __forceinline__ uint32_t bytes_f16(uint32_t w) {
 }
 
 // Bounded wait. Once one gave up nobody waits any more: the warps run through what is left of their
-// loops, with the barriers between them, and leave an output that the error code disowns.
+// loops, with the barriers between them, and leave an output that the error code, reported at the end, disowns.
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile int* gave_up, int code) {
   if (mbar_try_wait(bar, parity)) return true;
   uint64_t t0 = 0;
@@ -248,8 +247,7 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile in
     const uint64_t now = global_timer_ns();
     if (t0 == 0) t0 = now;
     if (now - t0 > 2000000000ull) {
-      atomicExch(&g_prompt_err, code);
-      *gave_up = 1;
+      *gave_up = code;
       return false;
     }
   }
@@ -621,7 +619,7 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_bf16_kernel(const PromptAr
   volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;  // (uniform)
   if (smem_u32(smem) & 1023) {  // the swizzle's rows would not fit (never seen: no static shared memory)
-    if (tid == 0) atomicExch(&g_prompt_err, 40);
+    if (tid == 0) ops_gave_up(a.err, 40);
     return;
   }
   if (tid == 0) {
@@ -861,6 +859,7 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_bf16_kernel(const PromptAr
   __syncwarp();
   before_sync();
   __syncthreads();
+  if (tid == 0 && *gave_up) ops_gave_up(a.err, *gave_up);
   if (warp == 7) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols));
 }
 
@@ -890,7 +889,7 @@ __global__ void __launch_bounds__(kThreads2, 1) prompt_f32_kernel(const PromptAr
   volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;  // (uniform)
   if (smem_u32(smem) & 1023) {
-    if (tid == 0) atomicExch(&g_prompt_err, 40);
+    if (tid == 0) ops_gave_up(a.err, 40);
     return;
   }
   if (tid == 0) {
@@ -1148,6 +1147,7 @@ __global__ void __launch_bounds__(kThreads2, 1) prompt_f32_kernel(const PromptAr
   __syncwarp();
   before_sync();
   __syncthreads();
+  if (tid == 0 && *gave_up) ops_gave_up(a.err, *gave_up);
   if (warp == 15) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols2));
 }
 
@@ -1194,28 +1194,16 @@ cudaError_t launch(PromptArgs a, int max_len, cudaStream_t s) {
 cudaError_t kv8_prompt_attention(const Kv8& c, const void* q, long long q_seq, long long q_row, void* out,
                                  long long o_seq, long long o_row, OpsDtype dt, int rows, int heads, const int* starts,
                                  const int* counts, int idx_stride, float scale, int max_len,
-                                 int splits, cudaStream_t s) {
+                                 int splits, OpsErrors* err, cudaStream_t s) {
+  if (!err) return cudaErrorInvalidValue;
   auto vec = [&](const void* p, long long seq, long long row) {
     const int es = dt == OPS_BF16 ? 2 : 4;
     return (uintptr_t)p % 16 == 0 && seq * es % 16 == 0 && row * es % 16 == 0;
   };
   const PromptArgs a{c, q, out, q_seq, q_row, o_seq, o_row, starts, counts, idx_stride, rows, heads / c.n_kv, scale,
-                     vec(q, q_seq, q_row), vec(out, o_seq, o_row), splits};
+                     vec(q, q_seq, q_row), vec(out, o_seq, o_row), splits, err};
   if (c.head_dim == 128) return dt == OPS_BF16 ? launch<128, true>(a, max_len, s) : launch<128, false>(a, max_len, s);
   return dt == OPS_BF16 ? launch<64, true>(a, max_len, s) : launch<64, false>(a, max_len, s);
-}
-
-int kv8_prompt_error() {
-  int e = 0;
-  if (cudaMemcpyFromSymbol(&e, g_prompt_err, sizeof(int)) != cudaSuccess) {
-    cudaGetLastError();
-    return -1;
-  }
-  if (e) {
-    const int zero = 0;
-    cudaMemcpyToSymbol(g_prompt_err, &zero, sizeof(int));
-  }
-  return e;
 }
 
 }  // namespace qasr

@@ -41,8 +41,6 @@ constexpr int kEpiWarps = 8;
 constexpr int kThreads = 64 + 32 * kEpiWarps;
 constexpr int kMaxCluster = 8;
 
-__device__ int g_wait_err;  // nonzero once a bounded wait gave up
-
 template <int NT, bool PAIR = false>
 struct Shape {
   static constexpr int kStage = kCh * kKb + (PAIR ? NT / 2 : NT) * kKb;
@@ -65,6 +63,7 @@ struct LinArgs {
   const void* resid;
   long long ldr, ldo;
   void* out;
+  OpsErrors* err;
 };
 
 __device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr) {
@@ -142,8 +141,10 @@ __device__ __forceinline__ void commit(uint64_t* bar) {
 }
 
 // A wait of a whole warp, as one answer.
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int code) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, &g_wait_err, code));
+__device__ __forceinline__ bool warp_wait(const LinArgs& a, uint64_t* bar, uint32_t parity, int code) {
+  if (__all_sync(0xffffffffu, mbar_wait(bar, parity, nullptr, 0))) return true;
+  if ((threadIdx.x & 31) == 0) ops_gave_up(a.err, code);
+  return false;
 }
 
 #define QASR_R8(r, i) "=r"((r)[i]), "=r"((r)[i + 1]), "=r"((r)[i + 2]), "=r"((r)[i + 3]), "=r"((r)[i + 4]), \
@@ -329,7 +330,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
       const int ch0 = u % a.ct * kTileCh + (PAIR ? rank * kCh : 0), m0 = u / a.ct * a.nt + (PAIR ? rank * (a.nt / 2) : 0);
       for (int kt = k0; kt < k1; ++kt, ++it) {
         const int st = it % ST;
-        if (it >= ST && !warp_wait(&empty[st], (uint32_t)((it / ST) - 1) & 1u, 31)) {
+        if (it >= ST && !warp_wait(a, &empty[st], (uint32_t)((it / ST) - 1) & 1u, 31)) {
           *abort_flag = 1;
           break;
         }
@@ -347,7 +348,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
     // (a pair's first CTA issues for both)
     for (int u = PAIR && rank > 0 ? a.tiles : unit0; u < a.tiles && !__any_sync(0xffffffffu, *abort_flag); u += step, ++lt) {
       const int ab = lt & 1;
-      if (lt >= 2 && !warp_wait(&acc_empty[ab], (uint32_t)((lt >> 1) - 1) & 1u, 32)) {
+      if (lt >= 2 && !warp_wait(a, &acc_empty[ab], (uint32_t)((lt >> 1) - 1) & 1u, 32)) {
         *abort_flag = 1;
         break;
       }
@@ -356,7 +357,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
       bool ok = true;
       for (int kt = k0; kt < k1; ++kt, ++it) {
         const int st = it % ST;
-        if (!warp_wait(&full[st], (uint32_t)(it / ST) & 1u, 33)) {
+        if (!warp_wait(a, &full[st], (uint32_t)(it / ST) & 1u, 33)) {
           ok = false;
           break;
         }
@@ -391,8 +392,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
       uint32_t r[C];
       if constexpr (EPI == LINEAR_RESID)
         if (a.split == 1) load_resid<C, BF16>(a, m0, ch, r);
-      const bool ok = mbar_wait(&acc_full[ab], (uint32_t)(lt >> 1) & 1u, &g_wait_err, 34);
-      if (!ok) {
+      if (!warp_wait(a, &acc_full[ab], (uint32_t)(lt >> 1) & 1u, 34)) {
         *abort_flag = 1;
         break;
       }
@@ -525,9 +525,11 @@ cudaError_t launch(const LinCall& c, const LinArgs& a, int grid, cudaStream_t s)
 
 cudaError_t linear_int8(const int8_t* xq, long long ldx, const float* xs, const int8_t* wq, long long ldw,
                         const float* ws, long long m, int n, int k, LinearEpi epi, const void* residual, long long ldr,
-                        void* out, long long ldo, OpsDtype dt, cudaStream_t s) {
+                        void* out, long long ldo, OpsDtype dt, OpsErrors* err, cudaStream_t s) {
   if (m <= 0 || n <= 0) return cudaSuccess;
+  if (!err) return cudaErrorInvalidValue;
   LinArgs a{};
+  a.err = err;
   a.m = m; a.n = n; a.xs = xs; a.ws = ws; a.resid = residual; a.ldr = ldr; a.ldo = ldo; a.out = out;
   const LinCall c{xq, wq, ldx, ldw, k, epi, dt == OPS_BF16};
   a.ct = ceil_div(n, kCh);
@@ -590,19 +592,6 @@ cudaError_t linear_int8(const int8_t* xq, long long ldx, const float* xs, const 
   if (a.nt <= 64) return launch<64>(c, a, grid, s);
   if (a.nt <= 128) return launch<128>(c, a, grid, s);
   return launch<256>(c, a, grid, s);
-}
-
-int linear_int8_error() {
-  int e = 0;
-  if (cudaMemcpyFromSymbol(&e, g_wait_err, sizeof(int)) != cudaSuccess) {
-    cudaGetLastError();
-    return -1;
-  }
-  if (e) {
-    const int zero = 0;
-    cudaMemcpyToSymbol(g_wait_err, &zero, sizeof(int));
-  }
-  return e;
 }
 
 }  // namespace qasr

@@ -224,3 +224,29 @@ def test_check_waits_for_every_stream(ops):
     assert not side.query()
     ops.check()
     assert side.query()
+
+
+def test_each_user_has_its_own_errors(tiny_dir):
+    """Two engines on one GPU and the operators beside them: whoever's wait gave up hears of it, once, and no other."""
+    import qwen_asr_b200 as Q
+    from qwen_asr_b200 import ops, synth
+    x = synth.synth_audio(16000 * 3, seed=97)
+    a, b = Q.Engine(tiny_dir), Q.Engine(tiny_dir)
+    for e in (a, b):
+        e.set_prefill_mode("int8")
+        e.set_kv_mode("int8")
+        e.set_force_n_tokens(4)
+    want = a.transcribe_pcm(x)
+    assert want is not None and b.transcribe_pcm(x) == want
+    report = Q.lib().qwen_asr_debug_report_ops_error
+    ops.check()
+    assert report(a._h, 33) == 0
+    assert b.transcribe_pcm(x) == want
+    ops.check()
+    assert a.transcribe_pcm(x) is None and "33" in Q.last_error()
+    assert a.transcribe_pcm(x) == want
+    assert report(None, 51) == 0
+    assert a.transcribe_pcm(x) == want and b.transcribe_pcm(x) == want
+    with pytest.raises(RuntimeError, match="51"):
+        ops.check()
+    ops.check()
