@@ -127,7 +127,8 @@ struct OncePerDevice {
 
 // Launch, optionally in clusters of `cluster` CTAs along x, with programmatic dependence on the
 // stream's previous kernel: the CTAs may start while it ends, so every kernel launched here waits
-// (pdl_wait) before it touches global memory, and lets its own successor start early in turn.
+// (pdl_wait) before it touches global memory, and lets its own successor start early in turn. None reads by the
+// read-only path (__ldg, ld.global.nc), which is for memory that nobody writes while the kernel is there.
 template <typename K, typename... A>
 inline cudaError_t ops_launch(K kernel, dim3 grid, dim3 block, size_t smem, cudaStream_t s, int cluster,
                               const A&... args) {

@@ -452,12 +452,13 @@ __device__ __forceinline__ long long out_row(const PromptArgs& a, const Work& t,
   return t.seq * a.o_seq + (long long)s * a.o_row + (long long)(t.kvh * a.group + rr - s * a.group) * hd;
 }
 
-// 16 bytes, or zeros.
+// 16 bytes, or zeros. (Not by the read-only path, here as for the scales: what the kernel before has written must be
+// seen, although this one may have started beside it.)
 __device__ __forceinline__ uint4 ld_if(const int8_t* p, bool there) {
   uint4 v;
   asm volatile(
       "{\n .reg .pred p;\n setp.ne.b32 p, %5, 0;\n mov.b32 %0, 0;\n mov.b32 %1, 0;\n mov.b32 %2, 0;\n mov.b32 %3, 0;\n"
-      " @p ld.global.nc.v4.b32 {%0,%1,%2,%3}, [%4];\n}\n"
+      " @p ld.global.v4.b32 {%0,%1,%2,%3}, [%4];\n}\n"
       : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w)
       : "l"(p), "r"((int)there));
   return v;
@@ -666,8 +667,8 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_bf16_kernel(const PromptAr
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
         const int tl = j * 4 + b;
-        kn[b] = tl < tiles ? __ldg(t.ks + tl) : 0.f;
-        vn[b] = tl < tiles ? __ldg(t.vs + tl) : 0.f;
+        kn[b] = tl < tiles ? t.ks[tl] : 0.f;
+        vn[b] = tl < tiles ? t.vs[tl] : 0.f;
       }
     };
     scales(0);
@@ -939,8 +940,8 @@ __global__ void __launch_bounds__(kThreads2, 1) prompt_f32_kernel(const PromptAr
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
         const int tl = j * 4 + half * 2 + b;
-        kn[b] = tl < t.tiles ? __ldg(t.ks + tl) : 0.f;
-        vn[b] = tl < t.tiles ? __ldg(t.vs + tl) : 0.f;
+        kn[b] = tl < t.tiles ? t.ks[tl] : 0.f;
+        vn[b] = tl < t.tiles ? t.vs[tl] : 0.f;
       }
     };
     float down = 0.f;          // 2^(r - kTop2) of the last block

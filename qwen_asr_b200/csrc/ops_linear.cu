@@ -385,9 +385,9 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
       const int ab = lt & 1;
       const int ch = u % a.ct * kTileCh + (PAIR ? rank * kCh : 0) + q * 32 + lane;
       const long long m0 = (long long)(u / a.ct) * a.nt + half * H;
-      const float wsc = ch < a.n ? __ldg(a.ws + ch) : 0.f;
+      const float wsc = ch < a.n ? a.ws[ch] : 0.f;
       __syncwarp();
-      for (int j = lane; j < H; j += 32) xs[j] = m0 + j < a.m ? __ldg(a.xs + m0 + j) : 0.f;
+      for (int j = lane; j < H; j += 32) xs[j] = m0 + j < a.m ? a.xs[m0 + j] : 0.f;
       __syncwarp();
       uint32_t r[C];
       if constexpr (EPI == LINEAR_RESID)
@@ -434,7 +434,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
       const int ch = unit0 % a.ct * kCh + q * 32 + lane;
       const int H = a.nt / 2;
       const long long m0 = (long long)(unit0 / a.ct) * a.nt + half * H;
-      const float wsc = ch < a.n ? __ldg(a.ws + ch) : 0.f;
+      const float wsc = ch < a.n ? a.ws[ch] : 0.f;
       const uint32_t part = smem_u32(smem) + (uint32_t)(half * H * kCh + q * 32 + lane) * 4u;
       const float* xs = xs_s + (warp - 2) * S::kHalf;
       const int each = H / a.split;  // tokens of a rank (H >= 8 = the largest split, and a multiple of it)

@@ -230,13 +230,12 @@ __global__ void __launch_bounds__(W * 32) norm_vec_kernel(const NormArgs a) {
       u[j][0] = 0.f;
       if (c < a.d) {
         if (a.h) E::store((T*)a.h + row * a.ldh + c, h[j][0]);
-        u[j][0] = __fmul_rn(h[j][0], a.w ? __ldg(a.w + c) : 1.f);
+        u[j][0] = __fmul_rn(h[j][0], a.w ? a.w[c] : 1.f);
       }
     } else if (c < a.d) {
-      if (a.h) *reinterpret_cast<uint4*>((T*)a.h + row * a.ldh + c) = raw[V > 1 ? j : 0];
 #pragma unroll
       for (int i = 0; i + 3 < V; i += 4) {
-        const float4 w = a.w ? __ldg(reinterpret_cast<const float4*>(a.w + c + i)) : make_float4(1.f, 1.f, 1.f, 1.f);
+        const float4 w = a.w ? *reinterpret_cast<const float4*>(a.w + c + i) : make_float4(1.f, 1.f, 1.f, 1.f);
         u[j][i] = __fmul_rn(h[j][i], w.x);
         u[j][i + 1] = __fmul_rn(h[j][i + 1], w.y);
         u[j][i + 2] = __fmul_rn(h[j][i + 2], w.z);
@@ -250,6 +249,13 @@ __global__ void __launch_bounds__(W * 32) norm_vec_kernel(const NormArgs a) {
     for (int i = 0; i < V; ++i) {
       mx = max_nan(mx, fabsf(u[j][i]));
       ss = fma((double)h[j][i], (double)h[j][i], ss);
+    }
+  }
+  if constexpr (V > 1) {  // (behind the weights' loads, which might alias it for all the compiler knows)
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = (threadIdx.x + j * N) * V;
+      if (a.h && c < a.d) *reinterpret_cast<uint4*>((T*)a.h + row * a.ldh + c) = raw[j];
     }
   }
   const unsigned mine = __float_as_uint(mx) & 0x7FFFFFFFu;

@@ -250,3 +250,41 @@ def test_each_user_has_its_own_errors(tiny_dir):
     with pytest.raises(RuntimeError, match="51"):
         ops.check()
     ops.check()
+
+
+# ------------------------------------------------------------------ calls in a row
+def test_every_call_sees_what_the_one_before_wrote(ops):
+    """Long runs of calls that start beside one another, each reading what its predecessor, or the one before that,
+    has just written over old values: the bits of the same calls with the device waited for in between."""
+    n, n_kv, hd, heads, d = 4, 2, 128, 8, 512
+    wq, ws = torch.randint(-127, 128, (2, (heads + 2 * n_kv) * hd, d), dtype=torch.int8, device="cuda"), rand(2, 1536, seed=1).abs() * 3e-4
+    steps = [1, 1, 40, 1, 3, 1, 1, 70, 1, 20, 1, 1] * 3
+
+    def run(wait):
+        cache = ops.kv8_cache(n, n_kv, 1024, hd)
+        w, scale, pos, out = torch.ones(d, device="cuda"), ws[0].clone(), torch.zeros(n, dtype=torch.int32, device="cuda"), []
+        g = torch.Generator(device="cuda")
+        g.manual_seed(5)
+        for i, rows in enumerate(steps):
+            x = torch.randn(n * rows, d, generator=g, device="cuda") * (1 + i % 3)
+            w.mul_(1.01)  # weights and their scales may have been written just before, too
+            q, s, h = ops.rms_norm_int8(x, w, residual=x)
+            wait()
+            scale.copy_(ws[i % 2])
+            y = ops.linear_int8(q, s, wq[i % 2], scale).view(n, rows, -1).unflatten(2, (heads + 2 * n_kv, hd))
+            wait()
+            before = ops.kv8_attention(y[:, :, :heads], cache, pos)
+            wait()
+            ops.kv8_append(cache, y[:, :, heads:heads + n_kv], y[:, :, heads + n_kv:], pos)
+            wait()
+            after = ops.kv8_attention(y[:, :, :heads], cache, pos)
+            wait()
+            out += [h, before, after, *ops.kv8_read(cache, pos, rows)]
+            pos += rows
+            wait()
+        torch.cuda.synchronize()
+        return out
+    want = run(torch.cuda.synchronize)
+    for _ in range(5):
+        for a, b in zip(run(lambda: None), want):
+            assert torch.equal(a, b)
