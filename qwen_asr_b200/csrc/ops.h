@@ -31,7 +31,7 @@ constexpr int kNormMaxD = 32768;  // the row is staged in shared memory as f32
 
 // rows r < rows of x (row pitch ldx elements): h = x + residual rounded to the type (h = x
 // without a residual), u = h * w, top = max |u|; q = rint(127 u / top) as if in exact
-// arithmetic, scale = top / sqrt(mean(h^2) + eps) / 127 (1 for a row of zeros). A row with a
+// arithmetic (where top is 2^-100 or more; below, top is taken to 2^-149), scale = top / sqrt(mean(h^2) + eps) / 127 (1 for a row of zeros). A row with a
 // NaN or an infinity (or a product beyond f32) gets scale NaN and q = 0. h may be null, x or
 // residual; q rows have pitch ldq bytes, of which bytes [d, ldq) are left as they were.
 cudaError_t rms_norm_int8(const void* x, long long ldx, const void* residual, long long ldr, const float* w, float eps,

@@ -8,9 +8,10 @@
 //
 // Rounding. q is the correctly rounded quotient. In f32, v = u * (127 / top) is off by at most
 // 127 * 4 * 2^-24 < 3.1e-5 (four roundings), so a v further than 3.2e-5 from a half rounds to the
-// right side; the others (6e-5 of all) are rounded again from the f64 product, whose factors are
-// exact. For them, and for the scale, top is exact too: the threads that hold the largest f32
-// product add its rounding error (one fma). The sum of squares is held in 64 bits, where no
+// right side; the others (6e-5 of all) are rounded again from the exact products u and top, which f64 holds
+// (top is the largest f32 product and its rounding error, one fma in the threads that hold it: exact down to 2^-100).
+// 127 u needs up to 55 bits, so where the f64 quotient is next to a half the side comes from 254 u - (2n + 1) top,
+// two products with their rounding errors (`rounded`). The sum of squares is held in 64 bits, where no
 // finite row overflows it.
 //
 // Bound: DRAM for many rows. What it took to get near: a bf16 sum as packed adds, one fmax a
@@ -56,39 +57,52 @@ struct NormArgs {
   float eps;  // negative: int8 rows without a norm (w null, scale = top / 127)
 };
 
-// Running row statistics: the sum of squares, and the largest |u| as (f32 rounding, error).
+// rint(127 u / top), correctly rounded, for exact u and top. (Of bf16 values 127 u is exact, too, and a quotient of
+// such products that is not a half is 2^-42 away from one at least, so its rounding to f64 does not matter.)
+template <bool BF16>
+__device__ __forceinline__ int rounded(double u, double top) {
+  if constexpr (BF16) return __double2int_rn(u * 127.0 / top);
+  const double v = fabs(u), x = v * 127.0 / top, n = floor(x);
+  double q = rint(x);
+  if (fabs(x - n - 0.5) < 1e-9) {
+    const double odd = 2.0 * n + 1.0, a = 254.0 * v, b = odd * top;
+    // (a and b are within a few steps of each other, and all three differences exact)
+    const double side = (a - b) + (fma(254.0, v, -a) - fma(odd, top, -b));
+    if (side > 0.0) q = n + 1.0;
+    if (side < 0.0) q = n;
+    if (side == 0.0) q = 2.0 * rint(0.5 * (n + 0.5));  // the even one
+  }
+  return (int)copysign(q, u);
+}
+
+// Running row statistics: the sum of squares, and the largest |u|, rounded (its bits) and exact.
 struct Stat {
-  double ss = 0.0;
-  unsigned top = 0u, low = 0u;  // bits of the rounded |u|; ordered bits of the error
+  double ss = 0.0, exact = 0.0;
+  unsigned top = 0u;
   __device__ void add(float h, float w) {
     ss = fma((double)h, (double)h, ss);
-    const float p = __fmul_rn(h, w);
-    const unsigned b = __float_as_uint(p) & 0x7FFFFFFFu;
+    const unsigned b = __float_as_uint(__fmul_rn(h, w)) & 0x7FFFFFFFu;
     if (b >= top) {
-      float e = __fmaf_rn(h, w, -p);
-      if (p < 0.f) e = -e;
-      const unsigned o = (unsigned)float_to_ordered(e) ^ 0x80000000u;
-      if (b > top || o > low) low = o;
+      exact = fmax(exact, fabs((double)h * (double)w));
       top = b;
     }
   }
   __device__ void warp() {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    const unsigned t = __reduce_max_sync(0xffffffffu, top);
-    low = __reduce_max_sync(0xffffffffu, top == t ? low : 0u);
-    top = t;
+    for (int o = 16; o > 0; o >>= 1) {
+      ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      exact = fmax(exact, __shfl_xor_sync(0xffffffffu, exact, o));
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
   }
   __device__ bool finite() const { return top < 0x7F800000u; }
-  __device__ double top64() const {
-    return (double)__uint_as_float(top) + (double)ordered_to_float((int)(low ^ 0x80000000u));
-  }
 };
 
+template <bool BF16>
 __device__ __forceinline__ int quant(float h, float w, float r127, const Stat& st) {
   const float v = __fmul_rn(__fmul_rn(h, w), r127);
   const float t = rintf(v);
-  if (fabsf(fabsf(__fsub_rn(v, t)) - 0.5f) < 1e-4f) return __double2int_rn((double)h * (double)w * 127.0 / st.top64());
+  if (fabsf(fabsf(__fsub_rn(v, t)) - 0.5f) < 1e-4f) return rounded<BF16>((double)h * (double)w, st.exact);
   return (int)t;
 }
 
@@ -102,7 +116,7 @@ __device__ __forceinline__ void write_scale(const NormArgs& a, long long row, co
   if (!st.finite())
     sc = __int_as_float(0x7FFFFFFF);
   else if (st.top)
-    sc = scale_of(a, st.top64(), st.ss);
+    sc = scale_of(a, st.exact, st.ss);
   a.scale[row] = sc;
 }
 
@@ -160,7 +174,7 @@ __device__ __forceinline__ void fix_near(const NormArgs& a, long long row, doubl
     const int c = ((int)threadIdx.x + b / V * step) * V + b % V;
     if (c >= a.d) break;
     const double w = a.w ? (double)a.w[c] : 1.0;
-    q[c] = (int8_t)__double2int_rn((double)Elem<BF16>::load(src + c) * w * 127.0 / top64);
+    q[c] = (int8_t)rounded<BF16>((double)Elem<BF16>::load(src + c) * w, top64);
   }
 }
 
@@ -350,8 +364,8 @@ __global__ void __launch_bounds__(512) norm_any_kernel(const NormArgs a) {
   for (int c = threadIdx.x; c < a.d; c += 512) {
     const float h = hrow[c], w = a.w ? a.w[c] : 1.0f;
     const int v = r127 == 0.f ? 0
-                  : tiny      ? __double2int_rn((double)h * (double)w * 127.0 / st.top64())
-                              : quant(h, w, r127, st);
+                  : tiny      ? rounded<BF16>((double)h * (double)w, st.exact)
+                              : quant<BF16>(h, w, r127, st);
     a.q[row * a.ldq + c] = (int8_t)v;
   }
   if (threadIdx.x == 0) write_scale(a, row, st);

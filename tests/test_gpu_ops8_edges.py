@@ -288,3 +288,33 @@ def test_every_call_sees_what_the_one_before_wrote(ops):
     for _ in range(5):
         for a, b in zip(run(lambda: None), want):
             assert torch.equal(a, b)
+
+
+# ------------------------------------------------------------------ values next to a rounding border
+# (a, b, c, d, n): 127 a b / (c d) is within half an f64 step of n + 1/2, above or below it; found by solving
+# 254 a b - (2 n + 1) c d = 1, -1, 2, ... in whole numbers under 2^24
+BORDER = [(9187418, 11738396, 14744709, 11124571, 83), (15514599, 11641642, 12066306, 16602699, 114),
+          (9678723, 15910658, 11891262, 15738585, 104), (10220674, 12154493, 10568986, 13886037, 107),
+          (15889422, 9953404, 13779419, 13948781, 104), (9270475, 8855139, 8706701, 14004943, 85),
+          (12467758, 12640073, 15177441, 13808285, 95), (9870208, 14882039, 13310854, 16016901, 87),
+          (13935253, 14249515, 16281284, 14543884, 106), (9350045, 8942833, 15864436, 13522678, 49),
+          (13429207, 9812132, 12548494, 14735921, 90), (11504340, 8951737, 16485217, 16358231, 48)]
+
+
+@pytest.mark.parametrize("d", [64, 49, 4096, 16384])
+def test_norm_values_within_an_f64_step_of_a_border(ops, d):
+    """int8 values as in exact arithmetic, at quotients that f64 rounds onto a half or over it."""
+    x, w = torch.zeros(4 * len(BORDER), d, device="cuda"), torch.ones(d, device="cuda")
+    want = []
+    for i, (a, b, c, e, n) in enumerate(BORDER):
+        w[2 * i], w[2 * i + 1] = b, e * 2.0 ** -20
+        assert 254 * a * b != (2 * n + 1) * c * e
+        q = n + 1 if 254 * a * b > (2 * n + 1) * c * e else n
+        for j, (s, t) in enumerate(((1, 1), (-1, 1), (1, -1), (-1, -1))):
+            x[4 * i + j, 2 * i], x[4 * i + j, 2 * i + 1] = s * a * 2.0 ** -20, t * c
+            want.append((s * q, t * 127))
+    q, _, _ = ops.rms_norm_int8(x, w)
+    q = q.cpu()
+    for r, (a, b) in enumerate(want):
+        i = r // 4
+        assert (q[r, 2 * i].item(), q[r, 2 * i + 1].item()) == (a, b), r
