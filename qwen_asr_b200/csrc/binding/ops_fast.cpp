@@ -18,11 +18,13 @@
 
 namespace {
 
-// The tensor of a plain torch.Tensor on a GPU that needs no gradient, or null.
+// The tensor of a plain torch.Tensor on a GPU that needs no gradient and has no tangent, or null.
 const at::Tensor* plain(PyObject* o) {
   if (!THPVariable_CheckExact(o)) return nullptr;
   const at::Tensor& t = THPVariable_Unpack(o);
-  if (!t.is_cuda() || t.layout() != at::kStrided || (t.requires_grad() && c10::GradMode::is_enabled())) return nullptr;
+  if (!t.is_cuda() || t.layout() != at::kStrided || (t.requires_grad() && c10::GradMode::is_enabled()) || t.is_neg() ||
+      t._fw_grad(0).defined())
+    return nullptr;
   return &t;
 }
 
@@ -193,6 +195,10 @@ PyObject* kv8_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
         !index_of(a[3], a[4], dev, c.n_seq, sp, cp, stride))
       Py_RETURN_NONE;
     if (qwen_asr_kv8_append(&c, &k, &v, dtype_of(*kt), (int32_t)rows, sp, cp, stride, dev, stream_of(dev))) return failed();
+    for (int i = 0; i < 4; ++i) {  // the cache has changed in place
+      const at::Tensor& t = THPVariable_Unpack(PyTuple_GET_ITEM(a[0], i));
+      if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+    }
     Py_RETURN_TRUE;
   });
 }

@@ -9,7 +9,8 @@
 
 Calls run on the current stream of the tensors' device, enqueue and return; outputs are new
 tensors. They keep no state and use no workspace, and can be captured into CUDA graphs. They
-have no gradients: an input that requires one is refused. Arguments that do not fit raise
+have no gradients: an input that requires one, or carries a forward-mode tangent, is refused, and
+kv8_append counts as an in-place change of the cache. Arguments that do not fit raise
 ValueError (TypeError for a wrong type) before anything is enqueued; a launch that CUDA refuses
 raises RuntimeError. There is no CPU form.
 """
@@ -20,6 +21,8 @@ import struct
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
+from torch.autograd.graph import increment_version as _increment_version
 
 from . import last_error, lib
 
@@ -56,6 +59,13 @@ def kv8_cache(n_seq: int, n_kv: int, capacity: int, head_dim: int = 128, device=
     return Kv8Cache(*q, *s)
 
 
+def _derives(t):
+    """Whether the call would have to differentiate: t requires a gradient, or has a tangent."""
+    if t.requires_grad and _grad():
+        return True
+    return _forward_ad._current_level >= 0 and _forward_ad.unpack_dual(t).tangent is not None
+
+
 # An ordinary call is checked and made in C++, which answers None to any other: unusual strides and
 # sizes, which ctypes handles here, and arguments that do not fit, which are named here.
 def _tensor(t, name, dims, dtypes, device=None, shape=None):
@@ -71,14 +81,16 @@ def _tensor(t, name, dims, dtypes, device=None, shape=None):
         raise ValueError(f"{name} must have {dims} dimensions, not {t.dim()}")
     if shape is not None and tuple(t.shape) != tuple(shape):
         raise ValueError(f"{name} must have shape {tuple(shape)}, not {tuple(t.shape)}")
-    if t.requires_grad and _grad():
-        raise ValueError(f"{name} requires a gradient, which the 8-bit operators do not have")
+    if _derives(t):
+        raise ValueError(f"{name} requires a gradient or has a tangent, which the 8-bit operators do not have")
+    if t.is_neg():
+        raise ValueError(f"{name} is a negated view (resolve_neg() makes a tensor of it)")
     return t
 
 
 def _is(t, dtype, device, shape):
     return (isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == device and t.shape == shape
-            and not (t.requires_grad and _grad()))
+            and not _derives(t) and not t.is_neg())
 
 
 def _pitch(t, name):
@@ -106,7 +118,7 @@ def rms_norm_int8(x, weight, eps: float = 1e-6, residual=None):
             return out
     _x = isinstance(x, torch.Tensor)
     code = _DTYPES.get(x.dtype) if _x else None
-    if code is None or x.dim() != 2 or not x.is_cuda or (x.requires_grad and _grad()):
+    if code is None or x.dim() != 2 or not x.is_cuda or _derives(x) or x.is_neg():
         _tensor(x, "x", 2, _FLOATS)
     dev, shape, dtype = x.get_device(), x.shape, x.dtype
     rows, d = shape
@@ -143,10 +155,11 @@ def linear_int8(xq, xs, wq, ws, residual=None, swiglu: bool = False, dtype=torch
         out = _fast.linear_int8(xq, xs, wq, ws, residual, bool(swiglu), dtype is torch.bfloat16)
         if out is not None:
             return out
-    if not (isinstance(xq, torch.Tensor) and xq.dtype is _INT8 and xq.is_cuda and xq.dim() == 2):
+    if not (isinstance(xq, torch.Tensor) and xq.dtype is _INT8 and xq.is_cuda and xq.dim() == 2 and not xq.is_neg()):
         _tensor(xq, "xq", 2, (_INT8,))
     dev, (m, k) = xq.get_device(), xq.shape
-    if not (isinstance(wq, torch.Tensor) and wq.dtype is _INT8 and wq.get_device() == dev and wq.dim() == 2):
+    if not (isinstance(wq, torch.Tensor) and wq.dtype is _INT8 and wq.get_device() == dev and wq.dim() == 2
+            and not wq.is_neg()):
         _tensor(wq, "wq", 2, (_INT8,), dev)
     n = wq.shape[0]
     if wq.shape[1] != k:
@@ -197,7 +210,7 @@ def _cache(cache):
                 and vs.shape == ks.shape and vs.stride() == ss and ss[1:] == (blocks, 1) and (hd == 128 or hd == 64)
                 and blocks > 0 and cap == blocks * BLOCK and dev >= 0 and v.get_device() == dev
                 and ks.get_device() == dev and vs.get_device() == dev
-                and not ((ks.requires_grad or vs.requires_grad) and _grad())):
+                and not (_derives(ks) or _derives(vs)) and not any(t.is_neg() for t in cache)):
             return (_KV8.pack(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), st[0], ss[0], n, h, cap, hd),
                     dev, n, h, hd)
     except (AttributeError, ValueError):
@@ -264,6 +277,8 @@ def kv8_append(cache: Kv8Cache, k, v, starts, counts=None) -> None:
     if rows and lib().qwen_asr_kv8_append(desc, _rows(k, "k"), _rows(v, "v"), code, rows, sp, cp, stride, dev,
                                           _raw_stream(dev)):
         _failed()
+    if rows:
+        _increment_version([t for t in cache if not t.is_inference()])
 
 
 def kv8_read(cache: Kv8Cache, starts, rows: int, counts=None, dtype=torch.float32):
@@ -306,7 +321,7 @@ def kv8_attention(q, cache: Kv8Cache, starts, counts=None, scale: float | None =
         _tensor(q, "q", 4, _FLOATS, dev)
     shape = q.shape
     rows, heads = shape[1], shape[2]
-    if shape != (n, rows, heads, hd) or q.get_device() != dev or (q.requires_grad and _grad()):
+    if shape != (n, rows, heads, hd) or q.get_device() != dev or _derives(q) or q.is_neg():
         _tensor(q, "q", 4, _FLOATS, dev, (n, rows, heads, hd))
     if heads < 1 or heads % h or heads > 256 * h:
         raise ValueError(f"{heads} query heads do not fit {h} cached ones")

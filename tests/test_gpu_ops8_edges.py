@@ -318,3 +318,57 @@ def test_norm_values_within_an_f64_step_of_a_border(ops, d):
     for r, (a, b) in enumerate(want):
         i = r // 4
         assert (q[r, 2 * i].item(), q[r, 2 * i + 1].item()) == (a, b), r
+
+
+# ------------------------------------------------------------------ tensors with derivatives
+def test_tangents_and_negated_views_are_refused(ops):
+    """A forward-mode tangent would be dropped, a negated view read without its sign."""
+    from torch.autograd import forward_ad
+    x, w = rand(4, 64), rand(64)
+    q8, s = torch.randint(-127, 128, (4, 64), dtype=torch.int8, device="cuda"), torch.ones(4, device="cuda")
+    c = ops.kv8_cache(2, 2, 32, 128)
+    z, k = torch.zeros(2, dtype=torch.int32, device="cuda"), rand(2, 1, 2, 128)
+    calls = [(lambda t: ops.rms_norm_int8(t, w), x), (lambda t: ops.rms_norm_int8(x, t), w),
+             (lambda t: ops.rms_norm_int8(x, w, residual=t), x), (lambda t: ops.linear_int8(q8, t, q8, s), s),
+             (lambda t: ops.linear_int8(q8, s, q8, t), s), (lambda t: ops.linear_int8(q8, s, q8, s, residual=t), rand(4, 4)),
+             (lambda t: ops.kv8_append(c, t, k, z), k), (lambda t: ops.kv8_append(c, k, t, z), k),
+             (lambda t: ops.kv8_attention(t, c, z), k), (lambda t: ops.kv8_attention(k, c._replace(v_scale=t), z), c.v_scale),
+             (lambda t: ops.kv8_read(c._replace(k_scale=t), z, 1), c.k_scale)]
+    ints = [(lambda t: ops.linear_int8(t, s, q8, s), q8), (lambda t: ops.linear_int8(q8, s, t, s), q8),
+            (lambda t: ops.kv8_read(c._replace(k=t), z, 1), c.k), (lambda t: ops.kv8_append(c, k, k, t), z),
+            (lambda t: ops.kv8_attention(k, c, z, t), z)]
+    for i, (f, t) in enumerate(calls + ints):
+        f(t)
+        with pytest.raises(ValueError, match="negated"):
+            f(torch._neg_view(t))
+        if i < len(calls):
+            with forward_ad.dual_level():
+                with pytest.raises(ValueError, match="tangent"):
+                    f(forward_ad.make_dual(t, torch.ones_like(t)))
+                f(t)
+
+
+def test_append_counts_as_a_change_of_the_cache(ops):
+    """A backward pass that saved the cache's values from before must not use those after."""
+    c = ops.kv8_cache(1, 1, 32, 64)
+    k, z = rand(1, 3, 1, 64), torch.zeros(1, dtype=torch.int32, device="cuda")
+    ops.kv8_append(c, k, k, z)
+    w = torch.ones(1, device="cuda", requires_grad=True)
+    for t in (c.k_scale, c.v_scale):
+        y = (t * w).sum()
+        y.backward()
+        y = (t * w).sum()
+        ops.kv8_append(c, 3 * k, 3 * k, z + 3)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    versions = [t._version for t in c]
+    ops.kv8_append(c, k[:, :0], k[:, :0], z)
+    ops.kv8_attention(k, c, z)
+    ops.kv8_read(c, z, 3)
+    assert [t._version for t in c] == versions
+    ops.kv8_append(c, k, k, z)
+    assert all(t._version > v for t, v in zip(c, versions))
+    with torch.inference_mode():
+        c = ops.kv8_cache(1, 1, 32, 64)
+        ops.kv8_append(c, k, k, z)
+        assert c.k_scale.any()
