@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import math
 import struct
+from operator import index
 from typing import NamedTuple
 
 import torch
@@ -35,6 +36,7 @@ BLOCK = 16  # cache tokens that share a scale
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
 _FLOATS = (torch.float32, torch.bfloat16)
+_MAX_INT32 = 2 ** 31 - 1
 _F32, _INT8, _INT32 = torch.float32, torch.int8, torch.int32
 _KV8 = struct.Struct("@PPPPqqiiii")  # QwenAsrKv8
 _ROWS = struct.Struct("@Pqq")        # QwenAsrRows
@@ -239,6 +241,8 @@ def _indices(starts, counts, dev, n):
     if not _is(starts, _INT32, dev, (n,)):
         _tensor(starts, "starts", 1, (_INT32,), dev, (n,))
     stride = starts.stride(0) if n > 1 else 1
+    if stride > _MAX_INT32:
+        starts, stride = starts.contiguous(), 1
     if counts is not None:
         if not _is(counts, _INT32, dev, (n,)):
             _tensor(counts, "counts", 1, (_INT32,), dev, (n,))
@@ -269,6 +273,8 @@ def kv8_append(cache: Kv8Cache, k, v, starts, counts=None) -> None:
     if code is None or k.dim() != 4:
         _tensor(k, "k", 4, _FLOATS, dev)
     rows = k.shape[1]
+    if rows > _MAX_INT32:
+        raise ValueError("k has 2^31 rows or more")
     shape = (n, rows, h, hd)
     if not (_is(k, k.dtype, dev, shape) and _is(v, k.dtype, dev, shape)):
         _tensor(k, "k", 4, _FLOATS, dev, shape)
@@ -292,8 +298,9 @@ def kv8_read(cache: Kv8Cache, starts, rows: int, counts=None, dtype=torch.float3
     code = _DTYPES.get(dtype)
     if code is None:
         raise TypeError(f"dtype must be torch.float32 or torch.bfloat16, not {dtype}")
-    if rows < 0:
-        raise ValueError("rows must not be negative")
+    rows = index(rows)
+    if not 0 <= rows <= _MAX_INT32:
+        raise ValueError("rows must be 0 .. 2^31 - 1")
     starts, counts, sp, cp, stride = _indices(starts, counts, dev, n)
     k = torch.empty((n, rows, h, hd), dtype=dtype, device=starts.device)
     v = torch.empty_like(k)
@@ -321,13 +328,17 @@ def kv8_attention(q, cache: Kv8Cache, starts, counts=None, scale: float | None =
         _tensor(q, "q", 4, _FLOATS, dev)
     shape = q.shape
     rows, heads = shape[1], shape[2]
+    if rows > 1 << 22:
+        raise ValueError("q must have at most 2^22 rows")
+    max_len = index(max_len)
+    if not 0 <= max_len <= cache[0].shape[2]:
+        max_len = 0  # (no bound: the capacity)
     if shape != (n, rows, heads, hd) or q.get_device() != dev or _derives(q) or q.is_neg():
         _tensor(q, "q", 4, _FLOATS, dev, (n, rows, heads, hd))
     if heads < 1 or heads % h or heads > 256 * h:
         raise ValueError(f"{heads} query heads do not fit {h} cached ones")
     starts, counts, sp, cp, stride = _indices(starts, counts, dev, n)
-    if scale is None:
-        scale = 1.0 / math.sqrt(hd)
+    scale = 1.0 / math.sqrt(hd) if scale is None else float(scale)
     out = torch.empty(shape, dtype=q.dtype, device=q.device)
     width = heads * hd
     if rows and lib().qwen_asr_kv8_attention(desc, _rows(q, "q"), _ROWS.pack(out.data_ptr(), rows * width, width),

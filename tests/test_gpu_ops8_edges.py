@@ -372,3 +372,43 @@ def test_append_counts_as_a_change_of_the_cache(ops):
         c = ops.kv8_cache(1, 1, 32, 64)
         ops.kv8_append(c, k, k, z)
         assert c.k_scale.any()
+
+
+# ------------------------------------------------------------------ arguments past 32 bits
+def test_arguments_past_32_bits(ops):
+    """A stride of positions, a number of rows and a length whose lower 32 bits are another number."""
+    n, cap = 2, 64
+    c = filled_cache(ops, n, 1, cap, 64, [cap, cap], seed=98)
+    cache = ops.Kv8Cache(*c)
+    q, k = rand(n, 1, 2, 64, seed=99), rand(n, 1, 1, 64, seed=100)
+    near = torch.tensor([3, 40], dtype=torch.int32, device="cuda")
+    table = torch.zeros(2 ** 32 + 2, dtype=torch.int32, device="cuda")
+    far = table[::2 ** 32 + 1]
+    far.copy_(near)
+    assert far.stride(0) == 2 ** 32 + 1
+    assert torch.equal(ops.kv8_attention(q, cache, far), ops.kv8_attention(q, cache, near))
+    assert torch.equal(ops.kv8_attention(q, cache, near, far), ops.kv8_attention(q, cache, near, near))
+    for a, b in zip(ops.kv8_read(cache, far, 5, far), ops.kv8_read(cache, near, 5, near)):
+        assert torch.equal(a, b)
+    before = [t.clone() for t in c]
+    ops.kv8_append(cache, k, k, far)
+    after = [t.clone() for t in c]
+    for t, b in zip(c, before):
+        t.copy_(b)
+    ops.kv8_append(cache, k, k, near)
+    assert all(torch.equal(a, b) for a, b in zip(c, after))
+    del table, far
+    many = k[:, :, :, :1].expand(n, 2 ** 32 + 1, 1, 64)
+    with pytest.raises(ValueError, match="rows"):
+        ops.kv8_append(cache, many, many, near)
+    with pytest.raises(ValueError, match="rows"):
+        ops.kv8_attention(many, cache, near)
+    with pytest.raises(ValueError, match="rows"):
+        ops.kv8_read(cache, near, 2 ** 31)
+    want = ops.kv8_attention(q, cache, near)
+    for m in (2 ** 32 + 16, 2 ** 80, -1, cap + 1):
+        assert torch.equal(ops.kv8_attention(q, cache, near, max_len=m), want)
+    with pytest.raises(TypeError):
+        ops.kv8_attention(q, cache, near, max_len=1.5)
+    assert torch.equal(ops.kv8_attention(q, cache, near, scale=torch.tensor(0.125)), want)
+    assert torch.equal(ops.kv8_attention(q, cache, near, scale=0.125, max_len=torch.tensor(64)), want)
