@@ -63,11 +63,17 @@ def build(force: bool = False, verbose: bool = True) -> str:
     return LIB
 
 
-def build_binding(force: bool = False, verbose: bool = True) -> str:
-    """_ops_fast.so: the C++ binding of the 8-bit operators (ops.py) against the installed torch."""
+def build_binding(force: bool = False, verbose: bool = True) -> str | None:
+    """_ops_fast.so: the C++ binding of the 8-bit operators (ops.py) against the installed torch. None
+    where torch is not installed: the engine and its C interface do without."""
     import sysconfig
-    import torch
-    from torch.utils import cpp_extension
+    try:
+        import torch
+        from torch.utils import cpp_extension
+    except ImportError:
+        if verbose:
+            print("no torch: the binding of qwen_asr_b200.ops is left out")
+        return None
     src = os.path.join(CSRC, "binding", "ops_fast.cpp")
     out = os.path.join(HERE, "_ops_fast.so")
     newest = _newest([src, LIB] + glob.glob(os.path.join(INC, "*.h")))

@@ -27,3 +27,15 @@ except RuntimeError as e:
     assert 'timed out' not in str(e), e
     print('reported')
 """, CUDA_VISIBLE_DEVICES="")
+
+
+def test_the_library_builds_without_torch():
+    assert "built" in python("""
+import sys
+sys.modules['torch'] = None  # an import of it fails
+import __graft_entry__
+__graft_entry__.build()
+from qwen_asr_b200 import build
+assert build.build_binding() is None
+print('built')
+""")
