@@ -412,3 +412,46 @@ def test_arguments_past_32_bits(ops):
         ops.kv8_attention(q, cache, near, max_len=1.5)
     assert torch.equal(ops.kv8_attention(q, cache, near, scale=torch.tensor(0.125)), want)
     assert torch.equal(ops.kv8_attention(q, cache, near, scale=0.125, max_len=torch.tensor(64)), want)
+
+
+# ------------------------------------------------------------------ refusals
+def test_refusals_are_of_the_documented_type(ops):
+    """A wrong type is a TypeError and an argument that does not fit a ValueError, before anything is enqueued: never
+    a launch that CUDA refuses, which is a RuntimeError."""
+    x, w, s = rand(4, 64), rand(64), torch.ones(4, device="cuda")
+    q8 = torch.ones(4, 64, dtype=torch.int8, device="cuda")
+    c, z, k = ops.kv8_cache(2, 2, 32, 128), torch.zeros(2, dtype=torch.int32, device="cuda"), rand(2, 1, 2, 128)
+    both = ops.Kv8Cache(*[t.expand(2, *t.shape[1:]) for t in ops.kv8_cache(1, 2, 32)])
+    bad = [
+        (TypeError, lambda: ops.rms_norm_int8(x.half(), w)), (TypeError, lambda: ops.rms_norm_int8(x, w.to(BF16))),
+        (TypeError, lambda: ops.rms_norm_int8(x, w, residual=x.to(BF16))),
+        (ValueError, lambda: ops.rms_norm_int8(x, w[:63])), (ValueError, lambda: ops.rms_norm_int8(x.T, rand(4))),
+        (ValueError, lambda: ops.rms_norm_int8(x, w, eps=-1.0)), (ValueError, lambda: ops.rms_norm_int8(x, w, eps=math.nan)),
+        (ValueError, lambda: ops.rms_norm_int8(x, w.cpu())), (ValueError, lambda: ops.rms_norm_int8(x.cpu(), w)),
+        (ValueError, lambda: ops.rms_norm_int8(x.clone().requires_grad_(), w)), (ValueError, lambda: ops.rms_norm_int8(x[0], w)),
+        (ValueError, lambda: ops.rms_norm_int8(rand(1, 40000), rand(40000))), (ValueError, lambda: ops.rms_norm_int8(x[:, :0], w[:0])),
+        (ValueError, lambda: ops.linear_int8(q8, s, q8[:, :32], s)), (ValueError, lambda: ops.linear_int8(q8[:, 1:33], s, q8[:, :32], s)),
+        (ValueError, lambda: ops.linear_int8(q8[:, :60].contiguous(), s, q8[:, :60], s)),
+        (ValueError, lambda: ops.linear_int8(q8, s[:3], q8, s)), (ValueError, lambda: ops.linear_int8(q8, s, q8[:3], s[:3], swiglu=True)),
+        (ValueError, lambda: ops.linear_int8(q8, s, q8, s, residual=rand(4, 4), swiglu=True)),
+        (ValueError, lambda: ops.linear_int8(q8, s, q8, s, residual=rand(4, 5))), (ValueError, lambda: ops.linear_int8(q8, s, q8[:0], s[:0])),
+        (ValueError, lambda: ops.linear_int8(q8[:1].expand(4, 64), s, q8, s)),
+        (TypeError, lambda: ops.linear_int8(q8, s, q8, s, dtype=torch.float16)), (TypeError, lambda: ops.linear_int8(x, s, q8, s)),
+        (TypeError, lambda: ops.linear_int8(q8, s, q8, s, residual=rand(4, 4).to(BF16))),
+        (ValueError, lambda: ops.kv8_append(c, k[:1], k[:1], z)), (ValueError, lambda: ops.kv8_append(c, k, k[..., :64], z)),
+        (TypeError, lambda: ops.kv8_append(c, k, k, z.long())), (TypeError, lambda: ops.kv8_append(c, k, k.to(BF16), z)),
+        (ValueError, lambda: ops.kv8_append(c, k, k, z[:1])), (ValueError, lambda: ops.kv8_append(c, k, k, z[:1].expand(2))),
+        (ValueError, lambda: ops.kv8_append(both, k, k, z)), (ValueError, lambda: ops.kv8_read(both, z, 1)),
+        (ValueError, lambda: ops.kv8_append(c, k.transpose(2, 3).contiguous().transpose(2, 3), k, z)),
+        (ValueError, lambda: ops.kv8_append(c._replace(v=c.v.transpose(1, 2)), k, k, z)),
+        (ValueError, lambda: ops.kv8_append(c, k, k, z, z.cpu())), (ValueError, lambda: ops.kv8_attention(k, both, z)),
+        (ValueError, lambda: ops.kv8_attention(rand(2, 1, 3, 128), c, z)), (ValueError, lambda: ops.kv8_attention(rand(2, 1, 4, 64), c, z)),
+        (ValueError, lambda: ops.kv8_attention(rand(2, 1, 1024, 128), c, z)), (ValueError, lambda: ops.kv8_read(c, z, -1)),
+        (ValueError, lambda: ops.kv8_read(ops.kv8_cache(1, 1, 16, 96), z[:1], 1)), (TypeError, lambda: ops.kv8_read(c, z, 1, dtype=torch.float16)),
+        (TypeError, lambda: ops.kv8_attention([1], c, z)), (TypeError, lambda: ops.kv8_read(c, z, 1.5)),
+    ]
+    for i, (err, f) in enumerate(bad):
+        with pytest.raises(Exception) as e:
+            f()
+        assert type(e.value) is err, (i, e.value)
+    assert not c.k.any() and not c.k_scale.any()
