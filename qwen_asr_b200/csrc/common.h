@@ -70,6 +70,7 @@ struct DevBuf {
     if (count == 0) count = 1;
     if (cudaMalloc(&p, count * sizeof(T)) != cudaSuccess) {
       p = nullptr;
+      cudaGetLastError();  // it is reported here, not by a later check of what a stage launched
       set_error("cudaMalloc failed for " + std::to_string(count * sizeof(T)) + " bytes");
       return false;
     }

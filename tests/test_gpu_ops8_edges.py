@@ -455,3 +455,34 @@ def test_refusals_are_of_the_documented_type(ops):
             f()
         assert type(e.value) is err, (i, e.value)
     assert not c.k.any() and not c.k_scale.any()
+
+
+def test_a_mode_that_does_not_fit_leaves_the_engine_as_it_was(tiny_dir):
+    """set_kv_mode without memory for the other cache: -1, and what follows runs as before."""
+    import qwen_asr_b200 as Q
+    from qwen_asr_b200 import synth
+    x = synth.synth_audio(16000 * 3, seed=101)
+    eng = Q.Engine(tiny_dir)
+    eng.set_force_n_tokens(4)
+    eng.grow_kv(1 << 18)  # (caches that do not fit into what the fill below leaves)
+    want, ids = eng.transcribe_pcm(x), eng.last_tokens()
+    torch.cuda.empty_cache()
+    for mode in (1, 0):
+        held = []
+        for size in (8 << 30, 1 << 30, 128 << 20, 16 << 20, 2 << 20):
+            try:
+                while True:
+                    held.append(torch.empty(size, dtype=torch.uint8, device="cuda"))
+            except torch.OutOfMemoryError:
+                pass
+        failed = Q.lib().qwen_asr_set_kv_mode(eng._h, mode)
+        del held
+        torch.cuda.empty_cache()
+        assert failed == -1
+        assert eng.transcribe_pcm(x) == want, Q.last_error()
+        if mode == 1:
+            assert eng.last_tokens() == ids
+            eng.set_kv_mode("int8")
+            want, ids = eng.transcribe_pcm(x), eng.last_tokens()
+        else:
+            assert eng.last_tokens() == ids
