@@ -48,7 +48,7 @@ namespace {
 
 constexpr int kTok = kKv8Block;  // tokens of a tile
 constexpr int kStepRows = 64;    // query rows of a KV head up to which its length is split
-constexpr float kNone = -1.0e30f;  // running maximum before any key (finite: differences stay defined)
+constexpr float kNone = -3.4028235e38f;  // running maximum before any key (finite: differences stay defined)
 
 struct AttnArgs {
   Kv8 c;
@@ -236,7 +236,7 @@ struct WarpState {
       for (int i = 0; i < 4; ++i) {
         const int nt = i >> 1, o = i & 1;
         const float sum = PL == 2 ? s[nt][o] + s[nt][2 + o] : s[nt][2 * h + o];
-        x[i] = pos0 + nt * 8 + 2 * t + o <= last[h] ? sum * f : -__int_as_float(0x7F800000);
+        x[i] = pos0 + nt * 8 + 2 * t + o <= last[h] ? __fmul_rn(sum, f) : -__int_as_float(0x7F800000);
         mx = fmaxf(mx, x[i]);
       }
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
@@ -712,7 +712,7 @@ __global__ void __launch_bounds__(kDigWarps * 32, RH == 1 ? 3 : 2) digit_kernel(
     }
     // ---- softmax state
     const bool partial = pos0 + 2 * kTok - 1 > all_see;
-    float f0[RH], f1[RH], v0[RH], v1[RH], mx[RH], most[RH];
+    float v0[RH], v1[RH], mx[RH], most[RH];
     bool grew = ++since > 2048;
     // the step's largest weight, within 4 times: its largest probability times its larger V scale, unless these are
     // further apart
@@ -721,17 +721,19 @@ __global__ void __launch_bounds__(kDigWarps * 32, RH == 1 ? 3 : 2) digit_kernel(
     for (int h = 0; h < RH; ++h) {
       // a block that the row sees nothing of gives it nothing of its scales either (they may be NaN)
       const bool see0 = pos0 <= last[h], see1 = pos0 + kTok <= last[h];
-      f0[h] = see0 ? fac[h] * sc.x : 0.f;
-      f1[h] = see1 ? fac[h] * sc.y : 0.f;
+      const float f0 = see0 ? fac[h] * sc.x : 0.f, f1 = see1 ? fac[h] * sc.y : 0.f;
       v0[h] = see0 ? sc.z : 0.f;
       v1[h] = see1 ? sc.w : 0.f;
       float t0 = kNone, t1 = kNone;
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
+      for (int e = 0; e < 4; ++e) {
+        // (rounded before the maximum is taken off, as that was: of scores of any size its own difference is 0)
+        x[h][e] = __fmul_rn(x[h][e], e < 2 ? f0 : f1);
         if (!partial || pos0 + (e >> 1) * 16 + (e & 1) * 8 + g <= last[h]) {
-          if (e < 2) t0 = fmaxf(t0, x[h][e] * f0[h]);
-          else t1 = fmaxf(t1, x[h][e] * f1[h]);
+          if (e < 2) t0 = fmaxf(t0, x[h][e]);
+          else t1 = fmaxf(t1, x[h][e]);
         }
+      }
       mx[h] = fmaxf(t0, t1);
 #pragma unroll
       for (int o = 4; o < 32; o *= 2) mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], o));
@@ -778,7 +780,7 @@ __global__ void __launch_bounds__(kDigWarps * 32, RH == 1 ? 3 : 2) digit_kernel(
       uint32_t z[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        float p = ex2(fmaf(x[h][e], e < 2 ? f0[h] : f1[h], -m[h]));
+        float p = ex2(x[h][e] - m[h]);
         // (not by the score: a masked one times a zero scale is no number)
         if (partial && pos0 + (e >> 1) * 16 + (e & 1) * 8 + g > last[h]) p = 0.f;
         l[h] += p;

@@ -49,7 +49,8 @@ namespace {
 
 constexpr int kMaxParts = 4;  // CTAs that share a row tile's keys
 constexpr int kRows = 128, kKeys = 64, kThreads = 256, kFill = 96;  // (threads that bring K and V)
-constexpr float kNone = -1.0e30f;
+constexpr float kNone = -3.4028235e38f;  // running maximum before any key: the lowest number, no score is below
+constexpr float kLarge = 65536.f;        // scores beyond are rounded before m is taken off (log2)
 constexpr float kLag = 8.f;  // what a score may exceed m by, and a bf16 row's weight 2^r (log2)
 constexpr int kTop1 = 7, kTop2 = 14;  // log2 of 2^r in P: 2^(kTop1 + kLag) and 2^kTop2 are in f16's range (to 65504)
 constexpr float kFaint = 80.f;  // probabilities under 2^-80 count as 2^-80 for r: P's factor stays finite
@@ -201,17 +202,22 @@ __device__ __forceinline__ uint32_t pack_rest(float a, float b, uint32_t hi) {
   const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
   return pack_f16(a - f.x, b - f.y);
 }
-// One tile of 16 scores: probabilities ex2(x f - m) (0 where seen says so), their sum to l, times w as f16 planes.
-template <int PL, bool PARTIAL>
+// One tile of 16 scores: probabilities ex2(x f - m), their sum to l, times w as f16 planes. CAREFUL: 0 where seen
+// says so, and x f rounded as m was, whose rounding would otherwise be the largest probability's exponent.
+template <int PL, bool CAREFUL>
 __device__ __forceinline__ void weigh(const float* x, float f, float m, float w, int seen, f32x2& l, uint32_t* hi,
                                       uint32_t* lo) {
   const f32x2 f2 = pair(f, f), m2 = pair(-m, -m), w2 = pair(w, w);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    float2 t = split(fma2(pair(x[2 * i], x[2 * i + 1]), f2, m2));
+    float2 t;
+    if (CAREFUL)  // (f32 pairs would be multiplied and added in one step all the same)
+      t = make_float2(__fsub_rn(__fmul_rn(x[2 * i], f), m), __fsub_rn(__fmul_rn(x[2 * i + 1], f), m));
+    else
+      t = split(fma2(pair(x[2 * i], x[2 * i + 1]), f2, m2));
     t.x = ex2(t.x);
     t.y = ex2(t.y);
-    if (PARTIAL) {  // (not by the score: -inf times a zero scale is no number)
+    if (CAREFUL) {  // (not by the score: -inf times a zero scale is no number)
       if (2 * i >= seen) t.x = 0.f;
       if (2 * i + 1 >= seen) t.y = 0.f;
     }
@@ -659,9 +665,10 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_bf16_kernel(const PromptAr
     const int last = (live ? min(start + s, a.c.capacity - 1) : -1) - t.first;
     const float fac = nb > 0 ? row_fac[tid] : 0.f;
     const uint32_t trow = tmem + ((uint32_t)(warp * 32) << 16);
-    // log2 of the largest weight so far; r + kLag, and 2^(kTop1 - r)
+    // log2 of the largest weight so far, relative to m; r + kLag, and 2^(kTop1 - r)
     float m = kNone, most = -__int_as_float(0x7F800000), full = -__int_as_float(0x7F800000), up = 1.f;
-    f32x2 l = 0;  // two partial sums
+    bool large = false;  // a row's m is beyond kLarge
+    f32x2 l = 0;         // two partial sums
     float kn[4], vn[4];  // the next block's scales
     auto scales = [&](int j) {
 #pragma unroll
@@ -701,28 +708,30 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_bf16_kernel(const PromptAr
         for (int i = 0; i < kKeys; ++i)
           if (pos0 + i > last) x[i] = -__int_as_float(0x7F800000);
       }
-      float mx = kNone, e = -__int_as_float(0x7F800000);  // the largest score, and log2 of the largest weight
+      float mx = kNone, e = -__int_as_float(0x7F800000), top[4];
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
         float t = x[16 * b];
 #pragma unroll
         for (int i = 1; i < 16; ++i) t = fmaxf(t, x[16 * b + i]);
-        t *= f[b];
-        mx = fmaxf(mx, t);  // (a masked tile's -inf, or no number: ignored)
-        e = fmaxf(e, t + wl[b]);
+        top[b] = __fmul_rn(t, f[b]);  // (not in one step with what is taken off)
+        mx = fmaxf(mx, top[b]);  // (a masked tile's -inf, or no number: ignored)
       }
-      const bool grow = mx > m + kLag || fmaxf(e - m, faint) > full, rescale = __any_sync(0xffffffffu, grow);
+#pragma unroll
+      for (int b = 0; b < 4; ++b) e = fmaxf(e, top[b] - mx + wl[b]);  // log2 of the largest weight, for a maximum of mx
+      const bool grow = mx > m + kLag || fmaxf(e + (mx - m), faint) > full, rescale = __any_sync(0xffffffffu, grow);
       float corr = 1.f, corr_o = 1.f;
       if (grow) {
         const float m1 = mx > m + kLag ? mx : m;
-        most = fmaxf(most, e);
-        const int r = exponent_of(fmaxf(most - m1, faint));
+        most = fmaxf(most + (m - m1), e + (mx - m1));
+        const int r = exponent_of(fmaxf(most, faint));
         corr = ex2(m - m1);
         corr_o = ex2(m - m1 + (full - (kLag + (float)r)));
         m = m1;
         full = kLag + (float)r;
         up = power(kTop1 - r);
       }
+      if (rescale) large = __any_sync(0xffffffffu, m > kNone && fabsf(m) > kLarge);
 #pragma unroll
       for (int b = 0; b < 4; ++b) w[b] *= up;
       if (j > 0) {
@@ -747,7 +756,7 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_bf16_kernel(const PromptAr
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
         uint32_t hi[8];
-        if (partial)
+        if (partial || large)
           weigh<1, true>(x + 16 * b, f[b], m, w[b], last + 1 - pos0 - 16 * b, sum, hi, nullptr);
         else
           weigh<1, false>(x + 16 * b, f[b], m, w[b], 16, sum, hi, nullptr);
@@ -932,6 +941,7 @@ __global__ void __launch_bounds__(kThreads2, 1) prompt_f32_kernel(const PromptAr
     const float fac = nb > 0 ? row_fac[row] : 0.f;
     const uint32_t trow = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     float m = kNone;
+    bool large = false;  // a row's m is beyond kLarge
     f32x2 l = 0, acc[kDims / 2];
 #pragma unroll
     for (f32x2& x : acc) x = 0;
@@ -986,29 +996,32 @@ __global__ void __launch_bounds__(kThreads2, 1) prompt_f32_kernel(const PromptAr
         for (int i = 0; i < 32; ++i)
           if (pos0 + i > last) x[i] = -__int_as_float(0x7F800000);
       }
-      float mx = kNone, e = -__int_as_float(0x7F800000);  // the largest score, and log2 of the largest weight
+      float mx = kNone, top[2];
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
         float t = x[16 * b];
 #pragma unroll
         for (int i = 1; i < 16; ++i) t = fmaxf(t, x[16 * b + i]);
-        t *= f[b];
-        mx = fmaxf(mx, t);  // (a masked tile's -inf, or no number: ignored)
-        e = fmaxf(e, t + wl[b]);
+        top[b] = __fmul_rn(t, f[b]);  // (not in one step with what is taken off)
+        mx = fmaxf(mx, top[b]);  // (a masked tile's -inf, or no number: ignored)
       }
-      e = fmaxf(e, mx - kFaint + fmaxf(wl[0], wl[1]));
+      // log2 of the largest weight, for a maximum of mx
+      float e = fmaxf(fmaxf(top[0] - mx + wl[0], top[1] - mx + wl[1]), fmaxf(wl[0], wl[1]) - kFaint);
       // over both halves of the row (two buffers: the next block's barrier keeps them apart)
       float2* shared_max = reinterpret_cast<float2*>(row_max) + (j & 1) * 2 * kRows;
       shared_max[half * kRows + row] = make_float2(mx, e);
       asm volatile("bar.sync 1, 256;" ::: "memory");
       const float2 other = shared_max[(half ^ 1) * kRows + row];
-      mx = fmaxf(mx, other.x);
-      const bool grow = mx > m + kLag;
-      const float corr = grow ? ex2(m - mx) : 1.f;
+      const float both = fmaxf(mx, other.x);
+      const bool grow = both > m + kLag;
+      const float corr = grow ? ex2(m - both) : 1.f;
       const bool rescale = __any_sync(0xffffffffu, grow);
-      if (grow) m = mx;
-      if (rescale) l = mul2(l, pair(corr, corr));
-      const int r = exponent_of(fmaxf(e, other.y) - m);
+      if (grow) m = both;
+      if (rescale) {
+        l = mul2(l, pair(corr, corr));
+        large = __any_sync(0xffffffffu, m > kNone && fabsf(m) > kLarge);
+      }
+      const int r = exponent_of(fmaxf(e + (mx - m), other.y + (other.x - m)));
 #pragma unroll
       for (int b = 0; b < 2; ++b) w[b] = min_nan(w[b] * power(kTop2 - r), 1e37f);
       // (P of block j - 2 has been read: its O was added in the last round)
@@ -1017,7 +1030,7 @@ __global__ void __launch_bounds__(kThreads2, 1) prompt_f32_kernel(const PromptAr
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
         uint32_t hi[8], lo[8];
-        if (partial)
+        if (partial || large)
           weigh<2, true>(x + 16 * b, f[b], m, w[b], last + 1 - pos0 - 16 * b, sum, hi, lo);
         else
           weigh<2, false>(x + 16 * b, f[b], m, w[b], 16, sum, hi, lo);

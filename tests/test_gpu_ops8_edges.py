@@ -486,3 +486,46 @@ def test_a_mode_that_does_not_fit_leaves_the_engine_as_it_was(tiny_dir):
             want, ids = eng.transcribe_pcm(x), eng.last_tokens()
         else:
             assert eng.last_tokens() == ids
+
+
+# ------------------------------------------------------------------ scores of any size
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("size", [1e3, 1e5, 1e7, 1e9, 1e15, 1e25, 1e33])
+@pytest.mark.parametrize("near,far", [(1.0, -0.5), (-0.25, -1.0), (1.0, 0.5)])
+@pytest.mark.parametrize("rows,group", [(1, 2), (1, 4), (3, 5), (70, 2)])
+def test_one_key_far_above_the_others(ops, dt, size, near, far, rows, group):
+    """Scores of about near * size, of one key, and far * size, of all others, as far as f32 goes: the output is the
+    one key's value (the weights of the others are 0 in f32), whatever the rounding of such scores."""
+    hd, cap = 64, 512
+    L = 300 + rows
+    for at in (0, 5, 299):
+        c = filled_cache(ops, 1, 1, cap, hd, [L], seed=102)
+        k = far * (1 + 0.1 * rand(1, L, 1, hd, seed=103).clamp(-2, 2))
+        k[0, at] = near
+        z = torch.zeros(1, dtype=torch.int32, device="cuda")
+        ops.kv8_append(ops.Kv8Cache(*c), k, rand(1, L, 1, hd, seed=104), z)
+        # (one sign and no cancellation: a score is off by 2^-6 of itself at most, int8 keys and rounding together)
+        q = (size / math.sqrt(hd) * (1 + 0.1 * rand(1, rows, group, hd, seed=105).clamp(-2, 2))).to(dt)
+        got = ops.kv8_attention(q, ops.Kv8Cache(*c), z + 300)
+        want = (c[1][0, 0, at].double() * c[3][0, 0, at // 16].double()).expand_as(got)
+        assert ((got.double() - want).abs() <= want.abs() * (2.0 ** -20 + HALF[dt])).all(), at
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("rows,group", [(1, 2), (1, 4), (3, 5), (70, 2)])
+def test_equal_scores_of_any_size(ops, dt, rows, group):
+    """Equal keys far below zero: the mean of the values."""
+    hd, cap, L = 64, 512, 300 + rows
+    v = rand(1, L, 1, hd, seed=106)
+    z = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for size in (1.0, 1e6, 1e12, 1e31, 1e36):
+        c = filled_cache(ops, 1, 1, cap, hd, [L], seed=107)
+        ops.kv8_append(ops.Kv8Cache(*c), torch.full_like(v, -math.sqrt(size)), v, z)
+        q = torch.full((1, rows, group, hd), math.sqrt(size) / math.sqrt(hd), device="cuda", dtype=dt)
+        got = ops.kv8_attention(q, ops.Kv8Cache(*c), z + 300)
+        vv = c[1][0, 0, :L].double() * c[3][0, 0].repeat_interleave(16)[:L, None].double()
+        for r in range(rows):
+            want = vv[:301 + r].mean(0)
+            # weights alike: 2^-11 of each in one f16 plane, 2^-22 in two and the f32 sums
+            slack = vv[:301 + r].abs().mean(0) * (2.0 ** -19 if dt == F32 else 2.0 ** -11)
+            assert ((got[0, r].double() - want).abs() <= slack + want.abs() * HALF[dt]).all(), (size, r)
