@@ -3,7 +3,7 @@
 // One CTA owns 128 query rows of one KV head (row = query position x head of the group) and walks
 // the keys they see in blocks of 64. Per block
 //   S = Q K^T          M = 128, N = 64, K = head_dim   -> TMEM
-//   p = exp2(S f - m)  f = scale * log2(e) * K scale of 16 tokens; running maximum m and sum l
+//   p = exp2(S f - m)  f = scale * log2(e) * K scale of 16 tokens (a tile); running maximum m and sum l
 //   O += P V           P = p * V scale * 2^(kTop - r), an operand in TMEM; N = head_dim
 // and at the end O * 2^(r - kTop) / l.
 //
@@ -16,9 +16,10 @@
 // 2^-37 of the block's (f32 rows, whose blocks are added outside TMEM, each with an r of its own). Not as fractions
 // of the largest V scale: a block of large values that a row gives no weight, or does not see, would cost it the
 // others' bits (1e-3 of the output behind a scale 1e4 times as large); and thousands of keys that have 2^-25 of the
-// weight each add up. (Against the largest V scale of the row tile, looked at once: 4 x 512 bf16 rows behind 1000 to
-// 7000 113 -> 117 us, f32 166 -> 170. Looking at a block's weights only where its V scales leave a window below 2^r,
-// in a branch of the warp: 121 and 182.)
+// weight each add up. All blocks take the same path: a score is taken relative to its tile's largest, which is exact
+// for scores of any size, and a masked one is -inf (4 x 512 bf16 rows behind 1000 to 7000 112 us, f32 168; with a path
+// each for whole, partly masked and large-scored blocks 125 and 178, by their length; 113 and 166 with fractions of
+// the largest V scale and two paths).
 // m is only raised when a score exceeds it by 2^kLag, and r of bf16 rows when a weight exceeds 2^(r + kLag): what has
 // been summed is then rescaled, which the first blocks of a row do and later ones hardly ever.
 //
@@ -30,8 +31,8 @@
 // and counts together, with an elected lane to issue, took 64 rows over 8064 f32 keys from 197 to 149 us.)
 //   bf16 rows: 256 threads, a softmax thread a row; two CTAs an SM, one's softmax beside the other's
 //   products. O stays in TMEM. 8 x 381 rows over up to 1403 keys, 8 KV heads of 2 x 128: 44 us; 2048 rows
-//   over 8048 keys, 4 KV heads of 4 x 64: 140 us; 592 heads' rows over 8064 keys: 198 us, 785 TFLOP/s.
-//   f32 rows: see below. The same shapes: 67, 208 and 310 us.
+//   over 8048 keys, 4 KV heads of 4 x 64: 145 us; 592 heads' rows over 8064 keys: 201 us, 773 TFLOP/s.
+//   f32 rows: see below. The same shapes: 70, 214 and 310 us.
 // Bound: the chain of a block's steps (scores, maximum, exp2, P V). bf16 rows: 0.9 us a block and CTA alone
 // on its SM, two CTAs an SM, in which exp2 takes 0.27 us an SM and the products 0.3 to 0.35 (a quarter of the exp2 as
 // polynomials on the FMA units was slower: 51 -> 55 us); f32 rows: 1.2 us, the products 0.7 of them.
@@ -50,9 +51,9 @@ namespace {
 constexpr int kMaxParts = 4;  // CTAs that share a row tile's keys
 constexpr int kRows = 128, kKeys = 64, kThreads = 256, kFill = 96;  // (threads that bring K and V)
 constexpr float kNone = -3.4028235e38f;  // running maximum before any key: the lowest number, no score is below
-constexpr float kLarge = 65536.f;        // scores beyond are rounded before m is taken off (log2)
 constexpr float kLag = 8.f;  // what a score may exceed m by, and a bf16 row's weight 2^r (log2)
 constexpr int kTop1 = 7, kTop2 = 14;  // log2 of 2^r in P: 2^(kTop1 + kLag) and 2^kTop2 are in f16's range (to 65504)
+constexpr float kTiny = 1.1754944e-38f;  // for a factor of 0: a masked score's -inf stays -inf
 constexpr float kFaint = 80.f;  // probabilities under 2^-80 count as 2^-80 for r: P's factor stays finite
 constexpr uint32_t kColS = 0, kColP = 64, kColO = 128, kCols = 256;  // TMEM columns
 
@@ -202,26 +203,15 @@ __device__ __forceinline__ uint32_t pack_rest(float a, float b, uint32_t hi) {
   const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
   return pack_f16(a - f.x, b - f.y);
 }
-// One tile of 16 scores: probabilities ex2(x f - m), their sum to l, times w as f16 planes. CAREFUL: 0 where seen
-// says so, and x f rounded as m was, whose rounding would otherwise be the largest probability's exponent.
-template <int PL, bool CAREFUL>
-__device__ __forceinline__ void weigh(const float* x, float f, float m, float w, int seen, f32x2& l, uint32_t* hi,
-                                      uint32_t* lo) {
-  const f32x2 f2 = pair(f, f), m2 = pair(-m, -m), w2 = pair(w, w);
+// One tile of 16 scores, the largest of which is t: probabilities ex2((x - t) f + d), their sum to l, times w as f16
+// planes. (Not ex2(x f - m): of large scores the rounding of m would be the largest probability's exponent.)
+template <int PL>
+__device__ __forceinline__ void weigh(const float* x, float t, float f, float d, float w, f32x2& l, uint32_t* hi, uint32_t* lo) {
+  const f32x2 t2 = pair(-t, -t), f2 = pair(f, f), d2 = pair(d, d), w2 = pair(w, w);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    float2 t;
-    if (CAREFUL)  // (f32 pairs would be multiplied and added in one step all the same)
-      t = make_float2(__fsub_rn(__fmul_rn(x[2 * i], f), m), __fsub_rn(__fmul_rn(x[2 * i + 1], f), m));
-    else
-      t = split(fma2(pair(x[2 * i], x[2 * i + 1]), f2, m2));
-    t.x = ex2(t.x);
-    t.y = ex2(t.y);
-    if (CAREFUL) {  // (not by the score: -inf times a zero scale is no number)
-      if (2 * i >= seen) t.x = 0.f;
-      if (2 * i + 1 >= seen) t.y = 0.f;
-    }
-    const f32x2 p = pair(t.x, t.y);
+    const float2 y = split(fma2(add2(pair(x[2 * i], x[2 * i + 1]), t2), f2, d2));
+    const f32x2 p = pair(ex2(y.x), ex2(y.y));
     l = add2(l, p);
     const f32x2 v = mul2(p, w2);
     const float2 u = split(v);
@@ -667,8 +657,7 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_bf16_kernel(const PromptAr
     const uint32_t trow = tmem + ((uint32_t)(warp * 32) << 16);
     // log2 of the largest weight so far, relative to m; r + kLag, and 2^(kTop1 - r)
     float m = kNone, most = -__int_as_float(0x7F800000), full = -__int_as_float(0x7F800000), up = 1.f;
-    bool large = false;  // a row's m is beyond kLarge
-    f32x2 l = 0;         // two partial sums
+    f32x2 l = 0;  // two partial sums
     float kn[4], vn[4];  // the next block's scales
     auto scales = [&](int j) {
 #pragma unroll
@@ -688,8 +677,9 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_bf16_kernel(const PromptAr
       for (int b = 0; b < 4; ++b) {
         f[b] = fac * kn[b];
         w[b] = vn[b];
-        // a row that sees nothing of a tile takes nothing of its scale either
-        if (partial && pos0 + b * kKv8Block > last) w[b] = 0.f;
+        if (f[b] == 0.f) f[b] = kTiny;
+        // a row that sees nothing of a tile takes nothing of its scales either (they may be NaN)
+        if (partial && pos0 + b * kKv8Block > last) f[b] = 1.f, w[b] = 0.f;
         wl[b] = lg2(w[b]);
       }
       const float faint = fmaxf(fmaxf(wl[0], wl[1]), fmaxf(wl[2], wl[3])) - kFaint;
@@ -708,17 +698,21 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_bf16_kernel(const PromptAr
         for (int i = 0; i < kKeys; ++i)
           if (pos0 + i > last) x[i] = -__int_as_float(0x7F800000);
       }
-      float mx = kNone, e = -__int_as_float(0x7F800000), top[4];
+      float mx = kNone, e = -__int_as_float(0x7F800000), top[4], d[4];  // a tile's largest x, and its score
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
-        float t = x[16 * b];
+        top[b] = x[16 * b];
 #pragma unroll
-        for (int i = 1; i < 16; ++i) t = fmaxf(t, x[16 * b + i]);
-        top[b] = __fmul_rn(t, f[b]);  // (not in one step with what is taken off)
-        mx = fmaxf(mx, top[b]);  // (a masked tile's -inf, or no number: ignored)
+        for (int i = 1; i < 16; ++i) top[b] = fmaxf(top[b], x[16 * b + i]);
+        top[b] = fmaxf(top[b], kNone);  // (a masked tile's -inf)
+        d[b] = __fmul_rn(top[b], f[b]);
+        mx = fmaxf(mx, d[b]);  // (no number: ignored)
       }
 #pragma unroll
-      for (int b = 0; b < 4; ++b) e = fmaxf(e, top[b] - mx + wl[b]);  // log2 of the largest weight, for a maximum of mx
+      for (int b = 0; b < 4; ++b) {
+        d[b] -= mx;
+        e = fmaxf(e, d[b] + wl[b]);  // log2 of the largest weight, for a maximum of mx
+      }
       const bool grow = mx > m + kLag || fmaxf(e + (mx - m), faint) > full, rescale = __any_sync(0xffffffffu, grow);
       float corr = 1.f, corr_o = 1.f;
       if (grow) {
@@ -731,7 +725,8 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_bf16_kernel(const PromptAr
         full = kLag + (float)r;
         up = power(kTop1 - r);
       }
-      if (rescale) large = __any_sync(0xffffffffu, m > kNone && fabsf(m) > kLarge);
+#pragma unroll
+      for (int b = 0; b < 4; ++b) d[b] += mx - m;
 #pragma unroll
       for (int b = 0; b < 4; ++b) w[b] *= up;
       if (j > 0) {
@@ -756,10 +751,7 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_bf16_kernel(const PromptAr
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
         uint32_t hi[8];
-        if (partial || large)
-          weigh<1, true>(x + 16 * b, f[b], m, w[b], last + 1 - pos0 - 16 * b, sum, hi, nullptr);
-        else
-          weigh<1, false>(x + 16 * b, f[b], m, w[b], 16, sum, hi, nullptr);
+        weigh<1>(x + 16 * b, top[b], f[b], d[b], w[b], sum, hi, nullptr);
         tmem_st8(trow + kColP + 8 * b, hi);
       }
       l = add2(l, sum);
@@ -941,7 +933,6 @@ __global__ void __launch_bounds__(kThreads2, 1) prompt_f32_kernel(const PromptAr
     const float fac = nb > 0 ? row_fac[row] : 0.f;
     const uint32_t trow = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     float m = kNone;
-    bool large = false;  // a row's m is beyond kLarge
     f32x2 l = 0, acc[kDims / 2];
 #pragma unroll
     for (f32x2& x : acc) x = 0;
@@ -978,8 +969,9 @@ __global__ void __launch_bounds__(kThreads2, 1) prompt_f32_kernel(const PromptAr
       for (int b = 0; b < 2; ++b) {
         f[b] = fac * kn[b];
         w[b] = vn[b];
-        // a row that sees nothing of a tile takes nothing of its scale either
-        if (partial && pos0 + b * kKv8Block > last) w[b] = 0.f;
+        if (f[b] == 0.f) f[b] = kTiny;
+        // a row that sees nothing of a tile takes nothing of its scales either (they may be NaN)
+        if (partial && pos0 + b * kKv8Block > last) f[b] = 1.f, w[b] = 0.f;
         wl[b] = lg2(w[b]);
       }
       if (j + 1 < nb) scales(j + 1);
@@ -996,17 +988,20 @@ __global__ void __launch_bounds__(kThreads2, 1) prompt_f32_kernel(const PromptAr
         for (int i = 0; i < 32; ++i)
           if (pos0 + i > last) x[i] = -__int_as_float(0x7F800000);
       }
-      float mx = kNone, top[2];
+      float mx = kNone, top[2], d[2];  // a tile's largest x, and its score
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
-        float t = x[16 * b];
+        top[b] = x[16 * b];
 #pragma unroll
-        for (int i = 1; i < 16; ++i) t = fmaxf(t, x[16 * b + i]);
-        top[b] = __fmul_rn(t, f[b]);  // (not in one step with what is taken off)
-        mx = fmaxf(mx, top[b]);  // (a masked tile's -inf, or no number: ignored)
+        for (int i = 1; i < 16; ++i) top[b] = fmaxf(top[b], x[16 * b + i]);
+        top[b] = fmaxf(top[b], kNone);  // (a masked tile's -inf)
+        d[b] = __fmul_rn(top[b], f[b]);
+        mx = fmaxf(mx, d[b]);  // (no number: ignored)
       }
+      d[0] -= mx;
+      d[1] -= mx;
       // log2 of the largest weight, for a maximum of mx
-      float e = fmaxf(fmaxf(top[0] - mx + wl[0], top[1] - mx + wl[1]), fmaxf(wl[0], wl[1]) - kFaint);
+      const float e = fmaxf(fmaxf(d[0] + wl[0], d[1] + wl[1]), fmaxf(wl[0], wl[1]) - kFaint);
       // over both halves of the row (two buffers: the next block's barrier keeps them apart)
       float2* shared_max = reinterpret_cast<float2*>(row_max) + (j & 1) * 2 * kRows;
       shared_max[half * kRows + row] = make_float2(mx, e);
@@ -1017,10 +1012,9 @@ __global__ void __launch_bounds__(kThreads2, 1) prompt_f32_kernel(const PromptAr
       const float corr = grow ? ex2(m - both) : 1.f;
       const bool rescale = __any_sync(0xffffffffu, grow);
       if (grow) m = both;
-      if (rescale) {
-        l = mul2(l, pair(corr, corr));
-        large = __any_sync(0xffffffffu, m > kNone && fabsf(m) > kLarge);
-      }
+      if (rescale) l = mul2(l, pair(corr, corr));
+      d[0] += mx - m;
+      d[1] += mx - m;
       const int r = exponent_of(fmaxf(e + (mx - m), other.y + (other.x - m)));
 #pragma unroll
       for (int b = 0; b < 2; ++b) w[b] = min_nan(w[b] * power(kTop2 - r), 1e37f);
@@ -1030,10 +1024,7 @@ __global__ void __launch_bounds__(kThreads2, 1) prompt_f32_kernel(const PromptAr
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
         uint32_t hi[8], lo[8];
-        if (partial || large)
-          weigh<2, true>(x + 16 * b, f[b], m, w[b], last + 1 - pos0 - 16 * b, sum, hi, lo);
-        else
-          weigh<2, false>(x + 16 * b, f[b], m, w[b], 16, sum, hi, lo);
+        weigh<2>(x + 16 * b, top[b], f[b], d[b], w[b], sum, hi, lo);
         tmem_st8(pcol + 8 * b, hi);
         tmem_st8(pcol + 32 + 8 * b, lo);
       }
