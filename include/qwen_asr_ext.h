@@ -262,7 +262,7 @@ int32_t qwen_asr_linear_int8(const int8_t* xq, int64_t ldx, const float* xs, con
                              int64_t ldr, void* out, int64_t ldo, int32_t dtype, int32_t device, void* stream);
 
 /* An int8 KV cache of n_seq sequences: k and v [n_seq][n_kv][capacity][head_dim], and an f32
- * scale for each block of 16 tokens of a head, [n_seq][n_kv][capacity / 16]. capacity is a
+ * scale (not negative) for each block of 16 tokens of a head, [n_seq][n_kv][capacity / 16]. capacity is a
  * multiple of 16, head_dim 64 or 128; seq_stride / scale_stride are the elements from one
  * sequence to the next (a layer of a larger cache is a pointer into it and its strides). */
 typedef struct QwenAsrKv8 {

@@ -346,7 +346,7 @@ __device__ __forceinline__ void rows_of(const AttnArgs& a, int seq, int& start, 
 
 // The CTA's sequence and its rows: a kernel's first reads. Where not all CTAs run at once, the longest of
 // every 32 sequences go first, so that none of them is left for the end (32 sequences of 0 to 8191 tokens in
-// ascending order: 61 us as they come, 49 so). All 32 lanes call it.
+// ascending order: 61 us as they come, 50 so). All 32 lanes call it.
 __device__ __forceinline__ int live_rows(const AttnArgs& a, int& start, int& count) {
   pdl_launch_dependents();
   pdl_wait();
@@ -916,9 +916,9 @@ __global__ void __launch_bounds__(kDigWarps * 32, RH == 1 ? 3 : 2) digit_kernel(
 // CTAs that share a sequence's length, for `ctas` CTAs unsplit: powers of two while all of them run
 // at once (two an SM; one an SM for 16, which wait long for room) and each keeps 256 tokens; between one and
 // two CTAs an SM two where sequences may be long, because lengths differ. 16 query heads on 8 x 128, measured
-// (us) at 1 / 2 / 4 / 8 / 16 splits: 8 CTAs of 436 tokens 7.5 / 6.6 / 5.7 / 6.3 / 8.2; 8 of 8000 49 / 28 / 17 /
-// 12.4 / 12.5; 16 of 0 to 8000 49 / 28 / 17 / 14 / 18; 64 of 0 to 8000 49 / 28 / 21 / 24 / 51; 256 of 0 to 8000
-// 63 / 48 / 62 / 93, of 8000 92 / 88 / 101 / 134, of 1000 15 / 22 / 33 / 61; 1024 of 0 to 1000 40 / 65 / 109.
+// (us) at 1 / 2 / 4 / 8 / 16 splits: 8 CTAs of 436 tokens 7.6 / 6.6 / 5.8 / 6.4 / 8.2; 8 of 8000 53 / 30 / 18 /
+// 12.9 / 12.7; 16 of 0 to 8000 53 / 30 / 18 / 14 / 19; 64 of 0 to 8000 53 / 30 / 22 / 24 / 52; 256 of 0 to 8000
+// 66 / 48 / 62 / 95, of 8000 93 / 90 / 101 / 131, of 1000 15 / 23 / 34 / 62; 1024 of 0 to 1000 41 / 66 / 111.
 int auto_splits(long long ctas, int max_len) {
   const int sms = ops_sm_count();
   const long long room = 2LL * sms;
@@ -947,7 +947,7 @@ cudaError_t launch(AttnArgs a, int max_len, int splits, cudaStream_t s) {
   constexpr int R = WarpState<HD, PL>::kRows;
   const int n_rows = a.rows * a.group;
   if (n_rows <= 2) return launch_digit<HD, 1, PL == 1>(a, max_len, splits, s);
-  // (8 rows as two digit tiles: 170 us for 32 x 8191 tokens, one f16 tile 147 us)
+  // (8 rows as two digit tiles: 170 us for 32 x 8191 tokens, one f16 tile 155 us)
   if (n_rows <= 4) return launch_digit<HD, 2, PL == 1>(a, max_len, splits, s);
   a.row_tiles = (n_rows + R - 1) / R;
   const long long ctas = (long long)a.c.n_kv * a.row_tiles * a.c.n_seq;

@@ -9,8 +9,8 @@
 //
 // Precision. int8 is exact in f16, so K and V enter the products as they are; their scales stay
 // outside, in f32. A query row is scaled by a power of two to [1/2, 1). For f32 rows q and P are two f16
-// planes, hi + lo, which hold a value to 2^-22 of itself (q, or 2^-25 of the row's largest); both planes add into the same f32 accumulator. For bf16
-// rows one plane: 2^-11 of a probability, an eighth of the output's own rounding.
+// planes, hi + lo, which hold a value to 2^-22 of itself (q, or 2^-25 of the row's largest); both planes add into
+// the same f32 accumulator. For bf16 rows one plane: 2^-11 of a probability, an eighth of the output's own rounding.
 // f16 has no step below 2^-24, so a row's weights p * V scale are held as fractions of about the largest of them,
 // 2^r, in the upper part of its range: none is off by more than 2^-30 of the row's largest so far (bf16 rows) or
 // 2^-37 of the block's (f32 rows, whose blocks are added outside TMEM, each with an r of its own). Not as fractions
@@ -1159,9 +1159,10 @@ __global__ void __launch_bounds__(kThreads2, 1) prompt_f32_kernel(const PromptAr
 // CTAs of a row tile, 1, 2 or 4, whose parts a cluster joins through shared memory: the number with the least
 // estimated time in blocks of keys, of which a CTA's prologue and output cost 8 and a joined one's 11; `room` CTAs
 // run at once. (Eight wait long for a place.) 16 heads on 8 x 128, measured (us) at 1 / 2 / 4: 128 rows behind 8000
-// bf16 116 / 66 / 39, f32 148 / 82 / 46, behind 900 22 / 19 / 15 and 27 / 22 / 16; 512 rows behind 7000 bf16 127 /
-// 85 / 53; 1500 rows behind 6000 bf16 181 / 137 / 146; 4 x 512 behind 1000 to 7000 bf16 163 / 112 / 141, f32 166 /
-// 186 / 245; 8 x 381 behind 0 to 1022 bf16 46 / 68 / 108.
+// bf16 124 / 70 / 42, f32 150 / 84 / 48, behind 100 11.5 / 12.9 / 11.1 and 13.1 / 13.7 / 12.1; 2 x 512 rows behind
+// 3000 and 7000 bf16 155 / 96 / 85, f32 146 / 120 / 144; 1500 rows behind 6000 bf16 174 / 138 / 148, f32 243 / 215 /
+// 247; 4 x 512 behind 1000 to 7000 bf16 169 / 113 / 139, f32 167 / 187 / 248; 8 x 381 behind 0 to 1022 bf16 45 / 65 /
+// 103, f32 70 / 114 / 181.
 int auto_splits(long long ctas, int room, int max_len) {
   const long long blocks = (max_len + kKeys - 1) / kKeys;
   int best = 1;

@@ -17,7 +17,7 @@
 // Bound: DRAM for many rows. What it took to get near: a bf16 sum as packed adds, one fmax a
 // value, rounding by the 1.5 * 2^23 trick whose low byte is the int8 value, and a warp that adds up
 // the squares behind the barrier while the others quantise (they do not need the norm). 16411
-// rows of 2048 bf16 values with a residual, call after call: 44 us, 5.3 TB/s; f32 67 us, 6.6 TB/s.
+// rows of 2048 bf16 values with a residual, call after call: 46 us, 5.1 TB/s; f32 68 us, 6.4 TB/s.
 #include <cuda_bf16.h>
 
 #include "bulk.cuh"
@@ -179,7 +179,7 @@ __device__ __forceinline__ void fix_near(const NormArgs& a, long long row, doubl
 }
 
 // One row by W warps, its values in registers: NV vectors of V a thread. V = 1: rows of any length, stride and
-// alignment (16411 x 2045 bf16 with residual 184 us by the kernel below, 92 so).
+// alignment (16411 x 2045 bf16 with residual 184 us by the kernel below, 87 so).
 template <bool BF16, int V, int W, int NV>
 __global__ void __launch_bounds__(W * 32) norm_vec_kernel(const NormArgs a) {
   using E = Elem<BF16>;

@@ -46,7 +46,7 @@ _raw_stream = torch._C._cuda_getCurrentRawStream  # the current stream's handle,
 
 class Kv8Cache(NamedTuple):
     """An int8 KV cache: k and v int8 [n_seq, n_kv, capacity, head_dim], k_scale and v_scale f32
-    [n_seq, n_kv, capacity / 16]. Slices along n_seq, or layers of a larger tensor, are caches too."""
+    [n_seq, n_kv, capacity / 16], not negative. Slices along n_seq, or layers of a larger tensor, are caches too."""
     k: torch.Tensor
     v: torch.Tensor
     k_scale: torch.Tensor
