@@ -314,30 +314,30 @@ bool Engine::ensure_kv(int needed) {
   if (kv_mode_ == KV_INT8) {
     if (!resize_kv8(slots_, nm, (size_t)(slots_ > 1 ? max_seq_ : kv_len_))) return false;
   } else {
-  size_t per = (size_t)slots_ * c.dec_layers * c.dec_kv_heads * nm * 128;
-  float *nk = nullptr, *nv = nullptr;
-  CUDA_OK(cudaMalloc(&nk, per * 4), false);
-  CUDA_OK(cudaMalloc(&nv, per * 4), false);
-  if (kc_.p && max_seq_ > 0) {
-    // copy every (slot, layer, head) row run into the wider layout (decoder.rs:199-231)
-    size_t rows = (size_t)slots_ * c.dec_layers * c.dec_kv_heads;
-    size_t used = (size_t)(slots_ > 1 ? max_seq_ : kv_len_) * 128 * 4;
-    if (used > 0) {
-      CUDA_OK(cudaMemcpy2DAsync(nk, (size_t)nm * 128 * 4, kc_.p, (size_t)max_seq_ * 128 * 4, used, rows,
-                                cudaMemcpyDeviceToDevice, stream_),
-              false);
-      CUDA_OK(cudaMemcpy2DAsync(nv, (size_t)nm * 128 * 4, vc_.p, (size_t)max_seq_ * 128 * 4, used, rows,
-                                cudaMemcpyDeviceToDevice, stream_),
-              false);
-      CUDA_OK(cudaStreamSynchronize(stream_), false);
+    size_t per = (size_t)slots_ * c.dec_layers * c.dec_kv_heads * nm * 128;
+    float *nk = nullptr, *nv = nullptr;
+    CUDA_OK(cudaMalloc(&nk, per * 4), false);
+    CUDA_OK(cudaMalloc(&nv, per * 4), false);
+    if (kc_.p && max_seq_ > 0) {
+      // copy every (slot, layer, head) row run into the wider layout (decoder.rs:199-231)
+      size_t rows = (size_t)slots_ * c.dec_layers * c.dec_kv_heads;
+      size_t used = (size_t)(slots_ > 1 ? max_seq_ : kv_len_) * 128 * 4;
+      if (used > 0) {
+        CUDA_OK(cudaMemcpy2DAsync(nk, (size_t)nm * 128 * 4, kc_.p, (size_t)max_seq_ * 128 * 4, used, rows,
+                                  cudaMemcpyDeviceToDevice, stream_),
+                false);
+        CUDA_OK(cudaMemcpy2DAsync(nv, (size_t)nm * 128 * 4, vc_.p, (size_t)max_seq_ * 128 * 4, used, rows,
+                                  cudaMemcpyDeviceToDevice, stream_),
+                false);
+        CUDA_OK(cudaStreamSynchronize(stream_), false);
+      }
     }
-  }
-  kc_.release();
-  vc_.release();
-  kc_.p = nk;
-  kc_.n = per;
-  vc_.p = nv;
-  vc_.n = per;
+    kc_.release();
+    vc_.release();
+    kc_.p = nk;
+    kc_.n = per;
+    vc_.p = nv;
+    vc_.n = per;
   }
   max_seq_ = nm;
   std::vector<float> rc, rs;
@@ -742,12 +742,12 @@ bool Engine::prefill_layers(float* x, int R, const std::vector<RowBlock>& blocks
                           OPS_F32, ops_err_.p, stream_),
               false);
     } else {
-    rms_norm_rows(x, pxn_.p, R, h, L.n1, c.dec_rms_norm_eps, stream_, pl_a_.p, plH);
-    GemmArgs a;
-    a.M = R; a.N = ldq; a.K = h; a.A = pxn_.p; a.lda = h; a.B = L.wqkv; a.ldb = h;
-    a.C = pqkv_.p; a.ldc = ldq;
-    a.a_split = pl_a_.p; a.a_split_ld = h; a.a_split_plane = plH;
-    gemm(a, stream_);
+      rms_norm_rows(x, pxn_.p, R, h, L.n1, c.dec_rms_norm_eps, stream_, pl_a_.p, plH);
+      GemmArgs a;
+      a.M = R; a.N = ldq; a.K = h; a.A = pxn_.p; a.lda = h; a.B = L.wqkv; a.ldb = h;
+      a.C = pqkv_.p; a.ldc = ldq;
+      a.a_split = pl_a_.p; a.a_split_ld = h; a.a_split_plane = plH;
+      gemm(a, stream_);
     }
     if (kv8) {
       // norm and RoPE of all rows in place, then each sequence's rows into its slot and over it
