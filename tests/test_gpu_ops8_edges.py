@@ -529,3 +529,57 @@ def test_equal_scores_of_any_size(ops, dt, rows, group):
             # weights alike: 2^-11 of each in one f16 plane, 2^-22 in two and the f32 sums
             slack = vv[:301 + r].abs().mean(0) * (2.0 ** -19 if dt == F32 else 2.0 ** -11)
             assert ((got[0, r].double() - want).abs() <= slack + want.abs() * HALF[dt]).all(), (size, r)
+
+
+# ------------------------------------------------------------------ the largest shapes
+def test_heads_past_2_gib_in_a_sequence_of_a_million_tokens():
+    """Positions near the end of a cache whose last heads start more than 2^31 bytes behind the first."""
+    from qwen_asr_b200 import ops
+    n_kv, hd, cap, new = 18, 128, (1 << 20) + 16, 100
+    c = ops.kv8_cache(1, n_kv, cap, hd)
+    assert (n_kv - 1) * cap * hd > 2 ** 31
+    start = (1 << 20) - 37
+    z = torch.full((1,), start, dtype=torch.int32, device="cuda")
+    k, v = rand(1, new, n_kv, hd, seed=110), rand(1, new, n_kv, hd, seed=111)
+    k *= 6  # (some of the new keys outweigh the million zeros)
+    ops.kv8_append(c, k, v, z)
+    kr, vr = ops.kv8_read(c, z, new)
+    assert not kr[0, cap - start:].any() and not vr[0, cap - start:].any()
+    for rows, heads, dt in ((1, 18, F32), (1, 36, BF16), (3, 36, F32), (6, 54, BF16), (60, 36, F32), (40, 54, BF16)):
+        q = rand(1, rows, heads, hd, seed=112).to(dt) * 2
+        got = ops.kv8_attention(q, c, z)
+        for h in (0, heads - 1):
+            kk, vv = kr[0, :, h * n_kv // heads].double(), vr[0, :, h * n_kv // heads].double()
+            x = q[0, :, h].double() @ kk.T / math.sqrt(hd)                      # the zeros before have a score of 0
+            x = x.masked_fill(torch.arange(new, device="cuda") > torch.arange(rows, device="cuda")[:, None], -math.inf)
+            top = x.amax(1, keepdim=True).clamp_min(0)
+            p = torch.exp(x - top)
+            l = p.sum(1, keepdim=True) + start * torch.exp(-top)
+            # scores off by d, weights held to 2^-22 or 2^-11 and by 2^-29 of the largest (the zeros have no value); l
+            # by at most 4096 sums in f32 one after the other (a million keys in blocks of 64, four parts): 2^-12
+            d = 2 * 2.0 ** -21 / math.sqrt(hd) * (q[0, :, h].double().abs().amax(1) * kk.abs().sum(1).amax())[:, None]
+            held = 2.0 ** -22 if dt == F32 else 2.0 ** -11
+            size = p @ vv.abs() / l
+            tol = size * (d + held + 2.0 ** -12 + 2.0 ** -22) + (p @ vv / l).abs() * HALF[dt]
+            tol += new * 2.0 ** -29 * vv.abs().max() / l
+            assert ((got[0, :, h].double() - p @ vv / l).abs() <= tol).all(), (rows, heads, dt, h)
+
+
+def test_many_sequences_and_many_heads():
+    """65535 sequences, and 4096 KV heads: the last ones as the first."""
+    from qwen_asr_b200 import ops
+    for n, n_kv, rows, group in ((65535, 1, 1, 1), (65535, 1, 7, 2), (65535, 1, 70, 1), (2, 4096, 1, 1), (2, 4096, 5, 2), (2, 4096, 40, 2)):
+        cap = 96
+        c = ops.kv8_cache(n, n_kv, cap, 64)
+        st = torch.randint(0, 20, (n,), generator=torch.Generator().manual_seed(n), dtype=torch.int32).cuda()
+        k = rand(n, rows + 20, n_kv, 64, seed=113)
+        ops.kv8_append(c, k, k, torch.zeros_like(st))
+        q = rand(n, rows, n_kv * group, 64, seed=114)
+        got = ops.kv8_attention(q, c, st)
+        for i in sorted({0, 1, n // 2, n - 1}):
+            for h in sorted({0, n_kv - 1}):
+                few = [t[i:i + 1, h:h + 1].contiguous() for t in c]
+                want, tol = weighed_ref(q[i:i + 1, :, h * group:(h + 1) * group], few, [st[i].item()], 1 / 8)
+                assert ((got[i:i + 1, :, h * group:(h + 1) * group].double() - want).abs() <= tol).all(), (n, rows, i, h)
+        back = ops.kv8_read(c, st, 2)[0]
+        assert torch.equal(back[-1, :, -1], few[0][0, 0, st[-1]:st[-1] + 2].float() * few[2][0, 0].repeat_interleave(16)[st[-1]:st[-1] + 2, None])
