@@ -19,35 +19,42 @@ class DeviceScope {
  public:
   explicit DeviceScope(int device) {
     if (device < 0) return;
-    if (!get_ || !set_ || !dev_) {
-      load("cuCtxGetCurrent", (void**)&get_);
-      load("cuCtxSetCurrent", (void**)&set_);
-      load("cuCtxGetDevice", (void**)&dev_);
-    }
-    if (!get_ || !set_ || !dev_) {
+    const Driver& d = driver();
+    if (!d.get || !d.set || !d.device) {
       ok_ = false;
       return;
     }
-    CUdevice d = -1;
-    if (get_(&prev_) == CUDA_SUCCESS && prev_ && dev_(&d) == CUDA_SUCCESS && (int)d == device) return;
+    CUdevice now = -1;
+    if (d.get(&prev_) == CUDA_SUCCESS && prev_ && d.device(&now) == CUDA_SUCCESS && (int)now == device) return;
     ok_ = cudaSetDevice(device) == cudaSuccess;
     restore_ = prev_ != nullptr;
   }
   ~DeviceScope() {
-    if (restore_) set_(prev_);
+    if (restore_) driver().set(prev_);
   }
   bool ok() const { return ok_; }
 
  private:
-  static void load(const char* name, void** fn) {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint(name, &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
-      *fn = p;
+  struct Driver {
+    CUresult (*get)(CUcontext*) = nullptr;
+    CUresult (*set)(CUcontext) = nullptr;
+    CUresult (*device)(CUdevice*) = nullptr;
+    Driver() {
+      load("cuCtxGetCurrent", (void**)&get);
+      load("cuCtxSetCurrent", (void**)&set);
+      load("cuCtxGetDevice", (void**)&device);
+    }
+    static void load(const char* name, void** fn) {
+      void* p = nullptr;
+      cudaDriverEntryPointQueryResult q;
+      if (cudaGetDriverEntryPoint(name, &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
+        *fn = p;
+    }
+  };
+  static const Driver& driver() {  // looked up once, whichever thread comes first
+    static const Driver d;
+    return d;
   }
-  static inline CUresult (*get_)(CUcontext*) = nullptr;
-  static inline CUresult (*set_)(CUcontext) = nullptr;
-  static inline CUresult (*dev_)(CUdevice*) = nullptr;
   CUcontext prev_ = nullptr;
   bool restore_ = false, ok_ = true;
 };

@@ -583,3 +583,40 @@ def test_many_sequences_and_many_heads():
                 assert ((got[i:i + 1, :, h * group:(h + 1) * group].double() - want).abs() <= tol).all(), (n, rows, i, h)
         back = ops.kv8_read(c, st, 2)[0]
         assert torch.equal(back[-1, :, -1], few[0][0, 0, st[-1]:st[-1] + 2].float() * few[2][0, 0].repeat_interleave(16)[st[-1]:st[-1] + 2, None])
+
+
+def test_first_calls_of_many_threads_at_once():
+    """Threads whose first calls come together, through the interface that does not hold the interpreter's lock."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import threading
+import torch
+from qwen_asr_b200 import ops
+ops._fast = None
+x, w = torch.randn(40, 512, device='cuda'), torch.ones(512, device='cuda')
+wq = torch.randint(-127, 128, (1024, 512), dtype=torch.int8, device='cuda')
+ws = torch.rand(1024, device='cuda')
+z = torch.zeros(1, dtype=torch.int32, device='cuda')
+start, out = threading.Barrier(16), [None] * 16
+torch.cuda.synchronize()
+def run(i):
+    with torch.cuda.stream(torch.cuda.Stream()):
+        c = ops.kv8_cache(1, 2, 64, 128)
+        start.wait()
+        q, s, h = ops.rms_norm_int8(x, w, residual=x)
+        y = ops.linear_int8(q, s, wq, ws)[None].unflatten(2, (8, 128))
+        ops.kv8_append(c, y[:, :, 4:6], y[:, :, 6:], z)
+        out[i] = (ops.kv8_attention(y[:, :, :4], c, z), ops.kv8_attention(y[:, :1, :4], c, z + 39))
+        torch.cuda.current_stream().synchronize()
+threads = [threading.Thread(target=run, args=(i,)) for i in range(16)]
+[t.start() for t in threads]
+[t.join() for t in threads]
+ops.check()
+assert all(o is not None and all(torch.equal(a, b) for a, b in zip(o, out[0])) for o in out)
+print('alike')
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "alike" in r.stdout, r.stderr[-2000:]
